@@ -8,8 +8,10 @@ A case is a dict of plain values. Its "op" names the operator:
   read       kvcache.read        a cache's keys and values back in 16 bits
   attend     kvcache.attention   attention of query rows over the 8-bit cache
 
-Layouts. MXFP4: codes uint8 [rows, k / 2], the even column in the low four bits, and scales
-uint8 [rows, 4 ceil(k / 128)], one exponent byte (bias 127) for each 32 columns, the rest 0.
+Layouts. MXFP4: codes uint8 [rows, k / 2], the even column in the low four bits, and one
+exponent byte (bias 127) for each 32 columns in the order the matrix cores take them: scales
+uint8 [ceil(k / 128), ceil(rows / 64), 4, 16, 4], indexed by k / 128, row / 64, k / 32 % 4,
+row % 16 and row / 16 % 4; 0 past the end of a row.
 Cache: k uint8 [pages, heads, block, d] and v uint8 [pages, heads, d, block], e4m3 codes, with
 float32 scales [pages, heads] that are powers of two. table int32 [sequences, pages of each].
 """
@@ -144,9 +146,9 @@ def prepare(case, seed):
         s["x"] = _activations(g, c["m"], c["k"], DT[c["dtype"]])
         # weights as a quantiser leaves them: any code, block exponents around 2^-7
         s["codes"] = _nibbles(g, c["n"], c["k"])
-        s["scales"] = torch.zeros((c["n"], 4 * -(-c["k"] // 128)), dtype=torch.uint8, device="cuda")
-        s["scales"][:, : c["k"] // 32] = torch.randint(
-            117, 122, (c["n"], c["k"] // 32), generator=g, device="cuda", dtype=torch.uint8)
+        s["scales"] = torch.randint(117, 122, (-(-c["k"] // 128), -(-c["n"] // 64), 4, 16, 4),
+                                    generator=g, device="cuda", dtype=torch.uint8)
+        s["scales"][c["k"] // 128:, :, c["k"] // 32 % 4:] = 0
         return s
     held, new = _counts(c)
     cap, h, d, blk = _capacity(c), c["hkv"], c["d"], c["block"]
@@ -207,7 +209,8 @@ def _mx_decode(codes, scales, k):
     """float32 [rows, k] of stored codes and scale bytes."""
     lut = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
     nib = torch.stack([codes & 15, codes >> 4], dim=-1).reshape(codes.shape[0], -1, 32)
-    return (lut[nib.int()] * _pow2(scales[:, : k // 32])[..., None]).reshape(codes.shape[0], k)
+    by_row = scales.permute(1, 4, 3, 0, 2).flatten(3).flatten(0, 2)[: codes.shape[0], : k // 32]
+    return (lut[nib.int()] * _pow2(by_row)[..., None]).reshape(codes.shape[0], k)
 
 
 def _e4m3_scale(amax):
@@ -443,7 +446,9 @@ def exact(case, seed):
         for half in (0, 1):
             nib = (s["codes"] >> (4 * half)) & 15
             w[:, half::2] = mag[(nib & 7).long()] * (1 - 2 * (nib >> 3).double())
-        e = s["scales"][:, : c["k"] // 32].int() - 127
+        row = torch.arange(c["n"], device="cuda")[:, None]
+        blk = torch.arange(c["k"] // 32, device="cuda")[None, :]
+        e = s["scales"][blk // 4, row // 64, blk % 4, row % 16, row // 16 % 4].int() - 127
         w *= _two(e).repeat_interleave(32, dim=1)
         return _exact_mx(s["x"]) @ w.t()
     if c["op"] == "write":
