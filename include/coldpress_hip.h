@@ -396,6 +396,89 @@ int cp_col_log_rms(const void* x, int x_dtype, int64_t nrow, int64_t n, int64_t 
  * No counterpart in the reference: it checks an implementation choice of this library. */
 int cp_check_division(int64_t n, uint64_t seed, int64_t* mismatches, void* stream);
 
+/* ---- low-bit serving: MXFP4 weights and activations, an 8-bit paged cache ----
+ * No counterpart in the reference, which leaves answering with a quantized model to
+ * llama.cpp. Work is enqueued on ``stream``; nothing here synchronizes or allocates. */
+
+enum cp_dtype { CP_F32 = 0, CP_BF16 = 1, CP_F16 = 2 };
+
+/* Bytes of the scale array of [rows, k] values in MXFP4: ceil(k / 128) x ceil(rows / 64) x
+ * 256. Byte ((s * ceil(rows / 64) + r / 64) * 64 + 16 * (b % 4) + r % 16) * 4 + r / 16 % 4
+ * holds the exponent (bias 127) of row r's 32-value block b, s = b / 4: the order the
+ * matrix cores take them in. */
+size_t cp_mx4_scale_bytes(int64_t rows, int64_t k);
+
+/* MXFP4 of x [rows, k] (element type cp_dtype, rows row_stride elements apart, 16-byte
+ * aligned): codes [rows, k / 2], the even column in the low four bits, and scales as above.
+ * Per block of 32 with largest magnitude a: exponent floor(log2 a) - 2 (at least -127),
+ * codes rounded to nearest even in e2m1 and saturating at 6; a block with a NaN or an
+ * infinity gets scale byte 255 and decodes to NaN. k % 32 == 0. */
+int cp_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t row_stride,
+                    uint8_t* codes, uint8_t* scales, void* stream);
+
+/* y [rows, k] = the codes' values, rounded once to y's type. */
+int cp_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k,
+                      void* y, int y_dtype, void* stream);
+
+/* y [m, n] = a [m, k] b [n, k]^T of two MXFP4 arrays, summed in float32, rounded once. */
+int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
+                  const uint8_t* b_codes, const uint8_t* b_scales, int64_t n, int64_t k, void* y,
+                  int y_dtype, void* stream);
+
+/* Workspace bytes of cp_mx4_linear (256-byte aligned). */
+size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k);
+
+/* y [m, n] = x w^T for MXFP4 weights w [n, k]: x [m, k] is quantized as cp_mx4_quantize
+ * does, then multiplied as cp_mx4_matmul does. */
+int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride,
+                  const uint8_t* w_codes, const uint8_t* w_scales, int64_t n, int64_t k, void* y,
+                  int y_dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* A paged key / value cache in e4m3. A page holds ``block`` tokens (16, 32, 64 or 128) of
+ * every head; a code stands for its value times its page and head's scale, a power of two. */
+typedef struct cp_kv_cache {
+  uint8_t* k;      /* [pages, heads, block, head_dim] */
+  uint8_t* v;      /* [pages, heads, head_dim, block] */
+  float* k_scale;  /* [pages, heads] */
+  float* v_scale;  /* [pages, heads] */
+  int64_t pages;
+  int heads, block, head_dim; /* head_dim: a multiple of 16 up to 256 */
+} cp_kv_cache;
+
+/* Quantizes and appends rows of k and v [rows, heads, head_dim] (strides in elements; heads
+ * and rows 16-byte aligned). Sequence b's rows are offsets[b] .. offsets[b + 1] (offsets
+ * NULL: row b), its tokens go to positions filled[b] onward; position p is slot p % block of
+ * page table[b][p / block] (table [batch, max_pages]). A page's scale is the least 2^e, e in
+ * [-60, 60], with max |x| <= 448 * 2^e over the finite values written, or the scale it had
+ * where it holds tokens already and that is larger; a scale that grows moves the codes held.
+ * Values beyond 448 * scale saturate, NaN stays. Tokens past the table's end or on a page
+ * outside [0, pages) are dropped. Sequences written in one call must not share a page. */
+int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t k_head,
+                const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows,
+                const int32_t* table, int64_t batch, int64_t max_pages, const int32_t* filled,
+                const int32_t* offsets, void* stream);
+
+/* The first offsets[b + 1] - offsets[b] tokens of every sequence into k and v [total, heads,
+ * head_dim]; tokens without a page read as 0. */
+int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, int64_t max_pages,
+               const int32_t* offsets, int64_t total, void* k, void* v, int dtype, void* stream);
+
+/* Workspace bytes of cp_kv_attention (0: none); ragged: offsets are given. */
+size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads,
+                                int64_t batch, int64_t max_pages, int ragged);
+
+/* out [rows, q_heads, head_dim] = attention of q over the cache. Sequence b has lens[b]
+ * tokens; its query rows (as in cp_kv_write) sit at its last positions, and query head x
+ * reads cache head x / (q_heads / heads). Row at position p sees token j where j < lens[b],
+ * j <= p (causal) and j > p - window (window > 0); tokens without a page are not seen. A row
+ * that sees nothing is 0 with lse -inf. lse [rows, q_heads] float32 (NULL: not wanted) is
+ * the natural log of the sum of exponentials. q and out: bfloat16 or float16. */
+int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head,
+                    int dtype, int64_t rows, int q_heads, const int32_t* table, int64_t batch,
+                    int64_t max_pages, const int32_t* lens, const int32_t* offsets, int causal,
+                    int window, float scale, void* out, float* lse, void* ws, size_t ws_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

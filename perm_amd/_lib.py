@@ -55,6 +55,16 @@ class ColTensor(ctypes.Structure):
 
 _col_p = ctypes.POINTER(ColTensor)
 
+
+class KvCacheDesc(ctypes.Structure):
+    """struct cp_kv_cache (include/coldpress_hip.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("pages", ctypes.c_int64), ("heads", ctypes.c_int), ("block", ctypes.c_int),
+                ("head_dim", ctypes.c_int)]
+
+
+_kv_p = ctypes.POINTER(KvCacheDesc)
+
 # name -> (restype, argtypes); every symbol include/coldpress_hip.h declares
 SIGNATURES = {
     "cp_last_error": (ctypes.c_char_p, []),
@@ -104,6 +114,19 @@ SIGNATURES = {
     "cp_check_division": (_i32, [_i64, ctypes.c_uint64, _vp, _vp]),
     "cp_sq_err_ws_bytes": (_sz, [_i64, _i64]),
     "cp_sq_err_sum": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "cp_mx4_scale_bytes": (_sz, [_i64, _i64]),
+    "cp_mx4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "cp_mx4_dequantize": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "cp_mx4_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "cp_mx4_linear_ws_bytes": (_sz, [_i64, _i64]),
+    "cp_mx4_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _sz,
+                             _vp]),
+    "cp_kv_write": (_i32, [_kv_p, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _vp, _i64, _i64,
+                           _vp, _vp, _vp]),
+    "cp_kv_read": (_i32, [_kv_p, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _vp]),
+    "cp_kv_attention_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32]),
+    "cp_kv_attention": (_i32, [_kv_p, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _i64, _vp,
+                               _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -1,0 +1,429 @@
+// Attention over the paged 8-bit cache on gfx950.
+//
+// Row i of a sequence with n query rows and len tokens sits at position p = len - n + i and
+// sees token j where j < len, j <= p (causal) and j > p - window (window > 0). With K and V
+// codes in e4m3 and power-of-two scales ks, vs of each page and head, in base 2:
+//
+//     t_j = (q . kcode_j) * ks_j * scale * log2 e + log2 vs_j
+//     w_j = 2^(t_j - m),  m the running maximum of t
+//     out = sum_j w_j vcode_j / sum_j (w_j / vs_j)
+//
+// V's scale rides in the exponent, so the codes feed the matrix cores unscaled and w is at
+// most 1 whatever the scales are: w is rounded to float16 (11 bits) as the operand of the
+// second product, for bf16 queries too. Scores, m, the sum and the output accumulate in
+// float32. K codes become q's own 16-bit type, which holds e4m3 exactly.
+#include <hip/hip_runtime.h>
+
+#include "kvcache.h"
+#include "lowbit.h"
+
+namespace cp {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 64;       // tokens per step of a wave
+constexpr float kNegInf = -__builtin_inff();
+
+struct AttnArgs {
+  KvCacheArgs c;
+  const void* q;                // [rows][q heads][d]
+  int64_t q_row, q_head;
+  const int* lens;              // [batch]
+  void* out;                    // [rows][q heads][d]
+  float* lse;                   // [rows][q heads] or null
+  float* part;                  // splits > 1: [rows][q heads][splits][d + 2]
+  int64_t rows;
+  int group;                    // q heads per kv head
+  int causal, window, splits;
+  float scale;                  // softmax scale * log2 e
+};
+
+// Eight e4m3 codes in q's type / in float16 (both exact).
+template <int DT>
+__device__ __forceinline__ u32x4 codes_to_16(uint32_t a, uint32_t b) {
+  u32x4 r;
+  if constexpr (DT == CP_BF16) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true));
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == CP_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// Bytes of w that are NaN codes (0x7F or 0xFF) as 0x80 flags: 0x7F is the only magnitude
+// that carries out of seven bits when one is added.
+__device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// Few query rows: a workgroup takes up to 16 (row, head of the group) pairs of one kv head
+// and one range of tokens; its four waves walk the range's 64-token tiles in turn and join
+// at the end. K is the A operand (16 tokens x 32 columns), q the B operand, so a lane's
+// scores belong to one query row (lane % 16), and its group lane / 16 owns 16 consecutive
+// tokens of the tile: score (t, i) of the lane is token 16 (lane / 16) + 4 t + i. Those are
+// the eight-token runs the second product's operands hold, so the weights go from one
+// product to the other without leaving their lanes.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
+  constexpr int NC = DP / 64, ND = DP / 16;
+  __shared__ float sm_m[4][16], sm_l[4][16];
+  __shared__ __align__(16) float sm_o[4][16][DP + 4];
+  const KvCacheArgs& c = a.c;
+  const int split = (int)(blockIdx.x % a.splits);
+  const int h = (int)(blockIdx.x / a.splits % c.heads);
+  int b, item, n_b;
+  int64_t row0;
+  if (!kv_locate(bt, (int)(blockIdx.x / a.splits / c.heads),
+                 [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item,
+                 &row0, &n_b))
+    return;
+  if (row0 < 0 || row0 + n_b > a.rows) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
+  const int d = c.d, blk = c.block;
+  const int64_t cap = (int64_t)c.max_pages * blk;
+  const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
+
+  // this lane's query row
+  const int64_t r = (int64_t)item * 16 + col;
+  const bool real = r < (int64_t)n_b * a.group;
+  const int qi = (int)(r / a.group), qh = h * a.group + (int)(r % a.group);
+  const int64_t pos = (int64_t)len - n_b + qi;
+  int hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len) : 0;
+  int lo = a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+  if (lo >= hi) lo = hi = 0;
+  // tokens any row of the workgroup sees
+  int jhi = hi, jlo = hi > lo ? lo : 0x7FFFFFFF;
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) {
+    jhi = max(jhi, __shfl_xor(jhi, s));
+    jlo = min(jlo, __shfl_xor(jlo, s));
+  }
+  jlo = min(jlo, jhi);
+  const int t0 = jlo / kTile, nt = (jhi + kTile - 1) / kTile - t0;
+  const int per = (nt + a.splits - 1) / a.splits;
+  const int tb = t0 + split * per, te = min(t0 + nt, tb + per);
+
+  u32x4 qf[NC][2];
+  {
+    typedef typename Elem<DT>::T T;
+    const T* qp = (const T*)a.q + (row0 + qi) * a.q_row + (int64_t)qh * a.q_head;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const bool in = real && 64 * k + 16 * g < d;
+      const u32x4 z = {0, 0, 0, 0};
+      qf[k][0] = in ? *reinterpret_cast<const u32x4*>(qp + 64 * k + 16 * g) : z;
+      qf[k][1] = in ? *reinterpret_cast<const u32x4*>(qp + 64 * k + 16 * g + 8) : z;
+    }
+  }
+  f32x4 o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i] = f32x4{0, 0, 0, 0};
+  float m = kNegInf, l = 0.0f;
+  const int* tab = c.table + (int64_t)b * c.max_pages;
+
+  for (int tile = tb + wave; tile < te; tile += 4) {
+    const int j0 = tile * kTile;
+    // pages of the two 16-token groups this lane reads: K rows by lane % 16 / 4, V and the
+    // scores' scales by lane / 16
+    const int jk = j0 + 16 * (col >> 2), jv = j0 + 16 * g;
+    int pk = jk < len ? tab[jk / blk] : -1, pv = jv < len ? tab[jv / blk] : -1;
+    if ((unsigned)pk >= (unsigned)c.pages) pk = -1;
+    if ((unsigned)pv >= (unsigned)c.pages) pv = -1;
+    const int64_t ak = ((int64_t)max(pk, 0) * c.heads + h) * blk * d;
+    const int64_t hv = (int64_t)max(pv, 0) * c.heads + h;
+    const uint8_t* kp = c.k + ak + (int64_t)(jk % blk + (col & 3)) * d + 16 * g;
+    const uint8_t* vp = c.v + hv * blk * d + (int64_t)col * blk + jv % blk;
+    f32x4 sc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
+    u32x4 kk[4][NC], vv[ND];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const u32x4 z = {0, 0, 0, 0};
+        kk[t][k] = 64 * k + 16 * g < d ? *reinterpret_cast<const u32x4*>(kp + 4 * t * d + 64 * k) : z;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const u32x4 z = {0, 0, 0, 0};
+      vv[i] = 16 * i < d ? *reinterpret_cast<const u32x4*>(vp + (int64_t)16 * i * blk) : z;
+    }
+    const float ks = c.k_scale[hv], vs = c.v_scale[hv];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        sc[t] = mfma16<DT>(codes_to_16<DT>(kk[t][k][0], kk[t][k][1]), qf[k][0], sc[t]);
+        sc[t] = mfma16<DT>(codes_to_16<DT>(kk[t][k][2], kk[t][k][3]), qf[k][1], sc[t]);
+      }
+    }
+    const float kc = ks * a.scale;
+    const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+    const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs) & 0x7F800000u));
+    float tm = kNegInf;
+    bool edge = false;  // a token of this lane that its row does not see
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = jv + 4 * t + i;
+        const bool see = j >= lo && j < hi && pv >= 0;
+        edge |= !see;
+        sc[t][i] = see ? __builtin_fmaf(sc[t][i], kc, lv) : kNegInf;
+        tm = fmaxf(tm, sc[t][i]);
+      }
+    }
+    tm = fmaxf(tm, __shfl_xor(tm, 16));
+    tm = fmaxf(tm, __shfl_xor(tm, 32));
+    const float mn = fmaxf(m, tm);
+    const float ms = mn == kNegInf ? 0.0f : mn;  // nothing seen yet: weights 2^-inf = 0
+    const float al = exp2_fast(m - ms);
+    m = mn;
+    u32x4 w[2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float e0 = exp2_fast(sc[t][i] - ms), e1 = exp2_fast(sc[t][i + 1] - ms);
+        sum += e0 + e1;
+        w[t >> 1][2 * (t & 1) + (i >> 1)] = pack2<CP_F16>(e0, e1);
+      }
+    }
+    l = l * al + sum * iv;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] *= al;
+    if (__any(edge)) {
+      // a code that a row does not see must not reach it, not even as 0 * NaN: NaN codes
+      // are taken out of the product and put back into the rows that do see them
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= nan_flags(vv[i][k]);
+      if (__any(any != 0)) {
+        u32x4 one[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int t = 2 * s + (k >> 1), i = 2 * (k & 1);
+            one[s][k] = (sc[t][i] != kNegInf ? 0x3C00u : 0u) | (sc[t][i + 1] != kNegInf ? 0x3C000000u : 0u);
+          }
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          f32x4 cnt = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t f = nan_flags(vv[i][k]);
+            vv[i][k] &= ~(((f >> 7) * 0xFFu));
+            // e4m3 1.0 = 0x38 where the code was NaN
+            const uint32_t ind = (f >> 7) * 0x38u;
+            const u32x4 z = codes_to_16<CP_F16>(ind, ind);
+            u32x4 av = {0, 0, 0, 0};
+            av[2 * (k & 1)] = z[0];
+            av[2 * (k & 1) + 1] = z[1];
+            cnt = mfma16<CP_F16>(av, one[k >> 1], cnt);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (cnt[k] > 0.0f) o[i][k] = __builtin_nanf("");
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(vv[i][0], vv[i][1]), w[0], o[i]);
+      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(vv[i][2], vv[i][3]), w[1], o[i]);
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) sm_m[wave][col] = m, sm_l[wave][col] = l;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4*>(&sm_o[wave][col][16 * i + 4 * g]) = o[i];
+  __syncthreads();
+  // join the four waves: thread -> row threadIdx / 16, columns strided by 16
+  const int row = threadIdx.x >> 4, c0 = threadIdx.x & 15;
+  const int64_t rr = (int64_t)item * 16 + row;
+  if (rr >= (int64_t)n_b * a.group) return;
+  float mm = kNegInf, f[4], ll = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w][row]);
+  const float ms = mm == kNegInf ? 0.0f : mm;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = exp2_fast(sm_m[w][row] - ms);
+    ll += sm_l[w][row] * f[w];
+  }
+  const int64_t orow = (row0 + rr / a.group) * ((int64_t)a.group * c.heads) + h * a.group + rr % a.group;
+  if (a.splits > 1) {
+    float* p = a.part + (orow * a.splits + split) * (d + 2);
+    if (c0 == 0) p[d] = mm, p[d + 1] = ll;
+    for (int x = c0; x < d; x += 16) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += sm_o[w][row][x] * f[w];
+      p[x] = v;
+    }
+    return;
+  }
+  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;  // a row that saw nothing: 0
+  typename Elem<DT>::T* op = (typename Elem<DT>::T*)a.out + orow * d;
+  for (int x = c0; x < d; x += 16) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v += sm_o[w][row][x] * f[w];
+    op[x] = (typename Elem<DT>::T)(v * inv);
+  }
+  if (a.lse && c0 == 0) a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+}
+
+// The splits of a row joined, in split order. One wave per row.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, int64_t rows,
+                                                        int d, int splits,
+                                                        typename Elem<DT>::T* __restrict__ out,
+                                                        float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const float* p = part + row * splits * (d + 2);
+  float mm = kNegInf;
+  for (int s = lane; s < splits; s += 64) mm = fmaxf(mm, p[(int64_t)s * (d + 2) + d]);
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) mm = fmaxf(mm, __shfl_xor(mm, k));
+  const float ms = mm == kNegInf ? 0.0f : mm;
+  float ll = 0.0f, v[4] = {0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s) {
+    const float* ps = p + (int64_t)s * (d + 2);
+    const float f = exp2_fast(ps[d] - ms);
+    ll += ps[d + 1] * f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 64 * i < d) v[i] += ps[lane + 64 * i] * f;
+  }
+  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 64 * i < d) out[row * d + lane + 64 * i] = (typename Elem<DT>::T)(v[i] * inv);
+  if (lse && lane == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+}
+
+struct AttnPlan {
+  int64_t items;  // upper bound of the batch's row tiles
+  int splits;
+};
+
+static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int64_t cap) {
+  AttnPlan p;
+  p.items = ragged ? rows * group / 16 + batch : batch * ((group + 15) / 16);
+  // enough workgroups for every CU four times over, none under 256 tokens (a tile a wave)
+  const int64_t want = 1024 / (p.items * heads > 0 ? p.items * heads : 1);
+  const int64_t most = (cap + 255) / 256;
+  p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+  return p;
+}
+
+template <int DT, int DP>
+static void attn_launch(const AttnArgs& a, const KvBatch& b, int64_t items, hipStream_t st) {
+  attn_few_kernel<DT, DP><<<dim3((unsigned)(items * a.c.heads * a.splits)), 256, 0, st>>>(a, b);
+}
+
+template <int DT>
+static void attn_launch_d(const AttnArgs& a, const KvBatch& b, int64_t items, hipStream_t st) {
+  if (a.c.d <= 64) attn_launch<DT, 64>(a, b, items, st);
+  else if (a.c.d <= 128) attn_launch<DT, 128>(a, b, items, st);
+  else attn_launch<DT, 256>(a, b, items, st);
+  if (a.splits > 1) {
+    const int64_t n = a.rows * a.group * a.c.heads;
+    attn_join_kernel<DT><<<dim3((unsigned)((n + 3) / 4)), 256, 0, st>>>(
+        a.part, n, a.c.d, a.splits, (typename Elem<DT>::T*)a.out, a.lse);
+  }
+}
+
+static int attn_check(const cp_kv_cache* cache, int64_t rows, int q_heads, const int32_t* table,
+                      int64_t batch, int64_t max_pages, const int32_t* offsets) {
+  if (int s = kv_check_cache(cache)) return s;
+  if (int s = kv_check_batch(table, batch, max_pages, rows, offsets)) return s;
+  if (q_heads < 1 || q_heads % cache->heads)
+    return set_error(CP_ERR_SHAPE, "%d query heads over %d cache heads", q_heads, cache->heads);
+  return CP_OK;
+}
+
+}  // namespace cp
+
+extern "C" {
+
+size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads, int64_t batch,
+                                int64_t max_pages, int ragged) {
+  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
+  const cp::AttnPlan p = cp::attn_plan(rows, batch, ragged != 0, q_heads / cache->heads, cache->heads,
+                                       max_pages * cache->block);
+  return p.splits > 1 ? (size_t)rows * q_heads * p.splits * (cache->head_dim + 2) * 4 : 0;
+}
+
+int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,
+                    int64_t rows, int q_heads, const int32_t* table, int64_t batch, int64_t max_pages,
+                    const int32_t* lens, const int32_t* offsets, int causal, int window, float scale,
+                    void* out, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  cp::clear_error();
+  if (int s = cp::attn_check(cache, rows, q_heads, table, batch, max_pages, offsets)) return s;
+  if (dtype != CP_BF16 && dtype != CP_F16) return cp::set_error(CP_ERR_ARG, "queries are bfloat16 or float16");
+  if (window < 0) return cp::set_error(CP_ERR_ARG, "window %d", window);
+  if (rows == 0 || batch == 0) return CP_OK;
+  if (!q || !lens || !out) return cp::set_error(CP_ERR_ARG, "null q / lens / out");
+  if (!cp::aligned(q, 16) || q_row * 2 % 16 || q_head * 2 % 16 || !cp::aligned(out, 16))
+    return cp::set_error(CP_ERR_ALIGN, "rows and heads of q and out need 16-byte alignment");
+  if (q_row < 0 || q_head < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of q");
+  const int group = q_heads / cache->heads;
+  const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads,
+                                       max_pages * cache->block);
+  const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr);
+  if (need && (!ws || ws_bytes < need))
+    return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
+  if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > (int64_t)0x7FFFFFFF * 4)
+    return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  cp::AttnArgs a;
+  a.c = cp::kv_args(cache, table, max_pages);
+  a.q = q;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.lens = lens;
+  a.out = out;
+  a.lse = lse;
+  a.part = (float*)ws;
+  a.rows = rows;
+  a.group = group;
+  a.causal = causal != 0;
+  a.window = window;
+  a.splits = p.splits;
+  a.scale = scale * cp::kLog2e;
+  const cp::KvBatch b = {offsets, (int)batch};
+  if (dtype == CP_BF16) cp::attn_launch_d<CP_BF16>(a, b, p.items, (hipStream_t)stream);
+  else cp::attn_launch_d<CP_F16>(a, b, p.items, (hipStream_t)stream);
+  CP_LAUNCHED("cache attention");
+  return CP_OK;
+}
+
+}  // extern "C"

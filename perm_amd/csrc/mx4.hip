@@ -1,0 +1,350 @@
+// MXFP4 (microscaled 4-bit floating point) on gfx950: quantisation, decode and product.
+//
+// A block is 32 consecutive values of a row with one power-of-two scale 2^e. With
+// a = max |x| over the block,
+//     e = floor(log2 a) - 2 (at least -127),  code = RNE to e2m1 of x * 2^-e,  |code| <= 6
+// so the largest magnitude lands in [4, 8) and saturates at 6. A block with a NaN or an
+// infinity gets the scale byte 255 and decodes to NaN; an all-zero block gets byte 0.
+// Scaling by a power of two is exact, so the e2m1 rounding is the only one.
+//
+// Layout. codes [rows][k / 2], two a byte, the even column in the low four bits. The scale
+// bytes (e + 127) lie as v_mfma_scale_f32_16x16x128_f8f6f4 takes them: its lane l holds row
+// l % 16 and the 32-block l / 16 of a 128-wide step, and picks one byte of a dword by an
+// immediate. So the dword of (step s, row group R of 64, lane l) holds that lane's four
+// 16-row tiles: byte ((s * ceil(rows / 64) + R) * 64 + l) * 4 + j is the scale of row
+// 64 R + 16 j + l % 16, block 4 s + l / 16. One 256-byte load serves 64 rows of a step.
+#include <hip/hip_runtime.h>
+
+#include "lowbit.h"
+
+namespace cp {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMxBlock = 32;    // values that share a scale
+constexpr int kMxStep = 128;    // values of one MFMA step
+constexpr int kMxGroup = 64;    // rows that share a scale dword's bytes
+
+inline int64_t mx_steps(int64_t k) { return (k + kMxStep - 1) / kMxStep; }
+inline int64_t mx_groups(int64_t rows) { return (rows + kMxGroup - 1) / kMxGroup; }
+
+// The scale byte of a block whose largest magnitude is a (NaN or infinity: 255).
+__device__ __forceinline__ int mx_scale_byte(float a) {
+  if (!(a < __builtin_inff())) return 255;
+  const int e = a == 0.0f ? -127 : frexp_e(a) - 3;
+  return (e < -127 ? -127 : e) + 127;
+}
+
+// 2^-e of a scale byte; e <= 125, so it is never below 2^-125.
+__device__ __forceinline__ float mx_inv_scale(int byte) {
+  return __uint_as_float((uint32_t)(254 - byte) << 23);
+}
+
+// Eight values' codes packed in a dword (values already scaled; saturating at 6).
+__device__ __forceinline__ uint32_t mx_pack8(const float (&v)[8], float inv) {
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0] * inv, v[1] * inv, 1.0f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2] * inv, v[3] * inv, 1.0f, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4] * inv, v[5] * inv, 1.0f, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6] * inv, v[7] * inv, 1.0f, 3);
+  return c;
+}
+
+// max |v| over the four lanes that hold a block, NaN if any value is one.
+__device__ __forceinline__ float mx_block_amax(const float (&v)[8]) {
+  uint32_t m = 0;
+  // |v| compares as an integer: infinity and NaN sort above every finite magnitude
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+    m = m > b ? m : b;
+  }
+  uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, true);
+  m = m > o ? m : o;
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, true);
+  return __uint_as_float(m > o ? m : o);
+}
+
+// One workgroup per (128 columns, 64 rows): thread t takes columns 8 (t % 16) .. + 7 of the
+// rows t / 16 + 16 j, j = 0..3, so four lanes share a block and the four bytes of a scale
+// dword come from one thread. Bound by HBM: each value is read once, each byte written once.
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const typename Elem<DT>::T* __restrict__ x,
+                                                           int64_t rows, int k, int64_t stride,
+                                                           uint8_t* __restrict__ codes,
+                                                           uint8_t* __restrict__ scales) {
+  const int t = threadIdx.x, step = blockIdx.x;
+  const int64_t group = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  const int64_t groups = (rows + kMxGroup - 1) / kMxGroup;
+  if (group >= groups) return;
+  const int col = step * kMxStep + 8 * (t & 15);
+  float v[4][8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = group * kMxGroup + 16 * j + (t >> 4);
+    if (r < rows && col < k) {
+      load8<DT>(x + r * stride + col, v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
+    }
+  }
+  uint32_t bytes = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = group * kMxGroup + 16 * j + (t >> 4);
+    const int b = mx_scale_byte(mx_block_amax(v[j]));
+    bytes |= (uint32_t)b << (8 * j);
+    if (r < rows && col < k)
+      *reinterpret_cast<uint32_t*>(codes + r * (k / 2) + col / 2) =
+          b == 255 ? 0u : mx_pack8(v[j], mx_inv_scale(b));
+  }
+  if ((t & 3) == 0)
+    *reinterpret_cast<uint32_t*>(
+        scales + ((step * groups + group) * 64 + 16 * ((t & 15) >> 2) + (t >> 4)) * 4) = bytes;
+}
+
+// The values of eight codes: sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+__device__ __forceinline__ void mx_unpack8(uint32_t c, float scale, float (&v)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2);
+  const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[i] = a[i] * scale;
+    v[2 + i] = b[i] * scale;
+    v[4 + i] = d[i] * scale;
+    v[6 + i] = e[i] * scale;
+  }
+}
+
+// The decode, over the same tiles as the quantiser.
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* __restrict__ codes,
+                                                             const uint8_t* __restrict__ scales,
+                                                             int64_t rows, int k,
+                                                             typename Elem<DT>::T* __restrict__ y) {
+  const int t = threadIdx.x, step = blockIdx.x;
+  const int64_t group = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+  const int64_t groups = (rows + kMxGroup - 1) / kMxGroup;
+  if (group >= groups) return;
+  const int col = step * kMxStep + 8 * (t & 15);
+  if (col >= k) return;
+  const uint32_t bytes = *reinterpret_cast<const uint32_t*>(
+      scales + ((step * groups + group) * 64 + 16 * ((t & 15) >> 2) + (t >> 4)) * 4);
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = group * kMxGroup + 16 * j + (t >> 4);
+    c[j] = r < rows ? *reinterpret_cast<const uint32_t*>(codes + r * (k / 2) + col / 2) : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = group * kMxGroup + 16 * j + (t >> 4);
+    if (r >= rows) break;
+    float v[8];
+    mx_unpack8(c[j], pow2_byte((bytes >> (8 * j)) & 255), v);
+    store8<DT>(y + r * k + col, v);
+  }
+}
+
+// ---------------------------------------------------------------- product
+// Y[m][n] = sum over k of a[m][k] b[n][k]. b's rows are the MFMA's A operand, so a lane's
+// four results are consecutive n of one m.
+
+struct MxOperand {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t rows;
+};
+
+// One lane's 32 codes of row r, block blk (zeros past the end: a zero code adds nothing).
+__device__ __forceinline__ u32x4 mx_load_block(const MxOperand& o, int64_t r, int blk, int k) {
+  u32x4 z = {0, 0, 0, 0};
+  if (r < o.rows && blk * kMxBlock < k)
+    z = *reinterpret_cast<const u32x4*>(o.codes + r * (k / 2) + blk * 16);
+  return z;
+}
+
+__device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int sa, int sb) {
+  const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, sa, 0, sb);
+}
+
+template <int DT>
+__device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, int64_t n0, int64_t M,
+                                          int64_t N, f32x4 c) {
+  if (m >= M) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n0 + i < N) y[m * N + n0 + i] = (typename Elem<DT>::T)c[i];
+}
+
+// One wave per 16 x 16 tile of Y, operands straight from memory.
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_tile_kernel(MxOperand a, MxOperand b, int k,
+                                                       typename Elem<DT>::T* __restrict__ y) {
+  const int lane = threadIdx.x & 63;
+  const int64_t nt = (b.rows + 15) / 16;
+  const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t m0 = tile / nt * 16, n0 = tile % nt * 16;
+  if (m0 >= a.rows) return;
+  const int steps = (k + kMxStep - 1) / kMxStep;
+  const int64_t ga = (a.rows + 63) / 64, gb = (b.rows + 63) / 64;
+  const uint32_t* sa = reinterpret_cast<const uint32_t*>(a.scales) + (m0 / 64) * 64 + lane;
+  const uint32_t* sb = reinterpret_cast<const uint32_t*>(b.scales) + (n0 / 64) * 64 + lane;
+  const int ja = (int)(m0 / 16 % 4) * 8, jb = (int)(n0 / 16 % 4) * 8;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s = 0; s < steps; ++s) {
+    const int blk = 4 * s + (lane >> 4);
+    const u32x4 av = mx_load_block(a, m0 + (lane & 15), blk, k);
+    const u32x4 bv = mx_load_block(b, n0 + (lane & 15), blk, k);
+    acc = mx_mfma(bv, av, acc, (int)(sb[s * gb * 64] >> jb), (int)(sa[s * ga * 64] >> ja));
+  }
+  mx_store4<DT>(y, m0 + (lane & 15), n0 + 4 * (lane >> 4), a.rows, b.rows, acc);
+}
+
+static int mx_shape(int64_t rows, int64_t k, const char* what) {
+  if (rows < 0 || k <= 0 || k % kMxBlock || k > (1 << 30) || rows > ((int64_t)1 << 40) / k)
+    return set_error(CP_ERR_SHAPE, "%s is [%lld, %lld]: rows hold whole blocks of 32 values", what,
+                     (long long)rows, (long long)k);
+  return CP_OK;
+}
+
+static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt,
+                             hipStream_t st) {
+  const int64_t tiles = ((a.rows + 15) / 16) * ((b.rows + 15) / 16), blocks = (tiles + 3) / 4;
+  if (blocks > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
+  const dim3 grid((unsigned)blocks);
+  if (dt == CP_F32) mx4_tile_kernel<CP_F32><<<grid, 256, 0, st>>>(a, b, k, (float*)y);
+  if (dt == CP_BF16) mx4_tile_kernel<CP_BF16><<<grid, 256, 0, st>>>(a, b, k, (__bf16*)y);
+  if (dt == CP_F16) mx4_tile_kernel<CP_F16><<<grid, 256, 0, st>>>(a, b, k, (_Float16*)y);
+  CP_LAUNCHED("MXFP4 product");
+  return CP_OK;
+}
+
+static int mx_quantize(const void* x, int dt, int64_t rows, int64_t k, int64_t stride,
+                       uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  const int64_t groups = mx_groups(rows);
+  const unsigned gy = (unsigned)(groups < 65535 ? groups : 65535);
+  const int64_t gz = (groups + gy - 1) / gy;
+  if (gz > 65535) return set_error(CP_ERR_SHAPE, "too many rows");
+  const dim3 grid((unsigned)mx_steps(k), gy, (unsigned)gz);
+  if (dt == CP_F32)
+    mx4_quantize_kernel<CP_F32><<<grid, 256, 0, st>>>((const float*)x, rows, (int)k, stride, codes, scales);
+  if (dt == CP_BF16)
+    mx4_quantize_kernel<CP_BF16><<<grid, 256, 0, st>>>((const __bf16*)x, rows, (int)k, stride, codes, scales);
+  if (dt == CP_F16)
+    mx4_quantize_kernel<CP_F16><<<grid, 256, 0, st>>>((const _Float16*)x, rows, (int)k, stride, codes, scales);
+  CP_LAUNCHED("MXFP4 quantize");
+  return CP_OK;
+}
+
+static int mx_check_x(const void* x, int dt, int64_t rows, int64_t k, int64_t stride) {
+  if (int s = mx_shape(rows, k, "x")) return s;
+  const int es = dtype_bytes(dt);
+  if (!es) return set_error(CP_ERR_ARG, "dtype code %d", dt);
+  if (rows > 1 && stride < k) return set_error(CP_ERR_SHAPE, "row stride %lld below %lld", (long long)stride, (long long)k);
+  if (rows && !x) return set_error(CP_ERR_ARG, "null x");
+  if (!aligned(x, 16) || (rows > 1 && stride * es % 16))
+    return set_error(CP_ERR_ALIGN, "rows of x need 16-byte alignment");
+  return CP_OK;
+}
+
+static int mx_check_packed(const uint8_t* codes, const uint8_t* scales, int64_t rows) {
+  if (rows && (!codes || !scales)) return set_error(CP_ERR_ARG, "null codes / scales");
+  if (!aligned(codes, 16) || !aligned(scales, 4))
+    return set_error(CP_ERR_ALIGN, "codes need 16-byte and scales 4-byte alignment");
+  return CP_OK;
+}
+
+}  // namespace cp
+
+extern "C" {
+
+size_t cp_mx4_scale_bytes(int64_t rows, int64_t k) {
+  if (rows < 0 || k < 0) return 0;
+  return (size_t)(cp::mx_steps(k) * cp::mx_groups(rows) * 256);
+}
+
+int cp_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t row_stride,
+                    uint8_t* codes, uint8_t* scales, void* stream) {
+  cp::clear_error();
+  if (int s = cp::mx_check_x(x, x_dtype, rows, k, row_stride)) return s;
+  if (int s = cp::mx_check_packed(codes, scales, rows)) return s;
+  if (rows == 0) return CP_OK;
+  return cp::mx_quantize(x, x_dtype, rows, k, row_stride, codes, scales, (hipStream_t)stream);
+}
+
+int cp_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* y,
+                      int y_dtype, void* stream) {
+  cp::clear_error();
+  if (int s = cp::mx_shape(rows, k, "y")) return s;
+  if (!cp::dtype_bytes(y_dtype)) return cp::set_error(CP_ERR_ARG, "dtype code %d", y_dtype);
+  if (int s = cp::mx_check_packed(codes, scales, rows)) return s;
+  if (rows && !y) return cp::set_error(CP_ERR_ARG, "null y");
+  if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
+  if (rows == 0) return CP_OK;
+  const int64_t groups = cp::mx_groups(rows);
+  const unsigned gy = (unsigned)(groups < 65535 ? groups : 65535);
+  const int64_t gz = (groups + gy - 1) / gy;
+  if (gz > 65535) return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  const dim3 grid((unsigned)cp::mx_steps(k), gy, (unsigned)gz);
+  hipStream_t st = (hipStream_t)stream;
+  if (y_dtype == CP_F32)
+    cp::mx4_dequantize_kernel<CP_F32><<<grid, 256, 0, st>>>(codes, scales, rows, (int)k, (float*)y);
+  if (y_dtype == CP_BF16)
+    cp::mx4_dequantize_kernel<CP_BF16><<<grid, 256, 0, st>>>(codes, scales, rows, (int)k, (__bf16*)y);
+  if (y_dtype == CP_F16)
+    cp::mx4_dequantize_kernel<CP_F16><<<grid, 256, 0, st>>>(codes, scales, rows, (int)k, (_Float16*)y);
+  CP_LAUNCHED("MXFP4 dequantize");
+  return CP_OK;
+}
+
+int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
+                  const uint8_t* b_codes, const uint8_t* b_scales, int64_t n, int64_t k, void* y,
+                  int y_dtype, void* stream) {
+  cp::clear_error();
+  if (int s = cp::mx_shape(m, k, "a")) return s;
+  if (int s = cp::mx_shape(n, k, "b")) return s;
+  if (!cp::dtype_bytes(y_dtype)) return cp::set_error(CP_ERR_ARG, "dtype code %d", y_dtype);
+  if (int s = cp::mx_check_packed(a_codes, a_scales, m)) return s;
+  if (int s = cp::mx_check_packed(b_codes, b_scales, n)) return s;
+  if (m == 0 || n == 0) return CP_OK;
+  if (!y) return cp::set_error(CP_ERR_ARG, "null y");
+  if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
+  return cp::mx_launch_product({a_codes, a_scales, m}, {b_codes, b_scales, n}, (int)k, y, y_dtype,
+                               (hipStream_t)stream);
+}
+
+size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k) {
+  if (m < 0 || k < 0) return 0;
+  return (size_t)((m * (k / 2) + 255) / 256 * 256) + cp_mx4_scale_bytes(m, k);
+}
+
+int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride, const uint8_t* w_codes,
+                  const uint8_t* w_scales, int64_t n, int64_t k, void* y, int y_dtype, void* ws,
+                  size_t ws_bytes, void* stream) {
+  cp::clear_error();
+  if (int s = cp::mx_check_x(x, x_dtype, m, k, row_stride)) return s;
+  if (int s = cp::mx_shape(n, k, "w")) return s;
+  if (!cp::dtype_bytes(y_dtype)) return cp::set_error(CP_ERR_ARG, "dtype code %d", y_dtype);
+  if (int s = cp::mx_check_packed(w_codes, w_scales, n)) return s;
+  if (m == 0 || n == 0) return CP_OK;
+  if (!y) return cp::set_error(CP_ERR_ARG, "null y");
+  if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
+  if (!ws || ws_bytes < cp_mx4_linear_ws_bytes(m, k))
+    return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes,
+                         cp_mx4_linear_ws_bytes(m, k));
+  if (!cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
+  uint8_t* xc = (uint8_t*)ws;
+  uint8_t* xs = xc + (m * (k / 2) + 255) / 256 * 256;
+  if (int s = cp::mx_quantize(x, x_dtype, m, k, row_stride, xc, xs, (hipStream_t)stream)) return s;
+  return cp::mx_launch_product({xc, xs, m}, {w_codes, w_scales, n}, (int)k, y, y_dtype,
+                               (hipStream_t)stream);
+}
+
+}  // extern "C"
