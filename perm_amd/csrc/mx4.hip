@@ -15,9 +15,22 @@
 // 64 R + 16 j + l % 16, block 4 s + l / 16. One 256-byte load serves 64 rows of a step.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "lowbit.h"
 
 namespace cp {
+
+// f(integral_constant 0), f(1), ... f(N - 1): indices that builtins take as immediates.
+template <class F, int... I>
+__device__ __forceinline__ void unrolled_impl(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled_impl(f, std::make_integer_sequence<int, N>{});
+}
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -168,10 +181,12 @@ __device__ __forceinline__ u32x4 mx_load_block(const MxOperand& o, int64_t r, in
   return z;
 }
 
-__device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int sa, int sb) {
+// c += a b over one step; SA and SB: which byte of the scale dwords is the operand's.
+template <int SA, int SB>
+__device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
   const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, sa, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, SA, (int)sa, SB, (int)sb);
 }
 
 template <int DT>
@@ -202,27 +217,256 @@ __global__ __launch_bounds__(256) void mx4_tile_kernel(MxOperand a, MxOperand b,
     const int blk = 4 * s + (lane >> 4);
     const u32x4 av = mx_load_block(a, m0 + (lane & 15), blk, k);
     const u32x4 bv = mx_load_block(b, n0 + (lane & 15), blk, k);
-    acc = mx_mfma(bv, av, acc, (int)(sb[s * gb * 64] >> jb), (int)(sa[s * ga * 64] >> ja));
+    acc = mx_mfma<0, 0>(bv, av, acc, sb[s * gb * 64] >> jb, sa[s * ga * 64] >> ja);
   }
   mx_store4<DT>(y, m0 + (lane & 15), n0 + 4 * (lane >> 4), a.rows, b.rows, acc);
 }
 
-static int mx_shape(int64_t rows, int64_t k, const char* what) {
-  if (rows < 0 || k <= 0 || k % kMxBlock || k > (1 << 30) || rows > ((int64_t)1 << 40) / k)
-    return set_error(CP_ERR_SHAPE, "%s is [%lld, %lld]: rows hold whole blocks of 32 values", what,
-                     (long long)rows, (long long)k);
+// A wave's FM x FN tiles of results to y. 16-bit results whose rows are 16-byte aligned go
+// through the wave's own LDS region, [16 FM][16 FN] with 16-byte chunks permuted by xor with
+// the row, and leave in whole row segments; others go straight from the registers.
+template <int FM, int FN, int DT>
+__device__ __forceinline__ void mx_store_tile(typename Elem<DT>::T* y, int64_t m0, int64_t n0, int64_t M,
+                                              int64_t N, const f32x4 (&acc)[FM][FN], uint8_t* lds) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  if (DT != CP_F32 && (N & 7) == 0) {
+    constexpr int CH = 2 * FN, MASK = (CH < 16 ? CH : 16) - 1;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int r = 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        u32x2 w;
+        w[0] = pack2<DT>(acc[i][j][0], acc[i][j][1]);
+        w[1] = pack2<DT>(acc[i][j][2], acc[i][j][3]);
+        const int c = (2 * j + (g >> 1)) ^ (r & MASK);
+        *reinterpret_cast<u32x2*>(lds + (r * CH + c) * 16 + 8 * (g & 1)) = w;
+      }
+    }
+    constexpr int RPI = 64 / CH;  // rows a store covers
+#pragma unroll
+    for (int i = 0; i < 16 * FM / RPI; ++i) {
+      const int r = i * RPI + lane / CH, c = lane % CH;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(lds + (r * CH + (c ^ (r & MASK))) * 16);
+      const int64_t m = m0 + r, n = n0 + 8 * c;
+      if (m < M && n < N) *reinterpret_cast<u32x4*>(y + m * N + n) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t m = m0 + 16 * i + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t n = n0 + 16 * j + 4 * g;
+      if (DT == CP_F32 && (N & 3) == 0) {
+        if (m < M && n < N) *reinterpret_cast<f32x4*>(y + m * N + n) = acc[i][j];
+      } else {
+        mx_store4<DT>(y, m, n, M, N, acc[i][j]);
+      }
+    }
+  }
+}
+
+// Large products: a workgroup of four waves (two by two) owns a tile of BM x BN results,
+// BM = 32 FM and BN = 32 FN; a wave owns FM x FN MFMA tiles. 256 columns of both operands
+// are staged in LDS a step ahead by loads that write LDS directly, 16 bytes a lane, in two
+// buffers; a row's eight 16-byte chunks are permuted by xor with the row's low three bits,
+// so that the 16 rows of an operand read spread over the banks. The direct loads fill LDS in
+// lane order, so the permutation is applied to the address they read. Scales come straight
+// from memory, one dword a lane for 64 rows and 128 columns.
+constexpr int kStage = 256;               // columns per stage
+constexpr int kStageBytes = kStage / 2;   // bytes per row
+constexpr uint32_t kOob = 0x80000000u;    // past any tile's bytes (at most 256 * 2^22)
+
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+template <int FM, int FN, int DT>
+__global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
+    MxOperand a, MxOperand b, int k, int mt, int nt, typename Elem<DT>::T* __restrict__ y) {
+  constexpr int BM = 32 * FM, BN = 32 * FN, ROWS = BM + BN;
+  constexpr int DA = FM > 4 ? FM / 4 : 1, DB = FN > 4 ? FN / 4 : 1;
+  extern __shared__ __align__(16) uint8_t lds[];  // [2][ROWS][128]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  // Workgroup w runs on XCD w % 8. Each XCD takes a contiguous run of tiles, ordered in
+  // columns of eight m tiles, so that the tiles in flight on one XCD form a block and share
+  // their operands in its L2.
+  int tm, tn;
+  {
+    const int tiles = mt * nt, w = blockIdx.x;
+    const int x = w & 7, q = tiles >> 3, r = tiles & 7;
+    const int t = x * q + min(x, r) + (w >> 3);
+    const int col = t / (8 * nt), h = min(8, mt - 8 * col), u = t - col * 8 * nt;
+    tn = u / h;
+    tm = 8 * col + u % h;
+  }
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int kb = k / 2, blocks = k / kMxBlock;
+  const int stages = (k + kStage - 1) / kStage, steps = (k + kMxStep - 1) / kMxStep;
+
+  // Buffer loads over the tile's rows: a row past the operand's end, and a lane whose chunk
+  // lies past the end of a row (given an offset past any buffer), reads zeros. A zero code
+  // adds nothing. Wave w loads rows 8 (FM w + i) + lane / 8 of a and the like of b.
+  const int chunk = (lane & 7) ^ (lane >> 3);
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(a.codes + m0 * kb), 0,
+                                                    (int)(min((int64_t)BM, a.rows - m0) * kb), 0x00020000);
+  const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(b.codes + n0 * kb), 0,
+                                                    (int)(min((int64_t)BN, b.rows - n0) * kb), 0x00020000);
+  const uint32_t va = (uint32_t)(8 * FM * wave + (lane >> 3)) * kb + 16 * chunk;
+  const uint32_t vb = (uint32_t)(8 * FN * wave + (lane >> 3)) * kb + 16 * chunk;
+  auto fetch = [&](int s) {
+    uint8_t* to = lds + (s & 1) * ROWS * kStageBytes;
+    const bool in = chunk < blocks - 8 * s;
+    const int at = __builtin_amdgcn_readfirstlane(s * kStageBytes);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + (FM * wave + i) * 1024), 16,
+                                               in ? va + 8 * i * kb : kOob, at, 0, 0);
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)(to + (FM * 4 + FN * wave + i) * 1024), 16,
+                                               in ? vb + 8 * i * kb : kOob, at, 0, 0);
+  };
+  const int64_t ga = (a.rows + 63) / 64, gb = (b.rows + 63) / 64;
+  uint32_t sa[2][DA], sb[2][DB], na[2][DA], nb[2][DB];  // [step][64-row group], this stage and next
+  const uint32_t* pa[DA];
+  const uint32_t* pb[DB];
+#pragma unroll
+  for (int i = 0; i < DA; ++i)
+    pa[i] = reinterpret_cast<const uint32_t*>(a.scales) + min(m0 / 64 + wm * FM / 4 + i, ga - 1) * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+    pb[i] = reinterpret_cast<const uint32_t*>(b.scales) + min(n0 / 64 + wn * FN / 4 + i, gb - 1) * 64 + lane;
+  auto fetch_scales = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t st = min(2 * s + j, steps - 1);
+#pragma unroll
+      for (int i = 0; i < DA; ++i) na[j][i] = pa[i][st * ga * 64] >> (FM < 4 ? 8 * (wm * FM & 3) : 0);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) nb[j][i] = pb[i][st * gb * 64] >> (FN < 4 ? 8 * (wn * FN & 3) : 0);
+    }
+  };
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  // operand reads: row lane % 16, chunk 4 step + lane / 16, permuted by the row's low bits
+  const int row = lane & 15;
+  const int at0 = row * kStageBytes + 16 * ((lane >> 4) ^ (row & 7));
+  const int at1 = row * kStageBytes + 16 * ((4 + (lane >> 4)) ^ (row & 7));
+  u32x4 fa[2][FM], fb[2][FN];  // [step of the stage]
+  auto read_a = [&](int s, auto P, int i) {
+    fa[P][i] = *reinterpret_cast<const u32x4*>(lds + (s & 1) * ROWS * kStageBytes +
+                                               (wm * FM + i) * 16 * kStageBytes + (P ? at1 : at0));
+  };
+  auto read_b = [&](int s, auto P, int j) {
+    fb[P][j] = *reinterpret_cast<const u32x4*>(lds + (s & 1) * ROWS * kStageBytes +
+                                               (BM + (wn * FN + j) * 16) * kStageBytes + (P ? at1 : at0));
+  };
+  auto mfmas = [&](auto P, auto I) {
+    unrolled<FN>([&](auto J) {
+      acc[I][J] = mx_mfma<J % 4, I % 4>(fb[P][J], fa[P][I], acc[I][J], sb[P][J / 4], sa[P][I / 4]);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::integral_constant<int, 0> P0{};
+  constexpr std::integral_constant<int, 1> P1{};
+  // The pipeline. Each row of FN MFMAs is issued with the operand reads of later rows, so
+  // no MFMA waits for a read issued just before it. A stage's last reads are issued halfway
+  // through its second step; there the workgroup meets once, the next stage has landed (it
+  // was fetched a stage ago), the buffer just read is free for the stage after it, and the
+  // rest of the step's MFMAs cover the first reads of the next stage.
+  auto scales_now = [&] {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < DA; ++i) sa[j][i] = na[j][i];
+#pragma unroll
+      for (int i = 0; i < DB; ++i) sb[j][i] = nb[j][i];
+    }
+  };
+  constexpr int HM = FM / 2, AHEAD = 2 < FM ? 2 : FM;
+  fetch(0);
+  fetch_scales(0);
+  __syncthreads();
+  fetch(1);
+  scales_now();
+#pragma unroll
+  for (int j = 0; j < FN; ++j) read_b(0, P0, j);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) read_a(0, P0, i);
+#pragma clang loop unroll(disable)
+  for (int s = 0; s < stages; ++s) {
+    fetch_scales(s + 1);
+    unrolled<FM>([&](auto I) {
+      if constexpr (I + AHEAD < FM) read_a(s, P0, I + AHEAD);
+      else read_a(s, P1, I + AHEAD - FM);
+#pragma unroll
+      for (int j = I * FN / FM; j < (I + 1) * FN / FM; ++j) read_b(s, P1, j);
+      mfmas(P0, I);
+    });
+    unrolled<HM>([&](auto I) {
+#pragma unroll
+      for (int i = AHEAD + I * (FM - AHEAD) / HM; i < AHEAD + (I + 1) * (FM - AHEAD) / HM; ++i) read_a(s, P1, i);
+      mfmas(P1, I);
+    });
+    __syncthreads();
+    fetch(s + 2);
+    unrolled<FM - HM>([&](auto I) {
+#pragma unroll
+      for (int j = I * FN / (FM - HM); j < (I + 1) * FN / (FM - HM); ++j) read_b(s + 1, P0, j);
+      if constexpr (I < AHEAD) read_a(s + 1, P0, I);
+      mfmas(P1, std::integral_constant<int, I + HM>{});
+    });
+    scales_now();
+  }
+  __syncthreads();  // the last fetches (zeros) are in before LDS is used again or given up
+  mx_store_tile<FM, FN, DT>(y, m0 + wm * FM * 16, n0 + wn * FN * 16, a.rows, b.rows, acc,
+                            lds + wave * FM * FN * 512);
+}
+
+template <int FM, int FN, int DT>
+static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
+  constexpr int lds = 2 * 32 * (FM + FN) * kStageBytes;
+  const int64_t mt = (a.rows + 32 * FM - 1) / (32 * FM), nt = (b.rows + 32 * FN - 1) / (32 * FN);
+  if (mt * nt > 0x7FFFFFFF || mt * 8 > 0x7FFFFFFF / nt) return set_error(CP_ERR_SHAPE, "product too large");
+  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<FM, FN, DT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (once != hipSuccess) return hip_fail(once, "LDS size of the MXFP4 product");
+  mx4_gemm_kernel<FM, FN, DT><<<dim3((unsigned)(mt * nt)), 256, lds, st>>>(a, b, k, (int)mt, (int)nt,
+                                                                      (typename Elem<DT>::T*)y);
+  CP_LAUNCHED("MXFP4 product");
+  return CP_OK;
+}
+
+template <int DT>
+static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
+  if (a.rows > 64 && b.rows > 64) {
+    if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<8, 8, DT>(a, b, k, y, st);
+    return mx_gemm<4, 4, DT>(a, b, k, y, st);
+  }
+  const int64_t tiles = ((a.rows + 15) / 16) * ((b.rows + 15) / 16), blocks = (tiles + 3) / 4;
+  if (blocks > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
+  mx4_tile_kernel<DT><<<dim3((unsigned)blocks), 256, 0, st>>>(a, b, k, (typename Elem<DT>::T*)y);
+  CP_LAUNCHED("MXFP4 product");
   return CP_OK;
 }
 
 static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt,
                              hipStream_t st) {
-  const int64_t tiles = ((a.rows + 15) / 16) * ((b.rows + 15) / 16), blocks = (tiles + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
-  const dim3 grid((unsigned)blocks);
-  if (dt == CP_F32) mx4_tile_kernel<CP_F32><<<grid, 256, 0, st>>>(a, b, k, (float*)y);
-  if (dt == CP_BF16) mx4_tile_kernel<CP_BF16><<<grid, 256, 0, st>>>(a, b, k, (__bf16*)y);
-  if (dt == CP_F16) mx4_tile_kernel<CP_F16><<<grid, 256, 0, st>>>(a, b, k, (_Float16*)y);
-  CP_LAUNCHED("MXFP4 product");
+  if (dt == CP_F32) return mx_product<CP_F32>(a, b, k, y, st);
+  if (dt == CP_BF16) return mx_product<CP_BF16>(a, b, k, y, st);
+  return mx_product<CP_F16>(a, b, k, y, st);
+}
+
+static int mx_shape(int64_t rows, int64_t k, const char* what) {
+  if (rows < 0 || k <= 0 || k % kMxBlock || k > (1 << 23) || rows > ((int64_t)1 << 40) / k)
+    return set_error(CP_ERR_SHAPE, "%s is [%lld, %lld]: rows hold whole blocks of 32 values", what,
+                     (long long)rows, (long long)k);
   return CP_OK;
 }
 
