@@ -268,27 +268,29 @@ __device__ __forceinline__ void mx_store_tile(typename Elem<DT>::T* y, int64_t m
   }
 }
 
-// Large products: a workgroup of four waves (two by two) owns a tile of BM x BN results,
-// BM = 32 FM and BN = 32 FN; a wave owns FM x FN MFMA tiles. 256 columns of both operands
-// are staged in LDS a step ahead by loads that write LDS directly, 16 bytes a lane, in two
-// buffers; a row's eight 16-byte chunks are permuted by xor with the row's low three bits,
-// so that the 16 rows of an operand read spread over the banks. The direct loads fill LDS in
-// lane order, so the permutation is applied to the address they read. Scales come straight
-// from memory, one dword a lane for 64 rows and 128 columns.
+// Large products: a workgroup of WM x WN waves owns a tile of BM x BN results, each wave
+// FM x FN MFMA tiles of it. 256 columns of both operands are staged in LDS a step ahead by
+// loads that write LDS directly, 16 bytes a lane, in two buffers; a row's eight 16-byte
+// chunks are permuted by xor with the row's low three bits, so that the 16 rows of an operand
+// read spread over the banks. The direct loads fill LDS in lane order, so the permutation is
+// applied to the address they read. Scales come straight from memory, one dword a lane for
+// 64 rows and 128 columns.
 constexpr int kStage = 256;               // columns per stage
 constexpr int kStageBytes = kStage / 2;   // bytes per row
 constexpr uint32_t kOob = 0x80000000u;    // past any tile's bytes (at most 256 * 2^22)
 
 typedef __attribute__((address_space(3))) void* lptr_t;
 
-template <int FM, int FN, int DT>
-__global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
-    MxOperand a, MxOperand b, int k, int mt, int nt, typename Elem<DT>::T* __restrict__ y) {
-  constexpr int BM = 32 * FM, BN = 32 * FN, ROWS = BM + BN;
+template <int WM, int WN, int FM, int FN, int DT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, MxOperand b, int k, int mt, int nt,
+                                                                   typename Elem<DT>::T* __restrict__ y) {
+  constexpr int W = WM * WN, BM = 16 * WM * FM, BN = 16 * WN * FN, ROWS = BM + BN;
+  constexpr int LA = BM / (8 * W), LB = BN / (8 * W);  // direct loads of a wave per stage, 8 rows each
   constexpr int DA = FM > 4 ? FM / 4 : 1, DB = FN > 4 ? FN / 4 : 1;
+  static_assert(LA * 8 * W == BM && LB * 8 * W == BN && FM % 2 == 0, "tile shape");
   extern __shared__ __align__(16) uint8_t lds[];  // [2][ROWS][128]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / WN, wn = wave % WN;
   // Workgroup w runs on XCD w % 8. Each XCD takes a contiguous run of tiles, ordered in
   // columns of eight m tiles, so that the tiles in flight on one XCD form a block and share
   // their operands in its L2.
@@ -307,25 +309,25 @@ __global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
 
   // Buffer loads over the tile's rows: a row past the operand's end, and a lane whose chunk
   // lies past the end of a row (given an offset past any buffer), reads zeros. A zero code
-  // adds nothing. Wave w loads rows 8 (FM w + i) + lane / 8 of a and the like of b.
+  // adds nothing. Wave w loads rows 8 (LA w + i) + lane / 8 of a and the like of b.
   const int chunk = (lane & 7) ^ (lane >> 3);
   const auto ra = __builtin_amdgcn_make_buffer_rsrc((void*)(a.codes + m0 * kb), 0,
                                                     (int)(min((int64_t)BM, a.rows - m0) * kb), 0x00020000);
   const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(b.codes + n0 * kb), 0,
                                                     (int)(min((int64_t)BN, b.rows - n0) * kb), 0x00020000);
-  const uint32_t va = (uint32_t)(8 * FM * wave + (lane >> 3)) * kb + 16 * chunk;
-  const uint32_t vb = (uint32_t)(8 * FN * wave + (lane >> 3)) * kb + 16 * chunk;
+  const uint32_t va = (uint32_t)(8 * LA * wave + (lane >> 3)) * kb + 16 * chunk;
+  const uint32_t vb = (uint32_t)(8 * LB * wave + (lane >> 3)) * kb + 16 * chunk;
   auto fetch = [&](int s) {
     uint8_t* to = lds + (s & 1) * ROWS * kStageBytes;
     const bool in = chunk < blocks - 8 * s;
     const int at = __builtin_amdgcn_readfirstlane(s * kStageBytes);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + (FM * wave + i) * 1024), 16,
+    for (int i = 0; i < LA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + (LA * wave + i) * 1024), 16,
                                                in ? va + 8 * i * kb : kOob, at, 0, 0);
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)(to + (FM * 4 + FN * wave + i) * 1024), 16,
+    for (int i = 0; i < LB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)(to + BM * kStageBytes + (LB * wave + i) * 1024), 16,
                                                in ? vb + 8 * i * kb : kOob, at, 0, 0);
   };
   const int64_t ga = (a.rows + 63) / 64, gb = (b.rows + 63) / 64;
@@ -358,10 +360,10 @@ __global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
   const int row = lane & 15;
   const int at0 = row * kStageBytes + 16 * ((lane >> 4) ^ (row & 7));
   const int at1 = row * kStageBytes + 16 * ((4 + (lane >> 4)) ^ (row & 7));
-  u32x4 fa[2][FM], fb[2][FN];  // [step of the stage]
+  u32x4 fa[FM], fb[2][FN];  // fb by step of the stage
   auto read_a = [&](int s, auto P, int i) {
-    fa[P][i] = *reinterpret_cast<const u32x4*>(lds + (s & 1) * ROWS * kStageBytes +
-                                               (wm * FM + i) * 16 * kStageBytes + (P ? at1 : at0));
+    fa[i] = *reinterpret_cast<const u32x4*>(lds + (s & 1) * ROWS * kStageBytes + (wm * FM + i) * 16 * kStageBytes +
+                                            (P ? at1 : at0));
   };
   auto read_b = [&](int s, auto P, int j) {
     fb[P][j] = *reinterpret_cast<const u32x4*>(lds + (s & 1) * ROWS * kStageBytes +
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
   };
   auto mfmas = [&](auto P, auto I) {
     unrolled<FN>([&](auto J) {
-      acc[I][J] = mx_mfma<J % 4, I % 4>(fb[P][J], fa[P][I], acc[I][J], sb[P][J / 4], sa[P][I / 4]);
+      acc[I][J] = mx_mfma<J % 4, I % 4>(fb[P][J], fa[I], acc[I][J], sb[P][J / 4], sa[P][I / 4]);
     });
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
       for (int i = 0; i < DB; ++i) sb[j][i] = nb[j][i];
     }
   };
-  constexpr int HM = FM / 2, AHEAD = 2 < FM ? 2 : FM;
+  constexpr int HM = FM / 2, AHEAD = 2;
   fetch(0);
   fetch_scales(0);
   __syncthreads();
@@ -429,16 +431,18 @@ __global__ __launch_bounds__(256, FM * FN > 32 ? 1 : 2) void mx4_gemm_kernel(
                             lds + wave * FM * FN * 512);
 }
 
-template <int FM, int FN, int DT>
+template <int WM, int WN, int FM, int FN, int DT>
 static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
-  constexpr int lds = 2 * 32 * (FM + FN) * kStageBytes;
-  const int64_t mt = (a.rows + 32 * FM - 1) / (32 * FM), nt = (b.rows + 32 * FN - 1) / (32 * FN);
+  constexpr int BM = 16 * WM * FM, BN = 16 * WN * FN, lds = 2 * (BM + BN) * kStageBytes;
+  static_assert(WM * WN * FM * FN * 512 <= lds, "the results pass through the staging buffers");
+  const int64_t mt = (a.rows + BM - 1) / BM, nt = (b.rows + BN - 1) / BN;
   if (mt * nt > 0x7FFFFFFF || mt * 8 > 0x7FFFFFFF / nt) return set_error(CP_ERR_SHAPE, "product too large");
-  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<FM, FN, DT>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  static const hipError_t once =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<WM, WN, FM, FN, DT>),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (once != hipSuccess) return hip_fail(once, "LDS size of the MXFP4 product");
-  mx4_gemm_kernel<FM, FN, DT><<<dim3((unsigned)(mt * nt)), 256, lds, st>>>(a, b, k, (int)mt, (int)nt,
-                                                                      (typename Elem<DT>::T*)y);
+  mx4_gemm_kernel<WM, WN, FM, FN, DT><<<dim3((unsigned)(mt * nt)), 64 * WM * WN, lds, st>>>(
+      a, b, k, (int)mt, (int)nt, (typename Elem<DT>::T*)y);
   CP_LAUNCHED("MXFP4 product");
   return CP_OK;
 }
@@ -446,8 +450,8 @@ static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, void* y, hipSt
 template <int DT>
 static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
   if (a.rows > 64 && b.rows > 64) {
-    if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<8, 8, DT>(a, b, k, y, st);
-    return mx_gemm<4, 4, DT>(a, b, k, y, st);
+    if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<2, 4, 8, 4, DT>(a, b, k, y, st);
+    return mx_gemm<2, 2, 4, 4, DT>(a, b, k, y, st);
   }
   const int64_t tiles = ((a.rows + 15) / 16) * ((b.rows + 15) / 16), blocks = (tiles + 3) / 4;
   if (blocks > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
