@@ -317,18 +317,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
                                                     (int)(min((int64_t)BN, b.rows - n0) * kb), 0x00020000);
   const uint32_t va = (uint32_t)(8 * LA * wave + (lane >> 3)) * kb + 16 * chunk;
   const uint32_t vb = (uint32_t)(8 * LB * wave + (lane >> 3)) * kb + 16 * chunk;
-  auto fetch = [&](int s) {
+  constexpr int L = LA + LB;
+  auto fetch = [&](int s, int i0, int i1) {  // loads i0 .. i1 - 1 of stage s
     uint8_t* to = lds + (s & 1) * ROWS * kStageBytes;
     const bool in = chunk < blocks - 8 * s;
     const int at = __builtin_amdgcn_readfirstlane(s * kStageBytes);
 #pragma unroll
-    for (int i = 0; i < LA; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + (LA * wave + i) * 1024), 16,
-                                               in ? va + 8 * i * kb : kOob, at, 0, 0);
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)(to + BM * kStageBytes + (LB * wave + i) * 1024), 16,
-                                               in ? vb + 8 * i * kb : kOob, at, 0, 0);
+    for (int i = i0; i < i1; ++i) {
+      if (i < LA)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr_t)(to + (LA * wave + i) * 1024), 16,
+                                                 in ? va + 8 * i * kb : kOob, at, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr_t)(to + BM * kStageBytes + (LB * wave + i - LA) * 1024), 16,
+                                                 in ? vb + 8 * (i - LA) * kb : kOob, at, 0, 0);
+    }
   };
   const int64_t ga = (a.rows + 63) / 64, gb = (b.rows + 63) / 64;
   uint32_t sa[2][DA], sb[2][DB], na[2][DA], nb[2][DB];  // [step][64-row group], this stage and next
@@ -381,7 +383,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
   // no MFMA waits for a read issued just before it. A stage's last reads are issued halfway
   // through its second step; there the workgroup meets once, the next stage has landed (it
   // was fetched a stage ago), the buffer just read is free for the stage after it, and the
-  // rest of the step's MFMAs cover the first reads of the next stage.
+  // rest of the step's MFMAs cover the first reads of the next stage. The fetches are spread
+  // over rows of MFMAs: a wave that issues eight at once waits for the address unit, which
+  // takes 16 clocks for each, while its MFMAs behind them wait too.
   auto scales_now = [&] {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -392,10 +396,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
     }
   };
   constexpr int HM = FM / 2, AHEAD = 2;
-  fetch(0);
+  fetch(0, 0, L);
   fetch_scales(0);
   __syncthreads();
-  fetch(1);
+  fetch(1, 0, L / 2);
   scales_now();
 #pragma unroll
   for (int j = 0; j < FN; ++j) read_b(0, P0, j);
@@ -403,8 +407,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
   for (int i = 0; i < AHEAD; ++i) read_a(0, P0, i);
 #pragma clang loop unroll(disable)
   for (int s = 0; s < stages; ++s) {
-    fetch_scales(s + 1);
     unrolled<FM>([&](auto I) {
+      if constexpr (I < HM) fetch(s + 1, L / 2 + I * L / FM, L / 2 + (I + 1) * L / FM);
+      if constexpr (I == HM) fetch_scales(s + 1);
       if constexpr (I + AHEAD < FM) read_a(s, P0, I + AHEAD);
       else read_a(s, P1, I + AHEAD - FM);
 #pragma unroll
@@ -417,8 +422,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
       mfmas(P1, I);
     });
     __syncthreads();
-    fetch(s + 2);
     unrolled<FM - HM>([&](auto I) {
+      fetch(s + 2, I * L / FM, (I + 1) * L / FM);
 #pragma unroll
       for (int j = I * FN / (FM - HM); j < (I + 1) * FN / (FM - HM); ++j) read_b(s + 1, P0, j);
       if constexpr (I < AHEAD) read_a(s + 1, P0, I);
