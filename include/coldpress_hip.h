@@ -425,7 +425,7 @@ int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
                   const uint8_t* b_codes, const uint8_t* b_scales, int64_t n, int64_t k, void* y,
                   int y_dtype, void* stream);
 
-/* Workspace bytes of cp_mx4_linear (256-byte aligned). */
+/* Workspace bytes of cp_mx4_linear (256-byte aligned; 0: none, ws may be NULL). */
 size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k);
 
 /* y [m, n] = x w^T for MXFP4 weights w [n, k]: x [m, k] is quantized as cp_mx4_quantize

@@ -15,6 +15,7 @@
 // 64 R + 16 j + l % 16, block 4 s + l / 16. One 256-byte load serves 64 rows of a step.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -198,28 +199,128 @@ __device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, in
     if (n0 + i < N) y[m * N + n0 + i] = (typename Elem<DT>::T)c[i];
 }
 
-// One wave per 16 x 16 tile of Y, operands straight from memory.
-template <int DT>
-__global__ __launch_bounds__(256) void mx4_tile_kernel(MxOperand a, MxOperand b, int k,
-                                                       typename Elem<DT>::T* __restrict__ y) {
-  const int lane = threadIdx.x & 63;
-  const int64_t nt = (b.rows + 15) / 16;
-  const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t m0 = tile / nt * 16, n0 = tile % nt * 16;
-  if (m0 >= a.rows) return;
-  const int steps = (k + kMxStep - 1) / kMxStep;
+// Few rows of a (at most 64): bound by reading b once. A workgroup takes NT 16-row tiles of b
+// and all of a; its waves take the 128-column steps in turn, up to four steps' loads in
+// flight in each, and join their sums in LDS in wave order. b's codes go from memory to the matrix cores
+// without LDS: each is used once. Four neighbouring workgroups of one XCD share the scale
+// dwords of 64 rows in its L2.
+//
+// XT >= 0: a's rows come as values of that type and are quantized by every workgroup into
+// its LDS ([row][k / 2] codes, then [row][k / 32] scale bytes), beside the first loads of b.
+template <int MT, int NT, int XT, int DT>
+__global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b, const void* x, int64_t stride, int k,
+                                                       int wgs, typename Elem<DT>::T* __restrict__ y) {
+  constexpr int U = MT * NT > 4 ? 2 : 4;  // within the 128 registers of a 16-wave workgroup
+  constexpr bool FUSED = XT >= 0;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, g = lane >> 4, W = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // blocks of 32 workgroups: XCD x (w % 8) takes four neighbours
+  int w = blockIdx.x;
+  if ((w | 31) < wgs) w = (w & ~31) + 4 * (w & 7) + ((w & 31) >> 3);
+  const int64_t n0 = (int64_t)w * NT * 16;
+  const int steps = (k + kMxStep - 1) / kMxStep, M = (int)a.rows, kb = k / 2, nblk = k / kMxBlock;
   const int64_t ga = (a.rows + 63) / 64, gb = (b.rows + 63) / 64;
-  const uint32_t* sa = reinterpret_cast<const uint32_t*>(a.scales) + (m0 / 64) * 64 + lane;
   const uint32_t* sb = reinterpret_cast<const uint32_t*>(b.scales) + (n0 / 64) * 64 + lane;
-  const int ja = (int)(m0 / 16 % 4) * 8, jb = (int)(n0 / 16 % 4) * 8;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < steps; ++s) {
-    const int blk = 4 * s + (lane >> 4);
-    const u32x4 av = mx_load_block(a, m0 + (lane & 15), blk, k);
-    const u32x4 bv = mx_load_block(b, n0 + (lane & 15), blk, k);
-    acc = mx_mfma<0, 0>(bv, av, acc, sb[s * gb * 64] >> jb, sa[s * ga * 64] >> ja);
+  const uint32_t* sa = reinterpret_cast<const uint32_t*>(a.scales) + lane;
+  const int jb = (int)(n0 / 16 & 3) * 8;
+  const uint8_t* pb[NT];
+  const uint8_t* pa[MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) pb[j] = b.codes + min(n0 + 16 * j + (lane & 15), b.rows - 1) * kb + 16 * g;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) pa[i] = a.codes + min((int64_t)(16 * i + (lane & 15)), a.rows - 1) * kb + 16 * g;
+
+  u32x4 fb[U][NT], fa[U][MT];
+  uint32_t vb[U], va[U];
+  const u32x4 zero = {0, 0, 0, 0};
+  // step s = base + W u + wave: rows past the end repeat the last (never stored), columns
+  // past the end are zero codes in a
+  auto load_b = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = base + W * u + wave, blk = 4 * s + g;
+      vb[u] = sb[min(s, steps - 1) * gb * 64] >> jb;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        fb[u][j] = blk < nblk ? *reinterpret_cast<const u32x4*>(pb[j] + (int64_t)s * 64) : zero;
+    }
+  };
+  const int pitch = kb + 16;
+  auto load_a = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = base + W * u + wave, blk = 4 * s + g;
+      if constexpr (FUSED) {
+        const bool in = blk < nblk && (lane & 15) < M;
+        fa[u][0] = in ? *reinterpret_cast<const u32x4*>(lds + (lane & 15) * pitch + 16 * blk) : zero;
+        va[u] = in ? lds[M * pitch + (lane & 15) * nblk + blk] : 0;
+      } else {
+        va[u] = sa[min(s, steps - 1) * ga * 64];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          fa[u][i] = blk < nblk ? *reinterpret_cast<const u32x4*>(pa[i] + (int64_t)s * 64) : zero;
+      }
+    }
+  };
+  load_b(0);
+  if constexpr (FUSED) {
+    typedef typename Elem<XT>::T T;
+    for (int m = 0; m < M; ++m) {
+      for (int c = threadIdx.x; c < k / 8; c += blockDim.x) {  // k % 32 == 0: whole blocks of four lanes
+        float v[8];
+        load8<XT>((const T*)x + m * stride + 8 * c, v);
+        const int e = mx_scale_byte(mx_block_amax(v));
+        *reinterpret_cast<uint32_t*>(lds + m * pitch + 4 * c) = e == 255 ? 0u : mx_pack8(v, mx_inv_scale(e));
+        if ((c & 3) == 0) lds[M * pitch + m * nblk + (c >> 2)] = (uint8_t)e;
+      }
+    }
+    __syncthreads();
   }
-  mx_store4<DT>(y, m0 + (lane & 15), n0 + 4 * (lane >> 4), a.rows, b.rows, acc);
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  load_a(0);
+  for (int base = 0;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unrolled<MT>([&](auto I) {
+        unrolled<NT>([&](auto J) {
+          acc[I][J] = mx_mfma<J, I>(fb[u][J], fa[u][I], acc[I][J], vb[u], va[u]);
+        });
+      });
+    }
+    base += U * W;
+    if (base >= steps) break;
+    load_b(base);
+    load_a(base);
+  }
+  // the waves' sums, joined in wave order; a slot is one lane's four results
+  f32x4* red = reinterpret_cast<f32x4*>(lds);
+  if constexpr (FUSED) __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int t = threadIdx.x; t < MT * NT * 64; t += blockDim.x) {
+    f32x4 c = red[t];
+    for (int v = 1; v < W; ++v) c += red[v * MT * NT * 64 + t];
+    const int l = t & 63, ij = t >> 6;
+    const int64_t m = 16 * (ij / NT) + (l & 15), n = n0 + 16 * (ij % NT) + 4 * (l >> 4);
+    if (DT != CP_F32 && (b.rows & 3) == 0) {
+      if (m < M && n < b.rows) {
+        u32x2 p;
+        p[0] = pack2<DT>(c[0], c[1]);
+        p[1] = pack2<DT>(c[2], c[3]);
+        *reinterpret_cast<u32x2*>(y + m * b.rows + n) = p;
+      }
+    } else {
+      mx_store4<DT>(y, m, n, a.rows, b.rows, c);
+    }
+  }
 }
 
 // A wave's FM x FN tiles of results to y. 16-bit results whose rows are 16-byte aligned go
@@ -452,17 +553,48 @@ static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, void* y, hipSt
   return CP_OK;
 }
 
-template <int DT>
-static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
-  if (a.rows > 64 && b.rows > 64) {
-    if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<2, 4, 8, 4, DT>(a, b, k, y, st);
-    return mx_gemm<2, 2, 4, 4, DT>(a, b, k, y, st);
-  }
-  const int64_t tiles = ((a.rows + 15) / 16) * ((b.rows + 15) / 16), blocks = (tiles + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
-  mx4_tile_kernel<DT><<<dim3((unsigned)blocks), 256, 0, st>>>(a, b, k, (typename Elem<DT>::T*)y);
+// Waves of a few-rows workgroup: four, or more while the launch has under eight waves a CU
+// and every wave keeps a step of its own.
+static int mx_few_waves(int64_t wgs, int steps) {
+  int w = 4;
+  while (w < 16 && wgs * w < 2048 && steps > 2 * w) w *= 2;
+  return w;
+}
+
+template <int MT, int NT, int XT, int DT>
+static int mx_few(const MxOperand& a, const MxOperand& b, const void* x, int64_t stride, int k, void* y,
+                  hipStream_t st) {
+  const int64_t wgs = (b.rows + 16 * NT - 1) / (16 * NT);
+  if (wgs > 0x7FFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
+  const int w = mx_few_waves(wgs, (k + kMxStep - 1) / kMxStep);
+  size_t lds = (size_t)w * MT * NT * 1024;
+  if (XT >= 0) lds = std::max(lds, (size_t)a.rows * (k / 2 + 16 + k / kMxBlock));
+  mx4_few_kernel<MT, NT, XT, DT><<<dim3((unsigned)wgs), 64 * w, lds, st>>>(a, b, x, stride, k, (int)wgs,
+                                                                      (typename Elem<DT>::T*)y);
   CP_LAUNCHED("MXFP4 product");
   return CP_OK;
+}
+
+template <int DT>
+static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
+  if (a.rows <= 16) return mx_few<1, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (a.rows <= 32) return mx_few<2, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (a.rows <= 64) return mx_few<4, 2, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<2, 4, 8, 4, DT>(a, b, k, y, st);
+  return mx_gemm<2, 2, 4, 4, DT>(a, b, k, y, st);
+}
+
+// x's rows quantized inside the product: up to four, whose codes every workgroup makes for
+// itself faster than a launch of their own takes.
+static bool mx_fuses(int64_t m, int64_t k) { return m <= 4 && m * (k / 2 + 16 + k / kMxBlock) <= 64 * 1024; }
+
+template <int XT>
+static int mx_fused(const void* x, int64_t m, int64_t stride, const MxOperand& b, int k, void* y, int dt,
+                    hipStream_t st) {
+  const MxOperand a = {nullptr, nullptr, m};
+  if (dt == CP_F32) return mx_few<1, 1, XT, CP_F32>(a, b, x, stride, k, y, st);
+  if (dt == CP_BF16) return mx_few<1, 1, XT, CP_BF16>(a, b, x, stride, k, y, st);
+  return mx_few<1, 1, XT, CP_F16>(a, b, x, stride, k, y, st);
 }
 
 static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt,
@@ -574,7 +706,7 @@ int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
 }
 
 size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k) {
-  if (m < 0 || k < 0) return 0;
+  if (m < 0 || k < 0 || cp::mx_fuses(m, k)) return 0;
   return (size_t)((m * (k / 2) + 255) / 256 * 256) + cp_mx4_scale_bytes(m, k);
 }
 
@@ -589,10 +721,16 @@ int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride, con
   if (m == 0 || n == 0) return CP_OK;
   if (!y) return cp::set_error(CP_ERR_ARG, "null y");
   if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
-  if (!ws || ws_bytes < cp_mx4_linear_ws_bytes(m, k))
+  if (cp_mx4_linear_ws_bytes(m, k) && (!ws || ws_bytes < cp_mx4_linear_ws_bytes(m, k)))
     return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes,
                          cp_mx4_linear_ws_bytes(m, k));
   if (!cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
+  if (cp::mx_fuses(m, k)) {
+    const cp::MxOperand b = {w_codes, w_scales, n};
+    if (x_dtype == CP_F32) return cp::mx_fused<CP_F32>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
+    if (x_dtype == CP_BF16) return cp::mx_fused<CP_BF16>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
+    return cp::mx_fused<CP_F16>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
+  }
   uint8_t* xc = (uint8_t*)ws;
   uint8_t* xs = xc + (m * (k / 2) + 255) / 256 * 256;
   if (int s = cp::mx_quantize(x, x_dtype, m, k, row_stride, xc, xs, (hipStream_t)stream)) return s;

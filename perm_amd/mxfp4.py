@@ -156,8 +156,8 @@ def linear(x, w, dtype=None):
     m = rows.shape[0]
     y = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=x.device)
     nws = lib.cp_mx4_linear_ws_bytes(m, k)
-    ws = _lib.workspace(nws, x.device)
+    ws = _lib.workspace(nws, x.device) if nws else None
     _lib.check(lib.cp_mx4_linear(rows.data_ptr(), xc, m, rows.stride(0), w.codes.data_ptr(),
-                                 w.scales.data_ptr(), n, k, y.data_ptr(), yc, ws.data_ptr(), nws,
+                                 w.scales.data_ptr(), n, k, y.data_ptr(), yc, _lib.ptr(ws), nws,
                                  _lib.stream_ptr()))
     return y
