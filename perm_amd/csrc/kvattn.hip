@@ -32,7 +32,7 @@ struct AttnArgs {
   const int* lens;              // [batch]
   void* out;                    // [rows][q heads][d]
   float* lse;                   // [rows][q heads] or null
-  float* part;                  // splits > 1: [rows][q heads][splits][d + 2]
+  float* part;                  // splits > 1: [rows][q heads][splits][d], then [..][splits][m, l]
   int64_t rows;
   int group;                    // q heads per kv head
   int causal, window, splits;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   if (row0 < 0 || row0 + n_b > a.rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
-  const int d = c.d, blk = c.block;
+  const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
   const int64_t cap = (int64_t)c.max_pages * blk;
   const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
 
@@ -138,19 +138,24 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   for (int i = 0; i < ND; ++i) o[i] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
   const int* tab = c.table + (int64_t)b * c.max_pages;
+  // columns past d read the row's first ones instead: their q is 0, and a NaN there makes the
+  // score NaN anyway
+  int kcol[NC];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) kcol[k] = 64 * k + 16 * g < d ? 64 * k + 16 * g : 0;
 
   for (int tile = tb + wave; tile < te; tile += 4) {
     const int j0 = tile * kTile;
     // pages of the two 16-token groups this lane reads: K rows by lane % 16 / 4, V and the
     // scores' scales by lane / 16
     const int jk = j0 + 16 * (col >> 2), jv = j0 + 16 * g;
-    int pk = jk < len ? tab[jk / blk] : -1, pv = jv < len ? tab[jv / blk] : -1;
+    int pk = jk < len ? tab[jk >> lb] : -1, pv = jv < len ? tab[jv >> lb] : -1;
     if ((unsigned)pk >= (unsigned)c.pages) pk = -1;
     if ((unsigned)pv >= (unsigned)c.pages) pv = -1;
     const int64_t ak = ((int64_t)max(pk, 0) * c.heads + h) * blk * d;
     const int64_t hv = (int64_t)max(pv, 0) * c.heads + h;
-    const uint8_t* kp = c.k + ak + (int64_t)(jk % blk + (col & 3)) * d + 16 * g;
-    const uint8_t* vp = c.v + hv * blk * d + (int64_t)col * blk + jv % blk;
+    const uint8_t* kp = c.k + ak + ((jk & (blk - 1)) + (col & 3)) * d;
+    const uint8_t* vp = c.v + hv * blk * d + col * blk + (jv & (blk - 1));
     f32x4 sc[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
@@ -159,14 +164,12 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
-        const u32x4 z = {0, 0, 0, 0};
-        kk[t][k] = 64 * k + 16 * g < d ? *reinterpret_cast<const u32x4*>(kp + 4 * t * d + 64 * k) : z;
+        kk[t][k] = *reinterpret_cast<const u32x4*>(kp + 4 * t * d + kcol[k]);
       }
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      const u32x4 z = {0, 0, 0, 0};
-      vv[i] = 16 * i < d ? *reinterpret_cast<const u32x4*>(vp + (int64_t)16 * i * blk) : z;
+      vv[i] = *reinterpret_cast<const u32x4*>(vp + (16 * i < d ? 16 * i : 0) * blk);  // rows past d are dropped
     }
     const float ks = c.k_scale[hv], vs = c.v_scale[hv];
 #pragma unroll
@@ -278,8 +281,9 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   }
   const int64_t orow = (row0 + rr / a.group) * ((int64_t)a.group * c.heads) + h * a.group + rr % a.group;
   if (a.splits > 1) {
-    float* p = a.part + (orow * a.splits + split) * (d + 2);
-    if (c0 == 0) p[d] = mm, p[d + 1] = ll;
+    float* p = a.part + (orow * a.splits + split) * d;
+    float* pm = a.part + a.rows * a.group * c.heads * a.splits * d + (orow * a.splits + split) * 2;
+    if (c0 == 0) pm[0] = mm, pm[1] = ll;
     for (int x = c0; x < d; x += 16) {
       float v = 0.0f;
 #pragma unroll
@@ -299,35 +303,48 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   if (a.lse && c0 == 0) a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
 }
 
-// The splits of a row joined, in split order. One wave per row.
+// The splits of a row joined: one workgroup per row, d / 4 threads over the columns and the
+// rest of the threads over the splits, whose sums are added in a fixed order.
 template <int DT>
-__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, int64_t rows,
-                                                        int d, int splits,
-                                                        typename Elem<DT>::T* __restrict__ out,
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, int64_t rows, int d,
+                                                        int splits, typename Elem<DT>::T* __restrict__ out,
                                                         float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const float* p = part + row * splits * (d + 2);
+  __shared__ float sm_m[4], sm_l[256];
+  __shared__ __align__(16) float sm_o[256 * 4];
+  const int64_t row = blockIdx.x;
+  const float* po = part + row * splits * d;
+  const float* pm = part + rows * splits * d + row * splits * 2;
   float mm = kNegInf;
-  for (int s = lane; s < splits; s += 64) mm = fmaxf(mm, p[(int64_t)s * (d + 2) + d]);
+  for (int s = threadIdx.x; s < splits; s += 256) mm = fmaxf(mm, pm[2 * s]);
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) mm = fmaxf(mm, __shfl_xor(mm, k));
+  if ((threadIdx.x & 63) == 0) sm_m[threadIdx.x >> 6] = mm;
+  __syncthreads();
+  mm = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
   const float ms = mm == kNegInf ? 0.0f : mm;
-  float ll = 0.0f, v[4] = {0, 0, 0, 0};
-  for (int s = 0; s < splits; ++s) {
-    const float* ps = p + (int64_t)s * (d + 2);
-    const float f = exp2_fast(ps[d] - ms);
-    ll += ps[d + 1] * f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < d) v[i] += ps[lane + 64 * i] * f;
+  const int T = d / 4, NG = 256 / T, grp = threadIdx.x / T, c = 4 * (threadIdx.x % T);
+  f32x4 v = {0, 0, 0, 0};
+  float ll = 0.0f;
+  if (grp < NG) {
+#pragma unroll 4
+    for (int s = grp; s < splits; s += NG) {
+      const float f = exp2_fast(pm[2 * s] - ms);
+      ll += pm[2 * s + 1] * f;
+      v += *reinterpret_cast<const f32x4*>(po + (int64_t)s * d + c) * f;
+    }
+    *reinterpret_cast<f32x4*>(&sm_o[grp * d + c]) = v;
+    sm_l[grp] = ll;  // the group's threads hold the same sum
   }
-  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < d) out[row * d + lane + 64 * i] = (typename Elem<DT>::T)(v[i] * inv);
-  if (lse && lane == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+  __syncthreads();
+  if ((int)threadIdx.x >= d) return;
+  float o = 0.0f;
+  ll = 0.0f;
+  for (int i = 0; i < NG; ++i) {
+    o += sm_o[i * d + threadIdx.x];
+    ll += sm_l[i];
+  }
+  out[row * d + threadIdx.x] = (typename Elem<DT>::T)(ll != 0.0f ? o / ll : 0.0f);
+  if (lse && threadIdx.x == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
 }
 
 struct AttnPlan {
@@ -357,7 +374,7 @@ static void attn_launch_d(const AttnArgs& a, const KvBatch& b, int64_t items, hi
   else attn_launch<DT, 256>(a, b, items, st);
   if (a.splits > 1) {
     const int64_t n = a.rows * a.group * a.c.heads;
-    attn_join_kernel<DT><<<dim3((unsigned)((n + 3) / 4)), 256, 0, st>>>(
+    attn_join_kernel<DT><<<dim3((unsigned)n), 256, 0, st>>>(
         a.part, n, a.c.d, a.splits, (typename Elem<DT>::T*)a.out, a.lse);
   }
 }
@@ -402,7 +419,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr);
   if (need && (!ws || ws_bytes < need))
     return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
-  if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > (int64_t)0x7FFFFFFF * 4)
+  if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > 0x7FFFFFFF)
     return cp::set_error(CP_ERR_SHAPE, "too many rows");
   cp::AttnArgs a;
   a.c = cp::kv_args(cache, table, max_pages);
