@@ -20,6 +20,7 @@
 namespace cp {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;       // tokens per step of a wave
@@ -303,6 +304,342 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   if (a.lse && c0 == 0) a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
 }
 
+// Many query rows: a workgroup takes 128 (row, head of the group) pairs of one kv head, 32 a
+// wave, and walks its range of tokens 64 at a time. The tile's K and V codes are staged in
+// LDS a tile ahead by loads that write LDS directly, and every wave turns the codes it reads
+// into 16 bits itself. The products are v_mfma_f32_32x32x16 with K and V as the A operand, so
+// a lane's scores belong to one query row (lane % 32): its half lane / 32 owns 16 consecutive
+// tokens of each 32, score i is token 16 (lane / 32) + i, and scores 8 s .. 8 s + 7 are the
+// second product's operand at step s as they stand.
+//
+// LDS rows hold 16-byte chunks permuted by xor, so that eight lanes of a read fall into
+// different banks: K rows (a token each) with bits 0, 1 and 4 of the token, V rows (a column
+// each, 64 tokens) with bits 2 and 3 of the column.
+template <int DP>
+__device__ __forceinline__ int k_swizzle(int token) {
+  const int f = DP >= 128 ? (token & 3) | ((token >> 2) & 4) : ((token >> 3) & 2) | (token & 1);
+  return 16 * f;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (DT == CP_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+typedef const __attribute__((address_space(1))) void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+constexpr int kManyRows = 128;
+
+template <int DT, int DP>
+__global__ __launch_bounds__(256, 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items) {
+  constexpr int NC = DP / 32, NL = DP / 64;          // 32-column chunks; direct loads of a wave for K, and for V
+  constexpr int KB = kTile * DP, BUF = 2 * KB;       // bytes of a K (or V) tile, of a buffer
+  extern __shared__ __align__(16) uint8_t lds[];     // [2][BUF]
+  const KvCacheArgs& c = a.c;
+  const int h = (int)(blockIdx.x % c.heads);
+  const int split = (int)(blockIdx.x / c.heads % a.splits);
+  int b, item, n_b;
+  int64_t row0;
+  // last items first: causal rows at the end of a prompt see the most tokens
+  if (!kv_locate(bt, items - 1 - (int)(blockIdx.x / c.heads / a.splits),
+                 [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b, &item,
+                 &row0, &n_b))
+    return;
+  if (row0 < 0 || row0 + n_b > a.rows) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q = lane & 31, hh = lane >> 5;
+  const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);
+  const int64_t cap = (int64_t)c.max_pages * blk;
+  const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
+
+  // token range [lo, hi) of row r of the sequence; rows past the end see nothing
+  auto range = [&](int64_t r, int* lo, int* hi) {
+    const bool real = r < (int64_t)n_b * a.group;
+    const int64_t pos = (int64_t)len - n_b + r / a.group;
+    *hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len) : 0;
+    *lo = a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+    if (*lo >= *hi) *lo = *hi = 0;
+  };
+  const int64_t r0 = (int64_t)item * kManyRows, r = r0 + 32 * wave + q;
+  int lo, hi;
+  range(r, &lo, &hi);
+  // what the workgroup's rows see together: rows are in order of position, so the first row
+  // that sees anything bounds it below and the last real row above
+  int jlo, jhi;
+  {
+    const int64_t last = min(r0 + kManyRows, (int64_t)n_b * a.group) - 1;
+    int x;
+    range(last, &x, &jhi);
+    // the lowest token of the first row whose position is not negative
+    const int64_t first = max(r0, (int64_t)(n_b - len) * a.group);
+    range(min(first, last), &jlo, &x);
+    if (jhi == 0) jlo = 0;
+  }
+  // every real row of this wave sees all of a tile inside [wlo, whi)
+  int wlo = lo, whi = hi;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    wlo = max(wlo, __shfl_xor(wlo, s));
+    whi = min(whi, __shfl_xor(whi, s));
+  }
+  wlo = __builtin_amdgcn_readfirstlane(wlo);
+  whi = __builtin_amdgcn_readfirstlane(whi);
+  const int t0 = jlo / kTile, nt = (jhi + kTile - 1) / kTile - t0;
+  const int per = (nt + a.splits - 1) / a.splits;
+  const int tb = t0 + split * per, te = min(t0 + nt, tb + per);
+
+  u32x4 qf[NC][2];
+  const int64_t qrow = row0 + r / a.group;
+  const int qh = h * a.group + (int)(r % a.group);
+  const bool real = r < (int64_t)n_b * a.group;
+  {
+    typedef typename Elem<DT>::T T;
+    const T* qp = (const T*)a.q + (real ? qrow * a.q_row + (int64_t)qh * a.q_head : 0);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const bool in = real && 32 * k + 16 * hh < d;
+      const u32x4 z = {0, 0, 0, 0};
+      qf[k][0] = in ? *reinterpret_cast<const u32x4*>(qp + 32 * k + 16 * hh) : z;
+      qf[k][1] = in ? *reinterpret_cast<const u32x4*>(qp + 32 * k + 16 * hh + 8) : z;
+    }
+  }
+  f32x16 o[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+  float m = kNegInf, l = 0.0f;
+
+  const int* tab = c.table + (int64_t)b * c.max_pages;
+  auto page_at = [&](int j) {  // of token j; -1: none
+    const int p = j < len ? tab[j >> lb] : -1;
+    return (unsigned)p < (unsigned)c.pages ? p : -1;
+  };
+  // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
+  // each, four token groups. Chunks past d repeat the row's first, rows past d its last 16
+  // (their q is 0, their results are dropped).
+  constexpr int CH = DP / 16;
+  const int kt = 16 * wave + lane / CH;                       // + 1024 / DP per load
+  const int vg = (lane & 3) ^ ((lane >> 4) & 3);
+  auto fetch = [&](int tile, int pk, int pv) {
+    uint8_t* to = lds + (tile & 1) * BUF;
+    const int j0 = tile * kTile;
+    const uint8_t* kp = c.k + ((int64_t)max(pk, 0) * c.heads + h) * blk * d;
+    const uint8_t* vp = c.v + ((int64_t)max(pv, 0) * c.heads + h) * blk * d;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int token = kt + i * (1024 / DP);
+      const int col = (16 * (lane % CH)) ^ k_swizzle<DP>(token);
+      const uint8_t* src = kp + ((j0 + token) & (blk - 1)) * d + (col < d ? col : 0);
+      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(to + (wave * NL + i) * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int column = min(16 * (wave * NL + i) + (lane >> 2), d - 1);
+      const uint8_t* src = vp + column * blk + ((j0 + 16 * vg) & (blk - 1));
+      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(to + KB + (wave * NL + i) * 1024), 16, 0, 0);
+    }
+  };
+  // this lane's K rows and V columns in LDS
+  const int token = 16 * ((q >> 2) & 1) + 4 * (q >> 3) + (q & 3);
+  const int ksw = k_swizzle<DP>(token);
+  const int vsw = 16 * ((q >> 2) & 3);
+
+  int pk = 0, pv = 0, pg[2] = {0, 0};
+  float ks[2], vs[2];
+  bool have[2];
+  auto pages = [&](int tile) {
+    const int j0 = tile * kTile;
+    pk = page_at(j0 + 16 * wave);
+    pv = page_at(j0 + 16 * vg);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) pg[s] = page_at(j0 + 32 * s + 16 * hh);
+  };
+  auto scales = [&] {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int64_t hv = (int64_t)max(pg[s], 0) * c.heads + h;
+      ks[s] = c.k_scale[hv];
+      vs[s] = c.v_scale[hv];
+      have[s] = pg[s] >= 0;
+    }
+  };
+  if (tb < te) {
+    pages(tb);
+    fetch(tb, pk, pv);
+  }
+  for (int tile = tb; tile < te; ++tile) {
+    scales();
+    const bool all = !__any(!have[0] || !have[1]);
+    __syncthreads();  // this tile has landed, and every wave is done with the one before
+    if (tile + 1 < te) {
+      pages(tile + 1);
+      fetch(tile + 1, pk, pv);
+    }
+    const uint8_t* lk = lds + (tile & 1) * BUF + token * DP;
+    const uint8_t* lv = lds + (tile & 1) * BUF + KB + q * 64;
+    const int j0 = tile * kTile;
+    f32x16 sc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[s][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((32 * k + 16 * hh) ^ ksw));
+        sc[s] = mfma32<DT>(codes_to_16<DT>(w[0], w[1]), qf[k][0], sc[s]);
+        sc[s] = mfma32<DT>(codes_to_16<DT>(w[2], w[3]), qf[k][1], sc[s]);
+        if (k & 1) __builtin_amdgcn_sched_barrier(0);  // or every read is hoisted, and registers spill
+      }
+    }
+    float kc[2], lg[2], iv[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      kc[s] = ks[s] * a.scale;
+      lg[s] = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
+      iv[s] = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
+    }
+    const bool edge = !all || j0 < wlo || j0 + kTile > whi;
+    if (edge) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + 32 * s + 16 * hh + i;
+          sc[s][i] = have[s] && j >= lo && j < hi ? sc[s][i] : kNegInf;
+        }
+    }
+    // the largest t of the tile: kc > 0, so t rises with the raw score
+    float tm = kNegInf;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float x = sc[s][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) x = fmaxf(x, sc[s][i]);
+      tm = fmaxf(tm, __builtin_fmaf(x, kc[s], lg[s]));
+    }
+    tm = fmaxf(tm, __shfl_xor(tm, 32));
+    if (__any(tm > m)) {
+      const float mn = fmaxf(m, tm);
+      const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i] *= al;
+    }
+    const float ms = m == kNegInf ? 0.0f : m;
+    u32x4 w[2][2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const float off = lg[s] - ms;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float e0 = exp2_fast(__builtin_fmaf(sc[s][i], kc[s], off));
+        const float e1 = exp2_fast(__builtin_fmaf(sc[s][i + 1], kc[s], off));
+        sum += e0 + e1;
+        w[s][i >> 3][(i >> 1) & 3] = pack2<CP_F16>(e0, e1);
+      }
+      l = __builtin_fmaf(sum, iv[s], l);
+    }
+    bool nan = false;
+    if (edge) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) any |= nan_flags(x[k]);
+        }
+      nan = __any(any != 0);
+    }
+    if (nan) {
+      // as in attn_few_kernel: NaN codes leave the product and return to the rows that see them
+      u32x4 one[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const int j = j0 + 32 * s + 16 * hh + i;
+          one[s][i >> 3][(i >> 1) & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
+                                         (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
+        }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        f32x16 cnt;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw)), f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t fl = nan_flags(x[k]) >> 7;
+            x[k] &= ~(fl * 0xFFu);
+            f[k] = fl * 0x38u;  // 1.0 where the code was NaN
+          }
+          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[s][0], cnt);
+          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[s][1], cnt);
+          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
+          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (cnt[j] > 0.0f) o[i][j] = __builtin_nanf("");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
+          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
+          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
+          if (s) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if (!real) return;
+  const int64_t orow = qrow * ((int64_t)a.group * c.heads) + qh;
+  // lane's results: columns 32 i + 8 (j / 4) + 4 hh + j % 4 of its row
+  if (a.splits > 1) {
+    float* p = a.part + (orow * a.splits + split) * d;
+    float* pm = a.part + a.rows * a.group * c.heads * a.splits * d + (orow * a.splits + split) * 2;
+    if (hh == 0) pm[0] = m, pm[1] = l;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int x = 32 * i + 8 * j + 4 * hh;
+        if (x < d) *reinterpret_cast<f32x4*>(p + x) = f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+      }
+    return;
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  typename Elem<DT>::T* op = (typename Elem<DT>::T*)a.out + orow * d;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int x = 32 * i + 8 * j + 4 * hh;
+      u32x2 v;
+      v[0] = pack2<DT>(o[i][4 * j] * inv, o[i][4 * j + 1] * inv);
+      v[1] = pack2<DT>(o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
+      if (x < d) *reinterpret_cast<u32x2*>(op + x) = v;
+    }
+  if (a.lse && hh == 0) a.lse[orow] = l == 0.0f ? kNegInf : (m + __builtin_amdgcn_logf(l)) / kLog2e;
+}
+
 // The splits of a row joined: one workgroup per row, d / 4 threads over the columns and the
 // rest of the threads over the splits, whose sums are added in a fixed order.
 template <int DT>
@@ -348,35 +685,52 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
 }
 
 struct AttnPlan {
+  bool many;
   int64_t items;  // upper bound of the batch's row tiles
   int splits;
 };
 
+// Row tiles of 16 while a sequence has no more (row, head of the group) pairs on average:
+// then reading the cache bounds the call; of 128 above that.
 static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int64_t cap) {
   AttnPlan p;
-  p.items = ragged ? rows * group / 16 + batch : batch * ((group + 15) / 16);
-  // enough workgroups for every CU four times over, none under 256 tokens (a tile a wave)
-  const int64_t want = 1024 / (p.items * heads > 0 ? p.items * heads : 1);
+  p.many = rows * group > 16 * batch;
+  const int tile = p.many ? kManyRows : 16;
+  p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
+  // workgroups for every CU four times over (two for the large tiles), none under 256 tokens
+  const int64_t n = p.items * heads, want = (p.many ? 512 : 1024) / (n > 0 ? n : 1);
   const int64_t most = (cap + 255) / 256;
   p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
   return p;
 }
 
 template <int DT, int DP>
-static void attn_launch(const AttnArgs& a, const KvBatch& b, int64_t items, hipStream_t st) {
-  attn_few_kernel<DT, DP><<<dim3((unsigned)(items * a.c.heads * a.splits)), 256, 0, st>>>(a, b);
+static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.items * a.c.heads * a.splits));
+  if (p.many) {
+    constexpr int lds = 4 * kTile * DP;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
+    attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
+  } else {
+    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b);
+  }
+  CP_LAUNCHED("cache attention");
+  return CP_OK;
 }
 
 template <int DT>
-static void attn_launch_d(const AttnArgs& a, const KvBatch& b, int64_t items, hipStream_t st) {
-  if (a.c.d <= 64) attn_launch<DT, 64>(a, b, items, st);
-  else if (a.c.d <= 128) attn_launch<DT, 128>(a, b, items, st);
-  else attn_launch<DT, 256>(a, b, items, st);
-  if (a.splits > 1) {
-    const int64_t n = a.rows * a.group * a.c.heads;
-    attn_join_kernel<DT><<<dim3((unsigned)n), 256, 0, st>>>(
-        a.part, n, a.c.d, a.splits, (typename Elem<DT>::T*)a.out, a.lse);
-  }
+static int attn_launch_d(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
+  const int s = a.c.d <= 64    ? attn_launch<DT, 64>(a, b, p, st)
+                : a.c.d <= 128 ? attn_launch<DT, 128>(a, b, p, st)
+                               : attn_launch<DT, 256>(a, b, p, st);
+  if (s || a.splits == 1) return s;
+  const int64_t n = a.rows * a.group * a.c.heads;
+  attn_join_kernel<DT><<<dim3((unsigned)n), 256, 0, st>>>(a.part, n, a.c.d, a.splits,
+                                                          (typename Elem<DT>::T*)a.out, a.lse);
+  CP_LAUNCHED("cache attention's join");
+  return CP_OK;
 }
 
 static int attn_check(const cp_kv_cache* cache, int64_t rows, int q_heads, const int32_t* table,
@@ -408,6 +762,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   if (int s = cp::attn_check(cache, rows, q_heads, table, batch, max_pages, offsets)) return s;
   if (dtype != CP_BF16 && dtype != CP_F16) return cp::set_error(CP_ERR_ARG, "queries are bfloat16 or float16");
   if (window < 0) return cp::set_error(CP_ERR_ARG, "window %d", window);
+  if (!(scale > 0.0f) || !(scale < 3e38f)) return cp::set_error(CP_ERR_ARG, "scale %g must be positive", scale);
   if (rows == 0 || batch == 0) return CP_OK;
   if (!q || !lens || !out) return cp::set_error(CP_ERR_ARG, "null q / lens / out");
   if (!cp::aligned(q, 16) || q_row * 2 % 16 || q_head * 2 % 16 || !cp::aligned(out, 16))
@@ -437,10 +792,8 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   a.splits = p.splits;
   a.scale = scale * cp::kLog2e;
   const cp::KvBatch b = {offsets, (int)batch};
-  if (dtype == CP_BF16) cp::attn_launch_d<CP_BF16>(a, b, p.items, (hipStream_t)stream);
-  else cp::attn_launch_d<CP_F16>(a, b, p.items, (hipStream_t)stream);
-  CP_LAUNCHED("cache attention");
-  return CP_OK;
+  return dtype == CP_BF16 ? cp::attn_launch_d<CP_BF16>(a, b, p, (hipStream_t)stream)
+                          : cp::attn_launch_d<CP_F16>(a, b, p, (hipStream_t)stream);
 }
 
 }  // extern "C"
