@@ -337,7 +337,7 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 constexpr int kManyRows = 128;
 
 template <int DT, int DP>
-__global__ __launch_bounds__(256, 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items) {
   constexpr int NC = DP / 32, NL = DP / 64;          // 32-column chunks; direct loads of a wave for K, and for V
   constexpr int KB = kTile * DP, BUF = 2 * KB;       // bytes of a K (or V) tile, of a buffer
   extern __shared__ __align__(16) uint8_t lds[];     // [2][BUF]
@@ -485,18 +485,33 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(AttnArgs a, KvBatch b
     const uint8_t* lk = lds + (tile & 1) * BUF + token * DP;
     const uint8_t* lv = lds + (tile & 1) * BUF + KB + q * 64;
     const int j0 = tile * kTile;
+    // LDS reads run one 32-column chunk ahead of their conversion; the barriers keep the
+    // compiler from hoisting every read, which spills
     f32x16 sc[2];
+    u32x4 kr[2][2], vr[2][2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) sc[s][j] = 0.0f;
+      kr[0][s] = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((16 * hh) ^ ksw));
+    }
+    auto read_v = [&](int i, int s) {
+      return *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
+    };
 #pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((32 * k + 16 * hh) ^ ksw));
-        sc[s] = mfma32<DT>(codes_to_16<DT>(w[0], w[1]), qf[k][0], sc[s]);
-        sc[s] = mfma32<DT>(codes_to_16<DT>(w[2], w[3]), qf[k][1], sc[s]);
-        if (k & 1) __builtin_amdgcn_sched_barrier(0);  // or every read is hoisted, and registers spill
+    for (int k = 0; k < NC; ++k) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (k + 1 < NC)
+          kr[(k + 1) & 1][s] = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((32 * (k + 1) + 16 * hh) ^ ksw));
+        else
+          vr[0][s] = read_v(0, s);
       }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k & 1][s][0], kr[k & 1][s][1]), qf[k][0], sc[s]);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k & 1][s][2], kr[k & 1][s][3]), qf[k][1], sc[s]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     float kc[2], lg[2], iv[2];
 #pragma unroll
@@ -525,7 +540,9 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(AttnArgs a, KvBatch b
       tm = fmaxf(tm, __builtin_fmaf(x, kc[s], lg[s]));
     }
     tm = fmaxf(tm, __shfl_xor(tm, 32));
-    if (__any(tm > m)) {
+    // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
+    // the outputs are then seldom rescaled
+    if (__any(tm > m + 8.0f)) {
       const float mn = fmaxf(m, tm);
       const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
       m = mn;
@@ -555,57 +572,51 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(AttnArgs a, KvBatch b
       for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
+          const u32x4 x = read_v(i, s);
 #pragma unroll
           for (int k = 0; k < 4; ++k) any |= nan_flags(x[k]);
         }
       nan = __any(any != 0);
     }
-    if (nan) {
-      // as in attn_few_kernel: NaN codes leave the product and return to the rows that see them
-      u32x4 one[2][2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < NC; ++i) {
+      if (i + 1 < NC) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const int j = j0 + 32 * s + 16 * hh + i;
-          one[s][i >> 3][(i >> 1) & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
-                                         (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
-        }
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
+        for (int s = 0; s < 2; ++s) vr[(i + 1) & 1][s] = read_v(i + 1, s);
+      }
+      if (nan) {
+        // as in attn_few_kernel: NaN codes leave the product and return to the rows that see them
         f32x16 cnt;
 #pragma unroll
         for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw)), f;
+          u32x4 f, one[2];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int j = j0 + 32 * s + 16 * hh + 2 * k;
+            one[k >> 2][k & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
+                                 (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t fl = nan_flags(x[k]) >> 7;
-            x[k] &= ~(fl * 0xFFu);
+            const uint32_t fl = nan_flags(vr[i & 1][s][k]) >> 7;
+            vr[i & 1][s][k] &= ~(fl * 0xFFu);
             f[k] = fl * 0x38u;  // 1.0 where the code was NaN
           }
-          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[s][0], cnt);
-          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[s][1], cnt);
-          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
-          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
+          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[0], cnt);
+          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[1], cnt);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (cnt[j] > 0.0f) o[i][j] = __builtin_nanf("");
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 16; ++j) o[i][j] = cnt[j] > 0.0f ? __builtin_nanf("") : o[i][j];
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
-          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
-          o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
-          if (s) __builtin_amdgcn_sched_barrier(0);
-        }
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 x = vr[i & 1][s];
+        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
+        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   l += __shfl_xor(l, 32);
