@@ -465,14 +465,14 @@ int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, in
 
 /* Workspace bytes of cp_kv_attention (0: none); ragged: offsets are given. */
 size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads,
-                                int64_t batch, int64_t max_pages, int ragged);
+                                int64_t batch, int64_t max_pages, int ragged, int window);
 
 /* out [rows, q_heads, head_dim] = attention of q over the cache. Sequence b has lens[b]
  * tokens; its query rows (as in cp_kv_write) sit at its last positions, and query head x
  * reads cache head x / (q_heads / heads). Row at position p sees token j where j < lens[b],
  * j <= p (causal) and j > p - window (window > 0); tokens without a page are not seen. A row
  * that sees nothing is 0 with lse -inf. lse [rows, q_heads] float32 (NULL: not wanted) is
- * the natural log of the sum of exponentials. q and out: bfloat16 or float16. */
+ * the natural log of the sum of exponentials. q and out: bfloat16 or float16. scale is positive. */
 int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head,
                     int dtype, int64_t rows, int q_heads, const int32_t* table, int64_t batch,
                     int64_t max_pages, const int32_t* lens, const int32_t* offsets, int causal,

@@ -124,7 +124,7 @@ SIGNATURES = {
     "cp_kv_write": (_i32, [_kv_p, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _vp, _i64, _i64,
                            _vp, _vp, _vp]),
     "cp_kv_read": (_i32, [_kv_p, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _vp]),
-    "cp_kv_attention_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32]),
+    "cp_kv_attention_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32, _i32]),
     "cp_kv_attention": (_i32, [_kv_p, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _i64, _vp,
                                _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
 }

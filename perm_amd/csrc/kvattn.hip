@@ -14,6 +14,8 @@
 // float32. K codes become q's own 16-bit type, which holds e4m3 exactly.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "kvcache.h"
 #include "lowbit.h"
 
@@ -33,12 +35,26 @@ struct AttnArgs {
   const int* lens;              // [batch]
   void* out;                    // [rows][q heads][d]
   float* lse;                   // [rows][q heads] or null
-  float* part;                  // splits > 1: [rows][q heads][splits][d], then [..][splits][m, l]
+  // splits > 1, a row being one of a sequence's and head: [row][splits][d] sums, then
+  // [row][splits] pairs (m, l), then [row] int: how many splits the row used, 0 if it is done
+  float* part;
   int64_t rows;
   int group;                    // q heads per kv head
   int causal, window, splits;
+  int least;                    // tiles of a split at least
   float scale;                  // softmax scale * log2 e
 };
+
+struct SplitParts {
+  float *sums, *ml;
+  int* used;
+};
+
+__host__ __device__ inline SplitParts split_parts(const AttnArgs& a) {
+  const int64_t n = a.rows * a.group * a.c.heads * a.splits;
+  float* ml = a.part + n * a.c.d;
+  return {a.part, ml, reinterpret_cast<int*>(ml + 2 * n)};
+}
 
 // Eight e4m3 codes in q's type / in float16 (both exact).
 template <int DT>
@@ -75,14 +91,21 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 // Few query rows: a workgroup takes up to 16 (row, head of the group) pairs of one kv head
-// and one range of tokens; its four waves walk the range's 64-token tiles in turn and join
-// at the end. K is the A operand (16 tokens x 32 columns), q the B operand, so a lane's
-// scores belong to one query row (lane % 16), and its group lane / 16 owns 16 consecutive
-// tokens of the tile: score (t, i) of the lane is token 16 (lane / 16) + 4 t + i. Those are
-// the eight-token runs the second product's operands hold, so the weights go from one
-// product to the other without leaving their lanes.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
+// and one range of tokens; its four waves walk the range 32 tokens at a time in turn and
+// join at the end. Bound by reading the cache, and for short ranges by the latencies a
+// workgroup starts with (length, page numbers, codes), which four workgroups on a CU hide
+// better than longer strides in fewer of them: hence small tiles and at most 128 registers.
+//
+// K is the A operand (16 tokens x 32 columns), q the B operand, so a lane's scores belong to
+// one query row (lane % 16), and its group lane / 16 owns 8 consecutive tokens of the tile:
+// score (t, i) of the lane is token 8 (lane / 16) + 4 t + i. Those are the eight-token runs
+// the second product's operands hold, so the weights go from one product to the other
+// without leaving their lanes.
+constexpr int kFewTile = 32;
+
+// FULL: d is DP, a constant the addresses fold in.
+template <int DT, int DP, bool FULL>
+__global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   constexpr int NC = DP / 64, ND = DP / 16;
   __shared__ float sm_m[4][16], sm_l[4][16];
   __shared__ __align__(16) float sm_o[4][16][DP + 4];
@@ -92,13 +115,12 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   int b, item, n_b;
   int64_t row0;
   if (!kv_locate(bt, (int)(blockIdx.x / a.splits / c.heads),
-                 [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item,
-                 &row0, &n_b))
+                 [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item, &row0, &n_b))
     return;
   if (row0 < 0 || row0 + n_b > a.rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
+  const int d = FULL ? DP : c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
   const int64_t cap = (int64_t)c.max_pages * blk;
   const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
 
@@ -117,21 +139,26 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
     jhi = max(jhi, __shfl_xor(jhi, s));
     jlo = min(jlo, __shfl_xor(jlo, s));
   }
-  jlo = min(jlo, jhi);
-  const int t0 = jlo / kTile, nt = (jhi + kTile - 1) / kTile - t0;
-  const int per = (nt + a.splits - 1) / a.splits;
+  jhi = __builtin_amdgcn_readfirstlane(jhi);
+  jlo = min(__builtin_amdgcn_readfirstlane(jlo), jhi);
+  const int t0 = jlo / kFewTile, nt = (jhi + kFewTile - 1) / kFewTile - t0;
+  // a row's tiles are shared evenly by the splits; one of few tiles uses few of them
+  const int per = max((nt + a.splits - 1) / a.splits, a.least), used = (nt + per - 1) / per;
+  if (split > 0 && split >= used) return;
   const int tb = t0 + split * per, te = min(t0 + nt, tb + per);
 
   u32x4 qf[NC][2];
   {
     typedef typename Elem<DT>::T T;
-    const T* qp = (const T*)a.q + (row0 + qi) * a.q_row + (int64_t)qh * a.q_head;
+    const T* qp = (const T*)a.q + (real ? (row0 + qi) * a.q_row + (int64_t)qh * a.q_head : 0);
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const bool in = real && 64 * k + 16 * g < d;
+      const bool in = real && (FULL || 64 * k + 16 * g < d);
       const u32x4 z = {0, 0, 0, 0};
-      qf[k][0] = in ? *reinterpret_cast<const u32x4*>(qp + 64 * k + 16 * g) : z;
-      qf[k][1] = in ? *reinterpret_cast<const u32x4*>(qp + 64 * k + 16 * g + 8) : z;
+      const T* p = qp + (FULL || 64 * k + 16 * g < d ? 64 * k + 16 * g : 0);
+      qf[k][0] = *reinterpret_cast<const u32x4*>(p);
+      qf[k][1] = *reinterpret_cast<const u32x4*>(p + 8);
+      if (!in) qf[k][0] = qf[k][1] = z;
     }
   }
   f32x4 o[ND];
@@ -143,38 +170,44 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   // score NaN anyway
   int kcol[NC];
 #pragma unroll
-  for (int k = 0; k < NC; ++k) kcol[k] = 64 * k + 16 * g < d ? 64 * k + 16 * g : 0;
+  for (int k = 0; k < NC; ++k) kcol[k] = FULL || 64 * k + 16 * g < d ? 64 * k + 16 * g : 0;
+  uint64_t marked = 0;  // bit 4 i + k: result (i, k) of this lane has seen a NaN code
+  u32x2* const mine = reinterpret_cast<u32x2*>(&sm_o[wave][0][0]) + lane;
 
+  // pages of the token runs this lane reads: K rows by lane % 16 / 4, V and the scores' scales
+  // by lane / 16. Looked up a tile ahead.
+  const int lastj = max(jhi - 1, 0);
+  auto page = [&](int j) { return tab[min(j, lastj) >> lb]; };
+  int pk = 0, pv = 0;
+  if (tb + wave < te) {
+    pk = page((tb + wave) * kFewTile + 8 * (col >> 2));
+    pv = page((tb + wave) * kFewTile + 8 * g);
+  }
+#pragma clang loop unroll(disable)
   for (int tile = tb + wave; tile < te; tile += 4) {
-    const int j0 = tile * kTile;
-    // pages of the two 16-token groups this lane reads: K rows by lane % 16 / 4, V and the
-    // scores' scales by lane / 16
-    const int jk = j0 + 16 * (col >> 2), jv = j0 + 16 * g;
-    int pk = jk < len ? tab[jk >> lb] : -1, pv = jv < len ? tab[jv >> lb] : -1;
-    if ((unsigned)pk >= (unsigned)c.pages) pk = -1;
-    if ((unsigned)pv >= (unsigned)c.pages) pv = -1;
-    const int64_t ak = ((int64_t)max(pk, 0) * c.heads + h) * blk * d;
-    const int64_t hv = (int64_t)max(pv, 0) * c.heads + h;
-    const uint8_t* kp = c.k + ak + ((jk & (blk - 1)) + (col & 3)) * d;
+    const int jk = tile * kFewTile + 8 * (col >> 2), jv = tile * kFewTile + 8 * g;
+    const bool hk = (unsigned)pk < (unsigned)c.pages, have = (unsigned)pv < (unsigned)c.pages;
+    const int64_t hv = (int64_t)(have ? pv : 0) * c.heads + h;
+    const uint8_t* kp = c.k + ((int64_t)(hk ? pk : 0) * c.heads + h) * blk * d + ((jk & (blk - 1)) + (col & 3)) * d;
     const uint8_t* vp = c.v + hv * blk * d + col * blk + (jv & (blk - 1));
-    f32x4 sc[4];
+    u32x4 kk[2][NC];
+    u32x2 vv[ND];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
-    u32x4 kk[4][NC], vv[ND];
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        kk[t][k] = *reinterpret_cast<const u32x4*>(kp + 4 * t * d + kcol[k]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      vv[i] = *reinterpret_cast<const u32x4*>(vp + (16 * i < d ? 16 * i : 0) * blk);  // rows past d are dropped
-    }
+      for (int k = 0; k < NC; ++k) kk[t][k] = *reinterpret_cast<const u32x4*>(kp + 4 * t * d + kcol[k]);
     const float ks = c.k_scale[hv], vs = c.v_scale[hv];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int i = 0; i < ND; ++i) {  // rows past d repeat the last one and are dropped
+      vv[i] = *reinterpret_cast<const u32x2*>(vp);
+      if (FULL || 16 * (i + 1) < d) vp += 16 * blk;
+    }
+    pk = page(jk + 4 * kFewTile);
+    pv = page(jv + 4 * kFewTile);
+    f32x4 sc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         sc[t] = mfma16<DT>(codes_to_16<DT>(kk[t][k][0], kk[t][k][1]), qf[k][0], sc[t]);
@@ -184,90 +217,98 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
     const float kc = ks * a.scale;
     const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
     const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs) & 0x7F800000u));
-    float tm = kNegInf;
     bool edge = false;  // a token of this lane that its row does not see
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = jv + 4 * t + i;
-        const bool see = j >= lo && j < hi && pv >= 0;
+        const bool see = have && j >= lo && j < hi;
         edge |= !see;
-        sc[t][i] = see ? __builtin_fmaf(sc[t][i], kc, lv) : kNegInf;
-        tm = fmaxf(tm, sc[t][i]);
+        sc[t][i] = see ? sc[t][i] : kNegInf;
       }
-    }
+    // kc > 0: the largest t of the lane's run comes from its largest raw score
+    float tm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                     fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    tm = __builtin_fmaf(tm, kc, lv);
     tm = fmaxf(tm, __shfl_xor(tm, 16));
     tm = fmaxf(tm, __shfl_xor(tm, 32));
-    const float mn = fmaxf(m, tm);
-    const float ms = mn == kNegInf ? 0.0f : mn;  // nothing seen yet: weights 2^-inf = 0
-    const float al = exp2_fast(m - ms);
-    m = mn;
-    u32x4 w[2];
+    // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
+    // the outputs are then seldom rescaled
+    if (__any(tm > m + 8.0f)) {
+      const float mn = fmaxf(m, tm);
+      const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[i] *= al;
+    }
+    const float off = lv - (m == kNegInf ? 0.0f : m);
+    u32x4 w;
     float sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const float e0 = exp2_fast(sc[t][i] - ms), e1 = exp2_fast(sc[t][i + 1] - ms);
+        const float e0 = exp2_fast(__builtin_fmaf(sc[t][i], kc, off));
+        const float e1 = exp2_fast(__builtin_fmaf(sc[t][i + 1], kc, off));
         sum += e0 + e1;
-        w[t >> 1][2 * (t & 1) + (i >> 1)] = pack2<CP_F16>(e0, e1);
+        w[2 * t + (i >> 1)] = pack2<CP_F16>(e0, e1);
       }
-    }
-    l = l * al + sum * iv;
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] *= al;
+    l = __builtin_fmaf(sum, iv, l);
+    // a code that a row does not see must not reach it, not even as 0 * NaN: NaN codes are
+    // taken out of the product and put back into the rows that do see them
+    bool nan = false;
     if (__any(edge)) {
-      // a code that a row does not see must not reach it, not even as 0 * NaN: NaN codes
-      // are taken out of the product and put back into the rows that do see them
       uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < ND; ++i)
+      for (int i = 0; i < ND; ++i) any |= nan_flags(vv[i][0]) | nan_flags(vv[i][1]);
+      nan = __any(any != 0);
+      if (nan) {
+        // through the wave's LDS in a loop: unrolled in registers, this rare path would make
+        // the common one spill
 #pragma unroll
-        for (int k = 0; k < 4; ++k) any |= nan_flags(vv[i][k]);
-      if (__any(any != 0)) {
-        u32x4 one[2];
+        for (int i = 0; i < ND; ++i) mine[64 * i] = vv[i];
+        u32x4 one = {0, 0, 0, 0};  // 1.0 where this lane's row sees the token
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int t = 2 * s + (k >> 1), i = 2 * (k & 1);
-            one[s][k] = (sc[t][i] != kNegInf ? 0x3C00u : 0u) | (sc[t][i + 1] != kNegInf ? 0x3C000000u : 0u);
-          }
-#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = jv + e;
+          if (have && j >= lo && j < hi) one[e >> 1] |= 0x3C00u << (16 * (e & 1));
+        }
+#pragma clang loop unroll(disable)
         for (int i = 0; i < ND; ++i) {
-          f32x4 cnt = {0, 0, 0, 0};
+          u32x2 y = mine[64 * i];
+          const uint32_t f0 = nan_flags(y[0]) >> 7, f1 = nan_flags(y[1]) >> 7;
+          y[0] &= ~(f0 * 0xFFu);
+          y[1] &= ~(f1 * 0xFFu);
+          mine[64 * i] = y;
+          // e4m3 1.0 where the code was NaN
+          const f32x4 cnt = mfma16<CP_F16>(codes_to_16<CP_F16>(f0 * 0x38u, f1 * 0x38u), one, f32x4{0, 0, 0, 0});
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t f = nan_flags(vv[i][k]);
-            vv[i][k] &= ~(((f >> 7) * 0xFFu));
-            // e4m3 1.0 = 0x38 where the code was NaN
-            const uint32_t ind = (f >> 7) * 0x38u;
-            const u32x4 z = codes_to_16<CP_F16>(ind, ind);
-            u32x4 av = {0, 0, 0, 0};
-            av[2 * (k & 1)] = z[0];
-            av[2 * (k & 1) + 1] = z[1];
-            cnt = mfma16<CP_F16>(av, one[k >> 1], cnt);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (cnt[k] > 0.0f) o[i][k] = __builtin_nanf("");
+          for (int k = 0; k < 4; ++k) marked |= cnt[k] > 0.0f ? (uint64_t)1 << (4 * i + k) : 0;
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(vv[i][0], vv[i][1]), w[0], o[i]);
-      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(vv[i][2], vv[i][3]), w[1], o[i]);
+      u32x2 y = vv[i];
+      if (nan) y = mine[64 * i];
+      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(y[0], y[1]), w, o[i]);
     }
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (g == 0) sm_m[wave][col] = m, sm_l[wave][col] = l;
+  if (__any(marked != 0)) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = marked >> (4 * i + k) & 1 ? __builtin_nanf("") : o[i][k];
+  }
 #pragma unroll
   for (int i = 0; i < ND; ++i) *reinterpret_cast<f32x4*>(&sm_o[wave][col][16 * i + 4 * g]) = o[i];
   __syncthreads();
-  // join the four waves: thread -> row threadIdx / 16, columns strided by 16
+  // join the four waves: thread -> row threadIdx / 16, four columns at a time
   const int row = threadIdx.x >> 4, c0 = threadIdx.x & 15;
   const int64_t rr = (int64_t)item * 16 + row;
   if (rr >= (int64_t)n_b * a.group) return;
@@ -281,27 +322,31 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnArgs a, KvBatch bt) {
     ll += sm_l[w][row] * f[w];
   }
   const int64_t orow = (row0 + rr / a.group) * ((int64_t)a.group * c.heads) + h * a.group + rr % a.group;
-  if (a.splits > 1) {
-    float* p = a.part + (orow * a.splits + split) * d;
-    float* pm = a.part + a.rows * a.group * c.heads * a.splits * d + (orow * a.splits + split) * 2;
-    if (c0 == 0) pm[0] = mm, pm[1] = ll;
-    for (int x = c0; x < d; x += 16) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v += sm_o[w][row][x] * f[w];
-      p[x] = v;
-    }
-    return;
-  }
-  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;  // a row that saw nothing: 0
+  const SplitParts sp = split_parts(a);
+  if (a.splits > 1 && split == 0 && c0 == 0) sp.used[orow] = used > 1 ? used : 0;
+  float* p = sp.sums + (orow * a.splits + split) * d;
   typename Elem<DT>::T* op = (typename Elem<DT>::T*)a.out + orow * d;
-  for (int x = c0; x < d; x += 16) {
-    float v = 0.0f;
+  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;  // a row that saw nothing: 0
+  for (int x = 4 * c0; x < d; x += 64) {
+    f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v += sm_o[w][row][x] * f[w];
-    op[x] = (typename Elem<DT>::T)(v * inv);
+    for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(&sm_o[w][row][x]) * f[w];
+    if (used > 1) {
+      *reinterpret_cast<f32x4*>(p + x) = v;
+    } else {
+      u32x2 y;
+      y[0] = pack2<DT>(v[0] * inv, v[1] * inv);
+      y[1] = pack2<DT>(v[2] * inv, v[3] * inv);
+      *reinterpret_cast<u32x2*>(op + x) = y;
+    }
   }
-  if (a.lse && c0 == 0) a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+  if (c0 != 0) return;
+  if (used > 1) {
+    float* pm = sp.ml + (orow * a.splits + split) * 2;
+    pm[0] = mm, pm[1] = ll;
+  } else if (a.lse) {
+    a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+  }
 }
 
 // Many query rows: a workgroup takes 128 (row, head of the group) pairs of one kv head, 32 a
@@ -391,7 +436,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   wlo = __builtin_amdgcn_readfirstlane(wlo);
   whi = __builtin_amdgcn_readfirstlane(whi);
   const int t0 = jlo / kTile, nt = (jhi + kTile - 1) / kTile - t0;
-  const int per = (nt + a.splits - 1) / a.splits;
+  const int per = max((nt + a.splits - 1) / a.splits, a.least), used = (nt + per - 1) / per;
+  if (split > 0 && split >= used) return;
   const int tb = t0 + split * per, te = min(t0 + nt, tb + per);
 
   u32x4 qf[NC][2];
@@ -623,9 +669,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   if (!real) return;
   const int64_t orow = qrow * ((int64_t)a.group * c.heads) + qh;
   // lane's results: columns 32 i + 8 (j / 4) + 4 hh + j % 4 of its row
-  if (a.splits > 1) {
-    float* p = a.part + (orow * a.splits + split) * d;
-    float* pm = a.part + a.rows * a.group * c.heads * a.splits * d + (orow * a.splits + split) * 2;
+  const SplitParts sp = split_parts(a);
+  if (a.splits > 1 && split == 0 && hh == 0) sp.used[orow] = used > 1 ? used : 0;
+  if (used > 1) {
+    float* p = sp.sums + (orow * a.splits + split) * d;
+    float* pm = sp.ml + (orow * a.splits + split) * 2;
     if (hh == 0) pm[0] = m, pm[1] = l;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -651,67 +699,84 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   if (a.lse && hh == 0) a.lse[orow] = l == 0.0f ? kNegInf : (m + __builtin_amdgcn_logf(l)) / kLog2e;
 }
 
-// The splits of a row joined: one workgroup per row, d / 4 threads over the columns and the
-// rest of the threads over the splits, whose sums are added in a fixed order.
-template <int DT>
-__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, int64_t rows, int d,
-                                                        int splits, typename Elem<DT>::T* __restrict__ out,
+// The splits of a row joined, in a fixed order. d / 4 threads (a group) take a row's columns;
+// with many splits the groups of a workgroup share one row's, otherwise each has its own row.
+template <int DT, bool ONE_ROW>
+__global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t rows, int d, int most,
+                                                        typename Elem<DT>::T* __restrict__ out,
                                                         float* __restrict__ lse) {
-  __shared__ float sm_m[4], sm_l[256];
+  __shared__ float sm_m[4], sm_l[16];
   __shared__ __align__(16) float sm_o[256 * 4];
-  const int64_t row = blockIdx.x;
-  const float* po = part + row * splits * d;
-  const float* pm = part + rows * splits * d + row * splits * 2;
+  const int T = d / 4, NG = min(256 / T, 16), grp = threadIdx.x / T, c = 4 * (threadIdx.x % T);
+  const int64_t row = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * NG + grp;
+  const bool mine = grp < NG && row < rows;
+  // a row that no sequence has was never given a count: bounded, its result means nothing
+  const int splits = mine || ONE_ROW ? min(max(sp.used[row], 0), most) : 0;
+  if (splits == 0) return;  // ONE_ROW: the whole workgroup leaves
+  const float* po = sp.sums + row * most * d;
+  const float* pm = sp.ml + row * most * 2;
   float mm = kNegInf;
-  for (int s = threadIdx.x; s < splits; s += 256) mm = fmaxf(mm, pm[2 * s]);
+  if constexpr (ONE_ROW) {
+    for (int s = threadIdx.x; s < splits; s += 256) mm = fmaxf(mm, pm[2 * s]);
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1) mm = fmaxf(mm, __shfl_xor(mm, k));
-  if ((threadIdx.x & 63) == 0) sm_m[threadIdx.x >> 6] = mm;
-  __syncthreads();
-  mm = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    for (int k = 1; k < 64; k <<= 1) mm = fmaxf(mm, __shfl_xor(mm, k));
+    if ((threadIdx.x & 63) == 0) sm_m[threadIdx.x >> 6] = mm;
+    __syncthreads();
+    mm = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+  } else {
+    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, pm[2 * s]);
+  }
   const float ms = mm == kNegInf ? 0.0f : mm;
-  const int T = d / 4, NG = 256 / T, grp = threadIdx.x / T, c = 4 * (threadIdx.x % T);
   f32x4 v = {0, 0, 0, 0};
   float ll = 0.0f;
-  if (grp < NG) {
+  if (mine) {
 #pragma unroll 4
-    for (int s = grp; s < splits; s += NG) {
+    for (int s = ONE_ROW ? grp : 0; s < splits; s += ONE_ROW ? NG : 1) {
       const float f = exp2_fast(pm[2 * s] - ms);
       ll += pm[2 * s + 1] * f;
       v += *reinterpret_cast<const f32x4*>(po + (int64_t)s * d + c) * f;
     }
-    *reinterpret_cast<f32x4*>(&sm_o[grp * d + c]) = v;
-    sm_l[grp] = ll;  // the group's threads hold the same sum
   }
-  __syncthreads();
-  if ((int)threadIdx.x >= d) return;
-  float o = 0.0f;
-  ll = 0.0f;
-  for (int i = 0; i < NG; ++i) {
-    o += sm_o[i * d + threadIdx.x];
-    ll += sm_l[i];
+  if constexpr (ONE_ROW) {
+    if (mine) {
+      *reinterpret_cast<f32x4*>(&sm_o[grp * d + c]) = v;
+      sm_l[grp] = ll;  // the group's threads hold the same sum
+    }
+    __syncthreads();
+    if (grp != 0) return;
+    for (int i = 1; i < NG; ++i) {
+      v += *reinterpret_cast<const f32x4*>(&sm_o[i * d + c]);
+      ll += sm_l[i];
+    }
   }
-  out[row * d + threadIdx.x] = (typename Elem<DT>::T)(ll != 0.0f ? o / ll : 0.0f);
-  if (lse && threadIdx.x == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+  const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+  u32x2 y;
+  y[0] = pack2<DT>(v[0] * inv, v[1] * inv);
+  y[1] = pack2<DT>(v[2] * inv, v[3] * inv);
+  *reinterpret_cast<u32x2*>(out + row * d + c) = y;
+  if (lse && c == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
 }
 
 struct AttnPlan {
   bool many;
   int64_t items;  // upper bound of the batch's row tiles
-  int splits;
+  int splits, least;  // at most so many pieces of a row's tiles, of at least so many tiles
 };
 
 // Row tiles of 16 while a sequence has no more (row, head of the group) pairs on average:
 // then reading the cache bounds the call; of 128 above that.
-static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int64_t cap) {
+static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int64_t cap, int window) {
   AttnPlan p;
   p.many = rows * group > 16 * batch;
-  const int tile = p.many ? kManyRows : 16;
+  const int tile = p.many ? kManyRows : 16, step = p.many ? kTile : kFewTile;
   p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
-  // workgroups for every CU four times over (two for the large tiles), none under 256 tokens
-  const int64_t n = p.items * heads, want = (p.many ? 512 : 1024) / (n > 0 ? n : 1);
-  const int64_t most = (cap + 255) / 256;
-  p.splits = (int)(want < 1 ? 1 : want > most ? most : want);
+  // The tokens of a row tile are split over as many workgroups as the CUs hold at once, but
+  // not into pieces shorter than joining them costs: 16 steps of the longest row tile there
+  // can be, or (few rows, where a step is 32 tokens) 8 of a shorter one's.
+  const int64_t n = p.items * heads, want = p.many ? 512 : 1024;
+  const int64_t span = window > 0 ? std::min(cap, (int64_t)window + tile + step) : cap;
+  p.least = p.many ? 16 : 8;
+  p.splits = (int)std::max((int64_t)1, std::min(want / std::max(n, (int64_t)1), span / (16 * step)));
   return p;
 }
 
@@ -725,7 +790,8 @@ static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, h
     if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
     attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
   } else {
-    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b);
+    if (a.c.d == DP) attn_few_kernel<DT, DP, true><<<grid, 256, 0, st>>>(a, b);
+    else attn_few_kernel<DT, DP, false><<<grid, 256, 0, st>>>(a, b);
   }
   CP_LAUNCHED("cache attention");
   return CP_OK;
@@ -738,8 +804,13 @@ static int attn_launch_d(const AttnArgs& a, const KvBatch& b, const AttnPlan& p,
                                : attn_launch<DT, 256>(a, b, p, st);
   if (s || a.splits == 1) return s;
   const int64_t n = a.rows * a.group * a.c.heads;
-  attn_join_kernel<DT><<<dim3((unsigned)n), 256, 0, st>>>(a.part, n, a.c.d, a.splits,
-                                                          (typename Elem<DT>::T*)a.out, a.lse);
+  typename Elem<DT>::T* out = (typename Elem<DT>::T*)a.out;
+  const int64_t groups = std::min(256 / (a.c.d / 4), 16);
+  if (a.splits > 8)
+    attn_join_kernel<DT, true><<<dim3((unsigned)n), 256, 0, st>>>(split_parts(a), n, a.c.d, a.splits, out, a.lse);
+  else
+    attn_join_kernel<DT, false><<<dim3((unsigned)((n + groups - 1) / groups)), 256, 0, st>>>(split_parts(a), n, a.c.d,
+                                                                                          a.splits, out, a.lse);
   CP_LAUNCHED("cache attention's join");
   return CP_OK;
 }
@@ -758,11 +829,11 @@ static int attn_check(const cp_kv_cache* cache, int64_t rows, int q_heads, const
 extern "C" {
 
 size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads, int64_t batch,
-                                int64_t max_pages, int ragged) {
+                                int64_t max_pages, int ragged, int window) {
   if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
   const cp::AttnPlan p = cp::attn_plan(rows, batch, ragged != 0, q_heads / cache->heads, cache->heads,
-                                       max_pages * cache->block);
-  return p.splits > 1 ? (size_t)rows * q_heads * p.splits * (cache->head_dim + 2) * 4 : 0;
+                                       max_pages * cache->block, window);
+  return p.splits > 1 ? (size_t)rows * q_heads * p.splits * (cache->head_dim + 2) * 4 + (size_t)rows * q_heads * 4 : 0;
 }
 
 int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,
@@ -781,8 +852,8 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   if (q_row < 0 || q_head < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of q");
   const int group = q_heads / cache->heads;
   const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads,
-                                       max_pages * cache->block);
-  const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr);
+                                       max_pages * cache->block, window);
+  const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window);
   if (need && (!ws || ws_bytes < need))
     return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
   if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > 0x7FFFFFFF)
@@ -801,6 +872,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   a.causal = causal != 0;
   a.window = window;
   a.splits = p.splits;
+  a.least = p.least;
   a.scale = scale * cp::kLog2e;
   const cp::KvBatch b = {offsets, (int)batch};
   return dtype == CP_BF16 ? cp::attn_launch_d<CP_BF16>(a, b, p, (hipStream_t)stream)

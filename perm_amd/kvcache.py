@@ -156,7 +156,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     Sequence b holds lens[b] tokens, and its query rows are its last ones (write them first):
     row i of n sits at position lens[b] - n + i and sees the tokens up to its own (causal) and,
     with window > 0, no more than the window's last ones. Query head x reads cache head
-    x // (q heads / cache heads). scale is head_dim ** -0.5 by default. A row that sees
+    x // (q heads / cache heads). scale is positive, head_dim ** -0.5 by default. A row that sees
     nothing is 0, its lse -inf."""
     lib = _lib.load()
     desc = _desc(cache)
@@ -173,7 +173,8 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     lse = torch.empty((rows, heads), device=q.device) if return_lse else None
     batch, max_pages = table.shape
     ragged = offsets is not None
-    nws = lib.cp_kv_attention_ws_bytes(ctypes.byref(desc), rows, heads, batch, max_pages, ragged)
+    nws = lib.cp_kv_attention_ws_bytes(ctypes.byref(desc), rows, heads, batch, max_pages, ragged,
+                                       window)
     ws = _lib.workspace(nws, q.device) if nws else None
     _lib.check(lib.cp_kv_attention(
         ctypes.byref(desc), q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], rows, heads,
