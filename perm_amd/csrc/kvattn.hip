@@ -463,10 +463,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   float m = kNegInf, l = 0.0f;
 
   const int* tab = c.table + (int64_t)b * c.max_pages;
-  auto page_at = [&](int j) {  // of token j; -1: none
-    const int p = j < len ? tab[j >> lb] : -1;
-    return (unsigned)p < (unsigned)c.pages ? p : -1;
-  };
   // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
   // each, four token groups. Chunks past d repeat the row's first, rows past d its last 16
   // (their q is 0, their results are dropped).
@@ -476,8 +472,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   auto fetch = [&](int tile, int pk, int pv) {
     uint8_t* to = lds + (tile & 1) * BUF;
     const int j0 = tile * kTile;
-    const uint8_t* kp = c.k + ((int64_t)max(pk, 0) * c.heads + h) * blk * d;
-    const uint8_t* vp = c.v + ((int64_t)max(pv, 0) * c.heads + h) * blk * d;
+    // no page: page 0's codes, which no row sees
+    const uint8_t* kp = c.k + ((int64_t)((unsigned)pk < (unsigned)c.pages ? pk : 0) * c.heads + h) * blk * d;
+    const uint8_t* vp = c.v + ((int64_t)((unsigned)pv < (unsigned)c.pages ? pv : 0) * c.heads + h) * blk * d;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int token = kt + i * (1024 / DP);
@@ -497,36 +494,45 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   const int ksw = k_swizzle<DP>(token);
   const int vsw = 16 * ((q >> 2) & 3);
 
-  int pk = 0, pv = 0, pg[2] = {0, 0};
-  float ks[2], vs[2];
-  bool have[2];
-  auto pages = [&](int tile) {
+  // Page numbers are looked up two tiles ahead and scales loaded one ahead, so that neither
+  // is waited for. Lookups past the last token repeat its own; such tokens are not seen.
+  const int lastj = max(jhi - 1, 0);
+  struct Pages {
+    int k, v, g[2];
+  } pn;
+  auto lookup = [&](int tile) {
     const int j0 = tile * kTile;
-    pk = page_at(j0 + 16 * wave);
-    pv = page_at(j0 + 16 * vg);
+    pn.k = tab[min(j0 + 16 * wave, lastj) >> lb];
+    pn.v = tab[min(j0 + 16 * vg, lastj) >> lb];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) pg[s] = page_at(j0 + 32 * s + 16 * hh);
+    for (int s = 0; s < 2; ++s) pn.g[s] = tab[min(j0 + 32 * s + 16 * hh, lastj) >> lb];
   };
-  auto scales = [&] {
+  float ks[2], vs[2], nks[2], nvs[2];
+  bool have[2], nhave[2];
+  auto next_scales = [&] {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int64_t hv = (int64_t)max(pg[s], 0) * c.heads + h;
-      ks[s] = c.k_scale[hv];
-      vs[s] = c.v_scale[hv];
-      have[s] = pg[s] >= 0;
+      nhave[s] = (unsigned)pn.g[s] < (unsigned)c.pages;
+      const int64_t hv = (int64_t)(nhave[s] ? pn.g[s] : 0) * c.heads + h;
+      nks[s] = c.k_scale[hv];
+      nvs[s] = c.v_scale[hv];
     }
   };
   if (tb < te) {
-    pages(tb);
-    fetch(tb, pk, pv);
+    lookup(tb);
+    fetch(tb, pn.k, pn.v);
+    next_scales();
+    lookup(tb + 1);
   }
   for (int tile = tb; tile < te; ++tile) {
-    scales();
-    const bool all = !__any(!have[0] || !have[1]);
     __syncthreads();  // this tile has landed, and every wave is done with the one before
+#pragma unroll
+    for (int s = 0; s < 2; ++s) ks[s] = nks[s], vs[s] = nvs[s], have[s] = nhave[s];
+    const bool all = !__any(!have[0] || !have[1]);
     if (tile + 1 < te) {
-      pages(tile + 1);
-      fetch(tile + 1, pk, pv);
+      fetch(tile + 1, pn.k, pn.v);
+      next_scales();
+      lookup(tile + 2);
     }
     const uint8_t* lk = lds + (tile & 1) * BUF + token * DP;
     const uint8_t* lv = lds + (tile & 1) * BUF + KB + q * 64;
