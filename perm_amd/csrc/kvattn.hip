@@ -574,11 +574,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     }
     const bool edge = !all || j0 < wlo || j0 + kTile > whi;
     if (edge) {
+      // this lane's first token, hidden from the compiler: it would compare all 32 on every
+      // tile, ahead of the branch
+      int j1 = j0 + 16 * hh;
+      asm volatile("" : "+v"(j1));
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * s + 16 * hh + i;
+          const int j = j1 + 32 * s + i;
           sc[s][i] = have[s] && j >= lo && j < hi ? sc[s][i] : kNegInf;
         }
     }
@@ -641,12 +645,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         f32x16 cnt;
 #pragma unroll
         for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
+        int j1 = j0 + 16 * hh;
+        asm volatile("" : "+v"(j1));
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           u32x4 f, one[2];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const int j = j0 + 32 * s + 16 * hh + 2 * k;
+            const int j = j1 + 32 * s + 2 * k;
             one[k >> 2][k & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
                                  (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
           }
