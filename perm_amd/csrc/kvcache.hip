@@ -35,19 +35,10 @@ __device__ __forceinline__ float kv_clamp(float v) {
   return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f);
 }
 
-template <class T>
-__device__ __forceinline__ T block_max(T v, T* lds) {
+// Largest of v over the wave.
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) {
-    const T o = __shfl_xor(v, s);
-    v = v > o ? v : o;
-  }
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) v = v > lds[w] ? v : lds[w];
-  __syncthreads();
+  for (int s = 32; s >= 1; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
   return v;
 }
 
@@ -56,60 +47,71 @@ struct KvRows {
   int64_t row_st, head_st;  // element strides
 };
 
-// The largest finite magnitude of n rows from row r0 of head h.
-template <int DT>
-__device__ __forceinline__ float kv_amax(const KvRows& x, int64_t r0, int n, int h, int d) {
-  const typename Elem<DT>::T* p = (const typename Elem<DT>::T*)x.p + r0 * x.row_st + h * x.head_st;
-  float m = 0.0f;
-  const int dc = d / 8;
-  for (int c = threadIdx.x; c < n * dc; c += 256) {
-    const int row = c / dc;
-    float v[8];
-    load8<DT>(p + row * x.row_st + 8 * (c - row * dc), v);
+// The largest finite magnitude of eight values.
+__device__ __forceinline__ float amax8(const float (&v)[8], float m) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = fabsf(v[i]);
-      m = a < __builtin_inff() && a > m ? a : m;
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(v[i]);
+    m = a < __builtin_inff() && a > m ? a : m;
   }
   return m;
 }
 
-// Eight scaled values' codes.
-template <int DT>
-__device__ __forceinline__ u32x2 kv_codes(const typename Elem<DT>::T* p, float inv) {
-  float v[8];
-  load8<DT>(p, v);
+__device__ __forceinline__ u32x2 codes8(const float (&v)[8], float inv) {
+  float u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = kv_clamp(v[i] * inv);
-  return e4m3_encode8(v);
+  for (int i = 0; i < 8; ++i) u[i] = kv_clamp(v[i] * inv);
+  return e4m3_encode8(u);
 }
 
-__device__ __forceinline__ uint8_t kv_rescale(uint8_t c, float ratio) {
-  const float v = __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * ratio;
-  return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false);
+// Four codes times ratio, rounded again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t c, float ratio) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a[0] * ratio, a[1] * ratio, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * ratio, b[1] * ratio, w, true);
 }
 
-// One workgroup per (touched page, head). It takes the page's scales from the rows that
-// fall into it, moves the codes held to a larger scale where it has to, and writes the
-// rows' codes: K as they come, V through LDS, transposed. Bound by HBM for prompts, by
-// latency for single tokens.
-template <int DT>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, KvRows v,
-                                                       KvBatch q, int64_t rows, const int* filled) {
-  extern __shared__ __align__(16) uint8_t tile[];  // [n][d + 4]: V codes by token
-  __shared__ float red[4];
-  const int h = (int)(blockIdx.x % c.heads);
+// A 16-token slab of V passes through LDS as dwords of four columns, [d / 4][16 tokens] at
+// this pitch in dwords: rows stay 16-byte aligned and neighbouring rows 20 banks apart.
+constexpr int kSlabPitch = 20;
+constexpr int kSlabLds = 256 / 4 * kSlabPitch;  // dwords of a wave
+
+// Four dwords of four bytes, transposed: out[i] byte j = in[j] byte i.
+__device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(in[1], in[0], 0x05010400u), b = __builtin_amdgcn_perm(in[1], in[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(in[3], in[2], 0x05010400u), e = __builtin_amdgcn_perm(in[3], in[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(e, b, 0x07060302u);
+}
+
+// One wave per (touched page, head), so nothing waits for another wave. It takes the page's
+// scales from the rows that fall into it, moves the codes held to a larger scale where it has
+// to, and writes the rows' codes: K as they come, V transposed through LDS a slab of 16
+// tokens at a time. Bound by HBM for prompts, by latency for single tokens.
+//
+// KEEP: pages of 16 tokens and d up to 128, whose values stay in registers between the scale
+// and the codes; larger ones are read twice, the second time from the L2.
+template <int DT, bool KEEP>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, KvRows v, KvBatch q, int64_t rows,
+                                                       const int* filled) {
+  __shared__ __align__(16) uint32_t slabs[4][kSlabLds];
+  typedef typename Elem<DT>::T T;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t* slab = slabs[wave];
+  const int at = (int)blockIdx.x * 4 + wave, h = at % c.heads;
   int b, item, n_b;
   int64_t row0;
-  const bool ok = kv_locate(
-      q, (int)(blockIdx.x / c.heads),
-      [&](int s, int n) { return n ? (max(filled[s], 0) % c.block + n + c.block - 1) / c.block : 0; },
-      &b, &item, &row0, &n_b);
-  if (!ok) return;
+  if (!kv_locate(
+          q, at / c.heads,
+          [&](int s, int n) { return n ? (max(filled[s], 0) % c.block + n + c.block - 1) / c.block : 0; }, &b, &item,
+          &row0, &n_b))
+    return;
   const int held = max(filled[b], 0);
-  const int64_t pg = (int64_t)held / c.block + item;  // page of the sequence
-  const int s0 = item == 0 ? held % c.block : 0;      // first slot written
+  const int64_t pg = (int64_t)held / c.block + item;                 // page of the sequence
+  const int s0 = item == 0 ? held % c.block : 0;                     // first slot written
   const int done = item == 0 ? 0 : item * c.block - held % c.block;  // rows in earlier pages
   const int n = min(n_b - done, c.block - s0);
   const int64_t r0 = row0 + done;
@@ -117,113 +119,183 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, 
   const int page = c.table[(int64_t)b * c.max_pages + pg];
   if ((unsigned)page >= (unsigned)c.pages) return;
   const int64_t ph = (int64_t)page * c.heads + h;
-  const int d = c.d, blk = c.block, dc = d / 8;
+  const int d = c.d, blk = c.block, dc = d / 8, total = n * dc;
   uint8_t* kc = c.k + ph * blk * d;
   uint8_t* vc = c.v + ph * blk * d;
+  const T* kp = (const T*)k.p + r0 * k.row_st + h * k.head_st;
+  const T* vp = (const T*)v.p + r0 * v.row_st + h * v.head_st;
 
-  const float ka = block_max(kv_amax<DT>(k, r0, n, h, d), red);
-  const float va = block_max(kv_amax<DT>(v, r0, n, h, d), red);
-  float ks = kv_scale(ka), vs = kv_scale(va);
+  constexpr int CH = KEEP ? 4 : 1;
+  float kv[CH][8], vv[CH][8];
+  float ka = 0.0f, va = 0.0f;
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int i = lane + 64 * u, row = i / dc, col = 8 * (i - row * dc);
+      if (i < total) {
+        load8<DT>(kp + row * k.row_st + col, kv[u]);
+        load8<DT>(vp + row * v.row_st + col, vv[u]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) kv[u][x] = vv[u][x] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < CH; ++u) ka = amax8(kv[u], ka), va = amax8(vv[u], va);
+  } else {
+#pragma unroll 4
+    for (int i = lane; i < total; i += 64) {
+      const int row = i / dc, col = 8 * (i - row * dc);
+      load8<DT>(kp + row * k.row_st + col, kv[0]);
+      load8<DT>(vp + row * v.row_st + col, vv[0]);
+      ka = amax8(kv[0], ka);
+      va = amax8(vv[0], va);
+    }
+  }
+  float ks = kv_scale(wave_max(ka)), vs = kv_scale(wave_max(va)), vratio = 1.0f;
   if (s0 > 0) {  // codes held: keep the larger scale
     const float ko = c.k_scale[ph], vo = c.v_scale[ph];
     if (ks > ko) {
       const float ratio = ko * inv_pow2(ks);
-      for (int i = threadIdx.x; i < s0 * d; i += 256) kc[i] = kv_rescale(kc[i], ratio);
+      for (int i = lane; i < s0 * d / 4; i += 64) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(kc) + i;
+        *p = rescale4(*p, ratio);
+      }
     } else {
       ks = ko;
     }
-    if (vs > vo) {
-      const float ratio = vo * inv_pow2(vs);
-      for (int i = threadIdx.x; i < s0 * d; i += 256) {
-        const int at = i / s0 * blk + i % s0;
-        vc[at] = kv_rescale(vc[at], ratio);
-      }
-    } else {
-      vs = vo;
-    }
+    if (vs > vo) vratio = vo * inv_pow2(vs);
+    else vs = vo;
   }
-  __syncthreads();  // every thread has read the old scales
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     c.k_scale[ph] = ks;
     c.v_scale[ph] = vs;
   }
-  typedef typename Elem<DT>::T T;
-  const T* kp = (const T*)k.p + r0 * k.row_st + h * k.head_st;
-  const T* vp = (const T*)v.p + r0 * v.row_st + h * v.head_st;
   const float ki = inv_pow2(ks), vi = inv_pow2(vs);
-  const int pitch = d + 4;
-  for (int i = threadIdx.x; i < n * dc; i += 256) {
-    const int row = i / dc, col = 8 * (i - row * dc);
-    *reinterpret_cast<u32x2*>(kc + (int64_t)(s0 + row) * d + col) = kv_codes<DT>(kp + row * k.row_st + col, ki);
-    const u32x2 cv = kv_codes<DT>(vp + row * v.row_st + col, vi);
-    *reinterpret_cast<uint32_t*>(tile + row * pitch + col) = cv[0];
-    *reinterpret_cast<uint32_t*>(tile + row * pitch + col + 4) = cv[1];
-  }
-  __syncthreads();
-  const int groups = blk / 16;
-  for (int i = threadIdx.x; i < d * groups; i += 256) {
-    const int col = i % d, g = i / d;
-    const int lo = max(s0, 16 * g), hi = min(s0 + n, 16 * g + 16);
-    if (lo >= hi) continue;
-    uint8_t* out = vc + (int64_t)col * blk + 16 * g;
-    if (hi - lo == 16) {
-      u32x4 w = {0, 0, 0, 0};
+  // slabs with a row written, and, where codes move, the ones before
+  const int g0 = vratio != 1.0f ? 0 : s0 / 16, g1 = (s0 + n + 15) / 16;
+  for (int g = g0; g < g1; ++g) {
+    const int lo = max(s0 - 16 * g, 0), hi = min(s0 + n - 16 * g, 16);  // slots of the slab written
+    // rows of this slab: lo .. hi - 1, from row 16 g + lo - s0
+    const int first = 16 * g + lo - s0, cnt = max(hi - lo, 0) * dc;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) w[j / 4] |= (uint32_t)tile[(16 * g + j - s0) * pitch + col] << (8 * (j % 4));
-      *reinterpret_cast<u32x4*>(out) = w;
-    } else {
-      for (int j = lo; j < hi; ++j) out[j - 16 * g] = tile[(j - s0) * pitch + col];
+    for (int u = 0; u < 8; ++u) {
+      if (KEEP && u >= CH) break;
+      const int i = lane + 64 * u;
+      if (i >= cnt) break;
+      const int row = i / dc, cc = i - row * dc;
+      if constexpr (!KEEP) {
+        load8<DT>(kp + (first + row) * k.row_st + 8 * cc, kv[0]);
+        load8<DT>(vp + (first + row) * v.row_st + 8 * cc, vv[0]);
+      }
+      *reinterpret_cast<u32x2*>(kc + (int64_t)(16 * g + lo + row) * d + 8 * cc) = codes8(kv[KEEP ? u : 0], ki);
+      const u32x2 w = codes8(vv[KEEP ? u : 0], vi);
+      slab[2 * cc * kSlabPitch + lo + row] = w[0];
+      slab[(2 * cc + 1) * kSlabPitch + lo + row] = w[1];
     }
+    __builtin_amdgcn_wave_barrier();
+    // four columns a lane: 16 tokens of each
+    if (lane < d / 4) {
+      uint8_t* out = vc + (int64_t)(4 * lane) * blk + 16 * g;
+      u32x4 w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const u32x4 r = *reinterpret_cast<const u32x4*>(slab + lane * kSlabPitch + 4 * x);
+        const uint32_t in[4] = {r[0], r[1], r[2], r[3]};
+        uint32_t t[4];
+        transpose4(in, t);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w[y][x] = t[y];
+      }
+      if (lo > 0 || hi < 16) {  // the other slots keep their codes, the held ones moved
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          u32x4 old = *reinterpret_cast<const u32x4*>(out + y * blk);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t put = 0, move = 0;  // bytes written, bytes held before
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int slot = 4 * x + e;
+              put |= slot >= lo && slot < hi ? 0xFFu << (8 * e) : 0;
+              move |= 16 * g + slot < s0 ? 0xFFu << (8 * e) : 0;
+            }
+            uint32_t o = old[x];
+            if (vratio != 1.0f) o = (o & ~move) | (rescale4(o, vratio) & move);
+            w[y][x] = (o & ~put) | (w[y][x] & put);
+          }
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) *reinterpret_cast<u32x4*>(out + y * blk) = w[y];
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// One workgroup per (page held, head): the codes' values in rows [total][head][d].
+// One wave per (16 tokens held, head): the codes' values in rows [total][head][d]. V's slab
+// is transposed through LDS.
 template <int DT>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvCacheArgs c, KvBatch q, int64_t total,
                                                       typename Elem<DT>::T* __restrict__ ko,
                                                       typename Elem<DT>::T* __restrict__ vo) {
-  extern __shared__ __align__(16) uint8_t tile[];  // [block][d + 4]
-  const int h = (int)(blockIdx.x % c.heads);
+  __shared__ __align__(16) uint32_t slabs[4][kSlabLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t* slab = slabs[wave];
+  const int at = (int)blockIdx.x * 4 + wave, h = at % c.heads;
   int b, item, n_b;
   int64_t row0;
-  if (!kv_locate(q, (int)(blockIdx.x / c.heads),
-                 [&](int, int n) { return (n + c.block - 1) / c.block; }, &b, &item, &row0, &n_b))
-    return;
-  const int n = min(n_b - item * c.block, c.block);
-  const int64_t r0 = row0 + (int64_t)item * c.block;
+  if (!kv_locate(q, at / c.heads, [&](int, int n) { return (n + 15) / 16; }, &b, &item, &row0, &n_b)) return;
+  const int n = min(n_b - item * 16, 16);
+  const int64_t r0 = row0 + (int64_t)item * 16;
   if (r0 < 0 || r0 + n > total) return;
-  const int page = item < c.max_pages ? c.table[(int64_t)b * c.max_pages + item] : -1;
+  const int64_t pg = (int64_t)item * 16 / c.block;
+  const int page = pg < c.max_pages ? c.table[(int64_t)b * c.max_pages + pg] : -1;
   const bool have = (unsigned)page < (unsigned)c.pages;
   const int64_t ph = have ? (int64_t)page * c.heads + h : 0;
-  const int d = c.d, blk = c.block, dc = d / 8, pitch = d + 4;
-  const uint8_t* kc = c.k + ph * blk * d;
-  const uint8_t* vc = c.v + ph * blk * d;
+  const int d = c.d, blk = c.block, dc = d / 8, slot = item * 16 % blk;
+  const uint8_t* kc = c.k + ph * blk * d + slot * d;
+  const uint8_t* vc = c.v + ph * blk * d + slot;
   const float ks = have ? c.k_scale[ph] : 0.0f, vs = have ? c.v_scale[ph] : 0.0f;
-  for (int i = threadIdx.x; i < d * (blk / 16); i += 256) {
-    const int col = i % d, g = i / d;
-    if (16 * g >= n) continue;
-    u32x4 w = {0, 0, 0, 0};
-    if (have) w = *reinterpret_cast<const u32x4*>(vc + (int64_t)col * blk + 16 * g);
+  u32x4 w[4];
+  if (lane < d / 4) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) tile[(16 * g + j) * pitch + col] = (uint8_t)(w[j / 4] >> (8 * (j % 4)));
+    for (int y = 0; y < 4; ++y) w[y] = *reinterpret_cast<const u32x4*>(vc + (int64_t)(4 * lane + y) * blk);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * dc; i += 256) {
-    const int row = i / dc, col = 8 * (i - row * dc);
-    const int64_t at = ((r0 + row) * c.heads + h) * d + col;
-    u32x2 cd = {0, 0};
-    if (have) cd = *reinterpret_cast<const u32x2*>(kc + (int64_t)row * d + col);
+  u32x2 kk[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int i = lane + 64 * u;
+    if (i < n * dc) kk[u] = *reinterpret_cast<const u32x2*>(kc + 8 * i);
+  }
+  if (lane < d / 4) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t in[4] = {w[0][x], w[1][x], w[2][x], w[3][x]};
+      uint32_t t[4];
+      transpose4(in, t);
+      *reinterpret_cast<u32x4*>(slab + lane * kSlabPitch + 4 * x) = u32x4{t[0], t[1], t[2], t[3]};
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int i = lane + 64 * u;
+    if (i >= n * dc) break;
+    const int row = i / dc, cc = i - row * dc;
+    const int64_t to = ((r0 + row) * c.heads + h) * d + 8 * cc;
     float f[8];
-    e4m3_decode8(cd, f);
+    // no page: codes of page 0 were read, and 0 is what they stand for
+    const u32x2 zero = {0, 0};
+    e4m3_decode8(have ? kk[u] : zero, f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] *= ks;
-    store8<DT>(ko + at, f);
-    cd[0] = *reinterpret_cast<const uint32_t*>(tile + row * pitch + col);
-    cd[1] = *reinterpret_cast<const uint32_t*>(tile + row * pitch + col + 4);
-    e4m3_decode8(cd, f);
+    store8<DT>(ko + to, f);
+    const u32x2 cd = {slab[2 * cc * kSlabPitch + row], slab[(2 * cc + 1) * kSlabPitch + row]};
+    e4m3_decode8(have ? cd : zero, f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] *= vs;
-    store8<DT>(vo + at, f);
+    store8<DT>(vo + to, f);
   }
 }
 
@@ -283,16 +355,22 @@ int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t 
   if (int s = cp::kv_check_rows(v, es, v_row, v_head, "v")) return s;
   // pages touched: ceil((filled % block + n) / block) summed over the sequences
   const int64_t items = offsets ? rows / cache->block + 2 * batch : batch;
-  if (items * cache->heads > 0x7FFFFFFF) return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  if (items * cache->heads > 0x7FFFFF00) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvRows kr = {k, k_row, k_head}, vr = {v, v_row, v_head};
   const cp::KvBatch q = {offsets, (int)batch};
-  const dim3 grid((unsigned)(items * cache->heads));
-  const size_t lds = (size_t)cache->block * (cache->head_dim + 4);
+  const dim3 grid((unsigned)((items * cache->heads + 3) / 4));
+  const bool keep = cache->block == 16 && cache->head_dim <= 128;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CP_F32) cp::kv_write_kernel<CP_F32><<<grid, 256, lds, st>>>(a, kr, vr, q, rows, filled);
-  if (dtype == CP_BF16) cp::kv_write_kernel<CP_BF16><<<grid, 256, lds, st>>>(a, kr, vr, q, rows, filled);
-  if (dtype == CP_F16) cp::kv_write_kernel<CP_F16><<<grid, 256, lds, st>>>(a, kr, vr, q, rows, filled);
+#define CP_KV_WRITE(DT)                                                              \
+  if (dtype == DT) {                                                                 \
+    if (keep) cp::kv_write_kernel<DT, true><<<grid, 256, 0, st>>>(a, kr, vr, q, rows, filled); \
+    else cp::kv_write_kernel<DT, false><<<grid, 256, 0, st>>>(a, kr, vr, q, rows, filled);     \
+  }
+  CP_KV_WRITE(CP_F32)
+  CP_KV_WRITE(CP_BF16)
+  CP_KV_WRITE(CP_F16)
+#undef CP_KV_WRITE
   CP_LAUNCHED("cache write");
   return CP_OK;
 }
@@ -307,16 +385,15 @@ int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, in
   if (!offsets) return cp::set_error(CP_ERR_ARG, "null offsets");
   if (!k || !v) return cp::set_error(CP_ERR_ARG, "null k / v");
   if (!cp::aligned(k, 16) || !cp::aligned(v, 16)) return cp::set_error(CP_ERR_ALIGN, "k and v need 16-byte alignment");
-  const int64_t items = total / cache->block + batch;
-  if (items * cache->heads > 0x7FFFFFFF) return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  const int64_t items = total / 16 + batch;
+  if (items * cache->heads > 0x7FFFFF00) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvBatch q = {offsets, (int)batch};
-  const dim3 grid((unsigned)(items * cache->heads));
-  const size_t lds = (size_t)cache->block * (cache->head_dim + 4);
+  const dim3 grid((unsigned)((items * cache->heads + 3) / 4));
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CP_F32) cp::kv_read_kernel<CP_F32><<<grid, 256, lds, st>>>(a, q, total, (float*)k, (float*)v);
-  if (dtype == CP_BF16) cp::kv_read_kernel<CP_BF16><<<grid, 256, lds, st>>>(a, q, total, (__bf16*)k, (__bf16*)v);
-  if (dtype == CP_F16) cp::kv_read_kernel<CP_F16><<<grid, 256, lds, st>>>(a, q, total, (_Float16*)k, (_Float16*)v);
+  if (dtype == CP_F32) cp::kv_read_kernel<CP_F32><<<grid, 256, 0, st>>>(a, q, total, (float*)k, (float*)v);
+  if (dtype == CP_BF16) cp::kv_read_kernel<CP_BF16><<<grid, 256, 0, st>>>(a, q, total, (__bf16*)k, (__bf16*)v);
+  if (dtype == CP_F16) cp::kv_read_kernel<CP_F16><<<grid, 256, 0, st>>>(a, q, total, (_Float16*)k, (_Float16*)v);
   CP_LAUNCHED("cache read");
   return CP_OK;
 }
