@@ -14,6 +14,7 @@
 // Slots that no row is written to keep their codes.
 #include <hip/hip_runtime.h>
 
+#include "cp_device.h"
 #include "kvcache.h"
 #include "lowbit.h"
 
@@ -35,11 +36,14 @@ __device__ __forceinline__ float kv_clamp(float v) {
   return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f);
 }
 
-// Largest of v over the wave.
+// Largest of v over the wave (all lanes active): within 16 lanes on the VALU, then across.
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int s = 32; s >= 1; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
-  return v;
+  v = fmaxf(v, dpp<kDppXor1>(v));
+  v = fmaxf(v, dpp<kDppXor2>(v));
+  v = fmaxf(v, dpp<kDppHalfMirror>(v));
+  v = fmaxf(v, dpp<kDppRor8>(v));
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
 }
 
 struct KvRows {
@@ -72,6 +76,11 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t c, float ratio) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[0] * ratio, b[1] * ratio, w, true);
 }
 
+// The low n bytes of a dword (none for n <= 0, all for n >= 4).
+__device__ __forceinline__ uint32_t low_bytes(int n) {
+  return n <= 0 ? 0u : n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+}
+
 // A 16-token slab of V passes through LDS as dwords of four columns, [d / 4][16 tokens] at
 // this pitch in dwords: rows stay 16-byte aligned and neighbouring rows 20 banks apart.
 constexpr int kSlabPitch = 20;
@@ -95,7 +104,7 @@ __device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&o
 // KEEP: pages of 16 tokens and d up to 128, whose values stay in registers between the scale
 // and the codes; larger ones are read twice, the second time from the L2.
 template <int DT, bool KEEP>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, KvRows v, KvBatch q, int64_t rows,
+__global__ __launch_bounds__(256, KEEP ? 4 : 3) void kv_write_kernel(KvCacheArgs c, KvRows k, KvRows v, KvBatch q, int64_t rows,
                                                        const int* filled) {
   __shared__ __align__(16) uint32_t slabs[4][kSlabLds];
   typedef typename Elem<DT>::T T;
@@ -125,36 +134,47 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, 
   const T* kp = (const T*)k.p + r0 * k.row_st + h * k.head_st;
   const T* vp = (const T*)v.p + r0 * v.row_st + h * v.head_st;
 
+  // asked for before they are needed: the scales of the codes held, and (KEEP) the codes of V
+  const float ko = c.k_scale[ph], vo = c.v_scale[ph];
   constexpr int CH = KEEP ? 4 : 1;
-  float kv[CH][8], vv[CH][8];
+  Raw8<DT> kv[CH], vv[CH];
   float ka = 0.0f, va = 0.0f;
+  if constexpr (KEEP) {
+    // lanes past the rows repeat the last one's values, which changes no maximum
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int i = min(lane + 64 * u, total - 1), row = i / dc, col = 8 * (i - row * dc);
+      kv[u] = load_raw8<DT>(kp + row * k.row_st + col);
+      vv[u] = load_raw8<DT>(vp + row * v.row_st + col);
+    }
+  }
+  u32x4 old[4];
+  const bool partial = KEEP && n < 16;
+  if (partial && lane < d / 4) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y) old[y] = *reinterpret_cast<const u32x4*>(vc + (4 * lane + y) * blk);
+  }
+  float f[8];
   if constexpr (KEEP) {
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
-      const int i = lane + 64 * u, row = i / dc, col = 8 * (i - row * dc);
-      if (i < total) {
-        load8<DT>(kp + row * k.row_st + col, kv[u]);
-        load8<DT>(vp + row * v.row_st + col, vv[u]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < 8; ++x) kv[u][x] = vv[u][x] = 0.0f;
-      }
+      widen8<DT>(kv[u], f);
+      ka = amax8(f, ka);
+      widen8<DT>(vv[u], f);
+      va = amax8(f, va);
     }
-#pragma unroll
-    for (int u = 0; u < CH; ++u) ka = amax8(kv[u], ka), va = amax8(vv[u], va);
   } else {
 #pragma unroll 4
     for (int i = lane; i < total; i += 64) {
       const int row = i / dc, col = 8 * (i - row * dc);
-      load8<DT>(kp + row * k.row_st + col, kv[0]);
-      load8<DT>(vp + row * v.row_st + col, vv[0]);
-      ka = amax8(kv[0], ka);
-      va = amax8(vv[0], va);
+      load8<DT>(kp + row * k.row_st + col, f);
+      ka = amax8(f, ka);
+      load8<DT>(vp + row * v.row_st + col, f);
+      va = amax8(f, va);
     }
   }
   float ks = kv_scale(wave_max(ka)), vs = kv_scale(wave_max(va)), vratio = 1.0f;
   if (s0 > 0) {  // codes held: keep the larger scale
-    const float ko = c.k_scale[ph], vo = c.v_scale[ph];
     if (ks > ko) {
       const float ratio = ko * inv_pow2(ks);
       for (int i = lane; i < s0 * d / 4; i += 64) {
@@ -185,11 +205,13 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, 
       if (i >= cnt) break;
       const int row = i / dc, cc = i - row * dc;
       if constexpr (!KEEP) {
-        load8<DT>(kp + (first + row) * k.row_st + 8 * cc, kv[0]);
-        load8<DT>(vp + (first + row) * v.row_st + 8 * cc, vv[0]);
+        kv[0] = load_raw8<DT>(kp + (first + row) * k.row_st + 8 * cc);
+        vv[0] = load_raw8<DT>(vp + (first + row) * v.row_st + 8 * cc);
       }
-      *reinterpret_cast<u32x2*>(kc + (int64_t)(16 * g + lo + row) * d + 8 * cc) = codes8(kv[KEEP ? u : 0], ki);
-      const u32x2 w = codes8(vv[KEEP ? u : 0], vi);
+      widen8<DT>(kv[KEEP ? u : 0], f);
+      *reinterpret_cast<u32x2*>(kc + (int64_t)(16 * g + lo + row) * d + 8 * cc) = codes8(f, ki);
+      widen8<DT>(vv[KEEP ? u : 0], f);
+      const u32x2 w = codes8(f, vi);
       slab[2 * cc * kSlabPitch + lo + row] = w[0];
       slab[(2 * cc + 1) * kSlabPitch + lo + row] = w[1];
     }
@@ -210,17 +232,12 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, 
       if (lo > 0 || hi < 16) {  // the other slots keep their codes, the held ones moved
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          u32x4 old = *reinterpret_cast<const u32x4*>(out + y * blk);
+          if constexpr (!KEEP) old[y] = *reinterpret_cast<const u32x4*>(out + y * blk);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            uint32_t put = 0, move = 0;  // bytes written, bytes held before
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int slot = 4 * x + e;
-              put |= slot >= lo && slot < hi ? 0xFFu << (8 * e) : 0;
-              move |= 16 * g + slot < s0 ? 0xFFu << (8 * e) : 0;
-            }
-            uint32_t o = old[x];
+            // bytes written, and bytes held before
+            const uint32_t put = low_bytes(hi - 4 * x) & ~low_bytes(lo - 4 * x), move = low_bytes(s0 - 16 * g - 4 * x);
+            uint32_t o = old[y][x];
             if (vratio != 1.0f) o = (o & ~move) | (rescale4(o, vratio) & move);
             w[y][x] = (o & ~put) | (w[y][x] & put);
           }
@@ -236,7 +253,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvCacheArgs c, KvRows k, 
 // One wave per (16 tokens held, head): the codes' values in rows [total][head][d]. V's slab
 // is transposed through LDS.
 template <int DT>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvCacheArgs c, KvBatch q, int64_t total,
+__global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch q, int64_t total,
                                                       typename Elem<DT>::T* __restrict__ ko,
                                                       typename Elem<DT>::T* __restrict__ vo) {
   __shared__ __align__(16) uint32_t slabs[4][kSlabLds];

@@ -23,15 +23,28 @@ template <> struct Elem<CP_F16> { typedef _Float16 T; };
 
 inline int dtype_bytes(int dt) { return dt == CP_F32 ? 4 : dt == CP_BF16 || dt == CP_F16 ? 2 : 0; }
 
-// Eight consecutive values as float32 (p 16-byte aligned).
+// Eight consecutive values as they are stored.
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&v)[8]) {
+struct Raw8 {
+  u32x4 w[DT == CP_F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8(const typename Elem<DT>::T* p) {
+  Raw8<DT> r;
+  r.w[0] = *reinterpret_cast<const u32x4*>(p);
+  if constexpr (DT == CP_F32) r.w[1] = *reinterpret_cast<const u32x4*>(p + 4);
+  return r;
+}
+
+// ... and as float32.
+template <int DT>
+__device__ __forceinline__ void widen8(const Raw8<DT>& raw, float (&v)[8]) {
   if constexpr (DT == CP_F32) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i], v[i + 4] = b[i];
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(raw.w[0][i]), v[i + 4] = __uint_as_float(raw.w[1][i]);
   } else {
-    const u32x4 r = *reinterpret_cast<const u32x4*>(p);
+    const u32x4 r = raw.w[0];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (DT == CP_BF16) {
@@ -45,6 +58,12 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&v)[
       }
     }
   }
+}
+
+// Eight consecutive values as float32 (p 16-byte aligned).
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&v)[8]) {
+  widen8<DT>(load_raw8<DT>(p), v);
 }
 
 // Two float32 rounded to nearest even in a 16-bit type, packed.
