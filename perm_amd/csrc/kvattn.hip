@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kvcache.h"
 #include "lowbit.h"
@@ -381,11 +382,17 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 
 constexpr int kManyRows = 128;
 
+template <class F>
+__device__ __forceinline__ void unrolled2(F f) {
+  f(std::integral_constant<int, 0>{});
+  f(std::integral_constant<int, 1>{});
+}
+
 template <int DT, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items) {
   constexpr int NC = DP / 32, NL = DP / 64;          // 32-column chunks; direct loads of a wave for K, and for V
   constexpr int KB = kTile * DP, BUF = 2 * KB;       // bytes of a K (or V) tile, of a buffer
-  extern __shared__ __align__(16) uint8_t lds[];     // [2][BUF]
+  extern __shared__ __align__(16) uint8_t lds[];     // [3][BUF], then [4 waves][NC][64 lanes][16]
   const KvCacheArgs& c = a.c;
   const int h = (int)(blockIdx.x % c.heads);
   const int split = (int)(blockIdx.x / c.heads % a.splits);
@@ -469,8 +476,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   constexpr int CH = DP / 16;
   const int kt = 16 * wave + lane / CH;                       // + 1024 / DP per load
   const int vg = (lane & 3) ^ ((lane >> 4) & 3);
-  auto fetch = [&](int tile, int pk, int pv) {
-    uint8_t* to = lds + (tile & 1) * BUF;
+  auto fetch = [&](int into, int tile, int pk, int pv) {
+    uint8_t* to = lds + into * BUF;
     const int j0 = tile * kTile;
     // no page: page 0's codes, which no row sees
     const uint8_t* kp = c.k + ((int64_t)((unsigned)pk < (unsigned)c.pages ? pk : 0) * c.heads + h) * blk * d;
@@ -509,172 +516,173 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   };
   float ks[2], vs[2], nks[2], nvs[2];
   bool have[2], nhave[2];
-  auto next_scales = [&] {
+  auto next_scales = [&](const int (&pg)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      nhave[s] = (unsigned)pn.g[s] < (unsigned)c.pages;
-      const int64_t hv = (int64_t)(nhave[s] ? pn.g[s] : 0) * c.heads + h;
+      nhave[s] = (unsigned)pg[s] < (unsigned)c.pages;
+      const int64_t hv = (int64_t)(nhave[s] ? pg[s] : 0) * c.heads + h;
       nks[s] = c.k_scale[hv];
       nvs[s] = c.v_scale[hv];
     }
   };
+  // A tile is two units of 32 tokens. A unit's scores are multiplied while the weights of the
+  // unit before it are computed, so that the matrix cores and the VALU overlap within a wave.
+  f32x16 sc[2];
+  u32x4 kr[NC], vr[NC];
+  auto read_k = [&](int buf, int s, int k) {
+    kr[k] = *reinterpret_cast<const u32x4*>(lds + buf * BUF + token * DP + s * 32 * DP + ((32 * k + 16 * hh) ^ ksw));
+  };
+  auto read_v = [&](int buf, int s, int i) {
+    vr[i] = *reinterpret_cast<const u32x4*>(lds + buf * BUF + KB + q * 64 + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
+  };
+  auto scores = [&](int s) {  // of the unit whose K is in kr
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[s][j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[s]);
+      sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[s]);
+    }
+  };
+  uint64_t marked[NC > 4 ? 2 : 1] = {};  // bit 16 i + j (of a word for four i): result (i, j) has seen a NaN code
+  int buf = 0, nbuf = 1;                 // buffers of this tile and the next
+  int pg[2] = {0, 0};  // pages of the next tile's scales
   if (tb < te) {
     lookup(tb);
-    fetch(tb, pn.k, pn.v);
-    next_scales();
+    fetch(0, tb, pn.k, pn.v);
+    next_scales(pn.g);
     lookup(tb + 1);
+    fetch(1, tb + 1, pn.k, pn.v);
+    pg[0] = pn.g[0], pg[1] = pn.g[1];
+    lookup(tb + 2);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NC; ++k) read_k(0, 0, k);
+    scores(0);
   }
   for (int tile = tb; tile < te; ++tile) {
-    __syncthreads();  // this tile has landed, and every wave is done with the one before
+    const int j0 = tile * kTile;
 #pragma unroll
     for (int s = 0; s < 2; ++s) ks[s] = nks[s], vs[s] = nvs[s], have[s] = nhave[s];
     const bool all = !__any(!have[0] || !have[1]);
-    if (tile + 1 < te) {
-      fetch(tile + 1, pn.k, pn.v);
-      next_scales();
-      lookup(tile + 2);
-    }
-    const uint8_t* lk = lds + (tile & 1) * BUF + token * DP;
-    const uint8_t* lv = lds + (tile & 1) * BUF + KB + q * 64;
-    const int j0 = tile * kTile;
-    // LDS reads run one 32-column chunk ahead of their conversion; the barriers keep the
-    // compiler from hoisting every read, which spills
-    f32x16 sc[2];
-    u32x4 kr[2][2], vr[2][2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sc[s][j] = 0.0f;
-      kr[0][s] = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((16 * hh) ^ ksw));
-    }
-    auto read_v = [&](int i, int s) {
-      return *reinterpret_cast<const u32x4*>(lv + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
-    };
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (k + 1 < NC)
-          kr[(k + 1) & 1][s] = *reinterpret_cast<const u32x4*>(lk + s * 32 * DP + ((32 * (k + 1) + 16 * hh) ^ ksw));
-        else
-          vr[0][s] = read_v(0, s);
+    const bool edge = !all || j0 < wlo || j0 + kTile > whi;
+    const int last = nbuf == 2 ? 0 : nbuf + 1;  // the tile before this one's: the one after the next's
+    unrolled2([&](auto S) {
+      constexpr int s = S;
+      const float kc = ks[s] * a.scale;
+      const float lg = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
+      const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
+      if constexpr (s == 1) {
+        __syncthreads();  // the next tile has landed, and every wave is done with the one before this
+        next_scales(pg);
+        pg[0] = pn.g[0], pg[1] = pn.g[1];
+        fetch(last, tile + 2, pn.k, pn.v);  // past the end: some page's codes, never used
+        lookup(tile + 3);
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k & 1][s][0], kr[k & 1][s][1]), qf[k][0], sc[s]);
+      for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
+      if (edge) {
+        // this lane's first token, hidden from the compiler: it would compare all of them on
+        // every tile, ahead of the branch
+        int j1 = j0 + 32 * s + 16 * hh;
+        asm volatile("" : "+v"(j1));
 #pragma unroll
-      for (int s = 0; s < 2; ++s) sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k & 1][s][2], kr[k & 1][s][3]), qf[k][1], sc[s]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    float kc[2], lg[2], iv[2];
+        for (int i = 0; i < 16; ++i) sc[s][i] = have[s] && j1 + i >= lo && j1 + i < hi ? sc[s][i] : kNegInf;
+      }
+      // the largest t of the unit: kc > 0, so t rises with the raw score
+      float tm = sc[s][0];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      kc[s] = ks[s] * a.scale;
-      lg[s] = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
-      iv[s] = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
-    }
-    const bool edge = !all || j0 < wlo || j0 + kTile > whi;
-    if (edge) {
-      // this lane's first token, hidden from the compiler: it would compare all 32 on every
-      // tile, ahead of the branch
-      int j1 = j0 + 16 * hh;
-      asm volatile("" : "+v"(j1));
+      for (int i = 1; i < 16; ++i) tm = fmaxf(tm, sc[s][i]);
+      tm = __builtin_fmaf(tm, kc, lg);
+      tm = fmaxf(tm, __shfl_xor(tm, 32));
+      // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
+      // the outputs are then seldom rescaled
+      if (__any(tm > m + 8.0f)) {
+        const float mn = fmaxf(m, tm);
+        const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
+        m = mn;
+        l *= al;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < NC; ++i) o[i] *= al;
+      }
+      const float off = lg - (m == kNegInf ? 0.0f : m);
+      scores(1 - s);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = j1 + 32 * s + i;
-          sc[s][i] = have[s] && j >= lo && j < hi ? sc[s][i] : kNegInf;
-        }
-    }
-    // the largest t of the tile: kc > 0, so t rises with the raw score
-    float tm = kNegInf;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float x = sc[s][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) x = fmaxf(x, sc[s][i]);
-      tm = fmaxf(tm, __builtin_fmaf(x, kc[s], lg[s]));
-    }
-    tm = fmaxf(tm, __shfl_xor(tm, 32));
-    // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
-    // the outputs are then seldom rescaled
-    if (__any(tm > m + 8.0f)) {
-      const float mn = fmaxf(m, tm);
-      const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
-      m = mn;
-      l *= al;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) o[i] *= al;
-    }
-    const float ms = m == kNegInf ? 0.0f : m;
-    u32x4 w[2][2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const float off = lg[s] - ms;
+      for (int i = 0; i < NC; ++i) read_v(buf, s, i);
+      u32x4 w[2];
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float e0 = exp2_fast(__builtin_fmaf(sc[s][i], kc[s], off));
-        const float e1 = exp2_fast(__builtin_fmaf(sc[s][i + 1], kc[s], off));
+        const float e0 = exp2_fast(__builtin_fmaf(sc[s][i], kc, off));
+        const float e1 = exp2_fast(__builtin_fmaf(sc[s][i + 1], kc, off));
         sum += e0 + e1;
-        w[s][i >> 3][(i >> 1) & 3] = pack2<CP_F16>(e0, e1);
+        w[i >> 3][(i >> 1) & 3] = pack2<CP_F16>(e0, e1);
       }
-      l = __builtin_fmaf(sum, iv[s], l);
-    }
-    bool nan = false;
-    if (edge) {
-      uint32_t any = 0;
+      l = __builtin_fmaf(sum, iv, l);
+      if (edge) {
+        uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const u32x4 x = read_v(i, s);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) any |= nan_flags(x[k]);
-        }
-      nan = __any(any != 0);
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      if (i + 1 < NC) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) vr[(i + 1) & 1][s] = read_v(i + 1, s);
-      }
-      if (nan) {
-        // as in attn_few_kernel: NaN codes leave the product and return to the rows that see them
-        f32x16 cnt;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
-        int j1 = j0 + 16 * hh;
-        asm volatile("" : "+v"(j1));
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4 f, one[2];
+          for (int k = 0; k < 4; ++k) any |= nan_flags(vr[i][k]);
+        if (__any(any != 0)) {
+          // as in attn_few_kernel: NaN codes leave the product and return to the rows that see
+          // them, in a loop over the wave's LDS that costs the common path no registers
+          u32x4* const mine = reinterpret_cast<u32x4*>(lds + 3 * BUF) + wave * NC * 64 + lane;
+          u32x4 one[2];
+          int j1 = j0 + 32 * s + 16 * hh;
+          asm volatile("" : "+v"(j1));
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const int j = j1 + 32 * s + 2 * k;
+            const int j = j1 + 2 * k;
             one[k >> 2][k & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
                                  (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t fl = nan_flags(vr[i & 1][s][k]) >> 7;
-            vr[i & 1][s][k] &= ~(fl * 0xFFu);
-            f[k] = fl * 0x38u;  // 1.0 where the code was NaN
+          for (int i = 0; i < NC; ++i) mine[64 * i] = vr[i];
+#pragma unroll
+          for (int i0 = 0; i0 < NC; i0 += 4) {
+#pragma clang loop unroll(disable)
+            for (int i = i0; i < min(NC, i0 + 4); ++i) {
+              u32x4 x = mine[64 * i], f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t fl = nan_flags(x[k]) >> 7;
+                x[k] &= ~(fl * 0xFFu);
+                f[k] = fl * 0x38u;  // 1.0 where the code was NaN
+              }
+              mine[64 * i] = x;
+              f32x16 cnt;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
+              cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[0], cnt);
+              cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[1], cnt);
+              uint32_t bits = 0;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) bits |= cnt[j] > 0.0f ? 1u << j : 0;
+              marked[i0 >> 2] |= (uint64_t)bits << (16 * (i - i0));
+            }
           }
-          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[0], cnt);
-          cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[1], cnt);
+#pragma unroll
+          for (int i = 0; i < NC; ++i) vr[i] = mine[64 * i];
         }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[i][j] = cnt[j] > 0.0f ? __builtin_nanf("") : o[i][j];
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 x = vr[i & 1][s];
-        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[0], x[1]), w[s][0], o[i]);
-        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(x[2], x[3]), w[s][1], o[i]);
+      for (int i = 0; i < NC; ++i) {
+        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(vr[i][0], vr[i][1]), w[0], o[i]);
+        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(vr[i][2], vr[i][3]), w[1], o[i]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+    });
+    buf = nbuf;
+    nbuf = last;
+  }
+  __syncthreads();  // the last fetch is in before LDS is given up
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if (__any(marked[i >> 2] != 0)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        o[i][j] = marked[i >> 2] >> (16 * (i & 3) + j) & 1 ? __builtin_nanf("") : o[i][j];
     }
   }
   l += __shfl_xor(l, 32);
@@ -796,7 +804,7 @@ template <int DT, int DP>
 static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.items * a.c.heads * a.splits));
   if (p.many) {
-    constexpr int lds = 4 * kTile * DP;
+    constexpr int lds = 6 * kTile * DP + 4 * (DP / 32) * 1024;
     static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
