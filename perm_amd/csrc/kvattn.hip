@@ -535,15 +535,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   auto read_v = [&](int buf, int s, int i) {
     vr[i] = *reinterpret_cast<const u32x4*>(lds + buf * BUF + KB + q * 64 + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
   };
-  auto scores = [&](int s) {  // of the unit whose K is in kr
-#pragma unroll
-    for (int j = 0; j < 16; ++j) sc[s][j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[s]);
-      sc[s] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[s]);
-    }
-  };
+  float top = kNegInf;  // the largest raw score of the unit at hand (this lane's half of its row)
   uint64_t marked[NC > 4 ? 2 : 1] = {};  // bit 16 i + j (of a word for four i): result (i, j) has seen a NaN code
   int buf = 0, nbuf = 1;                 // buffers of this tile and the next
   int pg[2] = {0, 0};  // pages of the next tile's scales
@@ -558,7 +550,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < NC; ++k) read_k(0, 0, k);
-    scores(0);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[0][j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
+      sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
+    }
+    top = sc[0][0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]);
   }
   for (int tile = tb; tile < te; ++tile) {
     const int j0 = tile * kTile;
@@ -588,12 +589,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         asm volatile("" : "+v"(j1));
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[s][i] = have[s] && j1 + i >= lo && j1 + i < hi ? sc[s][i] : kNegInf;
+        top = sc[s][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[s][i]);
       }
       // the largest t of the unit: kc > 0, so t rises with the raw score
-      float tm = sc[s][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) tm = fmaxf(tm, sc[s][i]);
-      tm = __builtin_fmaf(tm, kc, lg);
+      float tm = __builtin_fmaf(top, kc, lg);
       tm = fmaxf(tm, __shfl_xor(tm, 32));
       // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
       // the outputs are then seldom rescaled
@@ -606,17 +607,28 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         for (int i = 0; i < NC; ++i) o[i] *= al;
       }
       const float off = lg - (m == kNegInf ? 0.0f : m);
-      scores(1 - s);
-#pragma unroll
-      for (int i = 0; i < NC; ++i) read_v(buf, s, i);
+      // one MFMA of the next unit's scores, then as many of this unit's weights as it covers
       u32x4 w[2];
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float e0 = exp2_fast(__builtin_fmaf(sc[s][i], kc, off));
-        const float e1 = exp2_fast(__builtin_fmaf(sc[s][i + 1], kc, off));
-        sum += e0 + e1;
-        w[i >> 3][(i >> 1) & 3] = pack2<CP_F16>(e0, e1);
+      for (int j = 0; j < 16; ++j) sc[1 - s][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * NC; ++k) {
+        const u32x4 x = kr[k >> 1];
+        sc[1 - s] = mfma32<DT>(k & 1 ? codes_to_16<DT>(x[2], x[3]) : codes_to_16<DT>(x[0], x[1]), qf[k >> 1][k & 1],
+                               sc[1 - s]);
+#pragma unroll
+        for (int i = 8 * k / (2 * NC); i < 8 * (k + 1) / (2 * NC); ++i) {
+          const float e0 = exp2_fast(__builtin_fmaf(sc[s][2 * i], kc, off));
+          const float e1 = exp2_fast(__builtin_fmaf(sc[s][2 * i + 1], kc, off));
+          sum += e0 + e1;
+          w[i >> 2][i & 3] = pack2<CP_F16>(e0, e1);
+        }
+        if (k == NC) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) read_v(buf, s, i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
       l = __builtin_fmaf(sum, iv, l);
       if (edge) {
@@ -667,10 +679,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
           for (int i = 0; i < NC; ++i) vr[i] = mine[64 * i];
         }
       }
+      // the second product, and the next unit's largest score beside it
+      top = sc[1 - s][0];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(vr[i][0], vr[i][1]), w[0], o[i]);
-        o[i] = mfma32<CP_F16>(codes_to_16<CP_F16>(vr[i][2], vr[i][3]), w[1], o[i]);
+      for (int k = 0; k < 2 * NC; ++k) {
+        const int i = k % NC;
+        const u32x4 x = vr[i];
+        o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), w[k / NC], o[i]);
+#pragma unroll
+        for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j) top = fmaxf(top, sc[1 - s][j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     });
     buf = nbuf;
