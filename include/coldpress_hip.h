@@ -420,13 +420,17 @@ int cp_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t
 int cp_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k,
                       void* y, int y_dtype, void* stream);
 
-/* y [m, n] = a [m, k] b [n, k]^T of two MXFP4 arrays, summed in float32, rounded once. */
+/* Workspace bytes of cp_mx4_matmul (256-byte aligned; 0: none, ws may be NULL). */
+size_t cp_mx4_matmul_ws_bytes(int64_t m, int64_t n, int64_t k);
+
+/* y [m, n] = a [m, k] b [n, k]^T of two MXFP4 arrays, summed in float32, rounded once. The
+ * order of the sums depends on the sizes alone: the same arrays give the same y bit for bit. */
 int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
                   const uint8_t* b_codes, const uint8_t* b_scales, int64_t n, int64_t k, void* y,
-                  int y_dtype, void* stream);
+                  int y_dtype, void* ws, size_t ws_bytes, void* stream);
 
 /* Workspace bytes of cp_mx4_linear (256-byte aligned; 0: none, ws may be NULL). */
-size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k);
+size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t n, int64_t k);
 
 /* y [m, n] = x w^T for MXFP4 weights w [n, k]: x [m, k] is quantized as cp_mx4_quantize
  * does, then multiplied as cp_mx4_matmul does. */

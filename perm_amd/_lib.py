@@ -117,8 +117,9 @@ SIGNATURES = {
     "cp_mx4_scale_bytes": (_sz, [_i64, _i64]),
     "cp_mx4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
     "cp_mx4_dequantize": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _vp]),
-    "cp_mx4_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
-    "cp_mx4_linear_ws_bytes": (_sz, [_i64, _i64]),
+    "cp_mx4_matmul_ws_bytes": (_sz, [_i64, _i64, _i64]),
+    "cp_mx4_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _sz, _vp]),
+    "cp_mx4_linear_ws_bytes": (_sz, [_i64, _i64, _i64]),
     "cp_mx4_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp, _sz,
                              _vp]),
     "cp_kv_write": (_i32, [_kv_p, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _vp, _i64, _i64,

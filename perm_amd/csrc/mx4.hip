@@ -199,9 +199,9 @@ __device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, in
     if (n0 + i < N) y[m * N + n0 + i] = (typename Elem<DT>::T)c[i];
 }
 
-// Few rows of a (at most 64): bound by reading b once. A workgroup takes NT 16-row tiles of b
-// and all of a; its waves take the 128-column steps in turn, up to four steps' loads in
-// flight in each, and join their sums in LDS in wave order. b's codes go from memory to the matrix cores
+// Few rows of a (at most 32): bound by reading b once. A workgroup takes NT 16-row tiles of b
+// and all of a; its waves take the 128-column steps in turn, four or eight steps' loads
+// in flight in each, and join their sums in LDS in wave order. b's codes go from memory to the matrix cores
 // without LDS: each is used once. Four neighbouring workgroups of one XCD share the scale
 // dwords of 64 rows in its L2.
 //
@@ -210,7 +210,7 @@ __device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, in
 template <int MT, int NT, int XT, int DT>
 __global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b, const void* x, int64_t stride, int k,
                                                        int wgs, typename Elem<DT>::T* __restrict__ y) {
-  constexpr int U = MT * NT > 4 ? 2 : 4;  // within the 128 registers of a 16-wave workgroup
+  constexpr int U = MT + NT > 2 ? 4 : 8;  // within the 128 registers of a 16-wave workgroup
   constexpr bool FUSED = XT >= 0;
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, g = lane >> 4, W = blockDim.x >> 6;
@@ -384,7 +384,7 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 
 template <int WM, int WN, int FM, int FN, int DT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, MxOperand b, int k, int mt, int nt,
-                                                                   typename Elem<DT>::T* __restrict__ y) {
+                                                                   int splits, typename Elem<DT>::T* __restrict__ y) {
   constexpr int W = WM * WN, BM = 16 * WM * FM, BN = 16 * WN * FN, ROWS = BM + BN;
   constexpr int LA = BM / (8 * W), LB = BN / (8 * W);  // direct loads of a wave per stage, 8 rows each
   constexpr int DA = FM > 4 ? FM / 4 : 1, DB = FN > 4 ? FN / 4 : 1;
@@ -395,18 +395,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
   // Workgroup w runs on XCD w % 8. Each XCD takes a contiguous run of tiles, ordered in
   // columns of eight m tiles, so that the tiles in flight on one XCD form a block and share
   // their operands in its L2.
-  int tm, tn;
+  int tm, tn, split;
   {
-    const int tiles = mt * nt, w = blockIdx.x;
+    const int tiles = mt * nt * splits, w = blockIdx.x;
     const int x = w & 7, q = tiles >> 3, r = tiles & 7;
-    const int t = x * q + min(x, r) + (w >> 3);
+    int t = x * q + min(x, r) + (w >> 3);
+    split = t / (mt * nt);
+    t -= split * mt * nt;
     const int col = t / (8 * nt), h = min(8, mt - 8 * col), u = t - col * 8 * nt;
     tn = u / h;
     tm = 8 * col + u % h;
   }
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const int kb = k / 2, blocks = k / kMxBlock;
+  // columns in stages of 256; a split takes an equal run of them and its own [rows][rows] sums
   const int stages = (k + kStage - 1) / kStage, steps = (k + kMxStep - 1) / kMxStep;
+  const int sb0 = split * stages / splits, sb1 = (split + 1) * stages / splits;
+  y += split * a.rows * b.rows;
 
   // Buffer loads over the tile's rows: a row past the operand's end, and a lane whose chunk
   // lies past the end of a row (given an offset past any buffer), reads zeros. A zero code
@@ -496,18 +501,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
       for (int i = 0; i < DB; ++i) sb[j][i] = nb[j][i];
     }
   };
-  constexpr int HM = FM / 2, AHEAD = 2;
-  fetch(0, 0, L);
-  fetch_scales(0);
+  constexpr int HM = FM / 2, AHEAD = FM > 2 ? 2 : 1;  // a row read ahead must not be one still in use
+  fetch(sb0, 0, L);
+  fetch_scales(sb0);
   __syncthreads();
-  fetch(1, 0, L / 2);
+  fetch(sb0 + 1, 0, L / 2);
   scales_now();
 #pragma unroll
-  for (int j = 0; j < FN; ++j) read_b(0, P0, j);
+  for (int j = 0; j < FN; ++j) read_b(sb0, P0, j);
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) read_a(0, P0, i);
+  for (int i = 0; i < AHEAD; ++i) read_a(sb0, P0, i);
 #pragma clang loop unroll(disable)
-  for (int s = 0; s < stages; ++s) {
+  for (int s = sb0; s < sb1; ++s) {
     unrolled<FM>([&](auto I) {
       if constexpr (I < HM) fetch(s + 1, L / 2 + I * L / FM, L / 2 + (I + 1) * L / FM);
       if constexpr (I == HM) fetch_scales(s + 1);
@@ -537,20 +542,85 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
                             lds + wave * FM * FN * 512);
 }
 
+// y = the splits' sums in split order.
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ part, int64_t count, int splits,
+                                                       typename Elem<DT>::T* __restrict__ y) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i + 4 <= count && (count & 3) == 0) {
+    f32x4 c = *reinterpret_cast<const f32x4*>(part + i);
+    for (int s = 1; s < splits; ++s) c += *reinterpret_cast<const f32x4*>(part + s * count + i);
+    if constexpr (DT == CP_F32) {
+      *reinterpret_cast<f32x4*>(y + i) = c;
+    } else {
+      u32x2 p;
+      p[0] = pack2<DT>(c[0], c[1]);
+      p[1] = pack2<DT>(c[2], c[3]);
+      *reinterpret_cast<u32x2*>(y + i) = p;
+    }
+  } else {
+    for (int64_t j = i; j < i + 4 && j < count; ++j) {
+      float c = part[j];
+      for (int s = 1; s < splits; ++s) c += part[s * count + j];
+      y[j] = (typename Elem<DT>::T)c;
+    }
+  }
+}
+
+// How a product of m x n results over k columns is cut up.
+struct MxPlan {
+  int few;     // a's rows in tiles of 16 on mx4_few_kernel, or 0
+  int edge;    // otherwise the edge of mx4_gemm_kernel's square tiles: 64, 128 or 256
+  int splits;  // of the columns
+};
+
+// Tiles are chosen by predicted time. A stage takes a tile of edge 64 / 128 / 256 at least
+// 0.47 / 0.73 / 1.9 us however empty the GPU is, and a CU with several tiles 0.23 / 0.69 /
+// 1.9 us a tile (measured at k = 4096: 512 x 4096 results 11.6 / 13.2 / 23.5 us, 256 x 14336
+// 18.4 / 15.2 / 25.1, 1024 x 14336 52 / 38 / 33). Columns are split while that leaves at least
+// 12 stages a split and no more than two small tiles (or one) a CU, where joining costs less
+// than it saves (over 14336 columns 128 x 4096 results take 17.5 us in four splits, 26.6 in
+// one; 1024 x 4096, in 256 tiles of 128, 44.7 in two and 41.1 in one).
+static MxPlan mx_plan(int64_t m, int64_t n, int64_t k) {
+  if (m <= 32) return {(int)((m + 15) / 16), 0, 1};
+  const int edges[3] = {64, 128, 256};
+  const double least[3] = {0.47, 0.73, 1.9}, each[3] = {0.23, 0.69, 1.9};
+  MxPlan p = {0, 0, 1};
+  double best = 0.0;
+  int64_t tiles = 1;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t t = ((m + edges[i] - 1) / edges[i]) * ((n + edges[i] - 1) / edges[i]);
+    // 256-wide tiles run one a CU, in whole rounds
+    const double load = i == 2 ? (double)((t + 255) / 256) : t / 256.0;
+    const double us = std::max(least[i], each[i] * load);
+    if (!p.edge || us < best) best = us, p.edge = edges[i], tiles = t;
+  }
+  const int64_t stages = (k + kStage - 1) / kStage;
+  p.splits = (int)std::max((int64_t)1, std::min(stages / 12, (p.edge == 64 ? 512 : 256) / tiles));
+  return p;
+}
+
 template <int WM, int WN, int FM, int FN, int DT>
-static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
+static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, int splits, void* y, hipStream_t st) {
   constexpr int BM = 16 * WM * FM, BN = 16 * WN * FN, lds = 2 * (BM + BN) * kStageBytes;
   static_assert(WM * WN * FM * FN * 512 <= lds, "the results pass through the staging buffers");
   const int64_t mt = (a.rows + BM - 1) / BM, nt = (b.rows + BN - 1) / BN;
-  if (mt * nt > 0x7FFFFFFF || mt * 8 > 0x7FFFFFFF / nt) return set_error(CP_ERR_SHAPE, "product too large");
+  if (mt > 0x7FFFFFF / nt / splits) return set_error(CP_ERR_SHAPE, "product too large");
   static const hipError_t once =
       hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<WM, WN, FM, FN, DT>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (once != hipSuccess) return hip_fail(once, "LDS size of the MXFP4 product");
-  mx4_gemm_kernel<WM, WN, FM, FN, DT><<<dim3((unsigned)(mt * nt)), 64 * WM * WN, lds, st>>>(
-      a, b, k, (int)mt, (int)nt, (typename Elem<DT>::T*)y);
+  mx4_gemm_kernel<WM, WN, FM, FN, DT><<<dim3((unsigned)(mt * nt * splits)), 64 * WM * WN, lds, st>>>(
+      a, b, k, (int)mt, (int)nt, splits, (typename Elem<DT>::T*)y);
   CP_LAUNCHED("MXFP4 product");
   return CP_OK;
+}
+
+template <int DT>
+static int mx_gemm_edge(const MxPlan& p, const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
+  if (p.edge == 64) return mx_gemm<2, 2, 2, 2, DT>(a, b, k, p.splits, y, st);
+  if (p.edge == 128) return mx_gemm<2, 2, 4, 4, DT>(a, b, k, p.splits, y, st);
+  return mx_gemm<2, 4, 8, 4, DT>(a, b, k, p.splits, y, st);
 }
 
 // Waves of a few-rows workgroup: four, or more while the launch has under eight waves a CU
@@ -575,13 +645,26 @@ static int mx_few(const MxOperand& a, const MxOperand& b, const void* x, int64_t
   return CP_OK;
 }
 
+static size_t mx_product_ws(int64_t m, int64_t n, int64_t k) {
+  const MxPlan p = mx_plan(m, n, k);
+  return p.splits > 1 ? (size_t)m * n * p.splits * 4 : 0;
+}
+
 template <int DT>
-static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, hipStream_t st) {
-  if (a.rows <= 16) return mx_few<1, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
-  if (a.rows <= 32) return mx_few<2, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
-  if (a.rows <= 64) return mx_few<4, 2, -1, DT>(a, b, nullptr, 0, k, y, st);
-  if (((a.rows + 255) / 256) * ((b.rows + 255) / 256) >= 192) return mx_gemm<2, 4, 8, 4, DT>(a, b, k, y, st);
-  return mx_gemm<2, 2, 4, 4, DT>(a, b, k, y, st);
+static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, void* ws, hipStream_t st) {
+  const MxPlan p = mx_plan(a.rows, b.rows, k);
+  // two tiles of b a workgroup where that still fills the CUs: a's rows are read half as often
+  // (16 x 14336 x 4096: 9.4 us against 10.6; 16 x 4096 x 14336: 14.0 against 9.9)
+  const bool wide = b.rows >= 8192;
+  if (p.few == 1) return wide ? mx_few<1, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<1, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (p.few == 2) return wide ? mx_few<2, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<2, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (p.splits == 1) return mx_gemm_edge<DT>(p, a, b, k, y, st);
+  if (int s = mx_gemm_edge<CP_F32>(p, a, b, k, ws, st)) return s;
+  const int64_t count = a.rows * b.rows;
+  mx4_join_kernel<DT><<<dim3((unsigned)((count + 1023) / 1024)), 256, 0, st>>>((const float*)ws, count, p.splits,
+                                                                              (typename Elem<DT>::T*)y);
+  CP_LAUNCHED("MXFP4 product's join");
+  return CP_OK;
 }
 
 // x's rows quantized inside the product: up to four, whose codes every workgroup makes for
@@ -597,11 +680,11 @@ static int mx_fused(const void* x, int64_t m, int64_t stride, const MxOperand& b
   return mx_few<1, 1, XT, CP_F16>(a, b, x, stride, k, y, st);
 }
 
-static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt,
+static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt, void* ws,
                              hipStream_t st) {
-  if (dt == CP_F32) return mx_product<CP_F32>(a, b, k, y, st);
-  if (dt == CP_BF16) return mx_product<CP_BF16>(a, b, k, y, st);
-  return mx_product<CP_F16>(a, b, k, y, st);
+  if (dt == CP_F32) return mx_product<CP_F32>(a, b, k, y, ws, st);
+  if (dt == CP_BF16) return mx_product<CP_BF16>(a, b, k, y, ws, st);
+  return mx_product<CP_F16>(a, b, k, y, ws, st);
 }
 
 static int mx_shape(int64_t rows, int64_t k, const char* what) {
@@ -638,6 +721,16 @@ static int mx_check_x(const void* x, int dt, int64_t rows, int64_t k, int64_t st
     return set_error(CP_ERR_ALIGN, "rows of x need 16-byte alignment");
   return CP_OK;
 }
+
+static int mx_check_ws(const void* ws, size_t have, size_t need) {
+  if (need && (!ws || have < need))
+    return set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", have, need);
+  if (need && !aligned(ws, 256)) return set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
+  return CP_OK;
+}
+
+// Bytes of the codes of m rows, a multiple of 256.
+static size_t mx_code_bytes(int64_t m, int64_t k) { return (size_t)((m * (k / 2) + 255) / 256 * 256); }
 
 static int mx_check_packed(const uint8_t* codes, const uint8_t* scales, int64_t rows) {
   if (rows && (!codes || !scales)) return set_error(CP_ERR_ARG, "null codes / scales");
@@ -689,9 +782,14 @@ int cp_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
   return CP_OK;
 }
 
-int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
-                  const uint8_t* b_codes, const uint8_t* b_scales, int64_t n, int64_t k, void* y,
-                  int y_dtype, void* stream) {
+size_t cp_mx4_matmul_ws_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || n < 1 || k < 1) return 0;
+  return cp::mx_product_ws(m, n, k);
+}
+
+int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, const uint8_t* b_codes,
+                  const uint8_t* b_scales, int64_t n, int64_t k, void* y, int y_dtype, void* ws, size_t ws_bytes,
+                  void* stream) {
   cp::clear_error();
   if (int s = cp::mx_shape(m, k, "a")) return s;
   if (int s = cp::mx_shape(n, k, "b")) return s;
@@ -701,13 +799,14 @@ int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
   if (m == 0 || n == 0) return CP_OK;
   if (!y) return cp::set_error(CP_ERR_ARG, "null y");
   if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
-  return cp::mx_launch_product({a_codes, a_scales, m}, {b_codes, b_scales, n}, (int)k, y, y_dtype,
+  if (int s = cp::mx_check_ws(ws, ws_bytes, cp_mx4_matmul_ws_bytes(m, n, k))) return s;
+  return cp::mx_launch_product({a_codes, a_scales, m}, {b_codes, b_scales, n}, (int)k, y, y_dtype, ws,
                                (hipStream_t)stream);
 }
 
-size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t k) {
-  if (m < 0 || k < 0 || cp::mx_fuses(m, k)) return 0;
-  return (size_t)((m * (k / 2) + 255) / 256 * 256) + cp_mx4_scale_bytes(m, k);
+size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m < 1 || n < 1 || k < 1 || cp::mx_fuses(m, k)) return 0;
+  return cp::mx_code_bytes(m, k) + cp_mx4_scale_bytes(m, k) + cp_mx4_matmul_ws_bytes(m, n, k);
 }
 
 int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride, const uint8_t* w_codes,
@@ -721,20 +820,18 @@ int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride, con
   if (m == 0 || n == 0) return CP_OK;
   if (!y) return cp::set_error(CP_ERR_ARG, "null y");
   if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
-  if (cp_mx4_linear_ws_bytes(m, k) && (!ws || ws_bytes < cp_mx4_linear_ws_bytes(m, k)))
-    return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes,
-                         cp_mx4_linear_ws_bytes(m, k));
-  if (!cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
+  if (int s = cp::mx_check_ws(ws, ws_bytes, cp_mx4_linear_ws_bytes(m, n, k))) return s;
   if (cp::mx_fuses(m, k)) {
     const cp::MxOperand b = {w_codes, w_scales, n};
     if (x_dtype == CP_F32) return cp::mx_fused<CP_F32>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
     if (x_dtype == CP_BF16) return cp::mx_fused<CP_BF16>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
     return cp::mx_fused<CP_F16>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
   }
+  // the rows' codes, their scales, the product's own
   uint8_t* xc = (uint8_t*)ws;
-  uint8_t* xs = xc + (m * (k / 2) + 255) / 256 * 256;
+  uint8_t* xs = xc + cp::mx_code_bytes(m, k);
   if (int s = cp::mx_quantize(x, x_dtype, m, k, row_stride, xc, xs, (hipStream_t)stream)) return s;
-  return cp::mx_launch_product({xc, xs, m}, {w_codes, w_scales, n}, (int)k, y, y_dtype,
+  return cp::mx_launch_product({xc, xs, m}, {w_codes, w_scales, n}, (int)k, y, y_dtype, xs + cp_mx4_scale_bytes(m, k),
                                (hipStream_t)stream);
 }
 

@@ -133,8 +133,10 @@ def matmul(a, b, dtype=torch.bfloat16):
     if k != kb:
         raise ValueError(f"rows of {k} times rows of {kb}")
     y = torch.empty((m, n), dtype=dtype, device=a.codes.device)
+    nws = lib.cp_mx4_matmul_ws_bytes(m, n, k)
+    ws = _lib.workspace(nws, y.device) if nws else None
     _lib.check(lib.cp_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(),
-                                 b.scales.data_ptr(), n, k, y.data_ptr(), code,
+                                 b.scales.data_ptr(), n, k, y.data_ptr(), code, _lib.ptr(ws), nws,
                                  _lib.stream_ptr()))
     return y
 
@@ -155,7 +157,7 @@ def linear(x, w, dtype=None):
     rows = _rows(x)
     m = rows.shape[0]
     y = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=x.device)
-    nws = lib.cp_mx4_linear_ws_bytes(m, k)
+    nws = lib.cp_mx4_linear_ws_bytes(m, n, k)
     ws = _lib.workspace(nws, x.device) if nws else None
     _lib.check(lib.cp_mx4_linear(rows.data_ptr(), xc, m, rows.stride(0), w.codes.data_ptr(),
                                  w.scales.data_ptr(), n, k, y.data_ptr(), yc, _lib.ptr(ws), nws,

@@ -247,3 +247,19 @@ def test_refusals(mx):
         mx.matmul(q, mx.MxTensor(q.codes.float(), q.scales))
     with pytest.raises(ValueError):
         mx.matmul(q, mx.MxTensor(q.codes.t(), q.scales))
+
+
+@pytest.mark.parametrize("m,n,k", [(33, 100, 14336), (64, 70, 6144), (70, 4100, 3104), (130, 66, 8224),
+                                   (300, 1100, 1056), (600, 4097, 288), (1030, 12400, 160), (257, 15000, 128)])
+def test_tiles_and_splits(mx, m, n, k):
+    """Sizes that take each tile of the product, columns split in several parts among them."""
+    x = _rows(m, k, torch.bfloat16, m).cuda()
+    w = _rows(n, k, torch.float32, n, 0.02).cuda()
+    qx, qw = mx.quantize(x), mx.quantize(w)
+    a = mx.dequantize(qx).double().cpu().numpy()
+    b = mx.dequantize(qw).double().cpu().numpy()
+    for dtype in DTYPES:
+        y = mx.matmul(qx, qw, dtype)
+        _check_product(y, a, b, k, dtype)
+        assert torch.equal(y, mx.matmul(qx, qw, dtype))
+    assert torch.equal(mx.linear(x, qw), mx.matmul(qx, qw))

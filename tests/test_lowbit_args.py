@@ -47,8 +47,9 @@ def test_linear(lib, kw, status):
 
 
 def test_few_rows_need_no_workspace(lib):
-    assert lib.cp_mx4_linear_ws_bytes(4, 64) == 0 and lib.cp_mx4_linear_ws_bytes(5, 64) > 0
-    assert lib.cp_mx4_linear_ws_bytes(4, 1 << 20) > 0
+    assert lib.cp_mx4_linear_ws_bytes(4, 8, 64) == 0 and lib.cp_mx4_linear_ws_bytes(5, 8, 64) > 0
+    assert lib.cp_mx4_linear_ws_bytes(4, 8, 1 << 20) > 0
+    assert lib.cp_mx4_matmul_ws_bytes(100, 4096, 14336) > 0 == lib.cp_mx4_matmul_ws_bytes(16, 4096, 14336)
 
 
 def _write(lib, cache, rows=3, batch=3, dt=1, k=P, k_row=128, k_head=64, offsets=None, table=P,
