@@ -252,9 +252,14 @@ __global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b,
     for (int u = 0; u < U; ++u) {
       const int s = base + W * u + wave, blk = 4 * s + g;
       if constexpr (FUSED) {
-        const bool in = blk < nblk && (lane & 15) < M;
-        fa[u][0] = in ? *reinterpret_cast<const u32x4*>(lds + (lane & 15) * pitch + 16 * blk) : zero;
-        va[u] = in ? lds[M * pitch + (lane & 15) * nblk + blk] : 0;
+        va[u] = 0;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int m = 16 * i + (lane & 15);
+          const bool in = blk < nblk && m < M;
+          fa[u][i] = in ? *reinterpret_cast<const u32x4*>(lds + m * pitch + 16 * blk) : zero;
+          va[u] |= in ? (uint32_t)lds[M * pitch + m * nblk + blk] << (8 * i) : 0;
+        }
       } else {
         va[u] = sa[min(s, steps - 1) * ga * 64];
 #pragma unroll
@@ -266,14 +271,15 @@ __global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b,
   load_b(0);
   if constexpr (FUSED) {
     typedef typename Elem<XT>::T T;
-    for (int m = 0; m < M; ++m) {
-      for (int c = threadIdx.x; c < k / 8; c += blockDim.x) {  // k % 32 == 0: whole blocks of four lanes
-        float v[8];
-        load8<XT>((const T*)x + m * stride + 8 * c, v);
-        const int e = mx_scale_byte(mx_block_amax(v));
-        *reinterpret_cast<uint32_t*>(lds + m * pitch + 4 * c) = e == 255 ? 0u : mx_pack8(v, mx_inv_scale(e));
-        if ((c & 3) == 0) lds[M * pitch + m * nblk + (c >> 2)] = (uint8_t)e;
-      }
+    const int chunks = k / 8;  // k % 32 == 0: four lanes hold a block
+#pragma unroll 4
+    for (int t = threadIdx.x; t < M * chunks; t += blockDim.x) {
+      const int m = t / chunks, c = t - m * chunks;
+      float v[8];
+      load8<XT>((const T*)x + m * stride + 8 * c, v);
+      const int e = mx_scale_byte(mx_block_amax(v));
+      *reinterpret_cast<uint32_t*>(lds + m * pitch + 4 * c) = e == 255 ? 0u : mx_pack8(v, mx_inv_scale(e));
+      if ((c & 3) == 0) lds[M * pitch + m * nblk + (c >> 2)] = (uint8_t)e;
     }
     __syncthreads();
   }
@@ -667,17 +673,25 @@ static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, vo
   return CP_OK;
 }
 
-// x's rows quantized inside the product: up to four, whose codes every workgroup makes for
-// itself faster than a launch of their own takes.
-static bool mx_fuses(int64_t m, int64_t k) { return m <= 4 && m * (k / 2 + 16 + k / kMxBlock) <= 64 * 1024; }
+// Few rows are quantized inside the product: every workgroup makes the codes for itself, beside
+// its first loads of b. A launch of their own takes 2.7 us and the gap behind it; fused, 1000 x
+// 1056 weights take 4.2 us with one row and 7.0 with 32 (3.4 without the quantization), 14336 x
+// 4096 ones 8.8 / 12.6 / 15.2 with 1 / 4 / 6 rows (9.1 without). So where a workgroup's share,
+// m k, and all workgroups', m k n, are small.
+static bool mx_fuses(int64_t m, int64_t n, int64_t k) {
+  return m <= 32 && m * k <= 32768 && m * k * n <= ((int64_t)1 << 28);
+}
 
 template <int XT>
 static int mx_fused(const void* x, int64_t m, int64_t stride, const MxOperand& b, int k, void* y, int dt,
                     hipStream_t st) {
   const MxOperand a = {nullptr, nullptr, m};
-  if (dt == CP_F32) return mx_few<1, 1, XT, CP_F32>(a, b, x, stride, k, y, st);
-  if (dt == CP_BF16) return mx_few<1, 1, XT, CP_BF16>(a, b, x, stride, k, y, st);
-  return mx_few<1, 1, XT, CP_F16>(a, b, x, stride, k, y, st);
+#define CP_MX_FUSED(DT) \
+  return m <= 16 ? mx_few<1, 1, XT, DT>(a, b, x, stride, k, y, st) : mx_few<2, 1, XT, DT>(a, b, x, stride, k, y, st)
+  if (dt == CP_F32) CP_MX_FUSED(CP_F32);
+  if (dt == CP_BF16) CP_MX_FUSED(CP_BF16);
+  CP_MX_FUSED(CP_F16);
+#undef CP_MX_FUSED
 }
 
 static int mx_launch_product(const MxOperand& a, const MxOperand& b, int k, void* y, int dt, void* ws,
@@ -805,7 +819,7 @@ int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m, co
 }
 
 size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t n, int64_t k) {
-  if (m < 1 || n < 1 || k < 1 || cp::mx_fuses(m, k)) return 0;
+  if (m < 1 || n < 1 || k < 1 || cp::mx_fuses(m, n, k)) return 0;
   return cp::mx_code_bytes(m, k) + cp_mx4_scale_bytes(m, k) + cp_mx4_matmul_ws_bytes(m, n, k);
 }
 
@@ -821,7 +835,7 @@ int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride, con
   if (!y) return cp::set_error(CP_ERR_ARG, "null y");
   if (!cp::aligned(y, 16)) return cp::set_error(CP_ERR_ALIGN, "y needs 16-byte alignment");
   if (int s = cp::mx_check_ws(ws, ws_bytes, cp_mx4_linear_ws_bytes(m, n, k))) return s;
-  if (cp::mx_fuses(m, k)) {
+  if (cp::mx_fuses(m, n, k)) {
     const cp::MxOperand b = {w_codes, w_scales, n};
     if (x_dtype == CP_F32) return cp::mx_fused<CP_F32>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);
     if (x_dtype == CP_BF16) return cp::mx_fused<CP_BF16>(x, m, row_stride, b, (int)k, y, y_dtype, (hipStream_t)stream);

@@ -263,3 +263,19 @@ def test_tiles_and_splits(mx, m, n, k):
         _check_product(y, a, b, k, dtype)
         assert torch.equal(y, mx.matmul(qx, qw, dtype))
     assert torch.equal(mx.linear(x, qw), mx.matmul(qx, qw))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 16, 32768), (31, 40, 1056), (32, 1000, 1024), (17, 50, 96), (2, 8200, 4096)])
+def test_rows_quantized_in_the_product(mx, m, n, k):
+    """Few rows: the codes made inside the product are those of quantize()."""
+    x = _rows(m, k, torch.bfloat16, m + k).cuda()
+    x[m // 2, 5] = float("nan")
+    w = mx.quantize(_rows(n, k, torch.float32, n, 0.02).cuda())
+    y = mx.linear(x, w)
+    want = mx.matmul(mx.quantize(x), w)
+    assert y[m // 2].isnan().all() and y.isnan().sum() == n
+    a = np.nan_to_num(mx.dequantize(mx.quantize(x)).double().cpu().numpy())
+    b = mx.dequantize(w).double().cpu().numpy()
+    a[m // 2] = 0
+    _check_product(torch.where(y.isnan(), 0, y), a, b, k, torch.bfloat16)
+    _check_product(torch.where(want.isnan(), 0, want), a, b, k, torch.bfloat16)

@@ -40,14 +40,14 @@ def test_quantize(lib, kw, status):
     (dict(ws=None), _lib.CP_ERR_WORKSPACE), (dict(ws=P + 16), _lib.CP_ERR_ALIGN), (dict(m=0), _lib.CP_OK),
     (dict(n=0), _lib.CP_OK)])
 def test_linear(lib, kw, status):
-    a = dict(m=5, n=8, k=64, ydt=1, y=P, ws=P, nws=1 << 20)
+    a = dict(m=40, n=8, k=64, ydt=1, y=P, ws=P, nws=1 << 20)
     a.update(kw)
     got = lib.cp_mx4_linear(P, 1, a["m"], 64, P, P, a["n"], a["k"], a["y"], a["ydt"], a["ws"], a["nws"], None)
     assert got == status
 
 
 def test_few_rows_need_no_workspace(lib):
-    assert lib.cp_mx4_linear_ws_bytes(4, 8, 64) == 0 and lib.cp_mx4_linear_ws_bytes(5, 8, 64) > 0
+    assert lib.cp_mx4_linear_ws_bytes(4, 8, 64) == 0 and lib.cp_mx4_linear_ws_bytes(33, 8, 64) > 0
     assert lib.cp_mx4_linear_ws_bytes(4, 8, 1 << 20) > 0
     assert lib.cp_mx4_matmul_ws_bytes(100, 4096, 14336) > 0 == lib.cp_mx4_matmul_ws_bytes(16, 4096, 14336)
 
