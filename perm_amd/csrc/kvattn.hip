@@ -408,7 +408,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   const int q = lane & 31, hh = lane >> 5;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);
   const int64_t cap = (int64_t)c.max_pages * blk;
-  const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
+  const int len = (int)min((int64_t)max(__builtin_amdgcn_readfirstlane(a.lens[b]), 0), cap);
 
   // token range [lo, hi) of row r of the sequence; rows past the end see nothing
   auto range = [&](int64_t r, int* lo, int* hi) {
@@ -473,28 +473,36 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
   // each, four token groups. Chunks past d repeat the row's first, rows past d its last 16
   // (their q is 0, their results are dropped).
+  // What changes from tile to tile is a page's start and where in the page the tile begins:
+  // j0 is a multiple of 64 and a page's length a power of two, so (j0 + x) mod block is the sum
+  // of the two parts' remainders for x < 64.
   constexpr int CH = DP / 16;
+  const uint32_t page = (uint32_t)c.heads * blk * d;          // at most 65535 * 128 * 256
   const int kt = 16 * wave + lane / CH;                       // + 1024 / DP per load
   const int vg = (lane & 3) ^ ((lane >> 4) & 3);
+  const uint8_t* const kbase = c.k + (int64_t)h * blk * d;
+  const uint8_t* const vbase = c.v + (int64_t)h * blk * d;
+  uint32_t koff[NL], voff[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int token = kt + i * (1024 / DP);
+    const int col = (16 * (lane % CH)) ^ k_swizzle<DP>(token);
+    koff[i] = (token & (blk - 1)) * d + (col < d ? col : 0);
+    voff[i] = min(16 * (wave * NL + i) + (lane >> 2), d - 1) * blk + ((16 * vg) & (blk - 1));
+  }
   auto fetch = [&](int into, int tile, int pk, int pv) {
     uint8_t* to = lds + into * BUF;
-    const int j0 = tile * kTile;
-    // no page: page 0's codes, which no row sees
-    const uint8_t* kp = c.k + ((int64_t)((unsigned)pk < (unsigned)c.pages ? pk : 0) * c.heads + h) * blk * d;
-    const uint8_t* vp = c.v + ((int64_t)((unsigned)pv < (unsigned)c.pages ? pv : 0) * c.heads + h) * blk * d;
+    const int in = (tile * kTile) & (blk - 1);
+    // no page: page 0's codes, which no row sees; K's page is the wave's
+    pk = __builtin_amdgcn_readfirstlane(pk);
+    const uint8_t* kp = kbase + (uint64_t)((unsigned)pk < (unsigned)c.pages ? pk : 0) * page + in * d;
+    const uint8_t* vp = vbase + in + (uint64_t)((unsigned)pv < (unsigned)c.pages ? (unsigned)pv : 0u) * page;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int token = kt + i * (1024 / DP);
-      const int col = (16 * (lane % CH)) ^ k_swizzle<DP>(token);
-      const uint8_t* src = kp + ((j0 + token) & (blk - 1)) * d + (col < d ? col : 0);
-      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(to + (wave * NL + i) * 1024), 16, 0, 0);
-    }
+    for (int i = 0; i < NL; ++i)
+      __builtin_amdgcn_global_load_lds((gptr_t)(kp + koff[i]), (lptr_t)(to + (wave * NL + i) * 1024), 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int column = min(16 * (wave * NL + i) + (lane >> 2), d - 1);
-      const uint8_t* src = vp + column * blk + ((j0 + 16 * vg) & (blk - 1));
-      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(to + KB + (wave * NL + i) * 1024), 16, 0, 0);
-    }
+    for (int i = 0; i < NL; ++i)
+      __builtin_amdgcn_global_load_lds((gptr_t)(vp + voff[i]), (lptr_t)(to + KB + (wave * NL + i) * 1024), 16, 0, 0);
   };
   // this lane's K rows and V columns in LDS
   const int token = 16 * ((q >> 2) & 1) + 4 * (q >> 3) + (q & 3);
@@ -507,12 +515,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   struct Pages {
     int k, v, g[2];
   } pn;
+  auto at = [&](int j) {  // 32-bit offsets: max_pages is at most 2^31 / 128
+    return *reinterpret_cast<const int*>(reinterpret_cast<const char*>(tab) + 4 * ((uint32_t)min(j, lastj) >> lb));
+  };
   auto lookup = [&](int tile) {
     const int j0 = tile * kTile;
-    pn.k = tab[min(j0 + 16 * wave, lastj) >> lb];
-    pn.v = tab[min(j0 + 16 * vg, lastj) >> lb];
+    pn.k = at(j0 + 16 * wave);
+    pn.v = at(j0 + 16 * vg);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) pn.g[s] = tab[min(j0 + 32 * s + 16 * hh, lastj) >> lb];
+    for (int s = 0; s < 2; ++s) pn.g[s] = at(j0 + 32 * s + 16 * hh);
   };
   float ks[2], vs[2], nks[2], nvs[2];
   bool have[2], nhave[2];
@@ -520,9 +531,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       nhave[s] = (unsigned)pg[s] < (unsigned)c.pages;
-      const int64_t hv = (int64_t)(nhave[s] ? pg[s] : 0) * c.heads + h;
-      nks[s] = c.k_scale[hv];
-      nvs[s] = c.v_scale[hv];
+      const uint64_t hv = (uint64_t)(nhave[s] ? (unsigned)pg[s] : 0u) * (uint32_t)(4 * c.heads);
+      nks[s] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(c.k_scale + h) + hv);
+      nvs[s] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(c.v_scale + h) + hv);
     }
   };
   // A tile is two units of 32 tokens. A unit's scores are multiplied while the weights of the
@@ -622,7 +633,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
           const float e0 = exp2_fast(__builtin_fmaf(sc[s][2 * i], kc, off));
           const float e1 = exp2_fast(__builtin_fmaf(sc[s][2 * i + 1], kc, off));
           sum += e0 + e1;
-          w[i >> 2][i & 3] = pack2<CP_F16>(e0, e1);
+          uint32_t e = pack2<CP_F16>(e0, e1);
+          asm volatile("" : "+v"(e));  // here, not past the branch below
+          w[i >> 2][i & 3] = e;
         }
         if (k == NC) {
 #pragma unroll

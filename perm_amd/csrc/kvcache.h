@@ -43,14 +43,14 @@ __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int
       const int o = __shfl_up(sum, k);
       if (lane >= k) sum += o;
     }
-    const int total = __shfl(sum, 63);
+    const int total = __builtin_amdgcn_readlane(sum, 63);
     if (at < total) {
       const unsigned long long hit = __ballot(sum > at);
       const int l = __ffsll(hit) - 1;
       *b = base + l;
-      *item = at - __shfl(sum - pieces, l);
-      *row0 = __shfl(r, l);
-      *n = __shfl(m, l);
+      *item = at - __builtin_amdgcn_readlane(sum - pieces, l);
+      *row0 = __builtin_amdgcn_readlane(r, l);
+      *n = __builtin_amdgcn_readlane(m, l);
       return true;
     }
     at -= total;
