@@ -232,11 +232,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     float tm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                      fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     tm = __builtin_fmaf(tm, kc, lv);
-    tm = fmaxf(tm, __shfl_xor(tm, 16));
-    tm = fmaxf(tm, __shfl_xor(tm, 32));
     // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
-    // the outputs are then seldom rescaled
+    // the row's lanes seldom have to exchange their largest and rescale the outputs
     if (__any(tm > m + 8.0f)) {
+      tm = fmaxf(tm, __shfl_xor(tm, 16));
+      tm = fmaxf(tm, __shfl_xor(tm, 32));
       const float mn = fmaxf(m, tm);
       const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
       m = mn;
@@ -606,10 +606,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       }
       // the largest t of the unit: kc > 0, so t rises with the raw score
       float tm = __builtin_fmaf(top, kc, lg);
-      tm = fmaxf(tm, __shfl_xor(tm, 32));
       // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
-      // the outputs are then seldom rescaled
+      // the row's two lanes seldom have to exchange their largest and rescale the outputs
       if (__any(tm > m + 8.0f)) {
+        tm = fmaxf(tm, __shfl_xor(tm, 32));
         const float mn = fmaxf(m, tm);
         const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
         m = mn;
