@@ -15,6 +15,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kvcache.h"
@@ -820,18 +821,33 @@ struct AttnPlan {
 
 // Row tiles of 16 while a sequence has no more (row, head of the group) pairs on average:
 // then reading the cache bounds the call; of 128 above that.
-static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int64_t cap, int window) {
+static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int d,
+                          int64_t cap, int window) {
   AttnPlan p;
   p.many = rows * group > 16 * batch;
   const int tile = p.many ? kManyRows : 16, step = p.many ? kTile : kFewTile;
   p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
-  // The tokens of a row tile are split over as many workgroups as the CUs hold at once, but
-  // not into pieces shorter than joining them costs: 16 steps of the longest row tile there
-  // can be, or (few rows, where a step is 32 tokens) 8 of a shorter one's.
-  const int64_t n = p.items * heads, want = p.many ? 512 : 1024;
+  // The tokens of a row tile are split over at most as many workgroups as the CUs hold at once.
+  const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  const int64_t n = std::max(p.items * heads, (int64_t)1), want = !p.many ? 1024 : dp > 128 ? 256 : 512;
   const int64_t span = window > 0 ? std::min(cap, (int64_t)window + tile + step) : cap;
-  p.least = p.many ? 16 : 8;
-  p.splits = (int)std::max((int64_t)1, std::min(want / std::max(n, (int64_t)1), span / (16 * step)));
+  int64_t s = want / n;
+  if (p.many) {
+    // A tile takes a workgroup 2.4 us at 128 columns. Joining takes a launch (4 us) and, for each
+    // split, the time in which its float32 outputs are written and read back at 4 TB/s. The
+    // fewest microseconds of tiles t / s + join j s are at s = sqrt(t / j): 124 pairs of one
+    // head x 3592 tokens 57 -> 22 us where pieces of no less than 16 tiles were taken before.
+    const double tile_us = 2.4 * dp / 128, join_us = (double)rows * group * heads * d * 8 / 4e6;
+    const int64_t tiles = (span + step - 1) / step;
+    s = std::min({s, tiles / 2, (int64_t)std::sqrt(tiles * tile_us / join_us)});
+    if (s < 2 || (tiles + s - 1) / s * tile_us + s * join_us + 4.0 >= tiles * tile_us) s = 1;
+  } else {
+    // pieces of no less than 16 steps of the longest row tile there can be, or 8 of a shorter
+    // one's: from a quarter to twice that, nothing measured changed by more than the noise
+    s = std::min(s, span / (16 * step));
+  }
+  p.least = p.many ? 2 : 8;
+  p.splits = (int)std::max(s, (int64_t)1);
   return p;
 }
 
@@ -887,7 +903,7 @@ size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_he
                                 int64_t max_pages, int ragged, int window) {
   if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
   const cp::AttnPlan p = cp::attn_plan(rows, batch, ragged != 0, q_heads / cache->heads, cache->heads,
-                                       max_pages * cache->block, window);
+                                       cache->head_dim, max_pages * cache->block, window);
   return p.splits > 1 ? (size_t)rows * q_heads * p.splits * (cache->head_dim + 2) * 4 + (size_t)rows * q_heads * 4 : 0;
 }
 
@@ -906,7 +922,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
     return cp::set_error(CP_ERR_ALIGN, "rows and heads of q and out need 16-byte alignment");
   if (q_row < 0 || q_head < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of q");
   const int group = q_heads / cache->heads;
-  const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads,
+  const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads, cache->head_dim,
                                        max_pages * cache->block, window);
   const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window);
   if (need && (!ws || ws_bytes < need))
