@@ -166,7 +166,8 @@ def load(require_gpu=True):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
         _lib = lib
-    if require_gpu and not torch.cuda.is_available():
+    # an initialised runtime has a device; asking the driver again costs 2 us a call
+    if require_gpu and not (torch.cuda.is_initialized() or torch.cuda.is_available()):
         raise RuntimeError("perm_amd needs a HIP device (torch.cuda.is_available() is False)")
     return _lib
 

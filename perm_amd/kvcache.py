@@ -49,20 +49,22 @@ def new(pages, heads, head_dim, block=16, device="cuda"):
 
 def _desc(c):
     """struct cp_kv_cache of a KvCache, its buffers checked against each other."""
-    if c.k.dim() != 4:
+    k, v, ks, vs = c
+    if k.dim() != 4:
         raise ValueError("k codes are [pages, heads, block, head_dim]")
-    pages, heads, block, d = c.k.shape
-    if c.v.shape != (pages, heads, d, block) or c.k_scale.shape != (pages, heads) \
-            or c.v_scale.shape != (pages, heads):
-        raise ValueError(f"cache buffers of {tuple(c.k.shape)}, {tuple(c.v.shape)}, "
-                         f"{tuple(c.k_scale.shape)}, {tuple(c.v_scale.shape)} do not fit")
-    if c.k.dtype != torch.uint8 or c.v.dtype != torch.uint8 \
-            or c.k_scale.dtype != torch.float32 or c.v_scale.dtype != torch.float32:
+    pages, heads, block, d = k.shape
+    if v.shape != (pages, heads, d, block) or ks.shape != (pages, heads) \
+            or vs.shape != (pages, heads):
+        raise ValueError(f"cache buffers of {tuple(k.shape)}, {tuple(v.shape)}, "
+                         f"{tuple(ks.shape)}, {tuple(vs.shape)} do not fit")
+    if k.dtype != torch.uint8 or v.dtype != torch.uint8 \
+            or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise TypeError("cache codes are uint8 and scales float32")
-    if not all(t.is_cuda and t.is_contiguous() for t in c):
+    if not (k.is_cuda and v.is_cuda and ks.is_cuda and vs.is_cuda and k.is_contiguous()
+            and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache buffers must be contiguous and on the GPU")
-    return _lib.KvCacheDesc(c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(),
-                            c.v_scale.data_ptr(), pages, heads, block, d)
+    return _lib.KvCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages,
+                            heads, block, d)
 
 
 def _index(t, dims, what):
@@ -139,8 +141,8 @@ def read(cache, table, offsets, total, dtype=torch.bfloat16):
     if offsets is None:
         raise ValueError("read needs offsets")
     table, _, offsets = _batch(table, None, "", offsets, total)
-    k, v = (torch.empty((total, desc.heads, desc.head_dim), dtype=dtype, device=cache.k.device)
-            for _ in range(2))
+    shape = total, desc.heads, desc.head_dim
+    k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
     _lib.check(lib.cp_kv_read(ctypes.byref(desc), table.data_ptr(), table.shape[0],
                               table.shape[1], offsets.data_ptr(), total, k.data_ptr(),
                               v.data_ptr(), DTYPES[dtype], _lib.stream_ptr()))
@@ -169,7 +171,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     lse = torch.empty((rows, heads), device=q.device) if return_lse else None
     batch, max_pages = table.shape
     ragged = offsets is not None

@@ -62,7 +62,8 @@ def _dtype(dt, what):
 def _rows(x):
     """x as [rows, k] whose rows the kernels can read in place: unit column stride, 16-byte
     aligned rows (copied where they are not)."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     step = 16 // x.element_size()
     if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (
             x.stride(0) % step or x.stride(0) < x.shape[1])):
@@ -97,8 +98,8 @@ def quantize(x):
         raise ValueError(f"rows of {tuple(x.shape)} do not hold whole blocks of {BLOCK}")
     x = _rows(x)
     rows, k = x.shape
-    codes = torch.empty((rows, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(scale_shape(rows, k), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((rows, k // 2), dtype=torch.uint8)
+    scales = x.new_empty(scale_shape(rows, k), dtype=torch.uint8)
     _lib.check(lib.cp_mx4_quantize(x.data_ptr(), code, rows, k, x.stride(0), codes.data_ptr(),
                                    scales.data_ptr(), _lib.stream_ptr()))
     return MxTensor(codes, scales)
@@ -109,7 +110,7 @@ def dequantize(q, dtype=torch.float32):
     lib = _lib.load()
     code = _dtype(dtype, "dtype")
     rows, k = _checked(q, "q")
-    y = torch.empty((rows, k), dtype=dtype, device=q.codes.device)
+    y = q.codes.new_empty((rows, k), dtype=dtype)
     _lib.check(lib.cp_mx4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, k,
                                      y.data_ptr(), code, _lib.stream_ptr()))
     return y
@@ -132,7 +133,7 @@ def matmul(a, b, dtype=torch.bfloat16):
     n, kb = _checked(b, "b")
     if k != kb:
         raise ValueError(f"rows of {k} times rows of {kb}")
-    y = torch.empty((m, n), dtype=dtype, device=a.codes.device)
+    y = a.codes.new_empty((m, n), dtype=dtype)
     nws = lib.cp_mx4_matmul_ws_bytes(m, n, k)
     ws = _lib.workspace(nws, y.device) if nws else None
     _lib.check(lib.cp_mx4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), m, b.codes.data_ptr(),
@@ -156,7 +157,7 @@ def linear(x, w, dtype=None):
         raise ValueError(f"x {tuple(x.shape)} for weights of {k} columns")
     rows = _rows(x)
     m = rows.shape[0]
-    y = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (n,), dtype=dtype)
     nws = lib.cp_mx4_linear_ws_bytes(m, n, k)
     ws = _lib.workspace(nws, x.device) if nws else None
     _lib.check(lib.cp_mx4_linear(rows.data_ptr(), xc, m, rows.stride(0), w.codes.data_ptr(),
