@@ -9,9 +9,9 @@
 //     out = sum_j w_j vcode_j / sum_j (w_j / vs_j)
 //
 // V's scale rides in the exponent, so the codes feed the matrix cores unscaled and w is at
-// most 1 whatever the scales are: w is rounded to float16 (11 bits) as the operand of the
-// second product, for bf16 queries too. Scores, m, the sum and the output accumulate in
-// float32. K codes become q's own 16-bit type, which holds e4m3 exactly.
+// most 2^8 whatever the scales are (m follows the maximum within eight binades): w is rounded
+// to float16 (11 bits) as the operand of the second product, for bf16 queries too. Scores, m,
+// the sum and the output accumulate in float32. K codes become q's own 16-bit type, which holds e4m3 exactly.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -105,8 +105,7 @@ __device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7
 // without leaving their lanes.
 constexpr int kFewTile = 32;
 
-// FULL: d is DP, a constant the addresses fold in.
-template <int DT, int DP, bool FULL>
+template <int DT, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt) {
   constexpr int NC = DP / 64, ND = DP / 16;
   __shared__ float sm_m[4][16], sm_l[4][16];
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   if (row0 < 0 || row0 + n_b > a.rows) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int d = FULL ? DP : c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
+  const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
   const int64_t cap = (int64_t)c.max_pages * blk;
   const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
 
@@ -155,9 +154,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     const T* qp = (const T*)a.q + (real ? (row0 + qi) * a.q_row + (int64_t)qh * a.q_head : 0);
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const bool in = real && (FULL || 64 * k + 16 * g < d);
+      const bool in = real && 64 * k + 16 * g < d;
       const u32x4 z = {0, 0, 0, 0};
-      const T* p = qp + (FULL || 64 * k + 16 * g < d ? 64 * k + 16 * g : 0);
+      const T* p = qp + (64 * k + 16 * g < d ? 64 * k + 16 * g : 0);
       qf[k][0] = *reinterpret_cast<const u32x4*>(p);
       qf[k][1] = *reinterpret_cast<const u32x4*>(p + 8);
       if (!in) qf[k][0] = qf[k][1] = z;
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   // score NaN anyway
   int kcol[NC];
 #pragma unroll
-  for (int k = 0; k < NC; ++k) kcol[k] = FULL || 64 * k + 16 * g < d ? 64 * k + 16 * g : 0;
+  for (int k = 0; k < NC; ++k) kcol[k] = 64 * k + 16 * g < d ? 64 * k + 16 * g : 0;
   uint64_t marked = 0;  // bit 4 i + k: result (i, k) of this lane has seen a NaN code
   u32x2* const mine = reinterpret_cast<u32x2*>(&sm_o[wave][0][0]) + lane;
 
@@ -202,7 +201,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 #pragma unroll
     for (int i = 0; i < ND; ++i) {  // rows past d repeat the last one and are dropped
       vv[i] = *reinterpret_cast<const u32x2*>(vp);
-      if (FULL || 16 * (i + 1) < d) vp += 16 * blk;
+      if (16 * (i + 1) < d) vp += 16 * blk;
     }
     pk = page(jk + 4 * kFewTile);
     pv = page(jv + 4 * kFewTile);
@@ -755,8 +754,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   if (a.lse && hh == 0) a.lse[orow] = l == 0.0f ? kNegInf : (m + __builtin_amdgcn_logf(l)) / kLog2e;
 }
 
-// The splits of a row joined, in a fixed order. d / 4 threads (a group) take a row's columns;
-// with many splits the groups of a workgroup share one row's, otherwise each has its own row.
+// The splits of a row joined, in a fixed order. Bound by latency, or by reading the splits'
+// sums. d / 4 threads (a group) take a row's columns; with more than eight splits the groups
+// of a workgroup share one row's, otherwise each has its own row (attention and join, one row
+// of 16 heads: on 32768 tokens in 64 splits 27.7 us a group a row, 19.5 a workgroup; on 64 x
+// 2048 in two 25.8 and 26.5).
 template <int DT, bool ONE_ROW>
 __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t rows, int d, int most,
                                                         typename Elem<DT>::T* __restrict__ out,
@@ -819,12 +821,17 @@ struct AttnPlan {
   int splits, least;  // at most so many pieces of a row's tiles, of at least so many tiles
 };
 
-// Row tiles of 16 while a sequence has no more (row, head of the group) pairs on average:
-// then reading the cache bounds the call; of 128 above that.
+// Row tiles of 16 while a sequence has up to 64 (row, head of the group) pairs on average, or
+// while all pairs times the tokens they can see are few: four small workgroups a CU start and
+// end faster, and what they read more often comes from the L2. Tiles of 128 above that, where
+// the weights' arithmetic counts. Rows of 8 heads on 4 x 8192 tokens, tiles of 16 / of 128: 16
+// rows 16 / 36 us, 64 25 / 50, 256 83 / 62; 16 heads, 1024 rows on as many tokens 22 / 30, 1024
+// on 2048 44 / 41, 512 on 4096 50 / 41.
 static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int d,
                           int64_t cap, int window) {
   AttnPlan p;
-  p.many = rows * group > 16 * batch;
+  p.many = rows * group > 64 * batch &&
+           (double)rows * group * heads * (window > 0 ? std::min(cap, (int64_t)window + kManyRows) : cap) > 1 << 24;
   const int tile = p.many ? kManyRows : 16, step = p.many ? kTile : kFewTile;
   p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
   // The tokens of a row tile are split over at most as many workgroups as the CUs hold at once.
@@ -835,18 +842,20 @@ static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, i
   if (p.many) {
     // A tile takes a workgroup 2.4 us at 128 columns. Joining takes a launch (4 us) and, for each
     // split, the time in which its float32 outputs are written and read back at 4 TB/s. The
-    // fewest microseconds of tiles t / s + join j s are at s = sqrt(t / j): 124 pairs of one
-    // head x 3592 tokens 57 -> 22 us where pieces of no less than 16 tiles were taken before.
+    // fewest microseconds of tiles t / s + join j s are at s = sqrt(t / j). Against pieces of no
+    // less than 16 tiles, two times 1024 rows of 8 heads of 64 on 4096 tokens take 34 us for 45,
+    // and calls whose tiles fill the CUs the same.
     const double tile_us = 2.4 * dp / 128, join_us = (double)rows * group * heads * d * 8 / 4e6;
     const int64_t tiles = (span + step - 1) / step;
     s = std::min({s, tiles / 2, (int64_t)std::sqrt(tiles * tile_us / join_us)});
     if (s < 2 || (tiles + s - 1) / s * tile_us + s * join_us + 4.0 >= tiles * tile_us) s = 1;
   } else {
-    // pieces of no less than 16 steps of the longest row tile there can be, or 8 of a shorter
-    // one's: from a quarter to twice that, nothing measured changed by more than the noise
-    s = std::min(s, span / (16 * step));
+    // pieces of no less than 8 steps of the longest row tile there can be, or 4 of a shorter
+    // one's (16 and 8, then 4 and 4, for one row of 16 heads on 4 x 1024 tokens 11.9, 9.8, 9.2
+    // us, on 8192 12.9, 10.6, 11.0, on 300 7.5, 7.5, 9.2)
+    s = std::min(s, span / (8 * step));
   }
-  p.least = p.many ? 2 : 8;
+  p.least = p.many ? 2 : 4;
   p.splits = (int)std::max(s, (int64_t)1);
   return p;
 }
@@ -861,8 +870,7 @@ static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, h
     if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
     attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
   } else {
-    if (a.c.d == DP) attn_few_kernel<DT, DP, true><<<grid, 256, 0, st>>>(a, b);
-    else attn_few_kernel<DT, DP, false><<<grid, 256, 0, st>>>(a, b);
+    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b);
   }
   CP_LAUNCHED("cache attention");
   return CP_OK;
@@ -927,6 +935,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window);
   if (need && (!ws || ws_bytes < need))
     return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
+  if (need && !cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
   if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > 0x7FFFFFFF)
     return cp::set_error(CP_ERR_SHAPE, "too many rows");
   cp::AttnArgs a;

@@ -174,14 +174,6 @@ struct MxOperand {
   int64_t rows;
 };
 
-// One lane's 32 codes of row r, block blk (zeros past the end: a zero code adds nothing).
-__device__ __forceinline__ u32x4 mx_load_block(const MxOperand& o, int64_t r, int blk, int k) {
-  u32x4 z = {0, 0, 0, 0};
-  if (r < o.rows && blk * kMxBlock < k)
-    z = *reinterpret_cast<const u32x4*>(o.codes + r * (k / 2) + blk * 16);
-  return z;
-}
-
 // c += a b over one step; SA and SB: which byte of the scale dwords is the operand's.
 template <int SA, int SB>
 __device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
@@ -207,13 +199,15 @@ __device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, in
 //
 // XT >= 0: a's rows come as values of that type and are quantized by every workgroup into
 // its LDS ([row][k / 2] codes, then [row][k / 32] scale bytes), beside the first loads of b.
+constexpr int kFewWaves = 4;
+
 template <int MT, int NT, int XT, int DT>
-__global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b, const void* x, int64_t stride, int k,
+__global__ __launch_bounds__(XT >= 0 ? 1024 : 64 * kFewWaves) void mx4_few_kernel(MxOperand a, MxOperand b, const void* x, int64_t stride, int k,
                                                        int wgs, typename Elem<DT>::T* __restrict__ y) {
-  constexpr int U = MT + NT > 2 ? 4 : 8;  // within the 128 registers of a 16-wave workgroup
+  constexpr int U = MT + NT > 2 ? 4 : 8;
   constexpr bool FUSED = XT >= 0;
   extern __shared__ __align__(16) uint8_t lds[];
-  const int lane = threadIdx.x & 63, g = lane >> 4, W = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, g = lane >> 4, W = FUSED ? blockDim.x >> 6 : kFewWaves;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // blocks of 32 workgroups: XCD x (w % 8) takes four neighbours
   int w = blockIdx.x;
@@ -273,7 +267,7 @@ __global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b,
     typedef typename Elem<XT>::T T;
     const int chunks = k / 8;  // k % 32 == 0: four lanes hold a block
 #pragma unroll 4
-    for (int t = threadIdx.x; t < M * chunks; t += blockDim.x) {
+    for (int t = threadIdx.x; t < M * chunks; t += 64 * W) {
       const int m = t / chunks, c = t - m * chunks;
       float v[8];
       load8<XT>((const T*)x + m * stride + 8 * c, v);
@@ -311,7 +305,7 @@ __global__ __launch_bounds__(1024) void mx4_few_kernel(MxOperand a, MxOperand b,
 #pragma unroll
     for (int j = 0; j < NT; ++j) red[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  for (int t = threadIdx.x; t < MT * NT * 64; t += blockDim.x) {
+  for (int t = threadIdx.x; t < MT * NT * 64; t += 64 * W) {
     f32x4 c = red[t];
     for (int v = 1; v < W; ++v) c += red[v * MT * NT * 64 + t];
     const int l = t & 63, ij = t >> 6;
@@ -629,20 +623,17 @@ static int mx_gemm_edge(const MxPlan& p, const MxOperand& a, const MxOperand& b,
   return mx_gemm<2, 4, 8, 4, DT>(a, b, k, p.splits, y, st);
 }
 
-// Waves of a few-rows workgroup: four, or more while the launch has under eight waves a CU
-// and every wave keeps a step of its own.
-static int mx_few_waves(int64_t wgs, int steps) {
-  int w = 4;
-  while (w < 16 && wgs * w < 2048 && steps > 2 * w) w *= 2;
-  return w;
-}
-
 template <int MT, int NT, int XT, int DT>
 static int mx_few(const MxOperand& a, const MxOperand& b, const void* x, int64_t stride, int k, void* y,
                   hipStream_t st) {
   const int64_t wgs = (b.rows + 16 * NT - 1) / (16 * NT);
   if (wgs > 0x7FFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
-  const int w = mx_few_waves(wgs, (k + kMxStep - 1) / kMxStep);
+  // Waves: four (more gain nothing: 1 x 1024 x 4096 3.3, 3.6, 4.2 us with 4, 8 and 16). Where
+  // they quantize, more while a thread has over four chunks of eight values and the launch
+  // under eight waves a CU (8 x 1024 x 4096 9.4 us with 4, 7.0 with 16).
+  int w = kFewWaves;
+  if (XT >= 0)
+    while (w < 16 && wgs * w < 2048 && a.rows * (k / 8) > 4 * 64 * w) w *= 2;
   size_t lds = (size_t)w * MT * NT * 1024;
   if (XT >= 0) lds = std::max(lds, (size_t)a.rows * (k / 2 + 16 + k / kMxBlock));
   mx4_few_kernel<MT, NT, XT, DT><<<dim3((unsigned)wgs), 64 * w, lds, st>>>(a, b, x, stride, k, (int)wgs,
