@@ -99,10 +99,12 @@ __device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&o
 // One wave per (touched page, head), so nothing waits for another wave. It takes the page's
 // scales from the rows that fall into it, moves the codes held to a larger scale where it has
 // to, and writes the rows' codes: K as they come, V transposed through LDS a slab of 16
-// tokens at a time. Bound by HBM for prompts, by latency for single tokens.
+// tokens at a time. Bound by HBM for prompts (17 000 tokens of 8 heads of 128 in bf16: 105 MB
+// in 24 us, 4.4 TB/s), by latency for single tokens (64 sequences 7.8 us: length, page number,
+// scale and codes are read one after the other).
 //
 // KEEP: pages of 16 tokens and d up to 128, whose values stay in registers between the scale
-// and the codes; larger ones are read twice, the second time from the L2.
+// and the codes; larger ones are read twice, the second time from the L2 (those prompts 32 us).
 template <int DT, bool KEEP>
 __global__ __launch_bounds__(256, KEEP ? 4 : 3) void kv_write_kernel(KvCacheArgs c, KvRows k, KvRows v, KvBatch q, int64_t rows,
                                                        const int* filled) {
@@ -251,7 +253,9 @@ __global__ __launch_bounds__(256, KEEP ? 4 : 3) void kv_write_kernel(KvCacheArgs
 }
 
 // One wave per (16 tokens held, head): the codes' values in rows [total][head][d]. V's slab
-// is transposed through LDS.
+// is transposed through LDS. Bound by HBM, two thirds of the bytes being written (45 000 tokens
+// of 8 heads of 128 to bf16: 276 MB in 53 us, 5.2 TB/s, a copy's rate). All of a wave's loads
+// are issued before the first is used, and five waves a SIMD keep enough of them in flight.
 template <int DT>
 __global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch q, int64_t total,
                                                       typename Elem<DT>::T* __restrict__ ko,

@@ -81,7 +81,9 @@ __device__ __forceinline__ float mx_block_amax(const float (&v)[8]) {
 
 // One workgroup per (128 columns, 64 rows): thread t takes columns 8 (t % 16) .. + 7 of the
 // rows t / 16 + 16 j, j = 0..3, so four lanes share a block and the four bytes of a scale
-// dword come from one thread. Bound by HBM: each value is read once, each byte written once.
+// dword come from one thread. Bound by HBM: each value is read once, each byte written once
+// (14336 x 4096 in float32 with the decode after it: 532 MB in 106.6 us, 104 at a copy's 5.1
+// TB/s). A token's row is a launch of 2.7 us.
 template <int DT>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const typename Elem<DT>::T* __restrict__ x,
                                                            int64_t rows, int k, int64_t stride,
@@ -134,7 +136,7 @@ __device__ __forceinline__ void mx_unpack8(uint32_t c, float scale, float (&v)[8
   }
 }
 
-// The decode, over the same tiles as the quantiser.
+// The decode, over the same tiles as the quantiser and bound as it is.
 template <int DT>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales,
@@ -191,19 +193,20 @@ __device__ __forceinline__ void mx_store4(typename Elem<DT>::T* y, int64_t m, in
     if (n0 + i < N) y[m * N + n0 + i] = (typename Elem<DT>::T)c[i];
 }
 
-// Few rows of a (at most 32): bound by reading b once. A workgroup takes NT 16-row tiles of b
-// and all of a; its waves take the 128-column steps in turn, four or eight steps' loads
-// in flight in each, and join their sums in LDS in wave order. b's codes go from memory to the matrix cores
-// without LDS: each is used once. Four neighbouring workgroups of one XCD share the scale
-// dwords of 64 rows in its L2.
+// Few rows of a (at most 32): bound by reading b once (1 x 14336 x 4096: 31 MB in 6.2 us, 5.0
+// TB/s, most of it from the last-level cache), and by a launch's own 3 us where b is small. A
+// workgroup takes NT 16-row tiles of b and all of a; its waves take the 128-column steps in
+// turn, four or eight steps' loads in flight in each, and join their sums in LDS in wave order.
+// b's codes go from memory to the matrix cores without LDS: each is used once. Four
+// neighbouring workgroups of one XCD share the scale dwords of 64 rows in its L2.
 //
 // XT >= 0: a's rows come as values of that type and are quantized by every workgroup into
 // its LDS ([row][k / 2] codes, then [row][k / 32] scale bytes), beside the first loads of b.
 constexpr int kFewWaves = 4;
 
 template <int MT, int NT, int XT, int DT>
-__global__ __launch_bounds__(XT >= 0 ? 1024 : 64 * kFewWaves) void mx4_few_kernel(MxOperand a, MxOperand b, const void* x, int64_t stride, int k,
-                                                       int wgs, typename Elem<DT>::T* __restrict__ y) {
+__global__ __launch_bounds__(XT >= 0 ? 1024 : 64 * kFewWaves) void mx4_few_kernel(
+    MxOperand a, MxOperand b, const void* x, int64_t stride, int k, int wgs, typename Elem<DT>::T* __restrict__ y) {
   constexpr int U = MT + NT > 2 ? 4 : 8;
   constexpr bool FUSED = XT >= 0;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -369,7 +372,10 @@ __device__ __forceinline__ void mx_store_tile(typename Elem<DT>::T* y, int64_t m
   }
 }
 
-// Large products: a workgroup of WM x WN waves owns a tile of BM x BN results, each wave
+// Large products, bound by the matrix cores where the tiles fill the GPU (8192 x 8192 x 8192:
+// 237 us, 4.6 PFLOP/s; the instruction alone reaches 5.9 on random codes, where power limits
+// it) and by a tile's start and end where there are few stages (4096 x 14336 x 4096: 3.5 rounds
+// of tiles, 3.4 PFLOP/s). A workgroup of WM x WN waves owns a tile of BM x BN results, each wave
 // FM x FN MFMA tiles of it. 256 columns of both operands are staged in LDS a step ahead by
 // loads that write LDS directly, 16 bytes a lane, in two buffers; a row's eight 16-byte
 // chunks are permuted by xor with the row's low three bits, so that the 16 rows of an operand
@@ -542,7 +548,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_gemm_kernel(MxOperand a, 
                             lds + wave * FM * FN * 512);
 }
 
-// y = the splits' sums in split order.
+// y = the splits' sums in split order. Bound by reading them: 4 bytes a split and result.
 template <int DT>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ part, int64_t count, int splits,
                                                        typename Elem<DT>::T* __restrict__ y) {
@@ -651,10 +657,13 @@ template <int DT>
 static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, void* ws, hipStream_t st) {
   const MxPlan p = mx_plan(a.rows, b.rows, k);
   // two tiles of b a workgroup where that still fills the CUs: a's rows are read half as often
-  // (16 x 14336 x 4096: 9.4 us against 10.6; 16 x 4096 x 14336: 14.0 against 9.9)
+  // (one / two: 16 x 8192 x 4096 6.1 / 4.9 us, 16 x 14336 x 4096 10.2 / 7.8, 16 x 4096 x 4096
+  // 3.9 / 4.9, 16 x 4096 x 14336 9.5 / 12.7)
   const bool wide = b.rows >= 8192;
-  if (p.few == 1) return wide ? mx_few<1, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<1, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
-  if (p.few == 2) return wide ? mx_few<2, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<2, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (p.few == 1)
+    return wide ? mx_few<1, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<1, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
+  if (p.few == 2)
+    return wide ? mx_few<2, 2, -1, DT>(a, b, nullptr, 0, k, y, st) : mx_few<2, 1, -1, DT>(a, b, nullptr, 0, k, y, st);
   if (p.splits == 1) return mx_gemm_edge<DT>(p, a, b, k, y, st);
   if (int s = mx_gemm_edge<CP_F32>(p, a, b, k, ws, st)) return s;
   const int64_t count = a.rows * b.rows;
@@ -665,12 +674,12 @@ static int mx_product(const MxOperand& a, const MxOperand& b, int k, void* y, vo
 }
 
 // Few rows are quantized inside the product: every workgroup makes the codes for itself, beside
-// its first loads of b. A launch of their own takes 2.7 us and the gap behind it; fused, 1000 x
-// 1056 weights take 4.2 us with one row and 7.0 with 32 (3.4 without the quantization), 14336 x
-// 4096 ones 8.8 / 12.6 / 15.2 with 1 / 4 / 6 rows (9.1 without). So where a workgroup's share,
-// m k, and all workgroups', m k n, are small.
+// its first loads of b. GPU time fused / in a launch before it: 4 rows x 1000 x 1056 4.3 / 5.2
+// us, 16 5.6 / 5.3, 1 x 4096 x 4096 4.4 / 5.5, 4 5.6 / 5.6, 8 7.2 / 5.8, 1 x 14336 x 4096 8.6 /
+// 8.9, 2 9.8 / 9.0: even where a workgroup's share m k reaches 2^14 values or all workgroups'
+// m k n 2^26. The second launch also costs the host 4 us, so the bounds are a little above.
 static bool mx_fuses(int64_t m, int64_t n, int64_t k) {
-  return m <= 32 && m * k <= 32768 && m * k * n <= ((int64_t)1 << 28);
+  return m <= 32 && m * k <= 24576 && m * k * n <= ((int64_t)1 << 27);
 }
 
 template <int XT>
