@@ -433,7 +433,8 @@ int cp_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t m,
 size_t cp_mx4_linear_ws_bytes(int64_t m, int64_t n, int64_t k);
 
 /* y [m, n] = x w^T for MXFP4 weights w [n, k]: x [m, k] is quantized as cp_mx4_quantize
- * does, then multiplied as cp_mx4_matmul does. */
+ * does, then multiplied as by cp_mx4_matmul (few rows in one launch, whose sums may be in
+ * another order, again one that depends on the sizes alone). */
 int cp_mx4_linear(const void* x, int x_dtype, int64_t m, int64_t row_stride,
                   const uint8_t* w_codes, const uint8_t* w_scales, int64_t n, int64_t k, void* y,
                   int y_dtype, void* ws, size_t ws_bytes, void* stream);
@@ -467,7 +468,8 @@ int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t 
 int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, int64_t max_pages,
                const int32_t* offsets, int64_t total, void* k, void* v, int dtype, void* stream);
 
-/* Workspace bytes of cp_kv_attention (0: none); ragged: offsets are given. */
+/* Workspace bytes of cp_kv_attention (256-byte aligned; 0: none, ws may be NULL); ragged:
+ * offsets are given. */
 size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads,
                                 int64_t batch, int64_t max_pages, int ragged, int window);
 

@@ -361,10 +361,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 // second product's operand at step s as they stand.
 //
 // Bound by the VALU and the matrix cores together (per 32 rows x 64 tokens a wave has 32 MFMAs
-// of 32 clocks and about 360 other instructions, a third of them the conversions; counters
-// show both busy 91 % of the time in sum): two times 4096 rows of 16 heads on 8192 tokens 309
-// us, 0.92 PFLOP/s, 8192 rows of 32 heads 558 us, 0.98. Codes converted once for the workgroup
-// and kept in 16 bits double what the waves read from LDS, and lose (367 us against 341).
+// of 32 clocks and about 360 other instructions, a third of them the conversions; counters show
+// the VALU busy 66 % and the matrix cores 40 % of the time, 57 and 34 before a wave gave way in
+// its second product): two times 4096 rows of 16 heads on 8192 tokens 309 us, 0.92 PFLOP/s,
+// 8192 rows of 32 heads 558 us, 0.98. Codes converted once for the workgroup and kept in 16
+// bits double what the waves read from LDS, and lose (367 us against 341).
 //
 // LDS rows hold 16-byte chunks permuted by xor, so that eight lanes of a read fall into
 // different banks: K rows (a token each) with bits 0, 1 and 4 of the token, V rows (a column

@@ -142,7 +142,8 @@ def read(cache, table, offsets, total, dtype=torch.bfloat16):
         raise ValueError("read needs offsets")
     table, _, offsets = _batch(table, None, "", offsets, total)
     shape = total, desc.heads, desc.head_dim
-    k, v = cache.k.new_empty(shape, dtype=dtype), cache.k.new_empty(shape, dtype=dtype)
+    k = cache.k.new_empty(shape, dtype=dtype)
+    v = torch.empty_like(k)
     _lib.check(lib.cp_kv_read(ctypes.byref(desc), table.data_ptr(), table.shape[0],
                               table.shape[1], offsets.data_ptr(), total, k.data_ptr(),
                               v.data_ptr(), DTYPES[dtype], _lib.stream_ptr()))
@@ -171,7 +172,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     lse = torch.empty((rows, heads), device=q.device) if return_lse else None
     batch, max_pages = table.shape
     ragged = offsets is not None
