@@ -843,29 +843,45 @@ static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, i
            (double)rows * group * heads * (window > 0 ? std::min(cap, (int64_t)window + kManyRows) : cap) > 1 << 24;
   const int tile = p.many ? kManyRows : 16, step = p.many ? kTile : kFewTile;
   p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
-  // The tokens of a row tile are split over at most as many workgroups as the CUs hold at once.
-  const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  const int64_t n = std::max(p.items * heads, (int64_t)1), want = !p.many ? 1024 : dp > 128 ? 256 : 512;
+  const int64_t n = std::max(p.items * heads, (int64_t)1);
   const int64_t span = window > 0 ? std::min(cap, (int64_t)window + tile + step) : cap;
-  int64_t s = want / n;
+  int64_t s = 1;
   if (p.many) {
-    // A tile takes a workgroup 2.4 us at 128 columns. Joining takes a launch (4 us) and, for each
-    // split, the time in which its float32 outputs are written and read back at 4 TB/s. The
-    // fewest microseconds of tiles t / s + join j s are at s = sqrt(t / j). Against pieces of no
-    // less than 16 tiles, two times 1024 rows of 8 heads of 64 on 4096 tokens take 34 us for 45,
-    // and calls whose tiles fill the CUs the same.
-    const double tile_us = 2.4 * dp / 128, join_us = (double)rows * group * heads * d * 8 / 4e6;
+    // The tokens of a row tile are split as takes the fewest predicted microseconds. A join takes
+    // a launch (4) and the time in which the splits' float32 outputs are written and read back.
+    const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    const double mb = (double)rows * group * heads * d * 8 / 1e6;  // those outputs, a split
     const int64_t tiles = (span + step - 1) / step;
-    s = std::min({s, tiles / 2, (int64_t)std::sqrt(tiles * tile_us / join_us)});
-    if (s < 2 || (tiles + s - 1) / s * tile_us + s * join_us + 4.0 >= tiles * tile_us) s = 1;
+    if (n < 128) {
+      // CUs to spare: a tile takes 2.2 (at 128 columns) while no more workgroups run than fit at
+      // once (two a CU), and tiles t / s + join j s are fewest at s = sqrt(t / j). 40 row tiles
+      // on 32768 tokens: 674 us in one, 127 in six, 100 in eight, 92 in sixteen (99 as chosen).
+      const double tile_us = 2.2 * dp / 128, join_us = mb / 4;
+      const int64_t x = std::min({(dp > 128 ? 256 : 512) / n, tiles / 2, (int64_t)std::sqrt(tiles * tile_us / join_us)});
+      if (x > 1 && (tiles + x - 1) / x * tile_us + x * join_us + 4.0 < tiles * tile_us) s = x;
+    } else {
+      // A CU or more for each: the tiles of all pieces at 1.6 a CU (two workgroups on one are
+      // hardly faster than one after the other), and half a piece for the last to end, lengths
+      // being ragged. 264 row tiles, 1000 rows each of two sequences up to 4096: 169 us in one,
+      // 110 in two, 88 in three, 89 in four, 101 in six; 616, 2400 rows of two up to 8192: 359,
+      // 280, 248, 268, 296; 520, 4096 rows of one on 8192: 255, 249, 261, 271, 296.
+      const double cus = dp > 128 ? 128 : 256, tile_us = dp > 128 ? 3.2 : 1.6;
+      double best = 0.0;
+      for (int64_t x = 1; x == 1 || (x <= 4 && x <= tiles / 2); ++x) {
+        const double us = (std::max(1.0, n * x / cus) + 0.5) * ((double)tiles / x + 1) * tile_us +
+                          (x > 1 ? 4.0 + x * mb / 6 : 0.0);
+        if (x == 1 || us < best) best = us, s = x;
+      }
+    }
   } else {
-    // pieces of no less than 8 steps of the longest row tile there can be, or 4 of a shorter
-    // one's (16 and 8, then 4 and 4, for one row of 16 heads on 4 x 1024 tokens 11.9, 9.8, 9.2
-    // us, on 8192 12.9, 10.6, 11.0, on 300 7.5, 7.5, 9.2)
-    s = std::min(s, span / (8 * step));
+    // As many workgroups as the CUs hold at once, but pieces of no less than 8 steps of the
+    // longest row tile there can be, or 4 of a shorter one's (16 and 8, then 4 and 4, for one row
+    // of 16 heads on 4 x 1024 tokens 11.9, 9.8, 9.2 us, on 8192 12.9, 10.6, 11.0, on 300 7.5,
+    // 7.5, 9.2).
+    s = std::max((int64_t)1, std::min(1024 / n, span / (8 * step)));
   }
   p.least = p.many ? 2 : 4;
-  p.splits = (int)std::max(s, (int64_t)1);
+  p.splits = (int)s;
   return p;
 }
 
