@@ -279,3 +279,10 @@ def test_rows_quantized_in_the_product(mx, m, n, k):
     a[m // 2] = 0
     _check_product(torch.where(y.isnan(), 0, y), a, b, k, torch.bfloat16)
     _check_product(torch.where(want.isnan(), 0, want), a, b, k, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 48, 24576), (9, 333, 1024), (16, 1000, 1536), (23, 77, 1056), (32, 130, 768),
+                                   (5, 24000, 1024)])
+def test_rows_quantized_by_more_waves(mx, m, n, k):
+    """The largest shares that are quantized inside the product, by eight and sixteen waves."""
+    test_rows_quantized_in_the_product(mx, m, n, k)
