@@ -5,13 +5,20 @@
 // codes in e4m3 and power-of-two scales ks, vs of each page and head, in base 2:
 //
 //     t_j = (q . kcode_j) * ks_j * scale * log2 e + log2 vs_j
-//     w_j = 2^(t_j - m),  m the running maximum of t
+//     w_j = 2^(t_j - m + 11),  m the running maximum of t within four binades
 //     out = sum_j w_j vcode_j / sum_j (w_j / vs_j)
 //
 // V's scale rides in the exponent, so the codes feed the matrix cores unscaled and w is at
-// most 2^8 whatever the scales are (m follows the maximum within eight binades): w is rounded
-// to float16 (11 bits) as the operand of the second product, for bf16 queries too. Scores, m,
-// the sum and the output accumulate in float32. K codes become q's own 16-bit type, which holds e4m3 exactly.
+// most 2^15 whatever the scales are. Scores, m, the sum and the output accumulate in float32. K
+// codes become q's own 16-bit type, which holds e4m3 exactly.
+//
+// w is rounded as the second product's operand, and must not be lost for being small beside
+// others: where a first token takes most of the softmax and has no values, or a page with a large
+// V scale holds zeros in a column, small weights are all that the result consists of. It is either
+// one float16, which has 11 bits of a weight down to 2^-14, 25 binades below the running
+// maximum; or two bfloat16 terms, 16 bits of it down to 2^-126, for twice the MFMAs. Few query rows
+// always take the two terms (bound by reading the cache, they cost nothing); of many rows, a wave
+// takes them from the first unit on in which one of its rows sees a smaller weight.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,6 +36,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;       // tokens per step of a wave
 constexpr float kNegInf = -__builtin_inff();
+// Weights are 2^kLift above 2^(t - m), which uses float16's range up to 2^15: m moves when a t
+// passes it by kLag. A t more than kDeep below m has a weight below float16's normal range.
+constexpr float kLift = 11.0f, kLag = 4.0f, kDeep = kLift + 14.0f;
 
 struct AttnArgs {
   KvCacheArgs c;
@@ -87,6 +97,27 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// Two weights as bfloat16 terms: hi rounded, lo the rest rounded.
+struct Weights2 {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Weights2 weights2(float e0, float e1) {
+  const uint32_t hi = pack2<CP_BF16>(e0, e1);
+  return {hi, pack2<CP_BF16>(e0 - __uint_as_float(hi << 16), e1 - __uint_as_float(hi & 0xFFFF0000u))};
+}
+
+// What sums over an old maximum m are multiplied by when it moves to mn: the square of this. The
+// sum of weights takes it in two steps, being as large as V's scales are small (up to 2^60 times
+// the weights), and outlives a move of more than 126 binades.
+__device__ __forceinline__ float half_move(float m, float mn) {
+  return exp2_fast(0.5f * (m - (mn == kNegInf ? 0.0f : mn)));
+}
+
+// Log-sum-exp of a row whose weights, lifted by 2^kLift, sum to l over the maximum m.
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? kNegInf : (m - kLift + __builtin_amdgcn_logf(l)) / kLog2e;
+}
 
 // Bytes of w that are NaN codes (0x7F or 0xFF) as 0x80 flags: 0x7F is the only magnitude
 // that carries out of seven bits when one is added.
@@ -219,7 +250,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     }
     const float kc = ks * a.scale;
     const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
-    const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs) & 0x7F800000u));
     bool edge = false;  // a token of this lane that its row does not see
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -234,20 +264,21 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     float tm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                      fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     tm = __builtin_fmaf(tm, kc, lv);
-    // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
-    // the row's lanes seldom have to exchange their largest and rescale the outputs
-    if (__any(tm > m + 8.0f)) {
+    // the running maximum moves only when a t passes it by kLag, so the row's lanes seldom have
+    // to exchange their largest and rescale the outputs
+    if (__any(tm > m + kLag)) {
       tm = fmaxf(tm, __shfl_xor(tm, 16));
       tm = fmaxf(tm, __shfl_xor(tm, 32));
-      const float mn = fmaxf(m, tm);
-      const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
+      const float mn = fmaxf(m, tm), ah = half_move(m, mn), al = ah * ah;
       m = mn;
-      l *= al;
+      l = l * ah * ah;
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= al;
     }
-    const float off = lv - (m == kNegInf ? 0.0f : m);
-    u32x4 w;
+    // w / vs, the sum's term, and w from it: where V's scales are far apart w may fall out of
+    // float32's range beside the other results, but its term does not beside the sum
+    const float off = kLift - (m == kNegInf ? 0.0f : m);
+    u32x4 wh, wl;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -256,9 +287,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
         const float e0 = exp2_fast(__builtin_fmaf(sc[t][i], kc, off));
         const float e1 = exp2_fast(__builtin_fmaf(sc[t][i + 1], kc, off));
         sum += e0 + e1;
-        w[2 * t + (i >> 1)] = pack2<CP_F16>(e0, e1);
+        const Weights2 x = weights2(e0 * vs, e1 * vs);
+        wh[2 * t + (i >> 1)] = x.hi, wl[2 * t + (i >> 1)] = x.lo;
       }
-    l = __builtin_fmaf(sum, iv, l);
+    l += sum;
     // a code that a row does not see must not reach it, not even as 0 * NaN: NaN codes are
     // taken out of the product and put back into the rows that do see them
     bool nan = false;
@@ -296,7 +328,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     for (int i = 0; i < ND; ++i) {
       u32x2 y = vv[i];
       if (nan) y = mine[64 * i];
-      o[i] = mfma16<CP_F16>(codes_to_16<CP_F16>(y[0], y[1]), w, o[i]);
+      const u32x4 x = codes_to_16<CP_BF16>(y[0], y[1]);
+      o[i] = mfma16<CP_BF16>(x, wh, o[i]);
+      o[i] = mfma16<CP_BF16>(x, wl, o[i]);
     }
   }
   l += __shfl_xor(l, 16);
@@ -321,8 +355,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   const float ms = mm == kNegInf ? 0.0f : mm;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    f[w] = exp2_fast(sm_m[w][row] - ms);
-    ll += sm_l[w][row] * f[w];
+    const float fh = half_move(sm_m[w][row], ms);
+    f[w] = fh * fh;
+    ll += sm_l[w][row] * fh * fh;
   }
   const int64_t orow = (row0 + rr / a.group) * ((int64_t)a.group * c.heads) + h * a.group + rr % a.group;
   const SplitParts sp = split_parts(a);
@@ -348,7 +383,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     float* pm = sp.ml + (orow * a.splits + split) * 2;
     pm[0] = mm, pm[1] = ll;
   } else if (a.lse) {
-    a.lse[orow] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+    a.lse[orow] = row_lse(mm, ll);
   }
 }
 
@@ -361,10 +396,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 // second product's operand at step s as they stand.
 //
 // Bound by the VALU and the matrix cores together (per 32 rows x 64 tokens a wave has 32 MFMAs
-// of 32 clocks and about 360 other instructions, a third of them the conversions; counters show
+// of 32 clocks and about 380 other instructions, a third of them the conversions; counters showed
 // the VALU busy 66 % and the matrix cores 40 % of the time, 57 and 34 before a wave gave way in
-// its second product): two times 4096 rows of 16 heads on 8192 tokens 309 us, 0.92 PFLOP/s,
-// 8192 rows of 32 heads 558 us, 0.98. Codes converted once for the workgroup and kept in 16
+// its second product): two times 4096 rows of 16 heads on 8192 tokens 320 us, 0.88 PFLOP/s,
+// 8192 rows of 32 heads 594 us, 0.93; 3 % of it goes into looking for weights that one float16
+// does not hold. Codes converted once for the workgroup and kept in 16
 // bits double what the waves read from LDS, and lose (367 us against 341).
 //
 // LDS rows hold 16-byte chunks permuted by xor, so that eight lanes of a read fall into
@@ -555,7 +591,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   auto read_v = [&](int buf, int s, int i) {
     vr[i] = *reinterpret_cast<const u32x4*>(lds + buf * BUF + KB + q * 64 + i * 32 * 64 + ((32 * s + 16 * hh) ^ vsw));
   };
-  float top = kNegInf;  // the largest raw score of the unit at hand (this lane's half of its row)
+  // the largest and least raw scores of the unit at hand (this lane's half of its row)
+  float top = kNegInf, bot = -kNegInf;
   uint64_t marked[NC > 4 ? 2 : 1] = {};  // bit 16 i + j (of a word for four i): result (i, j) has seen a NaN code
   int buf = 0, nbuf = 1;                 // buffers of this tile and the next
   int pg[2] = {0, 0};  // pages of the next tile's scales
@@ -568,8 +605,89 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     pg[0] = pn.g[0], pg[1] = pn.g[1];
     lookup(tb + 2);
     __syncthreads();
+  }
+  // masks the scores of unit s of the tile at j0, of which the row may not see every token
+  auto mask = [&](f32x16& x, int j0, int s, bool hv) {
+    // this lane's first token, hidden from the compiler: it would compare all of them on
+    // every tile, ahead of the branch
+    int j1 = j0 + 32 * s + 16 * hh;
+    asm volatile("" : "+v"(j1));
+    top = kNegInf, bot = -kNegInf;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) read_k(0, 0, k);
+    for (int i = 0; i < 16; ++i) {
+      const bool see = hv && j1 + i >= lo && j1 + i < hi;
+      bot = fminf(bot, see ? x[i] : -kNegInf);
+      x[i] = see ? x[i] : kNegInf;
+      top = fmaxf(top, x[i]);
+    }
+  };
+  // As in attn_few_kernel: V's NaN codes of that unit leave the product and return to the rows
+  // that see them, in a loop over the wave's LDS that costs the common path no registers.
+  u32x4* const mine = reinterpret_cast<u32x4*>(lds + 3 * BUF) + wave * NC * 64 + lane;
+  auto take_nan = [&](int j0, int s, bool hv) {
+    u32x4 one[2];
+    int j1 = j0 + 32 * s + 16 * hh;
+    asm volatile("" : "+v"(j1));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = j1 + 2 * k;
+      one[k >> 2][k & 3] = (hv && j >= lo && j < hi ? 0x3C00u : 0u) | (hv && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
+    }
+#pragma unroll
+    for (int i0 = 0; i0 < NC; i0 += 4) {
+#pragma clang loop unroll(disable)
+      for (int i = i0; i < min(NC, i0 + 4); ++i) {
+        u32x4 x = mine[64 * i], f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t fl = nan_flags(x[k]) >> 7;
+          x[k] &= ~(fl * 0xFFu);
+          f[k] = fl * 0x38u;  // 1.0 where the code was NaN
+        }
+        mine[64 * i] = x;
+        f32x16 cnt;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
+        cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[0], cnt);
+        cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[1], cnt);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) bits |= cnt[j] > 0.0f ? 1u << j : 0;
+        marked[i0 >> 2] |= (uint64_t)bits << (16 * (i - i0));
+      }
+    }
+  };
+  // the running maximum and what hangs on it, when a row's t passes it by kLag; called seldom
+  auto move_max = [&](float tm) {
+    tm = fmaxf(tm, __shfl_xor(tm, 32));
+    const float mn = fmaxf(m, tm), ah = half_move(m, mn), al = ah * ah;
+    m = mn;
+    l = l * ah * ah;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) o[i] *= al;
+  };
+  int tile = tb, last = 0;
+  int wide = -1;  // the unit of the tile at hand from which on weights take two terms; -1: none does
+  bool all, edge;
+  auto enter = [&] {  // the tile at hand
+    const int j0 = tile * kTile;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) ks[s] = nks[s], vs[s] = nvs[s], have[s] = nhave[s];
+    all = !__any(!have[0] || !have[1]);
+    edge = !all || j0 < wlo || j0 + kTile > whi;
+    last = nbuf == 2 ? 0 : nbuf + 1;  // the tile before this one's: the one after the next's
+  };
+  auto advance = [&] {  // ahead of a tile's second unit
+    __syncthreads();    // the next tile has landed, and every wave is done with the one before this
+    next_scales(pg);
+    pg[0] = pn.g[0], pg[1] = pn.g[1];
+    fetch(last, tile + 2, pn.k, pn.v);  // past the end: some page's codes, never used
+    lookup(tile + 3);
+  };
+  if (tb < te) enter();
+  while (tile < te) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) read_k(buf, 0, k);
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[0][j] = 0.0f;
 #pragma unroll
@@ -577,82 +695,137 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
     }
-    top = sc[0][0];
+    top = bot = sc[0][0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]);
-  }
-  for (int tile = tb; tile < te; ++tile) {
-    const int j0 = tile * kTile;
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
+    wide = -1;
+    while (tile < te) {
+      const int j0 = tile * kTile;
+      unrolled2([&](auto S) {
+        constexpr int s = S;
+        if (s == 1 && wide >= 0) return;
+        const float kc = ks[s] * a.scale;
+        const float lg = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
+        const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
+        if constexpr (s == 1) advance();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) ks[s] = nks[s], vs[s] = nvs[s], have[s] = nhave[s];
-    const bool all = !__any(!have[0] || !have[1]);
-    const bool edge = !all || j0 < wlo || j0 + kTile > whi;
-    const int last = nbuf == 2 ? 0 : nbuf + 1;  // the tile before this one's: the one after the next's
-    unrolled2([&](auto S) {
-      constexpr int s = S;
-      const float kc = ks[s] * a.scale;
-      const float lg = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
-      const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
-      if constexpr (s == 1) {
-        __syncthreads();  // the next tile has landed, and every wave is done with the one before this
-        next_scales(pg);
-        pg[0] = pn.g[0], pg[1] = pn.g[1];
-        fetch(last, tile + 2, pn.k, pn.v);  // past the end: some page's codes, never used
-        lookup(tile + 3);
+        for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
+        if (edge) mask(sc[s], j0, s, have[s]);
+        // the largest t of the unit: kc > 0, so t rises with the raw score
+        const float tm = __builtin_fmaf(top, kc, lg);
+        if (__any(tm > m + kLag)) move_max(tm);
+        if (__any(__builtin_fmaf(bot, kc, lg) < m - kDeep)) {
+          wide = s;
+          return;
+        }
+        const float off = lg + kLift - (m == kNegInf ? 0.0f : m);
+        // one MFMA of the next unit's scores, then as many of this unit's weights as it covers
+        u32x4 w[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[1 - s][j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2 * NC; ++k) {
+          const u32x4 x = kr[k >> 1];
+          sc[1 - s] = mfma32<DT>(k & 1 ? codes_to_16<DT>(x[2], x[3]) : codes_to_16<DT>(x[0], x[1]), qf[k >> 1][k & 1],
+                                 sc[1 - s]);
+#pragma unroll
+          for (int i = 8 * k / (2 * NC); i < 8 * (k + 1) / (2 * NC); ++i) {
+            const float e0 = exp2_fast(__builtin_fmaf(sc[s][2 * i], kc, off));
+            const float e1 = exp2_fast(__builtin_fmaf(sc[s][2 * i + 1], kc, off));
+            sum += e0 + e1;
+            uint32_t e = pack2<CP_F16>(e0, e1);
+            asm volatile("" : "+v"(e));  // here, not past the branch below
+            w[i >> 2][i & 3] = e;
+          }
+          if (k == NC) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) read_v(buf, s, i);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        l = __builtin_fmaf(sum, iv, l);
+        if (edge) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) any |= nan_flags(vr[i][k]);
+          if (__any(any != 0)) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) mine[64 * i] = vr[i];
+            take_nan(j0, s, have[s]);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) vr[i] = mine[64 * i];
+          }
+        }
+        // The second product, and the next unit's largest and least scores beside it. It gives way to the
+        // SIMD's other wave: its MFMAs need an issue slot in 32 clocks, the weights every slot, and
+        // two waves that keep out of step overlap (335 -> 309 us for two prompts of 4096 rows).
+        __builtin_amdgcn_s_setprio(0);
+        top = bot = sc[1 - s][0];
+#pragma unroll
+        for (int k = 0; k < 2 * NC; ++k) {
+          const int i = k % NC;
+          const u32x4 x = vr[i];
+          o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), w[k / NC], o[i]);
+#pragma unroll
+          for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
+            top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(1);
+      });
+      if (wide >= 0) break;
+      buf = nbuf;
+      nbuf = last;
+      ++tile;
+      enter();
+    }
+    // Weights in two terms, a unit at a time from its scores on, until a tile needs no more of
+    // them. Every tile has its one barrier in either loop, so waves of both kinds keep in step.
+    // Two prompts of 4096 rows whose scores' deviation is 5.5 (all units here) 495 us, 1.4 (a few) 331.
+    bool deep = true;  // the tile at hand needs them
+    for (bool ahead = wide == 1; tile < te;) {
+      const int s = wide, j0 = tile * kTile;
+      if (s == 1 && !ahead) advance();
+      ahead = false;
+      const bool hv = s ? have[1] : have[0];
+      const float v1 = s ? vs[1] : vs[0], kc = (s ? ks[1] : ks[0]) * a.scale;
+      const float lg = (float)((int)(__float_as_uint(v1) >> 23) - 127);
+      f32x16& x = sc[0];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        read_k(buf, s, k);
+        x = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], x);
+        x = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], x);
       }
-#pragma unroll
-      for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
       if (edge) {
-        // this lane's first token, hidden from the compiler: it would compare all of them on
-        // every tile, ahead of the branch
-        int j1 = j0 + 32 * s + 16 * hh;
-        asm volatile("" : "+v"(j1));
+        mask(x, j0, s, hv);
+      } else {
+        top = bot = x[0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[s][i] = have[s] && j1 + i >= lo && j1 + i < hi ? sc[s][i] : kNegInf;
-        top = sc[s][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[s][i]);
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
       }
-      // the largest t of the unit: kc > 0, so t rises with the raw score
-      float tm = __builtin_fmaf(top, kc, lg);
-      // the running maximum moves only when a weight would pass 2^8: float16 holds that, and
-      // the row's two lanes seldom have to exchange their largest and rescale the outputs
-      if (__any(tm > m + 8.0f)) {
-        tm = fmaxf(tm, __shfl_xor(tm, 32));
-        const float mn = fmaxf(m, tm);
-        const float al = exp2_fast(m - (mn == kNegInf ? 0.0f : mn));
-        m = mn;
-        l *= al;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) o[i] *= al;
-      }
-      const float off = lg - (m == kNegInf ? 0.0f : m);
-      // one MFMA of the next unit's scores, then as many of this unit's weights as it covers
-      u32x4 w[2];
+      const float tm = __builtin_fmaf(top, kc, lg);
+      if (__any(tm > m + kLag)) move_max(tm);
+      deep |= __any(__builtin_fmaf(bot, kc, lg) < m - kDeep);
+      // as in attn_few_kernel, the sum's terms and the weights from them
+      const float off = kLift - (m == kNegInf ? 0.0f : m);
+      u32x4 wh[2], wl[2];
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sc[1 - s][j] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 2 * NC; ++k) {
-        const u32x4 x = kr[k >> 1];
-        sc[1 - s] = mfma32<DT>(k & 1 ? codes_to_16<DT>(x[2], x[3]) : codes_to_16<DT>(x[0], x[1]), qf[k >> 1][k & 1],
-                               sc[1 - s]);
-#pragma unroll
-        for (int i = 8 * k / (2 * NC); i < 8 * (k + 1) / (2 * NC); ++i) {
-          const float e0 = exp2_fast(__builtin_fmaf(sc[s][2 * i], kc, off));
-          const float e1 = exp2_fast(__builtin_fmaf(sc[s][2 * i + 1], kc, off));
-          sum += e0 + e1;
-          uint32_t e = pack2<CP_F16>(e0, e1);
-          asm volatile("" : "+v"(e));  // here, not past the branch below
-          w[i >> 2][i & 3] = e;
-        }
-        if (k == NC) {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) read_v(buf, s, i);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 8; ++i) {
+        const float e0 = exp2_fast(__builtin_fmaf(x[2 * i], kc, off)), e1 = exp2_fast(__builtin_fmaf(x[2 * i + 1], kc, off));
+        sum += e0 + e1;
+        const Weights2 w = weights2(e0 * v1, e1 * v1);
+        wh[i >> 2][i & 3] = w.hi, wl[i >> 2][i & 3] = w.lo;
       }
-      l = __builtin_fmaf(sum, iv, l);
+      l += sum;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) read_v(buf, s, i);
       if (edge) {
         uint32_t any = 0;
 #pragma unroll
@@ -660,65 +833,30 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
 #pragma unroll
           for (int k = 0; k < 4; ++k) any |= nan_flags(vr[i][k]);
         if (__any(any != 0)) {
-          // as in attn_few_kernel: NaN codes leave the product and return to the rows that see
-          // them, in a loop over the wave's LDS that costs the common path no registers
-          u32x4* const mine = reinterpret_cast<u32x4*>(lds + 3 * BUF) + wave * NC * 64 + lane;
-          u32x4 one[2];
-          int j1 = j0 + 32 * s + 16 * hh;
-          asm volatile("" : "+v"(j1));
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int j = j1 + 2 * k;
-            one[k >> 2][k & 3] = (have[s] && j >= lo && j < hi ? 0x3C00u : 0u) |
-                                 (have[s] && j + 1 >= lo && j + 1 < hi ? 0x3C000000u : 0u);
-          }
 #pragma unroll
           for (int i = 0; i < NC; ++i) mine[64 * i] = vr[i];
-#pragma unroll
-          for (int i0 = 0; i0 < NC; i0 += 4) {
-#pragma clang loop unroll(disable)
-            for (int i = i0; i < min(NC, i0 + 4); ++i) {
-              u32x4 x = mine[64 * i], f;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t fl = nan_flags(x[k]) >> 7;
-                x[k] &= ~(fl * 0xFFu);
-                f[k] = fl * 0x38u;  // 1.0 where the code was NaN
-              }
-              mine[64 * i] = x;
-              f32x16 cnt;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) cnt[j] = 0.0f;
-              cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[0], f[1]), one[0], cnt);
-              cnt = mfma32<CP_F16>(codes_to_16<CP_F16>(f[2], f[3]), one[1], cnt);
-              uint32_t bits = 0;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) bits |= cnt[j] > 0.0f ? 1u << j : 0;
-              marked[i0 >> 2] |= (uint64_t)bits << (16 * (i - i0));
-            }
-          }
+          take_nan(j0, s, hv);
 #pragma unroll
           for (int i = 0; i < NC; ++i) vr[i] = mine[64 * i];
         }
       }
-      // The second product, and the next unit's largest score beside it. It gives way to the
-      // SIMD's other wave: its MFMAs need an issue slot in 32 clocks, the weights every slot, and
-      // two waves that keep out of step overlap (335 -> 309 us for two prompts of 4096 rows).
-      __builtin_amdgcn_s_setprio(0);
-      top = sc[1 - s][0];
 #pragma unroll
       for (int k = 0; k < 2 * NC; ++k) {
         const int i = k % NC;
-        const u32x4 x = vr[i];
-        o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), w[k / NC], o[i]);
-#pragma unroll
-        for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j) top = fmaxf(top, sc[1 - s][j]);
-        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 y = vr[i], c16 = k < NC ? codes_to_16<CP_BF16>(y[0], y[1]) : codes_to_16<CP_BF16>(y[2], y[3]);
+        o[i] = mfma32<CP_BF16>(c16, wh[k / NC], o[i]);
+        o[i] = mfma32<CP_BF16>(c16, wl[k / NC], o[i]);
       }
-      __builtin_amdgcn_s_setprio(1);
-    });
-    buf = nbuf;
-    nbuf = last;
+      wide = 1 - s;
+      if (s == 1) {
+        buf = nbuf;
+        nbuf = last;
+        ++tile;
+        enter();
+        if (!deep) break;
+        deep = false;
+      }
+    }
   }
   __syncthreads();  // the last fetch is in before LDS is given up
 #pragma unroll
@@ -760,7 +898,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       v[1] = pack2<DT>(o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv);
       if (x < d) *reinterpret_cast<u32x2*>(op + x) = v;
     }
-  if (a.lse && hh == 0) a.lse[orow] = l == 0.0f ? kNegInf : (m + __builtin_amdgcn_logf(l)) / kLog2e;
+  if (a.lse && hh == 0) a.lse[orow] = row_lse(m, l);
 }
 
 // The splits of a row joined, in a fixed order. Bound by latency, or by reading the splits'
@@ -799,9 +937,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
   if (mine) {
 #pragma unroll 4
     for (int s = ONE_ROW ? grp : 0; s < splits; s += ONE_ROW ? NG : 1) {
-      const float f = exp2_fast(pm[2 * s] - ms);
-      ll += pm[2 * s + 1] * f;
-      v += *reinterpret_cast<const f32x4*>(po + (int64_t)s * d + c) * f;
+      const float fh = half_move(pm[2 * s], ms);
+      ll += pm[2 * s + 1] * fh * fh;
+      v += *reinterpret_cast<const f32x4*>(po + (int64_t)s * d + c) * (fh * fh);
     }
   }
   if constexpr (ONE_ROW) {
@@ -821,7 +959,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
   y[0] = pack2<DT>(v[0] * inv, v[1] * inv);
   y[1] = pack2<DT>(v[2] * inv, v[3] * inv);
   *reinterpret_cast<u32x2*>(out + row * d + c) = y;
-  if (lse && c == 0) lse[row] = ll == 0.0f ? kNegInf : (mm + __builtin_amdgcn_logf(ll)) / kLog2e;
+  if (lse && c == 0) lse[row] = row_lse(mm, ll);
 }
 
 struct AttnPlan {
