@@ -464,7 +464,7 @@ int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t 
                 const int32_t* offsets, void* stream);
 
 /* The first offsets[b + 1] - offsets[b] tokens of every sequence into k and v [total, heads,
- * head_dim]; tokens without a page read as 0. */
+ * head_dim]; tokens without a page, and rows that no sequence has, read as 0. */
 int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, int64_t max_pages,
                const int32_t* offsets, int64_t total, void* k, void* v, int dtype, void* stream);
 
@@ -477,7 +477,8 @@ size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_he
  * tokens; its query rows (as in cp_kv_write) sit at its last positions, and query head x
  * reads cache head x / (q_heads / heads). Row at position p sees token j where j < lens[b],
  * j <= p (causal) and j > p - window (window > 0); tokens without a page are not seen. A row
- * that sees nothing is 0 with lse -inf. lse [rows, q_heads] float32 (NULL: not wanted) is
+ * that sees nothing, or that no sequence has, is 0 with lse -inf; so are those of a sequence whose
+ * rows are not all among the call's. lse [rows, q_heads] float32 (NULL: not wanted) is
  * the natural log of the sum of exponentials. q and out: bfloat16 or float16. scale is positive. */
 int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head,
                     int dtype, int64_t rows, int q_heads, const int32_t* table, int64_t batch,

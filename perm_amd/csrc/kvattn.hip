@@ -68,6 +68,35 @@ __host__ __device__ inline SplitParts split_parts(const AttnArgs& a) {
   return {a.part, ml, reinterpret_cast<int*>(ml + 2 * n)};
 }
 
+// Results of the rows [0, lead) and [tail, end): 0, lse -inf, nothing to join. Workgroup `at` of `of`.
+template <int DT>
+__device__ __forceinline__ void attn_clear(const AttnArgs& a, int64_t lead, int64_t tail, int64_t end, int at, int of) {
+  const int64_t per = (int64_t)a.group * a.c.heads, skip = (tail - lead) * per;
+  for (int64_t i = (int64_t)at * blockDim.x + threadIdx.x; i < end * per - skip; i += (int64_t)of * blockDim.x) {
+    const int64_t r = i < lead * per ? i : i + skip;
+    typename Elem<DT>::T* p = (typename Elem<DT>::T*)a.out + r * a.c.d;
+    for (int x = 0; x < a.c.d; x += 8) *reinterpret_cast<u32x4*>(p + x) = u32x4{0, 0, 0, 0};
+    if (a.lse) a.lse[r] = kNegInf;
+    if (a.splits > 1) split_parts(a).used[r] = 0;
+  }
+}
+
+// What a workgroup without rows of its own does. at: its item past the end, or -1 for a sequence
+// whose rows are not all among the call's: those that are have no results either.
+template <int DT>
+__device__ __forceinline__ void attn_unowned(const AttnArgs& a, const KvBatch& bt, int at, int of, int piece, int64_t row0,
+                                             int n_b) {
+  const int pieces = a.c.heads * a.splits;
+  if (at >= 0) {
+    if (!bt.offsets) return;
+    const KvUnowned u = kv_unowned(bt, a.rows);
+    attn_clear<DT>(a, u.lead, u.tail, a.rows, at * pieces + piece, of * pieces);
+  } else {
+    const int64_t end = min(row0 + n_b, a.rows), from = min(max(row0, (int64_t)0), end);
+    attn_clear<DT>(a, 0, from, end, piece, pieces);
+  }
+}
+
 // Eight e4m3 codes in q's type / in float16 (both exact).
 template <int DT>
 __device__ __forceinline__ u32x4 codes_to_16(uint32_t a, uint32_t b) {
@@ -139,7 +168,7 @@ __device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7
 constexpr int kFewTile = 32;
 
 template <int DT, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt) {
+__global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt, int items) {
   constexpr int NC = DP / 64, ND = DP / 16;
   __shared__ float sm_m[4][16], sm_l[4][16];
   __shared__ __align__(16) float sm_o[4][16][DP + 4];
@@ -148,10 +177,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   const int h = (int)(blockIdx.x / a.splits % c.heads);
   int b, item, n_b;
   int64_t row0;
-  if (!kv_locate(bt, (int)(blockIdx.x / a.splits / c.heads),
-                 [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item, &row0, &n_b))
+  const int at = (int)(blockIdx.x / a.splits / c.heads), piece = h * a.splits + split;
+  if (!kv_locate(bt, at, [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item, &row0, &n_b))
+    return attn_unowned<DT>(a, bt, item, items - at + item, piece, 0, 0);
+  if (row0 < 0 || row0 + n_b > a.rows) {
+    if (item == 0) attn_unowned<DT>(a, bt, -1, 0, piece, row0, n_b);
     return;
-  if (row0 < 0 || row0 + n_b > a.rows) return;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
@@ -444,11 +476,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   int b, item, n_b;
   int64_t row0;
   // last items first: causal rows at the end of a prompt see the most tokens
-  if (!kv_locate(bt, items - 1 - (int)(blockIdx.x / c.heads / a.splits),
-                 [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b, &item,
-                 &row0, &n_b))
+  const int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
+  if (!kv_locate(bt, from_end, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b,
+                 &item, &row0, &n_b))
+    return attn_unowned<DT>(a, bt, item, items - from_end + item, piece, 0, 0);
+  if (row0 < 0 || row0 + n_b > a.rows) {
+    if (item == 0) attn_unowned<DT>(a, bt, -1, 0, piece, row0, n_b);
     return;
-  if (row0 < 0 || row0 + n_b > a.rows) return;
+  }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 31, hh = lane >> 5;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);
@@ -915,7 +950,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
   const int T = d / 4, NG = min(256 / T, 16), grp = threadIdx.x / T, c = 4 * (threadIdx.x % T);
   const int64_t row = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * NG + grp;
   const bool mine = grp < NG && row < rows;
-  // a row that no sequence has was never given a count: bounded, its result means nothing
+  // bounded: offsets that decrease leave rows without a count
   const int splits = mine || ONE_ROW ? min(max(sp.used[row], 0), most) : 0;
   if (splits == 0) return;  // ONE_ROW: the whole workgroup leaves
   const float* po = sp.sums + row * most * d;
@@ -964,7 +999,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
 
 struct AttnPlan {
   bool many;
-  int64_t items;  // upper bound of the batch's row tiles
+  int64_t items;  // upper bound of the batch's row tiles, and one more where rows may have no sequence
   int splits, least;  // at most so many pieces of a row's tiles, of at least so many tiles
 };
 
@@ -984,7 +1019,9 @@ static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, i
   const int64_t n = std::max(p.items * heads, (int64_t)1);
   const int64_t span = window > 0 ? std::min(cap, (int64_t)window + tile + step) : cap;
   int64_t s = 1;
-  if (p.many) {
+  if (batch == 0) {
+    // no sequence: the rows are cleared
+  } else if (p.many) {
     // The tokens of a row tile are split as takes the fewest predicted microseconds. A join takes
     // a launch (4) and the time in which the splits' float32 outputs are written and read back.
     const int dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
@@ -1018,6 +1055,7 @@ static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, i
     // 7.5, 9.2).
     s = std::max((int64_t)1, std::min(1024 / n, span / (8 * step)));
   }
+  p.items += ragged;
   p.least = p.many ? 2 : 4;
   p.splits = (int)s;
   return p;
@@ -1033,7 +1071,7 @@ static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, h
     if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
     attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
   } else {
-    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b);
+    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b, (int)p.items);
   }
   CP_LAUNCHED("cache attention");
   return CP_OK;
@@ -1072,7 +1110,7 @@ extern "C" {
 
 size_t cp_kv_attention_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads, int64_t batch,
                                 int64_t max_pages, int ragged, int window) {
-  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
+  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 0 || max_pages < 1) return 0;
   const cp::AttnPlan p = cp::attn_plan(rows, batch, ragged != 0, q_heads / cache->heads, cache->heads,
                                        cache->head_dim, max_pages * cache->block, window);
   return p.splits > 1 ? (size_t)rows * q_heads * p.splits * (cache->head_dim + 2) * 4 + (size_t)rows * q_heads * 4 : 0;
@@ -1087,8 +1125,8 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   if (dtype != CP_BF16 && dtype != CP_F16) return cp::set_error(CP_ERR_ARG, "queries are bfloat16 or float16");
   if (window < 0) return cp::set_error(CP_ERR_ARG, "window %d", window);
   if (!(scale > 0.0f) || !(scale < 3e38f)) return cp::set_error(CP_ERR_ARG, "scale %g must be positive", scale);
-  if (rows == 0 || batch == 0) return CP_OK;
-  if (!q || !lens || !out) return cp::set_error(CP_ERR_ARG, "null q / lens / out");
+  if (rows == 0) return CP_OK;
+  if (!q || (batch && !lens) || !out) return cp::set_error(CP_ERR_ARG, "null q / lens / out");
   if (!cp::aligned(q, 16) || q_row * 2 % 16 || q_head * 2 % 16 || !cp::aligned(out, 16))
     return cp::set_error(CP_ERR_ALIGN, "rows and heads of q and out need 16-byte alignment");
   if (q_row < 0 || q_head < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of q");

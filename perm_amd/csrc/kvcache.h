@@ -23,7 +23,8 @@ struct KvBatch {
 // Work item `at` of a ragged batch: sequence b, its item'th piece, its first row and row
 // count, where count(b, rows of b) says how many pieces a sequence has. Every wave scans
 // the batch by itself, 64 sequences a step, so nothing is planned on the host, which does
-// not know the lengths. False: the grid is an upper bound and this item is past the end.
+// not know the lengths. False: the grid is an upper bound and this item is past the end; *item
+// is then which one past it.
 template <class F>
 __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int* b, int* item,
                                           int64_t* row0, int* n) {
@@ -55,7 +56,19 @@ __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int
     }
     at -= total;
   }
+  *item = at;
   return false;
+}
+
+// Rows that no sequence has: [0, lead) and [tail, rows). Work items past the end of the batch, of
+// which a launch with offsets has one at least, clear them in the outputs.
+struct KvUnowned {
+  int64_t lead, tail;
+};
+
+__device__ __forceinline__ KvUnowned kv_unowned(const KvBatch& q, int64_t rows) {
+  const int64_t lead = min(max((int64_t)q.offsets[0], (int64_t)0), rows);
+  return {lead, min(max((int64_t)q.offsets[q.batch], lead), rows)};
 }
 
 int kv_check_cache(const cp_kv_cache* c);

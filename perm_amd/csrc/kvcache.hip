@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256, KEEP ? 4 : 3) void kv_write_kernel(KvCacheArgs
 // of 8 heads of 128 to bf16: 276 MB in 53 us, 5.2 TB/s, a copy's rate). All of a wave's loads
 // are issued before the first is used, and five waves a SIMD keep enough of them in flight.
 template <int DT>
-__global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch q, int64_t total,
+__global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch q, int items, int64_t total,
                                                       typename Elem<DT>::T* __restrict__ ko,
                                                       typename Elem<DT>::T* __restrict__ vo) {
   __shared__ __align__(16) uint32_t slabs[4][kSlabLds];
@@ -266,10 +266,25 @@ __global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch 
   const int at = (int)blockIdx.x * 4 + wave, h = at % c.heads;
   int b, item, n_b;
   int64_t row0;
-  if (!kv_locate(q, at / c.heads, [&](int, int n) { return (n + 15) / 16; }, &b, &item, &row0, &n_b)) return;
-  const int n = min(n_b - item * 16, 16);
+  if (!kv_locate(q, at / c.heads, [&](int, int n) { return (n + 15) / 16; }, &b, &item, &row0, &n_b)) {
+    // the rows that no sequence has, a (row, head) a lane, shared by the waves past the end
+    if (at >= items * c.heads) return;
+    const KvUnowned u = kv_unowned(q, total);
+    const int64_t lead = u.lead * c.heads, skip = u.tail * c.heads - lead;
+    const int64_t waves = (int64_t)(items - at / c.heads + item) * c.heads;
+    for (int64_t i = ((int64_t)item * c.heads + h) * 64 + lane; i < total * c.heads - skip; i += waves * 64) {
+      const int64_t to = (i < lead ? i : i + skip) * c.d;
+      const float zero[8] = {};
+      for (int x = 0; x < c.d; x += 8) {
+        store8<DT>(ko + to + x, zero);
+        store8<DT>(vo + to + x, zero);
+      }
+    }
+    return;
+  }
   const int64_t r0 = row0 + (int64_t)item * 16;
-  if (r0 < 0 || r0 + n > total) return;
+  if (r0 < 0) return;
+  const int n = (int)min((int64_t)min(n_b - item * 16, 16), total - r0);  // rows that there are
   const int64_t pg = (int64_t)item * 16 / c.block;
   const int page = pg < c.max_pages ? c.table[(int64_t)b * c.max_pages + pg] : -1;
   const bool have = (unsigned)page < (unsigned)c.pages;
@@ -402,19 +417,19 @@ int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, in
   if (int s = cp::kv_check_cache(cache)) return s;
   if (int s = cp::kv_check_batch(table, batch, max_pages, total, offsets)) return s;
   if (!cp::dtype_bytes(dtype)) return cp::set_error(CP_ERR_ARG, "dtype code %d", dtype);
-  if (total == 0 || batch == 0) return CP_OK;
+  if (total == 0) return CP_OK;
   if (!offsets) return cp::set_error(CP_ERR_ARG, "null offsets");
   if (!k || !v) return cp::set_error(CP_ERR_ARG, "null k / v");
   if (!cp::aligned(k, 16) || !cp::aligned(v, 16)) return cp::set_error(CP_ERR_ALIGN, "k and v need 16-byte alignment");
-  const int64_t items = total / 16 + batch;
+  const int64_t items = total / 16 + batch + 1;  // one more than sequences can need
   if (items * cache->heads > 0x7FFFFF00) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvBatch q = {offsets, (int)batch};
   const dim3 grid((unsigned)((items * cache->heads + 3) / 4));
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == CP_F32) cp::kv_read_kernel<CP_F32><<<grid, 256, 0, st>>>(a, q, total, (float*)k, (float*)v);
-  if (dtype == CP_BF16) cp::kv_read_kernel<CP_BF16><<<grid, 256, 0, st>>>(a, q, total, (__bf16*)k, (__bf16*)v);
-  if (dtype == CP_F16) cp::kv_read_kernel<CP_F16><<<grid, 256, 0, st>>>(a, q, total, (_Float16*)k, (_Float16*)v);
+  if (dtype == CP_F32) cp::kv_read_kernel<CP_F32><<<grid, 256, 0, st>>>(a, q, (int)items, total, (float*)k, (float*)v);
+  if (dtype == CP_BF16) cp::kv_read_kernel<CP_BF16><<<grid, 256, 0, st>>>(a, q, (int)items, total, (__bf16*)k, (__bf16*)v);
+  if (dtype == CP_F16) cp::kv_read_kernel<CP_F16><<<grid, 256, 0, st>>>(a, q, (int)items, total, (_Float16*)k, (_Float16*)v);
   CP_LAUNCHED("cache read");
   return CP_OK;
 }

@@ -12,7 +12,9 @@ Ragged batches: ``offsets`` int32 [batch + 1] gives each sequence's first row of
 None means one row a sequence, as in decoding. table int32 [batch, max_pages], filled and
 lens int32 [batch] stay on the GPU and are read there: a call never waits for the device. An
 entry of table outside the cache's pages is no page: what is written there is dropped, it
-reads as 0, and attention does not see its tokens.
+reads as 0, and attention does not see its tokens. Offsets do not decrease; rows before the
+first and past the last (a padded batch) have no sequence: write leaves them out, read and
+attention give 0 there.
 """
 import ctypes
 from typing import NamedTuple
@@ -160,7 +162,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     row i of n sits at position lens[b] - n + i and sees the tokens up to its own (causal) and,
     with window > 0, no more than the window's last ones. Query head x reads cache head
     x // (q heads / cache heads). scale is positive, head_dim ** -0.5 by default. A row that sees
-    nothing is 0, its lse -inf."""
+    nothing, or has no sequence, is 0, its lse -inf."""
     lib = _lib.load()
     desc = _desc(cache)
     if q.dtype not in (torch.bfloat16, torch.float16):
