@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int k = 0; k < NC; ++k) kk[t][k] = *reinterpret_cast<const u32x4*>(kp + 4 * t * d + kcol[k]);
-    const float ks = c.k_scale[hv], vs = c.v_scale[hv];
+    const float ks0 = c.k_scale[hv], vs0 = c.v_scale[hv];
 #pragma unroll
     for (int i = 0; i < ND; ++i) {  // rows past d repeat the last one and are dropped
       vv[i] = *reinterpret_cast<const u32x2*>(vp);
@@ -270,6 +270,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     }
     pk = page(jk + 4 * kFewTile);
     pv = page(jv + 4 * kFewTile);
+    // no page: page 0's codes, which no row sees, but its scales may be anything and would reach them
+    const float ks = have ? ks0 : 1.0f, vs = have ? vs0 : 1.0f;
     f32x4 sc[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -707,7 +709,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   auto enter = [&] {  // the tile at hand
     const int j0 = tile * kTile;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) ks[s] = nks[s], vs[s] = nvs[s], have[s] = nhave[s];
+    for (int s = 0; s < 2; ++s) {
+      have[s] = nhave[s];
+      ks[s] = have[s] ? nks[s] : 1.0f, vs[s] = have[s] ? nvs[s] : 1.0f;  // as in attn_few_kernel
+    }
     all = !__any(!have[0] || !have[1]);
     edge = !all || j0 < wlo || j0 + kTile > whi;
     last = nbuf == 2 ? 0 : nbuf + 1;  // the tile before this one's: the one after the next's
