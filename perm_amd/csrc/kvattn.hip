@@ -1104,6 +1104,9 @@ static int attn_check(const cp_kv_cache* cache, int64_t rows, int q_heads, const
                       int64_t batch, int64_t max_pages, const int32_t* offsets) {
   if (int s = kv_check_cache(cache)) return s;
   if (int s = kv_check_batch(table, batch, max_pages, rows, offsets)) return s;
+  // pages are looked up, in 32 bits, up to three tiles past a sequence's last
+  if (max_pages * cache->block > 0x7FFFFFFF - 1023)
+    return set_error(CP_ERR_SHAPE, "table rows of %lld pages of %d tokens", (long long)max_pages, cache->block);
   if (q_heads < 1 || q_heads % cache->heads)
     return set_error(CP_ERR_SHAPE, "%d query heads over %d cache heads", q_heads, cache->heads);
   return CP_OK;
@@ -1138,12 +1141,14 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   const int group = q_heads / cache->heads;
   const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads, cache->head_dim,
                                        max_pages * cache->block, window);
+  // a join takes up to a workgroup a row and head
+  if (p.items * cache->heads * p.splits > cp::most_workgroups(256) || rows * q_heads > 0x7FFFFFFF ||
+      (p.splits > 1 && rows * q_heads > cp::most_workgroups(256)))
+    return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const size_t need = cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window);
   if (need && (!ws || ws_bytes < need))
     return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
   if (need && !cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
-  if (p.items * cache->heads * p.splits > 0x7FFFFFFF || rows * q_heads > 0x7FFFFFFF)
-    return cp::set_error(CP_ERR_SHAPE, "too many rows");
   cp::AttnArgs a;
   a.c = cp::kv_args(cache, table, max_pages);
   a.q = q;

@@ -352,7 +352,8 @@ int kv_check_cache(const cp_kv_cache* c) {
 int kv_check_batch(const int* table, int64_t batch, int64_t max_pages, int64_t rows, const int* offsets) {
   if (batch < 0 || max_pages < 1 || max_pages > 0x7FFFFFFF / 128 || batch > 0x7FFFFFF)
     return set_error(CP_ERR_SHAPE, "table of %lld rows of %lld pages", (long long)batch, (long long)max_pages);
-  if (rows < 0 || rows > 0x7FFFFFFF) return set_error(CP_ERR_SHAPE, "%lld rows", (long long)rows);
+  // a page of positions more than the rows still fits 32 bits
+  if (rows < 0 || rows > 0x7FFFFF00) return set_error(CP_ERR_SHAPE, "%lld rows", (long long)rows);
   if (!offsets && rows != batch)
     return set_error(CP_ERR_SHAPE, "%lld rows for %lld sequences need offsets", (long long)rows, (long long)batch);
   if (batch && !table) return set_error(CP_ERR_ARG, "null table");
@@ -391,7 +392,7 @@ int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t 
   if (int s = cp::kv_check_rows(v, es, v_row, v_head, "v")) return s;
   // pages touched: ceil((filled % block + n) / block) summed over the sequences
   const int64_t items = offsets ? rows / cache->block + 2 * batch : batch;
-  if (items * cache->heads > 0x7FFFFF00) return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  if (items * cache->heads > 4 * cp::most_workgroups(256)) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvRows kr = {k, k_row, k_head}, vr = {v, v_row, v_head};
   const cp::KvBatch q = {offsets, (int)batch};
@@ -422,7 +423,7 @@ int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, in
   if (!k || !v) return cp::set_error(CP_ERR_ARG, "null k / v");
   if (!cp::aligned(k, 16) || !cp::aligned(v, 16)) return cp::set_error(CP_ERR_ALIGN, "k and v need 16-byte alignment");
   const int64_t items = total / 16 + batch + 1;  // one more than sequences can need
-  if (items * cache->heads > 0x7FFFFF00) return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  if (items * cache->heads > 4 * cp::most_workgroups(256)) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvBatch q = {offsets, (int)batch};
   const dim3 grid((unsigned)((items * cache->heads + 3) / 4));

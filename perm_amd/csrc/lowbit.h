@@ -21,6 +21,9 @@ template <> struct Elem<CP_F32> { typedef float T; };
 template <> struct Elem<CP_BF16> { typedef __bf16 T; };
 template <> struct Elem<CP_F16> { typedef _Float16 T; };
 
+// A launch holds under 2^32 work items in x: so many workgroups of that many threads at most.
+inline int64_t most_workgroups(int threads) { return 0xFFFFFFFFll / threads; }
+
 inline int dtype_bytes(int dt) { return dt == CP_F32 ? 4 : dt == CP_BF16 || dt == CP_F16 ? 2 : 0; }
 
 // Eight consecutive values as they are stored.

@@ -611,7 +611,7 @@ static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, int splits, vo
   constexpr int BM = 16 * WM * FM, BN = 16 * WN * FN, lds = 2 * (BM + BN) * kStageBytes;
   static_assert(WM * WN * FM * FN * 512 <= lds, "the results pass through the staging buffers");
   const int64_t mt = (a.rows + BM - 1) / BM, nt = (b.rows + BN - 1) / BN;
-  if (mt > 0x7FFFFFF / nt / splits) return set_error(CP_ERR_SHAPE, "product too large");
+  if (mt > most_workgroups(64 * WM * WN) / nt / splits) return set_error(CP_ERR_SHAPE, "product too large");
   static const hipError_t once =
       hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<WM, WN, FM, FN, DT>),
                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -633,7 +633,7 @@ template <int MT, int NT, int XT, int DT>
 static int mx_few(const MxOperand& a, const MxOperand& b, const void* x, int64_t stride, int k, void* y,
                   hipStream_t st) {
   const int64_t wgs = (b.rows + 16 * NT - 1) / (16 * NT);
-  if (wgs > 0x7FFFFFF) return set_error(CP_ERR_SHAPE, "product too large");
+  if (wgs > most_workgroups(1024)) return set_error(CP_ERR_SHAPE, "product too large");
   // Waves: four (more gain nothing: 1 x 1024 x 4096 3.3, 3.6, 4.2 us with 4, 8 and 16). Where
   // they quantize, more while a thread has over four chunks of eight values and the launch
   // under eight waves a CU (8 x 1024 x 4096 9.4 us with 4, 7.0 with 16).
