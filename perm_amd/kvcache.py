@@ -17,6 +17,7 @@ first and past the last (a padded batch) have no sequence: write leaves them out
 attention give 0 there.
 """
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -171,6 +172,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     rows, heads = q.shape[0], q.shape[1]
     if heads == 0 or heads % desc.heads:
         raise ValueError(f"{heads} query heads over {desc.heads} cache heads")
+    window = min(operator.index(window), 2 ** 31 - 1)  # positions are below
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
@@ -184,6 +186,6 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     _lib.check(lib.cp_kv_attention(
         ctypes.byref(desc), q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], rows, heads,
         table.data_ptr(), batch, max_pages, lens.data_ptr(), _lib.ptr(offsets), int(causal),
-        int(window), desc.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+        window, desc.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
         _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr()))
     return (out, lse) if return_lse else out
