@@ -52,6 +52,8 @@ def new(pages, heads, head_dim, block=16, device="cuda"):
 
 def _desc(c):
     """struct cp_kv_cache of a KvCache, its buffers checked against each other."""
+    if not (isinstance(c, (tuple, list)) and len(c) == 4):
+        raise TypeError(f"cache must be a KvCache, got {type(c).__name__}")
     k, v, ks, vs = c
     if k.dim() != 4:
         raise ValueError("k codes are [pages, heads, block, head_dim]")
@@ -83,7 +85,7 @@ def _index(t, dims, what):
 def _batch(table, per_seq, what, offsets, rows):
     """table, per_seq and offsets as the kernels read them, their shapes checked."""
     table = _index(table, 2, "table")
-    if per_seq is not None:
+    if what:
         per_seq = _index(per_seq, 1, what)
         if per_seq.shape[0] != table.shape[0]:
             raise ValueError(f"{what} of {per_seq.shape[0]} for {table.shape[0]} sequences")
@@ -94,6 +96,13 @@ def _batch(table, per_seq, what, offsets, rows):
     elif rows != table.shape[0]:
         raise ValueError(f"{rows} rows for {table.shape[0]} sequences need offsets")
     return table, per_seq, offsets
+
+
+def _dtype(x, what):
+    """The element type of a tensor."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor, got {type(x).__name__}")
+    return x.dtype
 
 
 def _heads(x, heads, d, what):
@@ -116,8 +125,9 @@ def write(cache, k, v, table, filled, offsets=None):
     NaN), do not enter a scale. Sequences of one call must not share a page they write."""
     lib = _lib.load()
     desc = _desc(cache)
-    if k.dtype != v.dtype or k.dtype not in DTYPES:
-        raise TypeError(f"k and v must both be float32, bfloat16 or float16, got {k.dtype}, "
+    dtype = _dtype(k, "k")
+    if dtype != _dtype(v, "v") or dtype not in DTYPES:
+        raise TypeError(f"k and v must both be float32, bfloat16 or float16, got {dtype}, "
                         f"{v.dtype}")
     k = _heads(k, desc.heads, desc.head_dim, "k")
     v = _heads(v, desc.heads, desc.head_dim, "v")
@@ -129,7 +139,7 @@ def write(cache, k, v, table, filled, offsets=None):
         return
     _lib.check(lib.cp_kv_write(
         ctypes.byref(desc), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-        v.stride(1), DTYPES[k.dtype], rows, table.data_ptr(), table.shape[0], table.shape[1],
+        v.stride(1), DTYPES[dtype], rows, table.data_ptr(), table.shape[0], table.shape[1],
         filled.data_ptr(), _lib.ptr(offsets), _lib.stream_ptr()))
 
 
@@ -166,7 +176,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     nothing, or has no sequence, is 0, its lse -inf."""
     lib = _lib.load()
     desc = _desc(cache)
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if _dtype(q, "q") not in (torch.bfloat16, torch.float16):
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
     q = _heads(q, None, desc.head_dim, "q")
     rows, heads = q.shape[0], q.shape[1]

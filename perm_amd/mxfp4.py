@@ -73,6 +73,8 @@ def _rows(x):
 
 def _checked(q, what):
     """(rows, k) of an MxTensor whose buffers have the shapes they claim."""
+    if not (isinstance(q, tuple) and len(q) == 2):
+        raise TypeError(f"{what} must be an MxTensor, got {type(q).__name__}")
     codes, scales = q
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"{what}: codes and scales are uint8")
@@ -147,7 +149,7 @@ def linear(x, w, dtype=None):
     tensor and is quantized as quantize() does inside the call; the products of the codes
     are summed in float32 and rounded once."""
     lib = _lib.load()
-    xc = _dtype(x.dtype, "x")
+    xc = _dtype(x.dtype if isinstance(x, torch.Tensor) else type(x).__name__, "x")
     dtype = dtype or x.dtype
     yc = _dtype(dtype, "dtype")
     n, k = _checked(w, "w")
