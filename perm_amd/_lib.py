@@ -246,6 +246,26 @@ def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
 
+class _NoBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, name, x):
+        ctx.name = name
+        ctx.mark_dirty(y)  # the result itself, not a view of it
+        return y
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.name} has no backward pass")
+
+
+def no_backward(y, name, x):
+    """y, with a backward pass that raises where autograd would want one: an operator without
+    gradients must not pass for one that has none to give."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return _NoBackward.apply(y, name, x)
+    return y
+
+
 def to_device(a, dtype):
     """(contiguous device tensor of ``dtype``, True if ``a`` came from the host)."""
     if isinstance(a, torch.Tensor):

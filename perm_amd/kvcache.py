@@ -15,6 +15,9 @@ entry of table outside the cache's pages is no page: what is written there is dr
 reads as 0, and attention does not see its tokens. Offsets do not decrease; rows before the
 first and past the last (a padded batch) have no sequence: write leaves them out, read and
 attention give 0 there.
+
+For inference: rows written keep no graph, and a backward pass through attention raises
+NotImplementedError.
 """
 import ctypes
 import operator
@@ -198,4 +201,5 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
         table.data_ptr(), batch, max_pages, lens.data_ptr(), _lib.ptr(offsets), int(causal),
         window, desc.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
         _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr()))
-    return (out, lse) if return_lse else out
+    out = _lib.no_backward(out, "kvcache.attention", q)
+    return (out, _lib.no_backward(lse, "kvcache.attention", q)) if return_lse else out

@@ -12,6 +12,9 @@ such blocks directly at four times their 16-bit rate.
 
 k is a multiple of 32. The exponent of a block is floor(log2 max|x|) - 2; codes round to
 nearest even and saturate at 6; a block that holds a NaN or an infinity decodes to NaN.
+
+For inference: the codes carry no gradient, and a backward pass through roundtrip or linear
+raises NotImplementedError.
 """
 from typing import NamedTuple
 
@@ -124,7 +127,7 @@ def roundtrip(x):
     shape = tuple(x.shape)
     q = quantize(x)
     y = dequantize(q, torch.float32 if host else x.dtype).reshape(shape)
-    return _lib.to_host(y) if host else y
+    return _lib.to_host(y) if host else _lib.no_backward(y, "mxfp4.roundtrip", x)
 
 
 def matmul(a, b, dtype=torch.bfloat16):
@@ -165,4 +168,4 @@ def linear(x, w, dtype=None):
     _lib.check(lib.cp_mx4_linear(rows.data_ptr(), xc, m, rows.stride(0), w.codes.data_ptr(),
                                  w.scales.data_ptr(), n, k, y.data_ptr(), yc, _lib.ptr(ws), nws,
                                  _lib.stream_ptr()))
-    return y
+    return _lib.no_backward(y, "mxfp4.linear", x)
