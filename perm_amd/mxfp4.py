@@ -18,6 +18,7 @@ raises NotImplementedError.
 """
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -122,12 +123,15 @@ def dequantize(q, dtype=torch.float32):
 
 
 def roundtrip(x):
-    """x through MXFP4 and back, in its own dtype and shape (numpy in, numpy out)."""
-    host = not (isinstance(x, torch.Tensor) and x.is_cuda)
-    shape = tuple(x.shape)
-    q = quantize(x)
-    y = dequantize(q, torch.float32 if host else x.dtype).reshape(shape)
-    return _lib.to_host(y) if host else _lib.no_backward(y, "mxfp4.roundtrip", x)
+    """x through MXFP4 and back, in its own dtype and shape. Host data comes back as numpy, in
+    float32 where it is neither float16 nor float64."""
+    if isinstance(x, torch.Tensor) and x.is_cuda:
+        y = dequantize(quantize(x), x.dtype).reshape(x.shape)
+        return _lib.no_backward(y, "mxfp4.roundtrip", x)
+    x = x.detach() if isinstance(x, torch.Tensor) else np.asarray(x)
+    y = _lib.to_host(dequantize(quantize(x))).reshape(tuple(x.shape))
+    own = str(x.dtype).rpartition(".")[2]
+    return y.astype(own) if own in ("float16", "float64") else y
 
 
 def matmul(a, b, dtype=torch.bfloat16):
