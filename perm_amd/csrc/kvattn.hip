@@ -1071,9 +1071,9 @@ static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, h
   const dim3 grid((unsigned)(p.items * a.c.heads * a.splits));
   if (p.many) {
     constexpr int lds = 6 * kTile * DP + 4 * (DP / 32) * 1024;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (once != hipSuccess) return hip_fail(once, "LDS size of the cache attention");
+    static std::atomic<uint64_t> done{0};
+    if (int s = allow_lds(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP>), lds, &done, "LDS of the cache attention"))
+      return s;
     attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
   } else {
     attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b, (int)p.items);

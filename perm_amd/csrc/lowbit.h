@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "cp_host.h"
 
 namespace cp {
@@ -23,6 +25,19 @@ template <> struct Elem<CP_F16> { typedef _Float16 T; };
 
 // A launch holds under 2^32 work items in x: so many workgroups of that many threads at most.
 inline int64_t most_workgroups(int threads) { return 0xFFFFFFFFll / threads; }
+
+// Allows a kernel this much LDS on the current device. It is asked for once for each device (a
+// bit of done); a failure is reported and asked for again by the next call.
+inline int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>* done, const char* what) {
+  int dev = 0;
+  CP_HIP(hipGetDevice(&dev));
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return CP_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return hip_fail(e, what);
+  if (dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return CP_OK;
+}
 
 inline int dtype_bytes(int dt) { return dt == CP_F32 ? 4 : dt == CP_BF16 || dt == CP_F16 ? 2 : 0; }
 

@@ -612,10 +612,10 @@ static int mx_gemm(const MxOperand& a, const MxOperand& b, int k, int splits, vo
   static_assert(WM * WN * FM * FN * 512 <= lds, "the results pass through the staging buffers");
   const int64_t mt = (a.rows + BM - 1) / BM, nt = (b.rows + BN - 1) / BN;
   if (mt > most_workgroups(64 * WM * WN) / nt / splits) return set_error(CP_ERR_SHAPE, "product too large");
-  static const hipError_t once =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_gemm_kernel<WM, WN, FM, FN, DT>),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (once != hipSuccess) return hip_fail(once, "LDS size of the MXFP4 product");
+  static std::atomic<uint64_t> done{0};
+  if (int s = allow_lds(reinterpret_cast<const void*>(&mx4_gemm_kernel<WM, WN, FM, FN, DT>), lds, &done,
+                        "LDS of the MXFP4 product"))
+    return s;
   mx4_gemm_kernel<WM, WN, FM, FN, DT><<<dim3((unsigned)(mt * nt * splits)), 64 * WM * WN, lds, st>>>(
       a, b, k, (int)mt, (int)nt, splits, (typename Elem<DT>::T*)y);
   CP_LAUNCHED("MXFP4 product");
