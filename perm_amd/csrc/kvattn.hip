@@ -187,15 +187,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
-  const int64_t cap = (int64_t)c.max_pages * blk;
-  const int len = (int)min((int64_t)max(a.lens[b], 0), cap);
+  // rows sit at the end of len tokens, of which the table holds the first
+  const int len = max(a.lens[b], 0), held = (int)min((int64_t)len, (int64_t)c.max_pages * blk);
 
   // this lane's query row
   const int64_t r = (int64_t)item * 16 + col;
   const bool real = r < (int64_t)n_b * a.group;
   const int qi = (int)(r / a.group), qh = h * a.group + (int)(r % a.group);
   const int64_t pos = (int64_t)len - n_b + qi;
-  int hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len) : 0;
+  int hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)held, pos + 1)) : held) : 0;
   int lo = a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
   if (lo >= hi) lo = hi = 0;
   // tokens any row of the workgroup sees
@@ -489,14 +489,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 31, hh = lane >> 5;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);
-  const int64_t cap = (int64_t)c.max_pages * blk;
-  const int len = (int)min((int64_t)max(__builtin_amdgcn_readfirstlane(a.lens[b]), 0), cap);
+  const int len = max(__builtin_amdgcn_readfirstlane(a.lens[b]), 0);
+  const int held = (int)min((int64_t)len, (int64_t)c.max_pages * blk);  // by the table
 
   // token range [lo, hi) of row r of the sequence; rows past the end see nothing
   auto range = [&](int64_t r, int* lo, int* hi) {
     const bool real = r < (int64_t)n_b * a.group;
     const int64_t pos = (int64_t)len - n_b + r / a.group;
-    *hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)len, pos + 1)) : len) : 0;
+    *hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)held, pos + 1)) : held) : 0;
     *lo = a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
     if (*lo >= *hi) *lo = *hi = 0;
   };
@@ -504,10 +504,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   int lo, hi;
   range(r, &lo, &hi);
   // what the workgroup's rows see together: rows are in order of position, so the first row
-  // that sees anything bounds it below and the last real row above
+  // that sees anything bounds it below and the last one above
   int jlo, jhi;
   {
-    const int64_t last = min(r0 + kManyRows, (int64_t)n_b * a.group) - 1;
+    int64_t last = min(r0 + kManyRows, (int64_t)n_b * a.group) - 1;
+    // a row more than the window past the tokens held sees none of them
+    if (a.window > 0) last = max(r0, min(last, ((int64_t)held + a.window - 1 - len + n_b) * a.group - 1));
     int x;
     range(last, &x, &jhi);
     // the lowest token of the first row whose position is not negative
