@@ -158,7 +158,8 @@ __device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7
 // workgroup starts with (length, page numbers, codes), which four workgroups on a CU hide
 // better than longer strides in fewer of them: hence small tiles and at most 128 registers.
 // One token of 32 heads on 131072 tokens: 268 MB in 49 us, 5.4 TB/s. 64 sequences of up to 4096
-// tokens: 174 MB in 41 us, 34 with equal lengths; the longest sequence's splits end last.
+// tokens: 174 MB in 41 us, 34 with equal lengths; the longest sequence's splits end last. Weights in
+// two terms cost 1 % at 128 columns, 8 % at 80, whose products are 128 wide all the same.
 //
 // K is the A operand (16 tokens x 32 columns), q the B operand, so a lane's scores belong to
 // one query row (lane % 16), and its group lane / 16 owns 8 consecutive tokens of the tile:
@@ -430,11 +431,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 // second product's operand at step s as they stand.
 //
 // Bound by the VALU and the matrix cores together (per 32 rows x 64 tokens a wave has 32 MFMAs
-// of 32 clocks and about 380 other instructions, a third of them the conversions; counters showed
-// the VALU busy 66 % and the matrix cores 40 % of the time, 57 and 34 before a wave gave way in
-// its second product): two times 4096 rows of 16 heads on 8192 tokens 320 us, 0.88 PFLOP/s,
-// 8192 rows of 32 heads 594 us, 0.93; 3 % of it goes into looking for weights that one float16
-// does not hold. Codes converted once for the workgroup and kept in 16
+// of 32 clocks and about 390 other instructions, a third of them the conversions; counters show
+// the VALU busy 66 % and the matrix cores 37 % of the time): two times 4096 rows of 16 heads on
+// 8192 tokens 311 to 323 us, 0.9 PFLOP/s, 8192 rows of 32 heads 594 us, 0.93. Looking for weights
+// that one float16 does not hold takes 4 % of it (9 % at 64 columns). Codes converted once for the workgroup and kept in 16
 // bits double what the waves read from LDS, and lose (367 us against 341).
 //
 // LDS rows hold 16-byte chunks permuted by xor, so that eight lanes of a read fall into
@@ -593,8 +593,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   const int ksw = k_swizzle<DP>(token);
   const int vsw = 16 * ((q >> 2) & 3);
 
-  // Page numbers are looked up two tiles ahead and scales loaded one ahead, so that neither
-  // is waited for. Lookups past the last token repeat its own; such tokens are not seen.
+  // Page numbers are looked up two tiles ahead and scales loaded one ahead. The compiler waits
+  // for all loads in flight at a tile's end, where it moves these to the next tile's names: half
+  // a tile after they, and the direct loads with them, were issued. Lookups past the last token repeat its own; such tokens are not seen.
   const int lastj = max(jhi - 1, 0);
   struct Pages {
     int k, v, g[2];

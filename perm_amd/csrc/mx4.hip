@@ -372,10 +372,11 @@ __device__ __forceinline__ void mx_store_tile(typename Elem<DT>::T* y, int64_t m
   }
 }
 
-// Large products, bound by the matrix cores where the tiles fill the GPU (8192 x 8192 x 8192:
-// 237 us, 4.6 PFLOP/s; the instruction alone reaches 5.9 on random codes, where power limits
-// it) and by a tile's start and end where there are few stages (4096 x 14336 x 4096: 3.5 rounds
-// of tiles, 121 us, 4.0 PFLOP/s). A workgroup of WM x WN waves owns a tile of BM x BN results, each wave
+// Large products, bound by the matrix cores where the tiles fill the GPU (8192 x 8192 x 8192 of
+// normal values: 228 to 238 us, 4.6 to 4.8 PFLOP/s; the instruction alone reaches 5.9 on random
+// codes, where power limits it) and by a tile's start and end where there are few stages
+// (4096 x 14336 x 4096: 3.5 rounds of tiles, 117 us, 4.1 PFLOP/s; of uniformly random codes, which
+// draw more power, 124 to 142). A workgroup of WM x WN waves owns a tile of BM x BN results, each wave
 // FM x FN MFMA tiles of it. 256 columns of both operands are staged in LDS a step ahead by
 // loads that write LDS directly, 16 bytes a lane, in two buffers; a row's eight 16-byte
 // chunks are permuted by xor with the row's low three bits, so that the 16 rows of an operand
