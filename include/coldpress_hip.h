@@ -486,6 +486,67 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
                     int window, float scale, void* out, float* lse, void* ws, size_t ws_bytes,
                     void* stream);
 
+/* ---- the pages of a cache: several answers to one prompt ----
+ * refs [pages] counts the entries of table [batch, max_pages] that hold a page; a page without
+ * holders is free. Tables and counts stay on the GPU and are changed in place; what a call hands
+ * out depends on its inputs alone. One call at a time works on a table and its counts. */
+
+/* Entries of row children[i] become those of row parents[i] that hold its lens[parents[i]] tokens,
+ * -1 past them; every page copied gains a holder. A child's row should hold no pages, is named
+ * once, and is no parent of the same call. Rows outside the table, and a row that is its own child, are left out. */
+int cp_kv_fork(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, int64_t max_pages,
+               const int32_t* lens, int block, const int32_t* parents, const int32_t* children,
+               int64_t n, void* stream);
+
+/* Workspace bytes of cp_kv_grow (256-byte aligned). */
+size_t cp_kv_grow_ws_bytes(int64_t pages, int64_t batch);
+
+/* Pages for the next fresh[b] (fresh NULL: each) tokens of sequence b, which holds filled[b].
+ * Of the entries those tokens fall into, one without a page gets a free one (but not one that
+ * tokens held were in), and one whose page has other holders gets a free one in its place: where
+ * tokens held are in it, src[b] and dst[b] name the pages to copy from and to (otherwise -1).
+ * Sequences are served in order, each wholly or not at all: missing[b] is 0, or the pages it
+ * wanted, from the first on for which the free pages do not suffice; also where its tokens pass
+ * the end of its row. Free pages are handed out by number. */
+int cp_kv_grow(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, int64_t max_pages,
+               const int32_t* filled, const int32_t* fresh, int each, int block, int32_t* src,
+               int32_t* dst, int32_t* missing, void* ws, size_t ws_bytes, void* stream);
+
+/* The entries of rows[0 .. n) (rows NULL: of all rows) become -1 and their pages lose a holder. */
+int cp_kv_free(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, int64_t max_pages,
+               const int32_t* rows, int64_t n, void* stream);
+
+/* Workspace bytes of cp_kv_compact (256-byte aligned). */
+size_t cp_kv_compact_ws_bytes(int64_t pages);
+
+/* Numbers the pages in use 0 .. *used: those at or past *used, in order, take the free numbers
+ * before it, in order. refs and table are changed; src and dst [pages / 2] name the pages to copy,
+ * -1 past them. */
+int cp_kv_compact(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, int64_t max_pages,
+                  int32_t* src, int32_t* dst, int32_t* used, void* ws, size_t ws_bytes,
+                  void* stream);
+
+/* Codes and scales of page src[i] of one cache into page dst[i] of another of the same geometry, or
+ * of the same one, where no page written may be read or written twice in the call. Pairs
+ * with a page outside its cache are left out. */
+int cp_kv_copy(const cp_kv_cache* from, const cp_kv_cache* to, const int32_t* src,
+               const int32_t* dst, int64_t n, void* stream);
+
+/* token[r] = the next token of row r of logits [rows, vocab] (rows row_step elements apart), chosen by
+ * u[r] in [0, 1) (float32; float64 with u_f64). A token of logit x weighs e^((x - max) / temperature).
+ * In the order of falling logits, equal ones by number, the first top_k tokens are kept (0: all);
+ * of those the ones before which less than top_p of their sum lies; of those the ones of at least
+ * min_p times the largest weight; the first one always. In the order of numbers the token is the
+ * first at which the sum of the weights kept passes u times all of it. temperature 0 (or no positive
+ * number): the first in the order of logits. NaN counts as minus infinity, which is never
+ * chosen; -1 for a row of nothing else. Settings are arrays [rows], or NULL: the number beside
+ * them. A setting out of range counts as the nearest in it. Weights are whole multiples of 2^-s of
+ * the largest, s = 62 - ceil(log2 vocab) up to 51, and are summed exactly. vocab up to 2^24. */
+int cp_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_step,
+              const void* u, int u_f64, const float* temperature, double temperature_all,
+              const int32_t* top_k, int top_k_all, const float* top_p, double top_p_all,
+              const float* min_p, double min_p_all, int32_t* token, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,16 @@ SIGNATURES = {
     "cp_kv_attention_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32, _i32]),
     "cp_kv_attention": (_i32, [_kv_p, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _i64, _vp,
                                _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "cp_kv_fork": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _i64, _vp]),
+    "cp_kv_grow_ws_bytes": (_sz, [_i64, _i64]),
+    "cp_kv_grow": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp,
+                          _sz, _vp]),
+    "cp_kv_free": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "cp_kv_compact_ws_bytes": (_sz, [_i64]),
+    "cp_kv_compact": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "cp_kv_copy": (_i32, [_kv_p, _kv_p, _vp, _vp, _i64, _vp]),
+    "cp_sample": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _f64, _vp, _i32, _vp, _f64,
+                         _vp, _f64, _vp, _vp]),
 }
 
 
@@ -240,6 +250,13 @@ def stream_ptr():
     """The current stream's hipStream_t, without the Stream object torch.cuda.current_stream()
     builds each time (0.1 us instead of 2.8)."""
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+
+
+def here(device):
+    """Refuses tensors of another device than the current one, on whose stream kernels run."""
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, but the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
 
 
 def ptr(t):
