@@ -486,6 +486,31 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
                     int window, float scale, void* out, float* lse, void* ws, size_t ws_bytes,
                     void* stream);
 
+/* What cp_kv_attention_more adds to cp_kv_attention; every field may be 0 or NULL. */
+typedef struct cp_kv_more {
+  float softcap;         /* > 0: scores x become softcap tanh(x / softcap) */
+  const float* slopes;   /* [q_heads]: scores (capped) lose slopes[head] |p - j| */
+  const int32_t* first;  /* [rows]: a row sees no token before first[row] */
+  const int32_t* prefix; /* [batch]: tokens j < prefix[b] are seen whatever the row's position (causal) */
+  const int32_t* shared; /* [groups]: batch / groups consecutive sequences form a group, whose table */
+  int64_t groups;        /* rows begin with the same shared[g] pages: they are read once for all of it */
+} cp_kv_more;
+
+/* Workspace bytes of cp_kv_attention_more (256-byte aligned; 0: none); groups: 0 without shared. */
+size_t cp_kv_attention_more_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads,
+                                     int64_t batch, int64_t max_pages, int ragged, int window,
+                                     int64_t groups);
+
+/* As cp_kv_attention, with scores and masks changed as ``more`` says. A row at position p sees token j
+ * where j < lens[b], j <= p or j < prefix[b] (causal), j > p - window (window > 0), and j >= first[row].
+ * Common pages are looked up in the table row of a group's first sequence. With them, a group of
+ * sequences whose rows are not all among the call's has no results. */
+int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head,
+                         int dtype, int64_t rows, int q_heads, const int32_t* table, int64_t batch,
+                         int64_t max_pages, const int32_t* lens, const int32_t* offsets, int causal,
+                         int window, float scale, const cp_kv_more* more, void* out, float* lse,
+                         void* ws, size_t ws_bytes, void* stream);
+
 /* ---- the pages of a cache: several answers to one prompt ----
  * refs [pages] counts the entries of table [batch, max_pages] that hold a page; a page without
  * holders is free. Tables and counts stay on the GPU and are changed in place; what a call hands

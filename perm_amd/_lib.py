@@ -65,6 +65,15 @@ class KvCacheDesc(ctypes.Structure):
 
 _kv_p = ctypes.POINTER(KvCacheDesc)
 
+
+class KvMore(ctypes.Structure):
+    """struct cp_kv_more (include/coldpress_hip.h)."""
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", _vp), ("first", _vp), ("prefix", _vp),
+                ("shared", _vp), ("groups", ctypes.c_int64)]
+
+
+_more_p = ctypes.POINTER(KvMore)
+
 # name -> (restype, argtypes); every symbol include/coldpress_hip.h declares
 SIGNATURES = {
     "cp_last_error": (ctypes.c_char_p, []),
@@ -128,6 +137,10 @@ SIGNATURES = {
     "cp_kv_attention_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32, _i32]),
     "cp_kv_attention": (_i32, [_kv_p, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _i64, _vp,
                                _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "cp_kv_attention_more_ws_bytes": (_sz, [_kv_p, _i64, _i32, _i64, _i64, _i32, _i32, _i64]),
+    "cp_kv_attention_more": (_i32, [_kv_p, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _i64, _vp,
+                                    _vp, _i32, _i32, ctypes.c_float, _more_p, _vp, _vp, _vp, _sz,
+                                    _vp]),
     "cp_kv_fork": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _i64, _vp]),
     "cp_kv_grow_ws_bytes": (_sz, [_i64, _i64]),
     "cp_kv_grow": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp,

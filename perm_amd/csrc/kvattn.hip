@@ -39,6 +39,7 @@ constexpr float kNegInf = -__builtin_inff();
 // Weights are 2^kLift above 2^(t - m), which uses float16's range up to 2^15: m moves when a t
 // passes it by kLag. A t more than kDeep below m has a weight below float16's normal range.
 constexpr float kLift = 11.0f, kLag = 4.0f, kDeep = kLift + 14.0f;
+constexpr float kGone = kLift + 127.0f;  // a t more than this below m has no weight in bfloat16 either
 
 struct AttnArgs {
   KvCacheArgs c;
@@ -57,43 +58,174 @@ struct AttnArgs {
   float scale;                  // softmax scale * log2 e
 };
 
+// What changes the masks and scores above, in kernels of their own (MODE 1: which tokens a row sees,
+// MODE 2: scores too):
+//   first   a row sees no token before its own first one (the start of its document)
+//   prefix  a sequence's tokens before this are seen whatever a row's position
+//   shared  consecutive sequences (`group` of them) whose tables begin with the same pages: those are read once,
+//           by phase 1, for all rows of the group; phase 2 does the rest of every sequence. Each
+//           writes splits of its own, which are joined together
+//   cap     scores x become cap tanh(x / cap)
+//   slopes  and lose slope |p - j|
+struct AttnMore {
+  const int *first, *prefix, *shared;
+  int seqs;                // sequences of a group
+  int phase;               // 0: no shared pages
+  int slot0, slots;        // where this phase's splits lie among a row's
+  const float* slopes;     // [q heads]
+  float cap, over;         // cap * log2 e (0: none) and 2 / cap
+  int series;              // a large cap
+};
+struct AttnPlain {};
+template <int MODE>
+using More = std::conditional_t<MODE == 0, AttnPlain, AttnMore>;
+
 struct SplitParts {
   float *sums, *ml;
   int* used;
 };
 
-__host__ __device__ inline SplitParts split_parts(const AttnArgs& a) {
-  const int64_t n = a.rows * a.group * a.c.heads * a.splits;
+__host__ __device__ inline SplitParts split_parts(const AttnArgs& a, int slots) {
+  const int64_t n = a.rows * a.group * a.c.heads * slots;
   float* ml = a.part + n * a.c.d;
   return {a.part, ml, reinterpret_cast<int*>(ml + 2 * n)};
 }
+__host__ __device__ inline SplitParts split_parts(const AttnArgs& a, const AttnPlain&) { return split_parts(a, a.splits); }
+// sums and (m, l) of row r's split s are at [r][slot0 + s]; phase 2 counts its splits in an array of its own
+__host__ __device__ inline SplitParts split_parts(const AttnArgs& a, const AttnMore& x) {
+  SplitParts p = split_parts(a, x.slots);
+  if (x.phase == 2) p.used += a.rows * a.group * a.c.heads;
+  return p;
+}
+__device__ __forceinline__ int slot_of(const AttnArgs& a, const AttnPlain&, int split) { return split; }
+__device__ __forceinline__ int slot_of(const AttnArgs& a, const AttnMore& x, int split) { return x.slot0 + split; }
+__device__ __forceinline__ int slots_of(const AttnArgs& a, const AttnPlain&) { return a.splits; }
+__device__ __forceinline__ int slots_of(const AttnArgs& a, const AttnMore& x) { return x.slots; }
+// Whether a row of this many splits is joined, and writes what it has for that
+__device__ __forceinline__ bool joined(const AttnArgs& a, const AttnPlain&) { return a.splits > 1; }
+__device__ __forceinline__ bool joined(const AttnArgs& a, const AttnMore& x) { return x.slots > 1; }
+__device__ __forceinline__ int phase_of(const AttnPlain&) { return 0; }
+__device__ __forceinline__ int phase_of(const AttnMore& x) { return x.phase; }
+__device__ __forceinline__ int pieces_of(int used, const AttnPlain&) { return used > 1 ? used : 0; }
+__device__ __forceinline__ int pieces_of(int used, const AttnMore& x) { return x.phase || used > 1 ? used : 0; }
+// sequences that kv_locate takes as one
+__device__ __forceinline__ int each_of(const AttnPlain&) { return 1; }
+__device__ __forceinline__ int each_of(const AttnMore& x) { return x.phase == 1 ? x.seqs : 1; }
+
+// A row of the call: its position, the tokens [lo, hi) it sees in this phase (0, 0: none).
+struct SeenRow {
+  int64_t pos;
+  int lo, hi;
+};
+
+// Tokens that sequences' common pages hold.
+__device__ __forceinline__ int shared_tokens(const AttnArgs& a, const AttnMore& x, int group) {
+  return min(max(x.shared[group], 0), a.c.max_pages) * a.c.block;
+}
+
+// Row r of the call, of a sequence (or, in phase 1, a group of them) b whose rows begin at row0, n_b of them.
+__device__ __forceinline__ SeenRow seen_row(const AttnArgs& a, const AttnMore& x, const KvBatch& bt, bool real, int64_t r,
+                                            int b, int64_t row0, int n_b) {
+  SeenRow s = {0, 0, 0};
+  if (!real) return s;
+  int q = b, group = b;
+  if (x.phase == 1) {
+    q = b * x.seqs;
+    if (!bt.offsets) {
+      q = (int)r, row0 = r, n_b = 1;
+    } else {  // the last sequence that begins at or before the row
+      int end = q + x.seqs;
+      while (end - q > 1) {
+        const int mid = q + (end - q) / 2;
+        if (bt.offsets[mid] <= r) q = mid;
+        else end = mid;
+      }
+      row0 = bt.offsets[q], n_b = bt.offsets[q + 1] - bt.offsets[q];
+    }
+  } else if (x.phase == 2) {
+    group = b / x.seqs;
+  }
+  const int len = max(a.lens[q], 0), held = (int)min((int64_t)len, (int64_t)a.c.max_pages * a.c.block);
+  s.pos = (int64_t)len - n_b + (r - row0);
+  int64_t hi = held, lo = 0;
+  if (a.causal) hi = max(s.pos + 1, x.prefix ? (int64_t)x.prefix[q] : (int64_t)0);
+  if (a.window > 0) lo = s.pos - a.window + 1;
+  if (x.first) lo = max(lo, (int64_t)x.first[r]);
+  hi = min(hi, (int64_t)held), lo = max(lo, (int64_t)0);
+  if (x.phase) {
+    const int n = shared_tokens(a, x, group);
+    if (x.phase == 1) hi = min(hi, (int64_t)n);
+    else lo = max(lo, (int64_t)n);
+  }
+  if (lo < hi) s.lo = (int)lo, s.hi = (int)hi;
+  return s;
+}
+
+// A sequence of phase 2 whose group's rows are not all among the call's has no results.
+__device__ __forceinline__ bool whole_group(const AttnArgs&, const AttnPlain&, const KvBatch&, int) { return true; }
+__device__ __forceinline__ bool whole_group(const AttnArgs& a, const AttnMore& x, const KvBatch& bt, int b) {
+  if (x.phase != 2 || !bt.offsets) return true;
+  const int at = b / x.seqs * x.seqs;
+  return bt.offsets[at] >= 0 && bt.offsets[at + x.seqs] <= a.rows;
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// N scores of tokens that follow one another, in base 2: products times kc, capped, less the distance's
+// share. far: position less the first token. tanh z = 1 - 2 / (1 + e^2z) errs by 1.5 x 2^-23, a capped
+// score by cap times that: up to caps of 128 no more than 2^-15 of a weight. Larger caps, of which
+// most scores are a small part, take the series below |z| = 1/4, whose error is relative.
+template <int N, class V>
+__device__ __forceinline__ void change_scores(const AttnMore& x, V& v, float kc, float slope, float far) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] *= kc;
+  if (x.cap > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float z2 = v[i] * x.over, e = exp2_fast(z2);
+      float y = __builtin_fmaf(-2.0f * x.cap, __builtin_amdgcn_rcpf(1.0f + e), x.cap);
+      if (x.series) {
+        const float z = z2 * (0.5f / kLog2e), q = z * z;
+        float p = __builtin_fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f);
+        p = __builtin_fmaf(q, p, 2.0f / 15.0f);
+        p = __builtin_fmaf(q, p, -1.0f / 3.0f);
+        y = q < 0.0625f ? __builtin_fmaf(v[i] * q, p, v[i]) : y;
+      }
+      v[i] = y;
+    }
+  }
+  if (x.slopes) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __builtin_fmaf(-slope, fabsf(far - (float)i), v[i]);
+  }
+}
 
 // Results of the rows [0, lead) and [tail, end): 0, lse -inf, nothing to join. Workgroup `at` of `of`.
-template <int DT>
-__device__ __forceinline__ void attn_clear(const AttnArgs& a, int64_t lead, int64_t tail, int64_t end, int at, int of) {
+template <int DT, class X>
+__device__ __forceinline__ void attn_clear(const AttnArgs& a, const X& x, int64_t lead, int64_t tail, int64_t end, int at, int of) {
   const int64_t per = (int64_t)a.group * a.c.heads, skip = (tail - lead) * per;
   for (int64_t i = (int64_t)at * blockDim.x + threadIdx.x; i < end * per - skip; i += (int64_t)of * blockDim.x) {
     const int64_t r = i < lead * per ? i : i + skip;
     typename Elem<DT>::T* p = (typename Elem<DT>::T*)a.out + r * a.c.d;
-    for (int x = 0; x < a.c.d; x += 8) *reinterpret_cast<u32x4*>(p + x) = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < a.c.d; i += 8) *reinterpret_cast<u32x4*>(p + i) = u32x4{0, 0, 0, 0};
     if (a.lse) a.lse[r] = kNegInf;
-    if (a.splits > 1) split_parts(a).used[r] = 0;
+    if (joined(a, x)) split_parts(a, x).used[r] = 0;
   }
 }
 
 // What a workgroup without rows of its own does. at: its item past the end, or -1 for a sequence
 // whose rows are not all among the call's: those that are have no results either.
-template <int DT>
-__device__ __forceinline__ void attn_unowned(const AttnArgs& a, const KvBatch& bt, int at, int of, int piece, int64_t row0,
+template <int DT, class X>
+__device__ __forceinline__ void attn_unowned(const AttnArgs& a, const X& x, const KvBatch& bt, int at, int of, int piece, int64_t row0,
                                              int n_b) {
   const int pieces = a.c.heads * a.splits;
   if (at >= 0) {
     if (!bt.offsets) return;
-    const KvUnowned u = kv_unowned(bt, a.rows);
-    attn_clear<DT>(a, u.lead, u.tail, a.rows, at * pieces + piece, of * pieces);
+    const KvUnowned u = kv_unowned(bt, a.rows, each_of(x));
+    attn_clear<DT>(a, x, u.lead, u.tail, a.rows, at * pieces + piece, of * pieces);
   } else {
     const int64_t end = min(row0 + n_b, a.rows), from = min(max(row0, (int64_t)0), end);
-    attn_clear<DT>(a, 0, from, end, piece, pieces);
+    attn_clear<DT>(a, x, 0, from, end, piece, pieces);
   }
 }
 
@@ -124,8 +256,6 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-
-__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // Two weights as bfloat16 terms: hi rounded, lo the rest rounded.
 struct Weights2 {
@@ -168,8 +298,8 @@ __device__ __forceinline__ uint32_t nan_flags(uint32_t w) { return ((w & 0x7F7F7
 // without leaving their lanes.
 constexpr int kFewTile = 32;
 
-template <int DT, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt, int items) {
+template <int DT, int DP, int MODE>
+__global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArgs a, KvBatch bt, int items, More<MODE> ext) {
   constexpr int NC = DP / 64, ND = DP / 16;
   __shared__ float sm_m[4][16], sm_l[4][16];
   __shared__ __align__(16) float sm_o[4][16][DP + 4];
@@ -179,26 +309,33 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   int b, item, n_b;
   int64_t row0;
   const int at = (int)(blockIdx.x / a.splits / c.heads), piece = h * a.splits + split;
-  if (!kv_locate(bt, at, [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item, &row0, &n_b))
-    return attn_unowned<DT>(a, bt, item, items - at + item, piece, 0, 0);
-  if (row0 < 0 || row0 + n_b > a.rows) {
-    if (item == 0) attn_unowned<DT>(a, bt, -1, 0, piece, row0, n_b);
+  if (!kv_locate(bt, at, [&](int, int n) { return (int)(((int64_t)n * a.group + 15) / 16); }, &b, &item, &row0, &n_b,
+                 each_of(ext)))
+    return attn_unowned<DT>(a, ext, bt, item, items - at + item, piece, 0, 0);
+  if (row0 < 0 || row0 + n_b > a.rows || !whole_group(a, ext, bt, b)) {
+    if (item == 0) attn_unowned<DT>(a, ext, bt, -1, 0, piece, row0, n_b);
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);  // block is a power of two
   // rows sit at the end of len tokens, of which the table holds the first
-  const int len = max(a.lens[b], 0), held = (int)min((int64_t)len, (int64_t)c.max_pages * blk);
+  const int len = MODE ? 0 : max(a.lens[b], 0), held = (int)min((int64_t)len, (int64_t)c.max_pages * blk);
 
   // this lane's query row
   const int64_t r = (int64_t)item * 16 + col;
   const bool real = r < (int64_t)n_b * a.group;
   const int qi = (int)(r / a.group), qh = h * a.group + (int)(r % a.group);
-  const int64_t pos = (int64_t)len - n_b + qi;
+  int64_t pos = (int64_t)len - n_b + qi;
   int hi = real ? (a.causal ? (int)max((int64_t)0, min((int64_t)held, pos + 1)) : held) : 0;
   int lo = a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
   if (lo >= hi) lo = hi = 0;
+  float slope = 0.0f;
+  if constexpr (MODE > 0) {
+    const SeenRow s = seen_row(a, ext, bt, real, row0 + qi, b, row0, n_b);
+    pos = s.pos, lo = s.lo, hi = s.hi;
+    if (MODE > 1 && ext.slopes && real) slope = ext.slopes[qh] * kLog2e;
+  }
   // tokens any row of the workgroup sees
   int jhi = hi, jlo = hi > lo ? lo : 0x7FFFFFFF;
 #pragma unroll
@@ -232,7 +369,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 #pragma unroll
   for (int i = 0; i < ND; ++i) o[i] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
-  const int* tab = c.table + (int64_t)b * c.max_pages;
+  const int* tab = c.table + (int64_t)b * each_of(ext) * c.max_pages;
   // columns past d read the row's first ones instead: their q is 0, and a NaN there makes the
   // score NaN anyway
   int kcol[NC];
@@ -283,8 +420,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
         sc[t] = mfma16<DT>(codes_to_16<DT>(kk[t][k][2], kk[t][k][3]), qf[k][1], sc[t]);
       }
     }
-    const float kc = ks * a.scale;
+    const float kc = MODE > 1 ? 1.0f : ks * a.scale;
     const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+    if constexpr (MODE > 1) {
+      const float far = (float)(pos - jv);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) change_scores<4>(ext, sc[t], ks * a.scale, slope, far - 4.0f * t);
+    }
     bool edge = false;  // a token of this lane that its row does not see
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -395,16 +537,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     ll += sm_l[w][row] * fh * fh;
   }
   const int64_t orow = (row0 + rr / a.group) * ((int64_t)a.group * c.heads) + h * a.group + rr % a.group;
-  const SplitParts sp = split_parts(a);
-  if (a.splits > 1 && split == 0 && c0 == 0) sp.used[orow] = used > 1 ? used : 0;
-  float* p = sp.sums + (orow * a.splits + split) * d;
+  const SplitParts sp = split_parts(a, ext);
+  const int pieces = pieces_of(used, ext);
+  if (joined(a, ext) && split == 0 && c0 == 0) sp.used[orow] = pieces;
+  if (MODE && phase_of(ext) && pieces == 0) return;
+  const int64_t slot = orow * slots_of(a, ext) + slot_of(a, ext, split);
+  float* p = sp.sums + slot * d;
   typename Elem<DT>::T* op = (typename Elem<DT>::T*)a.out + orow * d;
   const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;  // a row that saw nothing: 0
   for (int x = 4 * c0; x < d; x += 64) {
     f32x4 v = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(&sm_o[w][row][x]) * f[w];
-    if (used > 1) {
+    if (pieces > 0) {
       *reinterpret_cast<f32x4*>(p + x) = v;
     } else {
       u32x2 y;
@@ -414,8 +559,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
     }
   }
   if (c0 != 0) return;
-  if (used > 1) {
-    float* pm = sp.ml + (orow * a.splits + split) * 2;
+  if (pieces > 0) {
+    float* pm = sp.ml + slot * 2;
     pm[0] = mm, pm[1] = ll;
   } else if (a.lse) {
     a.lse[orow] = row_lse(mm, ll);
@@ -467,8 +612,9 @@ __device__ __forceinline__ void unrolled2(F f) {
   f(std::integral_constant<int, 1>{});
 }
 
-template <int DT, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items) {
+template <int DT, int DP, int MODE>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnArgs a, KvBatch bt, int items,
+                                                                          More<MODE> ext) {
   constexpr int NC = DP / 32, NL = DP / 64;          // 32-column chunks; direct loads of a wave for K, and for V
   constexpr int KB = kTile * DP, BUF = 2 * KB;       // bytes of a K (or V) tile, of a buffer
   extern __shared__ __align__(16) uint8_t lds[];     // [3][BUF], then [4 waves][NC][64 lanes][16]
@@ -480,16 +626,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   // last items first: causal rows at the end of a prompt see the most tokens
   const int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
   if (!kv_locate(bt, from_end, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b,
-                 &item, &row0, &n_b))
-    return attn_unowned<DT>(a, bt, item, items - from_end + item, piece, 0, 0);
-  if (row0 < 0 || row0 + n_b > a.rows) {
-    if (item == 0) attn_unowned<DT>(a, bt, -1, 0, piece, row0, n_b);
+                 &item, &row0, &n_b, each_of(ext)))
+    return attn_unowned<DT>(a, ext, bt, item, items - from_end + item, piece, 0, 0);
+  if (row0 < 0 || row0 + n_b > a.rows || !whole_group(a, ext, bt, b)) {
+    if (item == 0) attn_unowned<DT>(a, ext, bt, -1, 0, piece, row0, n_b);
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 31, hh = lane >> 5;
   const int d = c.d, blk = c.block, lb = 31 - __clz(c.block);
-  const int len = max(__builtin_amdgcn_readfirstlane(a.lens[b]), 0);
+  const int len = MODE ? 0 : max(__builtin_amdgcn_readfirstlane(a.lens[b]), 0);
   const int held = (int)min((int64_t)len, (int64_t)c.max_pages * blk);  // by the table
 
   // token range [lo, hi) of row r of the sequence; rows past the end see nothing
@@ -502,11 +648,32 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   };
   const int64_t r0 = (int64_t)item * kManyRows, r = r0 + 32 * wave + q;
   int lo, hi;
-  range(r, &lo, &hi);
+  int64_t pos = 0;
+  if constexpr (MODE > 0) {
+    const SeenRow seen = seen_row(a, ext, bt, r < (int64_t)n_b * a.group, row0 + r / a.group, b, row0, n_b);
+    pos = seen.pos, lo = seen.lo, hi = seen.hi;
+  } else {
+    range(r, &lo, &hi);
+  }
   // what the workgroup's rows see together: rows are in order of position, so the first row
   // that sees anything bounds it below and the last one above
   int jlo, jhi;
-  {
+  if constexpr (MODE > 0) {  // in any order: the least and the most of all
+    jlo = hi > lo ? lo : 0x7FFFFFFF, jhi = hi;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      jlo = min(jlo, __shfl_xor(jlo, s));
+      jhi = max(jhi, __shfl_xor(jhi, s));
+    }
+    int* const ends = reinterpret_cast<int*>(lds);
+    if (lane == 0) ends[wave] = jlo, ends[4 + wave] = jhi;
+    __syncthreads();
+    jlo = min(min(ends[0], ends[1]), min(ends[2], ends[3]));
+    jhi = max(max(ends[4], ends[5]), max(ends[6], ends[7]));
+    __syncthreads();  // before tiles are fetched into it
+    jhi = __builtin_amdgcn_readfirstlane(jhi);
+    jlo = min(__builtin_amdgcn_readfirstlane(jlo), jhi);
+  } else {
     int64_t last = min(r0 + kManyRows, (int64_t)n_b * a.group) - 1;
     // a row more than the window past the tokens held sees none of them
     if (a.window > 0) last = max(r0, min(last, ((int64_t)held + a.window - 1 - len + n_b) * a.group - 1));
@@ -553,7 +720,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
   float m = kNegInf, l = 0.0f;
 
-  const int* tab = c.table + (int64_t)b * c.max_pages;
+  float slope = 0.0f;
+  if constexpr (MODE > 1) {
+    if (ext.slopes && real) slope = ext.slopes[qh] * kLog2e;
+  }
+  const int* tab = c.table + (int64_t)b * each_of(ext) * c.max_pages;
   // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
   // each, four token groups. Chunks past d repeat the row's first, rows past d its last 16
   // (their q is 0, their results are dropped).
@@ -697,6 +868,21 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       }
     }
   };
+  // MODE 2: the scores of unit s of the tile at j0, and the largest and least of them
+  auto change = [&](f32x16& x, int j0, int s, float kc) {
+    if constexpr (MODE > 1) {
+      change_scores<16>(ext, x, kc, slope, (float)(pos - (j0 + 32 * s + 16 * hh)));
+      top = bot = x[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
+    }
+  };
+  // Whether a row's weights need two terms: one is too small for float16, and not all of them for any.
+  // (A distance's share leaves many rows' far tokens with no weight at all.)
+  auto deep_scores = [&](float kc, float lg) {
+    const bool small = __builtin_fmaf(bot, kc, lg) < m - kDeep;
+    return MODE > 1 ? small && __builtin_fmaf(top, kc, lg) > m - kGone : small;
+  };
   // the running maximum and what hangs on it, when a row's t passes it by kLag; called seldom
   auto move_max = [&](float tm) {
     tm = fmaxf(tm, __shfl_xor(tm, 32));
@@ -738,26 +924,29 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
     }
-    top = bot = sc[0][0];
+    if constexpr (MODE < 2) {
+      top = bot = sc[0][0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
+    }
     wide = -1;
     while (tile < te) {
       const int j0 = tile * kTile;
       unrolled2([&](auto S) {
         constexpr int s = S;
         if (s == 1 && wide >= 0) return;
-        const float kc = ks[s] * a.scale;
+        const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale;
         const float lg = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
         const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
         if constexpr (s == 1) advance();
 #pragma unroll
         for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
+        change(sc[s], j0, s, ks[s] * a.scale);
         if (edge) mask(sc[s], j0, s, have[s]);
         // the largest t of the unit: kc > 0, so t rises with the raw score
         const float tm = __builtin_fmaf(top, kc, lg);
         if (__any(tm > m + kLag)) move_max(tm);
-        if (__any(__builtin_fmaf(bot, kc, lg) < m - kDeep)) {
+        if (__any(deep_scores(kc, lg))) {
           wide = s;
           return;
         }
@@ -806,15 +995,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         // SIMD's other wave: its MFMAs need an issue slot in 32 clocks, the weights every slot, and
         // two waves that keep out of step overlap (335 -> 309 us for two prompts of 4096 rows).
         __builtin_amdgcn_s_setprio(0);
-        top = bot = sc[1 - s][0];
+        if constexpr (MODE < 2) top = bot = sc[1 - s][0];
 #pragma unroll
         for (int k = 0; k < 2 * NC; ++k) {
           const int i = k % NC;
           const u32x4 x = vr[i];
           o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), w[k / NC], o[i]);
+          if constexpr (MODE < 2) {
 #pragma unroll
-          for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
-            top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
+            for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
+              top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(1);
@@ -834,7 +1025,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       if (s == 1 && !ahead) advance();
       ahead = false;
       const bool hv = s ? have[1] : have[0];
-      const float v1 = s ? vs[1] : vs[0], kc = (s ? ks[1] : ks[0]) * a.scale;
+      const float v1 = s ? vs[1] : vs[0], kc0 = (s ? ks[1] : ks[0]) * a.scale, kc = MODE > 1 ? 1.0f : kc0;
       const float lg = (float)((int)(__float_as_uint(v1) >> 23) - 127);
       f32x16& x = sc[0];
 #pragma unroll
@@ -845,16 +1036,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         x = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], x);
         x = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], x);
       }
+      change(x, j0, s, kc0);
       if (edge) {
         mask(x, j0, s, hv);
-      } else {
+      } else if constexpr (MODE < 2) {
         top = bot = x[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
       }
       const float tm = __builtin_fmaf(top, kc, lg);
       if (__any(tm > m + kLag)) move_max(tm);
-      deep |= __any(__builtin_fmaf(bot, kc, lg) < m - kDeep);
+      deep |= __any(deep_scores(kc, lg));
       // as in attn_few_kernel, the sum's terms and the weights from them
       const float off = kLift - (m == kNegInf ? 0.0f : m);
       u32x4 wh[2], wl[2];
@@ -914,11 +1106,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   if (!real) return;
   const int64_t orow = qrow * ((int64_t)a.group * c.heads) + qh;
   // lane's results: columns 32 i + 8 (j / 4) + 4 hh + j % 4 of its row
-  const SplitParts sp = split_parts(a);
-  if (a.splits > 1 && split == 0 && hh == 0) sp.used[orow] = used > 1 ? used : 0;
-  if (used > 1) {
-    float* p = sp.sums + (orow * a.splits + split) * d;
-    float* pm = sp.ml + (orow * a.splits + split) * 2;
+  const SplitParts sp = split_parts(a, ext);
+  const int pieces = pieces_of(used, ext);
+  if (joined(a, ext) && split == 0 && hh == 0) sp.used[orow] = pieces;
+  if (pieces > 0) {
+    const int64_t slot = orow * slots_of(a, ext) + slot_of(a, ext, split);
+    float* p = sp.sums + slot * d;
+    float* pm = sp.ml + slot * 2;
     if (hh == 0) pm[0] = m, pm[1] = l;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -929,6 +1123,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       }
     return;
   }
+  if (phase_of(ext)) return;  // nothing of this phase to join
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   typename Elem<DT>::T* op = (typename Elem<DT>::T*)a.out + orow * d;
 #pragma unroll
@@ -949,8 +1144,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
 // of a workgroup share one row's, otherwise each has its own row (attention and join, one row
 // of 16 heads: on 32768 tokens in 64 splits 27.7 us a group a row, 19.5 a workgroup; on 64 x
 // 2048 in two 25.8 and 26.5).
-template <int DT, bool ONE_ROW>
-__global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t rows, int d, int most,
+//
+// TWO: a row has the splits of two phases, the second's from slot1 on, and is written here even if it has none.
+template <int DT, bool ONE_ROW, bool TWO>
+__global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t rows, int d, int most, int slot1,
                                                         typename Elem<DT>::T* __restrict__ out,
                                                         float* __restrict__ lse) {
   __shared__ float sm_m[4], sm_l[16];
@@ -959,27 +1156,30 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
   const int64_t row = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * NG + grp;
   const bool mine = grp < NG && row < rows;
   // bounded: offsets that decrease leave rows without a count
-  const int splits = mine || ONE_ROW ? min(max(sp.used[row], 0), most) : 0;
-  if (splits == 0) return;  // ONE_ROW: the whole workgroup leaves
+  const int splits1 = mine || ONE_ROW ? min(max(sp.used[row], 0), TWO ? slot1 : most) : 0;
+  const int splits = splits1 + (TWO && (mine || ONE_ROW) ? min(max(sp.used[rows + row], 0), most - slot1) : 0);
+  if (!TWO && splits == 0) return;  // ONE_ROW: the whole workgroup leaves
+  auto slot = [&](int s) { return TWO && s >= splits1 ? slot1 + s - splits1 : s; };
   const float* po = sp.sums + row * most * d;
   const float* pm = sp.ml + row * most * 2;
   float mm = kNegInf;
   if constexpr (ONE_ROW) {
-    for (int s = threadIdx.x; s < splits; s += 256) mm = fmaxf(mm, pm[2 * s]);
+    for (int s = threadIdx.x; s < splits; s += 256) mm = fmaxf(mm, pm[2 * slot(s)]);
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) mm = fmaxf(mm, __shfl_xor(mm, k));
     if ((threadIdx.x & 63) == 0) sm_m[threadIdx.x >> 6] = mm;
     __syncthreads();
     mm = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
   } else {
-    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, pm[2 * s]);
+    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, pm[2 * slot(s)]);
   }
   const float ms = mm == kNegInf ? 0.0f : mm;
   f32x4 v = {0, 0, 0, 0};
   float ll = 0.0f;
   if (mine) {
 #pragma unroll 4
-    for (int s = ONE_ROW ? grp : 0; s < splits; s += ONE_ROW ? NG : 1) {
+    for (int i = ONE_ROW ? grp : 0; i < splits; i += ONE_ROW ? NG : 1) {
+      const int s = slot(i);
       const float fh = half_move(pm[2 * s], ms);
       ll += pm[2 * s + 1] * fh * fh;
       v += *reinterpret_cast<const f32x4*>(po + (int64_t)s * d + c) * (fh * fh);
@@ -997,6 +1197,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
       ll += sm_l[i];
     }
   }
+  if (TWO && !mine) return;
   const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
   u32x2 y;
   y[0] = pack2<DT>(v[0] * inv, v[1] * inv);
@@ -1018,12 +1219,12 @@ struct AttnPlan {
 // rows 16 / 36 us, 64 25 / 50, 256 83 / 62; 16 heads, 1024 rows on as many tokens 22 / 30, 1024
 // on 2048 44 / 41, 512 on 4096 50 / 41.
 static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, int heads, int d,
-                          int64_t cap, int window) {
+                          int64_t cap, int window, int64_t rows_each = 1) {
   AttnPlan p;
   p.many = rows * group > 64 * batch &&
            (double)rows * group * heads * (window > 0 ? std::min(cap, (int64_t)window + kManyRows) : cap) > 1 << 24;
   const int tile = p.many ? kManyRows : 16, step = p.many ? kTile : kFewTile;
-  p.items = ragged ? rows * group / tile + batch : batch * ((group + tile - 1) / tile);
+  p.items = ragged ? rows * group / tile + batch : batch * ((rows_each * group + tile - 1) / tile);
   const int64_t n = std::max(p.items * heads, (int64_t)1);
   const int64_t span = window > 0 ? std::min(cap, (int64_t)window + tile + step) : cap;
   int64_t s = 1;
@@ -1069,38 +1270,81 @@ static AttnPlan attn_plan(int64_t rows, int64_t batch, bool ragged, int group, i
   return p;
 }
 
-template <int DT, int DP>
-static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
+template <int DT, int DP, int MODE>
+static int attn_launch(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, const More<MODE>& x, hipStream_t st) {
   const dim3 grid((unsigned)(p.items * a.c.heads * a.splits));
   if (p.many) {
     constexpr int lds = 6 * kTile * DP + 4 * (DP / 32) * 1024;
     static std::atomic<uint64_t> done{0};
-    if (int s = allow_lds(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP>), lds, &done, "LDS of the cache attention"))
+    if (int s = allow_lds(reinterpret_cast<const void*>(&attn_many_kernel<DT, DP, MODE>), lds, &done,
+                          "LDS of the cache attention"))
       return s;
-    attn_many_kernel<DT, DP><<<grid, 256, lds, st>>>(a, b, (int)p.items);
+    attn_many_kernel<DT, DP, MODE><<<grid, 256, lds, st>>>(a, b, (int)p.items, x);
   } else {
-    attn_few_kernel<DT, DP><<<grid, 256, 0, st>>>(a, b, (int)p.items);
+    attn_few_kernel<DT, DP, MODE><<<grid, 256, 0, st>>>(a, b, (int)p.items, x);
   }
   CP_LAUNCHED("cache attention");
   return CP_OK;
 }
 
-template <int DT>
-static int attn_launch_d(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
-  const int s = a.c.d <= 64    ? attn_launch<DT, 64>(a, b, p, st)
-                : a.c.d <= 128 ? attn_launch<DT, 128>(a, b, p, st)
-                               : attn_launch<DT, 256>(a, b, p, st);
-  if (s || a.splits == 1) return s;
+template <int DT, int MODE>
+static int attn_launch_d(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, const More<MODE>& x, hipStream_t st) {
+  return a.c.d <= 64    ? attn_launch<DT, 64, MODE>(a, b, p, x, st)
+         : a.c.d <= 128 ? attn_launch<DT, 128, MODE>(a, b, p, x, st)
+                        : attn_launch<DT, 256, MODE>(a, b, p, x, st);
+}
+
+// slots of a row, the second phase's (TWO) from slot1 on
+template <int DT, bool TWO>
+static int attn_join(const AttnArgs& a, int slots, int slot1, hipStream_t st) {
   const int64_t n = a.rows * a.group * a.c.heads;
   typename Elem<DT>::T* out = (typename Elem<DT>::T*)a.out;
   const int64_t groups = std::min(256 / (a.c.d / 4), 16);
-  if (a.splits > 8)
-    attn_join_kernel<DT, true><<<dim3((unsigned)n), 256, 0, st>>>(split_parts(a), n, a.c.d, a.splits, out, a.lse);
+  const SplitParts sp = split_parts(a, slots);
+  if (slots > 8)
+    attn_join_kernel<DT, true, TWO><<<dim3((unsigned)n), 256, 0, st>>>(sp, n, a.c.d, slots, slot1, out, a.lse);
   else
-    attn_join_kernel<DT, false><<<dim3((unsigned)((n + groups - 1) / groups)), 256, 0, st>>>(split_parts(a), n, a.c.d,
-                                                                                          a.splits, out, a.lse);
+    attn_join_kernel<DT, false, TWO><<<dim3((unsigned)((n + groups - 1) / groups)), 256, 0, st>>>(sp, n, a.c.d, slots,
+                                                                                               slot1, out, a.lse);
   CP_LAUNCHED("cache attention's join");
   return CP_OK;
+}
+
+template <int DT>
+static int attn_run(const AttnArgs& a, const KvBatch& b, const AttnPlan& p, hipStream_t st) {
+  const int s = attn_launch_d<DT, 0>(a, b, p, AttnPlain{}, st);
+  return s || a.splits == 1 ? s : attn_join<DT, false>(a, a.splits, 0, st);
+}
+
+// The plans of a call with common pages: of the groups' rows over those, of the sequences over the rest.
+struct SharedPlan {
+  AttnPlan front, rest;
+};
+
+static SharedPlan shared_plan(int64_t rows, int64_t batch, int64_t groups, bool ragged, int group, int heads, int d,
+                              int64_t cap, int window) {
+  return {attn_plan(rows, groups, ragged, group, heads, d, cap, window, groups ? rows / groups : 0),
+          attn_plan(rows, batch, ragged, group, heads, d, cap, window)};
+}
+
+template <int DT, int MODE>
+static int attn_run_more(AttnArgs a, KvBatch b, AttnMore x, const AttnPlan& p, const SharedPlan& sp, int groups,
+                         hipStream_t st) {
+  if (!x.shared) {
+    x.slots = a.splits = p.splits, a.least = p.least;
+    const int s = attn_launch_d<DT, MODE>(a, b, p, x, st);
+    return s || a.splits == 1 ? s : attn_join<DT, false>(a, a.splits, 0, st);
+  }
+  x.slots = sp.front.splits + sp.rest.splits;
+  x.phase = 1;
+  a.splits = sp.front.splits, a.least = sp.front.least;
+  const KvBatch bg = {b.offsets, groups};
+  if (int s = attn_launch_d<DT, MODE>(a, bg, sp.front, x, st)) return s;
+  x.phase = 2;
+  x.slot0 = sp.front.splits;
+  a.splits = sp.rest.splits, a.least = sp.rest.least;
+  if (int s = attn_launch_d<DT, MODE>(a, b, sp.rest, x, st)) return s;
+  return attn_join<DT, true>(a, x.slots, sp.front.splits, st);
 }
 
 static int attn_check(const cp_kv_cache* cache, int64_t rows, int q_heads, const int32_t* table,
@@ -1169,8 +1413,89 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   a.least = p.least;
   a.scale = scale * cp::kLog2e;
   const cp::KvBatch b = {offsets, (int)batch};
-  return dtype == CP_BF16 ? cp::attn_launch_d<CP_BF16>(a, b, p, (hipStream_t)stream)
-                          : cp::attn_launch_d<CP_F16>(a, b, p, (hipStream_t)stream);
+  return dtype == CP_BF16 ? cp::attn_run<CP_BF16>(a, b, p, (hipStream_t)stream)
+                          : cp::attn_run<CP_F16>(a, b, p, (hipStream_t)stream);
+}
+
+size_t cp_kv_attention_more_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads, int64_t batch,
+                                     int64_t max_pages, int ragged, int window, int64_t groups) {
+  if (groups <= 0) return cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, ragged, window);
+  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
+  const cp::SharedPlan p = cp::shared_plan(rows, batch, groups, ragged != 0, q_heads / cache->heads, cache->heads,
+                                           cache->head_dim, max_pages * cache->block, window);
+  return (size_t)rows * q_heads * ((size_t)(p.front.splits + p.rest.splits) * (cache->head_dim + 2) + 2) * 4;
+}
+
+int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head, int dtype,
+                         int64_t rows, int q_heads, const int32_t* table, int64_t batch, int64_t max_pages,
+                         const int32_t* lens, const int32_t* offsets, int causal, int window, float scale,
+                         const cp_kv_more* more, void* out, float* lse, void* ws, size_t ws_bytes, void* stream) {
+  cp::clear_error();
+  if (int s = cp::attn_check(cache, rows, q_heads, table, batch, max_pages, offsets)) return s;
+  if (dtype != CP_BF16 && dtype != CP_F16) return cp::set_error(CP_ERR_ARG, "queries are bfloat16 or float16");
+  if (window < 0) return cp::set_error(CP_ERR_ARG, "window %d", window);
+  if (!(scale > 0.0f) || !(scale < 3e38f)) return cp::set_error(CP_ERR_ARG, "scale %g must be positive", scale);
+  if (!more) return cp::set_error(CP_ERR_ARG, "null more");
+  if (!(more->softcap >= 0.0f) || !(more->softcap < 1e30f) || (more->softcap > 0.0f && more->softcap < 1e-30f))
+    return cp::set_error(CP_ERR_ARG, "softcap %g must be 0 or positive", more->softcap);
+  const int64_t groups = more->shared ? more->groups : 0;
+  if (more->shared && (groups < 1 || batch % groups))
+    return cp::set_error(CP_ERR_SHAPE, "%lld sequences in %lld groups", (long long)batch, (long long)groups);
+  if (rows == 0) return CP_OK;
+  if (!q || (batch && !lens) || !out) return cp::set_error(CP_ERR_ARG, "null q / lens / out");
+  if (!cp::aligned(q, 16) || q_row * 2 % 16 || q_head * 2 % 16 || !cp::aligned(out, 16))
+    return cp::set_error(CP_ERR_ALIGN, "rows and heads of q and out need 16-byte alignment");
+  if (q_row < 0 || q_head < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of q");
+  const int group = q_heads / cache->heads;
+  const int64_t cap = max_pages * cache->block;
+  // a call without sequences only clears its rows
+  const bool two = groups > 0 && batch > 0;
+  const cp::AttnPlan p = cp::attn_plan(rows, batch, offsets != nullptr, group, cache->heads, cache->head_dim, cap, window);
+  const cp::SharedPlan sp = cp::shared_plan(rows, batch, two ? groups : 1, offsets != nullptr, group, cache->heads,
+                                            cache->head_dim, cap, window);
+  const int64_t slots = two ? sp.front.splits + sp.rest.splits : p.splits;
+  const int64_t most = two ? std::max(sp.front.items * sp.front.splits, sp.rest.items * sp.rest.splits) : p.items * p.splits;
+  if (most * cache->heads > cp::most_workgroups(256) || rows * q_heads > 0x7FFFFFFF ||
+      (slots > 1 && rows * q_heads > cp::most_workgroups(256)))
+    return cp::set_error(CP_ERR_SHAPE, "too many rows");
+  const size_t need = cp_kv_attention_more_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window,
+                                                    two ? groups : 0);
+  if (need && (!ws || ws_bytes < need))
+    return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, need);
+  if (need && !cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
+  cp::AttnArgs a;
+  a.c = cp::kv_args(cache, table, max_pages);
+  a.q = q;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.lens = lens;
+  a.out = out;
+  a.lse = lse;
+  a.part = (float*)ws;
+  a.rows = rows;
+  a.group = group;
+  a.causal = causal != 0;
+  a.window = window;
+  a.splits = p.splits;
+  a.least = p.least;
+  a.scale = scale * cp::kLog2e;
+  cp::AttnMore x = {};
+  x.first = more->first;
+  x.prefix = more->prefix;
+  x.shared = two ? more->shared : nullptr;
+  x.seqs = two ? (int)(batch / groups) : 1;
+  x.slopes = more->slopes;
+  x.cap = more->softcap * cp::kLog2e;
+  x.over = more->softcap > 0.0f ? 2.0f / more->softcap : 0.0f;
+  x.series = more->softcap > 128.0f;
+  const cp::KvBatch b = {offsets, (int)batch};
+  hipStream_t st = (hipStream_t)stream;
+  const bool scores = more->softcap > 0.0f || more->slopes;
+  if (dtype == CP_BF16)
+    return scores ? cp::attn_run_more<CP_BF16, 2>(a, b, x, p, sp, (int)groups, st)
+                  : cp::attn_run_more<CP_BF16, 1>(a, b, x, p, sp, (int)groups, st);
+  return scores ? cp::attn_run_more<CP_F16, 2>(a, b, x, p, sp, (int)groups, st)
+                : cp::attn_run_more<CP_F16, 1>(a, b, x, p, sp, (int)groups, st);
 }
 
 }  // extern "C"

@@ -24,17 +24,18 @@ struct KvBatch {
 // count, where count(b, rows of b) says how many pieces a sequence has. Every wave scans
 // the batch by itself, 64 sequences a step, so nothing is planned on the host, which does
 // not know the lengths. False: the grid is an upper bound and this item is past the end; *item
-// is then which one past it.
+// is then which one past it. each: so many consecutive sequences count as one, of which q.batch
+// are given.
 template <class F>
 __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int* b, int* item,
-                                          int64_t* row0, int* n) {
+                                          int64_t* row0, int* n, int each = 1) {
   const int lane = threadIdx.x & 63;
   for (int base = 0; base < q.batch; base += 64) {
     const int s = base + lane;
     int r = 0, m = 0, pieces = 0;
     if (s < q.batch) {
-      r = q.offsets ? q.offsets[s] : s;
-      m = q.offsets ? q.offsets[s + 1] - r : 1;
+      r = q.offsets ? q.offsets[s * each] : s * each;
+      m = q.offsets ? q.offsets[(s + 1) * each] - r : each;
       m = m < 0 ? 0 : m;
       pieces = count(s, m);
     }
@@ -66,9 +67,9 @@ struct KvUnowned {
   int64_t lead, tail;
 };
 
-__device__ __forceinline__ KvUnowned kv_unowned(const KvBatch& q, int64_t rows) {
+__device__ __forceinline__ KvUnowned kv_unowned(const KvBatch& q, int64_t rows, int each = 1) {
   const int64_t lead = min(max((int64_t)q.offsets[0], (int64_t)0), rows);
-  return {lead, min(max((int64_t)q.offsets[q.batch], lead), rows)};
+  return {lead, min(max((int64_t)q.offsets[q.batch * each], lead), rows)};
 }
 
 int kv_check_cache(const cp_kv_cache* c);

@@ -166,8 +166,37 @@ def read(cache, table, offsets, total, dtype=torch.bfloat16):
     return k, v
 
 
+def _more(desc, table, rows, heads, device, softcap, slopes, first, prefix, shared):
+    """struct cp_kv_more of attention's arguments, and what keeps its arrays alive."""
+    _lib.here(device)
+    softcap = float(softcap)
+    if not 0.0 <= softcap < 1e30 or 0.0 < softcap < 1e-30:
+        raise ValueError(f"softcap {softcap} must be 0 (none) or positive")
+    if slopes is not None:
+        if not (isinstance(slopes, torch.Tensor) and slopes.is_cuda):
+            raise ValueError("slopes must be a CUDA tensor")
+        if slopes.dtype != torch.float32 or slopes.shape != (heads,):
+            raise ValueError(f"slopes must be float32 [{heads}], got {slopes.dtype} "
+                             f"{tuple(slopes.shape)}")
+        slopes = slopes.contiguous()
+    batch = table.shape[0]
+    for t, n, what in ((first, rows, "first"), (prefix, batch, "prefix")):
+        if t is not None and _index(t, 1, what).shape[0] != n:
+            raise ValueError(f"{what} of {t.shape[0]}, not {n}")
+    first = first if first is None else first.contiguous()
+    prefix = prefix if prefix is None else prefix.contiguous()
+    groups = 0
+    if shared is not None:
+        shared = _index(shared, 1, "shared")
+        groups = shared.shape[0]
+        if groups == 0 or batch % groups:
+            raise ValueError(f"{batch} sequences in {groups} groups")
+    keep = slopes, first, prefix, shared
+    return _lib.KvMore(softcap, *(None if t is None else t.data_ptr() for t in keep), groups), keep
+
+
 def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, scale=None,
-              return_lse=False):
+              return_lse=False, softcap=0.0, slopes=None, first=None, prefix=None, shared=None):
     """softmax(scale * q K^T) V over the cache: q [rows, q heads, head_dim] in bfloat16 or
     float16 -> the same shape and type (and, with return_lse, float32 [rows, q heads]: the
     natural log of each row's sum of exponentials).
@@ -176,7 +205,18 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     row i of n sits at position lens[b] - n + i and sees the tokens up to its own (causal) and,
     with window > 0, no more than the window's last ones. Query head x reads cache head
     x // (q heads / cache heads). scale is positive, head_dim ** -0.5 by default. A row that sees
-    nothing, or has no sequence, is 0, its lse -inf."""
+    nothing, or has no sequence, is 0, its lse -inf.
+
+    softcap > 0 turns scores s into softcap * tanh(s / softcap); slopes (float32 [q heads]) then
+    take slopes[x] * |p - j| from the score of token j for a row at position p (float32: a score as large as
+    2^k errs by 2^(k - 24)). first (int32 [rows]): a row sees no token before first[row],
+    as the start of its document. prefix (int32 [batch]): a row sees its sequence's tokens before prefix[b] also
+    where they come after it (causal); window and first hold for those too.
+
+    shared (int32 [groups]): the batch is groups of as many consecutive sequences each, and in
+    group g all rows of the table begin with the same shared[g] pages, as ``kvpages.fork``
+    leaves them. Those pages are read once for the whole group (from the row of its first
+    sequence). The result is the same, up to the order of the sums."""
     lib = _lib.load()
     desc = _desc(cache)
     if _dtype(q, "q") not in (torch.bfloat16, torch.float16):
@@ -189,17 +229,27 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
+    more = None
+    if softcap or slopes is not None or first is not None or prefix is not None or shared is not None:
+        more, keep = _more(desc, table, rows, heads, q.device, softcap, slopes, first, prefix, shared)
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     lse = torch.empty((rows, heads), device=q.device) if return_lse else None
     batch, max_pages = table.shape
     ragged = offsets is not None
-    nws = lib.cp_kv_attention_ws_bytes(ctypes.byref(desc), rows, heads, batch, max_pages, ragged,
-                                       window)
+    if more is None:
+        nws = lib.cp_kv_attention_ws_bytes(ctypes.byref(desc), rows, heads, batch, max_pages,
+                                           ragged, window)
+    else:
+        nws = lib.cp_kv_attention_more_ws_bytes(ctypes.byref(desc), rows, heads, batch, max_pages,
+                                                ragged, window, more.groups)
     ws = _lib.workspace(nws, q.device) if nws else None
-    _lib.check(lib.cp_kv_attention(
-        ctypes.byref(desc), q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], rows, heads,
-        table.data_ptr(), batch, max_pages, lens.data_ptr(), _lib.ptr(offsets), int(causal),
-        window, desc.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
-        _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr()))
+    args = [ctypes.byref(desc), q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], rows,
+            heads, table.data_ptr(), batch, max_pages, lens.data_ptr(), _lib.ptr(offsets),
+            int(causal), window, desc.head_dim ** -0.5 if scale is None else float(scale)]
+    ends = [out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr()]
+    if more is None:
+        _lib.check(lib.cp_kv_attention(*args, *ends))
+    else:
+        _lib.check(lib.cp_kv_attention_more(*args, ctypes.byref(more), *ends))
     out = _lib.no_backward(out, "kvcache.attention", q)
     return (out, _lib.no_backward(lse, "kvcache.attention", q)) if return_lse else out

@@ -87,3 +87,29 @@ def test_sample(lib, kw, status):  # noqa: F811
     got = lib.cp_sample(a["logits"], a["dt"], a["rows"], a["vocab"], a["step"], a["u"], a["u64"], None, 1.0, None, 0, None,
                         1.0, None, 0.0, a["token"], None)
     assert got == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(heads=3), SHAPE), (dict(dt=0), ARG), (dict(window=-1), ARG), (dict(lens=None), ARG), (dict(q=P + 8), ALIGN),
+    (dict(rows=3), SHAPE), (dict(nws=64, shared=P), WS), (dict(ws=P + 8, shared=P), ALIGN), (dict(softcap=-1.0), ARG),
+    (dict(softcap=float("nan")), ARG), (dict(softcap=float("inf")), ARG), (dict(softcap=1e-38), ARG), (dict(more=False), ARG),
+    (dict(shared=P, groups=0), SHAPE), (dict(shared=P, groups=4), SHAPE), (dict(shared=P, groups=-1), SHAPE),
+    (dict(rows=0, batch=0), OK), (dict(rows=2 ** 24, batch=2 ** 24, max_pages=1, shared=P, groups=1), SHAPE)])
+def test_attention_more(lib, kw, status):  # noqa: F811
+    a = dict(q=P, dt=1, rows=6, heads=4, batch=6, max_pages=2, lens=P, window=0, nws=1 << 50, ws=P, softcap=0.0, shared=None,
+             groups=2, more=True)
+    a.update(kw)
+    m = _lib.KvMore(a["softcap"], None, None, None, a["shared"], a["groups"])
+    got = lib.cp_kv_attention_more(ctypes.byref(_cache()), a["q"], 256, 64, a["dt"], a["rows"], a["heads"], P, a["batch"],
+                                   a["max_pages"], a["lens"], None, 1, a["window"], 1.0, ctypes.byref(m) if a["more"] else None,
+                                   P, None, a["ws"], a["nws"], None)
+    assert got == status
+
+
+def test_workspaces_of_common_pages(lib):  # noqa: F811
+    c = ctypes.byref(_cache())
+    plain = lib.cp_kv_attention_ws_bytes(c, 64, 4, 64, 512, 0, 0)
+    assert lib.cp_kv_attention_more_ws_bytes(c, 64, 4, 64, 512, 0, 0, 0) == plain
+    # two phases: two splits of every row and head at the least, and two counts
+    assert lib.cp_kv_attention_more_ws_bytes(c, 64, 4, 64, 1, 0, 0, 1) >= 64 * 4 * (2 * (64 + 2) + 2) * 4
+    assert lib.cp_kv_attention_more_ws_bytes(c, 0, 4, 64, 1, 0, 0, 1) == 0
