@@ -557,6 +557,9 @@ int cp_kv_compact(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, i
 int cp_kv_copy(const cp_kv_cache* from, const cp_kv_cache* to, const int32_t* src,
                const int32_t* dst, int64_t n, void* stream);
 
+/* Workspace bytes of cp_sample (256-byte aligned). */
+size_t cp_sample_ws_bytes(int64_t rows, int64_t vocab);
+
 /* token[r] = the next token of row r of logits [rows, vocab] (rows row_step elements apart), chosen by
  * u[r] in [0, 1) (float32; float64 with u_f64). A token of logit x weighs e^((x - max) / temperature).
  * In the order of falling logits, equal ones by number, the first top_k tokens are kept (0: all);
@@ -570,7 +573,8 @@ int cp_kv_copy(const cp_kv_cache* from, const cp_kv_cache* to, const int32_t* sr
 int cp_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_step,
               const void* u, int u_f64, const float* temperature, double temperature_all,
               const int32_t* top_k, int top_k_all, const float* top_p, double top_p_all,
-              const float* min_p, double min_p_all, int32_t* token, void* stream);
+              const float* min_p, double min_p_all, int32_t* token, void* ws, size_t ws_bytes,
+              void* stream);
 
 #ifdef __cplusplus
 }

@@ -150,7 +150,8 @@ SIGNATURES = {
     "cp_kv_compact": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "cp_kv_copy": (_i32, [_kv_p, _kv_p, _vp, _vp, _i64, _vp]),
     "cp_sample": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _f64, _vp, _i32, _vp, _f64,
-                         _vp, _f64, _vp, _vp]),
+                         _vp, _f64, _vp, _vp, _sz, _vp]),
+    "cp_sample_ws_bytes": (_sz, [_i64, _i64]),
 }
 
 

@@ -23,8 +23,10 @@
 namespace cp {
 
 constexpr int kBins = 2048;    // of a histogram
-constexpr int kList = 1024;    // tokens that are sorted at most: one a thread
-constexpr int kChunks = 2048;  // pieces of a row whose weights are summed by themselves
+constexpr int kList = 2048;    // tokens that are sorted at most: two a thread
+constexpr int kChunks = 1024;  // pieces of a row whose weights are summed by themselves, at most
+constexpr int kChunkUnits = 256;  // of 16 bytes in a piece, at least
+constexpr int kSplits = 64;     // workgroups of a row at most
 constexpr float kDead = -__builtin_inff();
 
 struct SampleArgs {
@@ -38,6 +40,9 @@ struct SampleArgs {
   double t, p, m;
   int k;
   int* token;          // [rows]
+  struct RowWork* work;  // [rows]
+  int splits;          // workgroups of a row, where it is read by several
+  int chunk_units, chunks, per;  // units of a chunk, chunks of a row and of a workgroup
 };
 
 // Order-preserving whole numbers of float32 (larger ones first do not: -0 is made 0 by the reader).
@@ -53,30 +58,35 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 __device__ __forceinline__ uint64_t place(uint32_t key, int i) { return (uint64_t)key << 32 | (0xFFFFFFFFu - (uint32_t)i); }
 __device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFFFu - (uint32_t)place); }
 
-// round(2^s e^((x - max) / T)) with scale = log2 e / T. 2^f for |f| <= 1/2 by its series to the 12th
-// term, off by 6e-15; the product with 2^s rounds as 2^52 is added.
+// round(2^s e^((x - max) / T)) with scale = log2 e / T: 2^n times the series of 2^f, |f| <= 1/2, to the 12th
+// term, off by 6e-15. Numbers round as 1.5 x 2^52 (n) and 2^52 (the weight) are added, and lie in
+// the low bits then. NaN and minus infinity weigh 0: fmax leaves the other. The largest logit is finite here.
 struct Weigh {
-  double top, scale, unit;  // unit = 2^s
+  double top, scale;
+  int shift;  // s
   __device__ __forceinline__ uint64_t operator()(float x) const {
     const double r = fmax(((double)x - top) * scale, -64.0);
-    const double n = rint(r), f = (r - n) * 0.69314718055994530942;
-    double y = 1.0 / 39916800.0;
-    y = __builtin_fma(y, f, 1.0 / 3628800.0);
-    y = __builtin_fma(y, f, 1.0 / 362880.0);
-    y = __builtin_fma(y, f, 1.0 / 40320.0);
-    y = __builtin_fma(y, f, 1.0 / 5040.0);
-    y = __builtin_fma(y, f, 1.0 / 720.0);
-    y = __builtin_fma(y, f, 1.0 / 120.0);
-    y = __builtin_fma(y, f, 1.0 / 24.0);
-    y = __builtin_fma(y, f, 1.0 / 6.0);
-    y = __builtin_fma(y, f, 0.5);
+    const double big = r + 6755399441055744.0, f = r - (big - 6755399441055744.0);
+    double y = 4.44553827187081e-10;  // ln2^k / k!
+    y = __builtin_fma(y, f, 7.054911620801121e-09);
+    y = __builtin_fma(y, f, 1.0178086009239696e-07);
+    y = __builtin_fma(y, f, 1.3215486790144305e-06);
+    y = __builtin_fma(y, f, 1.5252733804059838e-05);
+    y = __builtin_fma(y, f, 1.5403530393381606e-04);
+    y = __builtin_fma(y, f, 1.3333558146428441e-03);
+    y = __builtin_fma(y, f, 9.618129107628477e-03);
+    y = __builtin_fma(y, f, 5.5504108664821576e-02);
+    y = __builtin_fma(y, f, 2.402265069591007e-01);
+    y = __builtin_fma(y, f, 6.931471805599453e-01);
     y = __builtin_fma(y, f, 1.0);
-    y = __builtin_fma(y, f, 1.0);
-    const double two_n = __builtin_bit_cast(double, (uint64_t)((int64_t)(int)n + 1023) << 52);
-    // x = max where that is an infinity: its difference is no number
-    const double w = (double)x == top ? unit : y * (two_n * unit);
-    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) - 0x4330000000000000ull;
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, big) + shift;
+    const uint64_t b = __builtin_bit_cast(uint64_t, y);
+    const double w = __builtin_bit_cast(double, ((uint64_t)((uint32_t)(b >> 32) + (n << 20)) << 32) | (uint32_t)b) +
+                     4503599627370496.0;
+    return __builtin_bit_cast(uint64_t, w) & 0xFFFFFFFFFFFFFull;
   }
+  // Where the largest may be an infinity, too.
+  __device__ __forceinline__ uint64_t any(float x) const { return (double)x == top ? (uint64_t)1 << shift : (*this)(x); }
 };
 
 // One row's elements, 16 bytes a thread and step.
@@ -115,26 +125,167 @@ struct RowReader {
     }
     return fmaxf(x, kDead) + 0.0f;
   }
-  // f(unit, its 16 bytes) for the units first, first + by, ...; four loads in flight.
+  // f(unit, its 16 bytes) for the units first, first + by, ... before `end`; four loads in flight.
   template <class F>
-  __device__ __forceinline__ void each(int first, int by, F f) const {
+  __device__ __forceinline__ void each(int first, int by, int end, F f) const {
     constexpr int U = 4;
-    for (int g = first; g < units; g += U * by) {
+    for (int g = first; g < end; g += U * by) {
       u32x4 w[U];
 #pragma unroll
       for (int x = 0; x < U; ++x)
-        if (g + x * by < units) w[x] = load(g + x * by);
+        if (g + x * by < end) w[x] = load(g + x * by);
 #pragma unroll
       for (int x = 0; x < U; ++x)
-        if (g + x * by < units) f(g + x * by, w[x]);
+        if (g + x * by < end) f(g + x * by, w[x]);
     }
   }
 };
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int s) {
-  const uint32_t lo = __shfl_xor((int)(uint32_t)v, s), hi = __shfl_xor((int)(v >> 32), s);
-  return (uint64_t)hi << 32 | lo;
+// What the launches of a call hand on about a row.
+struct RowWork {
+  uint64_t mass[kBins];
+  uint32_t count[kBins];
+  uint64_t list[kList];
+  uint64_t chunk[kChunks];
+  uint64_t top[kSplits], least[kSplits];  // of every workgroup: its largest place, its least key's complement
+  uint64_t before, goal;  // weight ahead of the border's bin, and the border's
+  uint64_t cut;           // place of the last token kept
+  uint32_t n;             // tokens on the list, or that there were for it
+  uint32_t done;          // the row has its token
+};
+
+// How a row is dealt with.
+enum RowKind { kGreedy, kWhole, kFront, kShare, kAll };
+
+struct RowSettings {
+  double t, p, m, u;
+  uint64_t k;
+  RowKind kind;
+};
+
+__device__ __forceinline__ RowSettings settings(const SampleArgs& a, int r) {
+  RowSettings s;
+  s.t = a.temperature ? (double)a.temperature[r] : a.t;
+  s.p = a.top_p ? (double)a.top_p[r] : a.p;
+  const double m = a.min_p ? (double)a.min_p[r] : a.m;
+  s.m = m > 0.0 ? fmin(m, 1.0) : 0.0;
+  s.u = a.u64 ? ((const double*)a.u)[r] : (double)((const float*)a.u)[r];
+  const int k = max(a.top_k ? a.top_k[r] : a.k, 0);
+  s.k = k >= a.vocab ? 0 : k;
+  s.kind = !(s.t > 0.0) ? kGreedy : s.k > kList ? kWhole : s.k ? kFront : s.p < 1.0 ? kShare : kAll;
+  return s;
 }
+
+// Least whole number that is no less than p times the sum, and at least 1: the first token stays.
+__device__ __forceinline__ uint64_t mass_goal(double p, uint64_t total) {
+  const double g = ceil(fmax(p, 0.0) * (double)total);
+  return g >= (double)total ? total : max((uint64_t)g, (uint64_t)1);
+}
+__device__ __forceinline__ uint64_t pick_goal(double u, uint64_t total) {
+  const double g = floor(fmax(u, 0.0) * (double)total);
+  return g >= (double)(total - 1) ? total - 1 : (uint64_t)g;
+}
+
+__device__ __forceinline__ uint64_t join64(int lo, int hi) { return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo; }
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int s) {
+  return join64(__shfl_xor((int)(uint32_t)v, s), __shfl_xor((int)(v >> 32), s));
+}
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int s) {
+  return join64(__shfl_up((int)(uint32_t)v, s), __shfl_up((int)(v >> 32), s));
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) v += shfl_xor64(v, s);
+  return v;
+}
+
+// Sum of v over the threads before this one, and over all W waves.
+template <int W>
+__device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t sum = v;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint64_t o = shfl_up64(sum, s);
+    if (lane >= s) sum += o;
+  }
+  if (lane == 63) red[wave] = sum;
+  __syncthreads();
+  uint64_t base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    base += w < wave ? red[w] : 0;
+    all += red[w];
+  }
+  __syncthreads();
+  *total = all;
+  return base + sum - v;
+}
+
+template <int W>
+__device__ __forceinline__ uint64_t max_block(uint64_t v, uint64_t* red) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint64_t o = shfl_xor64(v, s);
+    v = o > v ? o : v;
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) v = red[w] > v ? red[w] : v;
+  __syncthreads();
+  return v;
+}
+
+// Up to 1024 E values, number t + 1024 e in thread t's v[e], sorted, the largest first; n of them are not
+// 0. Steps within a wave exchange by shuffles: up to 64 values need no other.
+template <int E>
+__device__ __forceinline__ void sort_block(uint64_t (&v)[E], int n, uint64_t* list) {
+  const int t = threadIdx.x;
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (E > 1 && j == 1024) {
+        const uint64_t a = v[0], b = v[E - 1];
+        v[0] = a > b ? a : b, v[E - 1] = a > b ? b : a;
+        continue;
+      }
+      uint64_t o[E];
+      if (j < 64) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = shfl_xor64(v[e], j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) list[t + 1024 * e] = v[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = list[(t ^ j) + 1024 * e];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool first = !(t & j), down = !((t + 1024 * e) & k);  // down: the larger one first
+        v[e] = (first == down) == (v[e] > o[e]) ? v[e] : o[e];
+      }
+    }
+}
+
+// Bins of falling logits, as many as bring the least logit, or the one from which on weights are 0, to the
+// last of them. Monotone, as subtraction, product and conversion round monotonically; where the
+// largest is an infinity, the others' differences or their products with 0 go to the last bin.
+struct Bins {
+  float top, per;
+  __device__ __forceinline__ Bins() {}
+  __device__ __forceinline__ Bins(float largest, float least, int shift, double t) : top(largest) {
+    const double span = fmin((double)largest - (double)least, (shift + 2) * 0.6931471805599453 * t);
+    per = span > 0.0 ? (float)fmin((double)kBins / span, 3e38) : 0.0f;
+    if (!(per > 0.0f)) per = 0.0f;
+  }
+  __device__ __forceinline__ int operator()(float x) const {
+    return x == top ? 0 : min((int)fminf((top - x) * per, 4e6f), kBins - 1);
+  }
+};
 
 struct SampleShared {
   uint64_t mass[kBins];  // of a histogram
@@ -146,71 +297,130 @@ struct SampleShared {
   uint64_t pick[4];
 };
 
-// Sum of v over the threads before this one, and over all 1024.
-__device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64_t* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t sum = v;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint64_t o = (uint64_t)(uint32_t)__shfl_up((int)(sum >> 32), s) << 32 | (uint32_t)__shfl_up((int)(uint32_t)sum, s);
-    if (lane >= s) sum += o;
-  }
-  if (lane == 63) red[wave] = sum;
-  __syncthreads();
-  uint64_t base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    base += w < wave ? red[w] : 0;
-    all += red[w];
-  }
-  __syncthreads();
-  *total = all;
-  return base + sum - v;
-}
-
-__device__ __forceinline__ uint64_t max_block(uint64_t v, uint64_t* red) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint64_t o = shfl_xor64(v, s);
-    v = o > v ? o : v;
-  }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 16; ++w) v = red[w] > v ? red[w] : v;
-  __syncthreads();
-  return v;
-}
-
-// The first n threads' values sorted, the largest first (threads past them: 0). Steps within a wave
-// exchange by shuffles; n <= 64 needs no other.
-__device__ __forceinline__ uint64_t sort_block(uint64_t v, int n, uint64_t* list) {
+// Chooses among the n tokens of the list in LDS, all that may be kept, by their places: k, p, m and u as
+// in the file's heading (k 0: all n).
+template <int E>
+__device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int n, const RowSettings& s) {
   const int t = threadIdx.x;
-  int size = 64;
-  while (size < n) size <<= 1;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      uint64_t o;
-      if (j < 64) {
-        o = shfl_xor64(v, j);
-      } else {
-        list[t] = v;
-        __syncthreads();
-        o = list[t ^ j];
-        __syncthreads();
-      }
-      const bool first = !(t & j), down = !(t & k);  // down: the larger one first
-      v = (first == down) == (v > o) ? v : o;
-    }
-  return v;
+  const double unit = (double)((uint64_t)1 << weigh.shift);
+  uint64_t v[E], w[E], before[E], total = 0, kept = 0, sum;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
+  __syncthreads();
+  sort_block<E>(v, n, sm.list);
+  const int last = s.k ? min(n, (int)s.k) : n;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    w[e] = t + 1024 * e < last ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
+    before[e] = total + scan_block<16>(w[e], sm.red, &sum);
+    total += sum;
+  }
+  const uint64_t share = s.p < 1.0 ? mass_goal(s.p, total) : total;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool keep = t + 1024 * e < last && (t + 1024 * e == 0 || (before[e] < share && (double)w[e] >= s.m * unit));
+    w[e] = keep ? w[e] : 0;
+    sm.mass[t + 1024 * e] = w[e];
+    // by rising number, the kept ones first
+    v[e] = keep ? (uint64_t)(uint32_t)v[e] << 32 | (uint32_t)(t + 1024 * e) : 0;
+    scan_block<16>(w[e], sm.red, &sum);
+    kept += sum;
+  }
+  const uint64_t goal = pick_goal(s.u, kept);
+  sort_block<E>(v, n, sm.list);
+  total = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint64_t mine = v[e] ? sm.mass[(uint32_t)v[e]] : 0;
+    const uint64_t b = total + scan_block<16>(mine, sm.red, &sum);
+    total += sum;
+    if (b <= goal && b + mine > goal) sm.pick[2] = (uint64_t)(0xFFFFFFFFu - (uint32_t)(v[e] >> 32));
+  }
+  __syncthreads();
+  return (int)sm.pick[2];
 }
 
-// Threshold of a front: what is kept is every token whose place is at least this.
-struct Cut {
-  uint64_t place;
-  bool list;  // LDS holds the n tokens at or before the cut's bin, unsorted
-  int n;
-};
+// The place of the last token kept among the n of the list in LDS: the one before which, `before` included,
+// less than goal lies.
+template <int E>
+__device__ __forceinline__ uint64_t last_kept(SampleShared& sm, const Weigh& weigh, int n, uint64_t before,
+                                              uint64_t goal) {
+  const int t = threadIdx.x;
+  uint64_t v[E], sum, least = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
+  __syncthreads();
+  sort_block<E>(v, n, sm.list);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint64_t w = t + 1024 * e < n ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
+    const uint64_t b = before + scan_block<16>(w, sm.red, &sum);
+    before += sum;
+    if (t + 1024 * e < n && b < goal && ~v[e] > least) least = ~v[e];
+  }
+  return ~max_block<16>(least, sm.red);
+}
+
+// The sum of value(i, x) over chunk c, by one wave.
+template <int DT, class F>
+__device__ __forceinline__ uint64_t chunk_sum(const SampleArgs& a, const RowReader<DT>& row, int c, F value) {
+  const int lane = threadIdx.x & 63, g0 = c * a.chunk_units, g1 = min(row.units, g0 + a.chunk_units);
+  uint64_t v = 0;
+  for (int g = g0 + lane; g < g1; g += 256) {
+    u32x4 w[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (g + 64 * x < g1) w[x] = row.load(g + 64 * x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (g + 64 * x < g1) {
+#pragma unroll
+        for (int j = 0; j < RowReader<DT>::E; ++j)
+          v += value((g + 64 * x) * RowReader<DT>::E - row.off + j, RowReader<DT>::value(w[x], j));
+      }
+  }
+  return wave_sum64(v);
+}
+
+// The number of the first token at which the sum of value(i, x) in the order of numbers passes goal, which
+// is less than the whole. The chunks' sums are in LDS. 1024 threads.
+template <int DT, class F>
+__device__ __forceinline__ int find(const SampleArgs& a, SampleShared& sm, const RowReader<DT>& row, uint64_t goal,
+                                    F value) {
+  constexpr int E = RowReader<DT>::E;
+  uint64_t sum;
+  const uint64_t mine = (int)threadIdx.x < a.chunks ? sm.chunk[threadIdx.x] : 0;
+  const uint64_t before = scan_block<16>(mine, sm.red, &sum);
+  if (before <= goal && before + mine > goal) sm.pick[0] = threadIdx.x, sm.pick[1] = before;
+  __syncthreads();
+  const int c = (int)sm.pick[0], g1 = min(row.units, (c + 1) * a.chunk_units);
+  uint64_t base = sm.pick[1];
+  for (int g0 = c * a.chunk_units; g0 < g1 && base <= goal; g0 += 1024) {
+    const int g = g0 + threadIdx.x;
+    uint64_t v[E], all = 0;
+    if (g < g1) {
+      const u32x4 w = row.load(g);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        v[j] = value(g * E - row.off + j, RowReader<DT>::value(w, j));
+        all += v[j];
+      }
+    }
+    uint64_t b = base + scan_block<16>(all, sm.red, &sum);
+    if (b <= goal && b + all > goal) {
+      int j = 0;
+#pragma unroll
+      for (int x = 0; x < E; ++x) {
+        b += v[x];
+        if (b <= goal) j = x + 1;
+      }
+      sm.pick[2] = (uint64_t)(g * E - row.off + min(j, E - 1));
+    }
+    base += sum;
+  }
+  __syncthreads();
+  return (int)sm.pick[2];
+}
 
 template <int DT>
 struct Sampler {
@@ -218,21 +428,13 @@ struct Sampler {
   SampleShared& sm;
   RowReader<DT> row;
   Weigh weigh;
-  double unit;
-  float top;      // largest logit
-  float per_bin;  // bins a logit of one
+  Bins bin;
 
   static constexpr int E = RowReader<DT>::E;
 
-  // Bins of falling logits: monotone, as subtraction, product and conversion round monotonically. Where
-  // the largest is an infinity, the others' differences or their products with 0 go to the last bin.
-  __device__ __forceinline__ int bin(float x) const {
-    return x == top ? 0 : min((int)fminf((top - x) * per_bin, 4e6f), kBins - 1);
-  }
-
   template <class F>
   __device__ __forceinline__ void tokens(F f) const {
-    row.each(threadIdx.x, 1024, [&](int unit, const u32x4& w) {
+    row.each(threadIdx.x, 1024, row.units, [&](int unit, const u32x4& w) {
       const int i0 = unit * E - row.off;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -254,7 +456,7 @@ struct Sampler {
     const int i = 2 * threadIdx.x;
     uint64_t all;
     const uint64_t c0 = sm.count[i], c1 = sm.count[i + 1], m0 = sm.mass[i], m1 = sm.mass[i + 1];
-    const uint64_t c = scan_block(c0 + c1, sm.red, &all), m = scan_block(m0 + m1, sm.red, &all);
+    const uint64_t c = scan_block<16>(c0 + c1, sm.red, &all), m = scan_block<16>(m0 + m1, sm.red, &all);
     if (threadIdx.x == 0) sm.pick[0] = kBins - 1, sm.pick[1] = sm.pick[2] = 0;
     __syncthreads();
     const uint64_t goal = by_count ? by_count : by_mass;
@@ -286,7 +488,7 @@ struct Sampler {
 
   // The least key of a bin: keys rise as bins fall.
   __device__ __forceinline__ uint32_t least_key(int b) const {
-    uint32_t lo = key_of(kDead) + 1, hi = key_of(top);  // bin(hi) = 0 <= b
+    uint32_t lo = key_of(kDead) + 1, hi = key_of(bin.top);  // bin(hi) = 0 <= b
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo) / 2;
       if (bin(value_of(mid)) <= b) hi = mid;
@@ -296,30 +498,32 @@ struct Sampler {
   }
 
   // Of the tokens at or above `cut`, the place of the last one kept: by_count tokens, or those before which
-  // less than by_mass lies. Afterwards *kept is their weight (by_mass only).
+  // less than by_mass lies.
   //
   // A histogram finds the bin the border lies in; the bin's keys are split again until its tokens fit
   // the list, or are all equal.
-  __device__ __forceinline__ Cut front(uint64_t cut, uint64_t by_count, uint64_t by_mass, int at, uint64_t count,
+  __device__ __forceinline__ uint64_t front(uint64_t cut, uint64_t by_count, uint64_t by_mass, int at, uint64_t count,
                                        uint64_t mass) {
-    uint32_t hi = at == 0 ? key_of(top) : least_key(at - 1) - 1, lo = least_key(at);
+    uint32_t hi = at == 0 ? key_of(bin.top) : least_key(at - 1) - 1, lo = least_key(at);
     for (;;) {
       int n;
       const uint64_t in_bin = sm.count[at];
-      if (count + in_bin <= kList) {  // everything down to the border fits
-        collect(lo, 0xFFFFFFFFu, cut, &n);
-        return {0, true, n};
-      }
       if (in_bin <= kList) {
         collect(lo, hi, cut, &n);
-        const uint64_t v = sort_block(threadIdx.x < n ? sm.list[threadIdx.x] : 0, n, sm.list);
-        const uint64_t w = threadIdx.x < n ? weigh(value_of((uint32_t)(v >> 32))) : 0;
-        uint64_t all;
-        const uint64_t before = mass + scan_block(w, sm.red, &all);
-        const bool keep = threadIdx.x < n && (by_count ? count + threadIdx.x < by_count : before < by_mass);
-        // the last kept: the smallest place
-        const uint64_t last = ~max_block(keep ? ~v : 0, sm.red);
-        return {last, false, 0};
+        if (by_count) {
+          uint64_t v[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) v[e] = (int)threadIdx.x + 1024 * e < n ? sm.list[threadIdx.x + 1024 * e] : 0;
+          __syncthreads();
+          sort_block<2>(v, n, sm.list);
+          const int at = (int)(by_count - count) - 1;  // of the sorted list
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if ((int)threadIdx.x + 1024 * e == at) sm.pick[3] = v[e];
+          __syncthreads();
+          return sm.pick[3];
+        }
+        return last_kept<2>(sm, weigh, n, mass, by_mass);
       }
       if (lo == hi) break;
       const int s = max(0, 32 - __clz(hi - lo) - 11);
@@ -330,7 +534,7 @@ struct Sampler {
         if (k >= lo && k <= top_key && place(k, i) >= cut) {
           const uint32_t b = (top_key - k) >> s;
           atomicAdd(&sm.count[b], 1u);
-          if (by_mass) atomicAdd((unsigned long long*)&sm.mass[b], (unsigned long long)weigh(x));
+          if (by_mass) atomicAdd((unsigned long long*)&sm.mass[b], (unsigned long long)weigh.any(x));
         }
       });
       __syncthreads();
@@ -345,291 +549,424 @@ struct Sampler {
     if (by_count) {
       need = by_count - count;
     } else {
-      const uint64_t w = weigh(value_of(hi));
+      const uint64_t w = weigh.any(value_of(hi));
       need = w ? (by_mass - mass + w - 1) / w : 1;
     }
-    return {nth(hi, cut, need), false, 0};
-  }
-
-  // Elements of a chunk, a power of two of the units a wave takes in a step.
-  __device__ __forceinline__ int chunk_shift() const {
-    int s = 6;
-    while (((row.units - 1) >> s) >= kChunks) ++s;
-    return s;
+    return nth(hi, cut, need);
   }
 
   // Sums value(i, x) over chunks of the row into sm.chunk, then finds the chunk in which the sum in the
   // order of numbers passes `goal`: the number of the first token at which it does.
   template <class F>
   __device__ __forceinline__ void chunk_sums(F value) {
-    for (int i = threadIdx.x; i < kChunks; i += 1024) sm.chunk[i] = 0;
     __syncthreads();
-    const int s = chunk_shift();
-    for (int unit = threadIdx.x; unit - (int)(threadIdx.x & 63) < row.units; unit += 1024) {  // whole waves
-      const int i0 = unit * E - row.off;
-      uint64_t v = 0;
-      if (unit < row.units) {
-        const u32x4 w = row.load(unit);
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float x = RowReader<DT>::value(w, j);
-          if (x != kDead) v += value(i0 + j, x);
-        }
-      }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) v += shfl_xor64(v, k);
-      if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&sm.chunk[unit >> s], (unsigned long long)v);
+    for (int c = threadIdx.x >> 6; c < a.chunks; c += 16) {
+      const uint64_t v = chunk_sum<DT>(a, row, c, value);
+      if ((threadIdx.x & 63) == 0) sm.chunk[c] = v;
     }
     __syncthreads();
-  }
-
-  template <class F>
-  __device__ __forceinline__ int find(uint64_t goal, F value) {
-    const int i = 2 * threadIdx.x;
-    uint64_t all;
-    const uint64_t c0 = sm.chunk[i], c1 = sm.chunk[i + 1], c = scan_block(c0 + c1, sm.red, &all);
-    if (c <= goal && c + c0 > goal) sm.pick[0] = i, sm.pick[1] = c;
-    else if (c + c0 <= goal && c + c0 + c1 > goal) sm.pick[0] = i + 1, sm.pick[1] = c + c0;
-    __syncthreads();
-    const int at = (int)sm.pick[0], s = chunk_shift();
-    if (threadIdx.x < 64) {  // 64 units a step, in order
-      uint64_t base = sm.pick[1];
-      const int end = min(row.units, (at + 1) << s);
-      for (int g = (at << s) + threadIdx.x; __any(g < end); g += 64) {
-        uint64_t v[E], sum = 0;
-        u32x4 w = {};
-        if (g < end) w = row.load(g);
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float x = RowReader<DT>::value(w, j);
-          v[j] = g < end && x != kDead ? value(g * E - row.off + j, x) : 0;
-          sum += v[j];
-        }
-        uint64_t incl = sum;
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) {
-          const uint64_t o =
-              (uint64_t)(uint32_t)__shfl_up((int)(incl >> 32), k) << 32 | (uint32_t)__shfl_up((int)(uint32_t)incl, k);
-          if ((int)threadIdx.x >= k) incl += o;
-        }
-        const unsigned long long hit = __ballot(base + incl > goal);
-        if (hit) {
-          const int l = __ffsll(hit) - 1;
-          if ((int)threadIdx.x == l) {
-            uint64_t b = base + incl - sum;
-            int j = 0;
-#pragma unroll
-            for (int x = 0; x < E; ++x) {
-              b += v[x];
-              if (b <= goal) j = x + 1;
-            }
-            sm.pick[2] = (uint64_t)(g * E - row.off + min(j, E - 1));
-          }
-          break;
-        }
-        base += (uint64_t)(uint32_t)__shfl((int)(incl >> 32), 63) << 32 | (uint32_t)__shfl((int)(uint32_t)incl, 63);
-      }
-    }
-    __syncthreads();
-    return (int)sm.pick[2];
   }
 
   // The place of the need'th token with this key at or above `cut`, by number.
   __device__ __forceinline__ uint64_t nth(uint32_t key, uint64_t cut, uint64_t need) {
-    auto one = [&](int i, float x) -> uint64_t { return key_of(x) == key && place(key, i) >= cut; };
+    auto one = [&](int i, float x) -> uint64_t { return x != kDead && key_of(x) == key && place(key, i) >= cut; };
     chunk_sums(one);
-    uint64_t v = 0, all;
-    for (int i = threadIdx.x; i < kChunks; i += 1024) v += sm.chunk[i];
-    scan_block(v, sm.red, &all);
+    uint64_t all;
+    scan_block<16>((int)threadIdx.x < a.chunks ? sm.chunk[threadIdx.x] : 0, sm.red, &all);
     if (all == 0) return cut;  // no such token: not reached
-    return place(key, find(min(need, all) - 1, one));
+    return place(key, find<DT>(a, sm, row, min(need, all) - 1, one));
   }
 
-  // The tokens of the list, sorted, are all that is left to choose from.
-  __device__ __forceinline__ int choose(int n, uint64_t k, double p, double m, double u) {
-    const int t = threadIdx.x;
-    const uint64_t v = sort_block(t < n ? sm.list[t] : 0, n, sm.list);
-    uint64_t total, kept;
-    const bool in = t < n && (k == 0 || (uint64_t)t < k);
-    const uint64_t w = in ? weigh(value_of((uint32_t)(v >> 32))) : 0;
-    const uint64_t before = scan_block(w, sm.red, &total);
-    const bool keep = in && (t == 0 || ((!(p < 1.0) || before < mass_goal(p, total)) && (double)w >= m * unit));
-    scan_block(keep ? w : 0, sm.red, &kept);
-    const uint64_t goal = pick_goal(u, kept);
-    __syncthreads();
-    sm.mass[t] = keep ? w : 0;
-    // by rising number, the kept ones first
-    const uint64_t by_number = sort_block(keep ? (uint64_t)(uint32_t)v << 32 | (uint32_t)t : 0, n, sm.list);
-    const uint64_t mine = by_number ? sm.mass[(uint32_t)by_number] : 0;
-    const uint64_t b = scan_block(mine, sm.red, &total);
-    if (b <= goal && b + mine > goal) sm.pick[2] = (uint64_t)(0xFFFFFFFFu - (uint32_t)(by_number >> 32));
-    __syncthreads();
-    return (int)sm.pick[2];
-  }
-
-  // Least whole number that is no less than p times the sum, and at least 1: the first token stays.
-  static __device__ __forceinline__ uint64_t mass_goal(double p, uint64_t total) {
-    const double g = ceil(fmax(p, 0.0) * (double)total);
-    return g >= (double)total ? total : max((uint64_t)g, (uint64_t)1);
-  }
-  static __device__ __forceinline__ uint64_t pick_goal(double u, uint64_t total) {
-    const double g = floor(fmax(u, 0.0) * (double)total);
-    return g >= (double)(total - 1) ? total - 1 : (uint64_t)g;
+  // A row by one workgroup, whatever it holds.
+  __device__ __forceinline__ int whole(const RowSettings& s) {
+    uint64_t all, k = s.k, alive = 0, cut = 0, count, mass;
+    int at;
+    tokens([&](int, float) { ++alive; });
+    scan_block<16>(alive, sm.red, &all);
+    if (k >= all) k = 0;
+    if (k) {
+      clear_bins();
+      tokens([&](int, float x) { atomicAdd(&sm.count[bin(x)], 1u); });
+      __syncthreads();
+      border(k, 0, &at, &count, &mass);
+      cut = front(0, k, 0, at, count, 0);
+    }
+    if (s.p < 1.0) {
+      clear_bins();
+      tokens([&](int i, float x) {
+        if (place(key_of(x), i) < cut) return;
+        const int b = bin(x);
+        atomicAdd(&sm.count[b], 1u);
+        atomicAdd((unsigned long long*)&sm.mass[b], (unsigned long long)weigh.any(x));
+      });
+      __syncthreads();
+      scan_block<16>(sm.mass[threadIdx.x] + sm.mass[threadIdx.x + 1024], sm.red, &all);
+      const uint64_t goal = mass_goal(s.p, all);
+      border(0, goal, &at, &count, &mass);
+      cut = front(cut, 0, goal, at, count, mass);
+    }
+    const double least = s.m * (double)((uint64_t)1 << weigh.shift);
+    auto value = [&](int i, float x) -> uint64_t {
+      if (place(key_of(x), i) < cut) return 0;
+      const uint64_t w = weigh.any(x);
+      return (double)w >= least ? w : 0;
+    };
+    chunk_sums(value);
+    scan_block<16>((int)threadIdx.x < a.chunks ? sm.chunk[threadIdx.x] : 0, sm.red, &all);
+    return find<DT>(a, sm, row, pick_goal(s.u, all), value);
   }
 };
 
-// A workgroup a row.
+// A row's largest and least logit as its first launch left them (nothing but minus infinity: kDead).
+struct RowRange {
+  float top, least;
+};
+__device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork& w) {
+  uint64_t top = 0, least = 0;
+  for (int i = 0; i < a.splits; ++i) top = max(top, w.top[i]), least = max(least, w.least[i]);
+  return {top ? value_of((uint32_t)(top >> 32)) : kDead, value_of(~(uint32_t)least)};
+}
+
+// Launch 1, a.splits workgroups a row as all others that read it: its largest logit (and the first token that
+// has it, where that is the answer), its least, and what the next ones add to cleared.
 template <int DT>
-__global__ __launch_bounds__(1024) void sample_kernel(SampleArgs a) {
+__global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a) {
+  __shared__ uint64_t red[4];
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
+  const RowSettings s = settings(a, r);
+  const RowReader<DT> row(a, r);
+  RowWork& w = a.work[r];
+  const int g0 = at * a.per * a.chunk_units, g1 = min(row.units, (at + 1) * a.per * a.chunk_units);
+  constexpr int E = RowReader<DT>::E;
+  if (s.kind == kGreedy) {
+    uint64_t best = 0;
+    row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& v) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float x = RowReader<DT>::value(v, j);
+        const uint64_t p = place(key_of(x), unit * E - row.off + j);
+        best = x != kDead && p > best ? p : best;
+      }
+    });
+    best = max_block<4>(best, red);
+    if (threadIdx.x == 0) w.top[at] = best;
+  } else {
+    float top = kDead, least = __builtin_inff();
+    row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float x = RowReader<DT>::value(v, j);
+        top = fmaxf(top, x);
+        least = fminf(least, x == kDead ? __builtin_inff() : x);
+      }
+    });
+    const uint64_t hi = max_block<4>(top == kDead ? 0 : place(key_of(top), 0), red);
+    const uint64_t lo = max_block<4>(~key_of(least), red);
+    if (threadIdx.x == 0) w.top[at] = hi, w.least[at] = lo;
+    if (s.kind == kShare)
+      for (int i = at * 256 + threadIdx.x; i < kBins; i += a.splits * 256) w.mass[i] = 0;
+    if (s.kind == kFront)
+      for (int i = at * 256 + threadIdx.x; i < kBins; i += a.splits * 256) w.count[i] = 0;
+  }
+  if (at == 0 && threadIdx.x == 0) w.n = w.done = 0;
+}
+
+// Launch 2. top_k: how many tokens are in each bin, as far as this workgroup's part reaches k. top_p: the bins'
+// weights. Neither: the chunks' weights.
+template <int DT>
+__global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint64_t red[4];
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
+  const RowSettings s = settings(a, r);
+  if (s.kind == kGreedy || s.kind == kWhole) return;
+  const RowReader<DT> row(a, r);
+  RowWork& w = a.work[r];
+  const RowRange range = row_range(a, w);
+  if (!(fabsf(range.top) < __builtin_inff())) return;  // an infinity: one workgroup deals with it
+  const int c0 = at * a.per, c1 = min(a.chunks, c0 + a.per);
+  const int g0 = c0 * a.chunk_units, g1 = min(row.units, c1 * a.chunk_units);
+  constexpr int E = RowReader<DT>::E;
+  const Weigh weigh = {(double)range.top, 1.4426950408889634074 / s.t, a.shift};
+  if (s.kind == kAll) {
+    const uint64_t least = (uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift));
+    for (int c = c0 + (threadIdx.x >> 6); c < c1; c += 4) {
+      const uint64_t v = chunk_sum<DT>(a, row, c, [&](int, float x) {
+        const uint64_t y = weigh(x);
+        return y >= least ? y : 0;
+      });
+      if ((threadIdx.x & 63) == 0) w.chunk[c] = v;
+    }
+    return;
+  }
+  const Bins bin(range.top, range.least, a.shift, s.t);
+  if (s.kind == kShare) {
+    for (int i = threadIdx.x; i < kBins; i += 256) mass[i] = 0;
+    __syncthreads();
+    row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float x = RowReader<DT>::value(v, j);
+        const uint64_t y = weigh(x);
+        if (y) atomicAdd((unsigned long long*)&mass[bin(x)], (unsigned long long)y);
+      }
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += 256)
+      if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
+    return;
+  }
+  uint32_t* count = reinterpret_cast<uint32_t*>(mass);
+  for (int i = threadIdx.x; i < kBins; i += 256) count[i] = 0;
+  __syncthreads();
+  row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float x = RowReader<DT>::value(v, j);
+      if (x != kDead) atomicAdd(&count[bin(x)], 1u);
+    }
+  });
+  __syncthreads();
+  uint64_t sum = 0, all;
+  for (int i = 0; i < kBins / 256; ++i) sum += count[threadIdx.x * (kBins / 256) + i];
+  uint64_t before = scan_block<4>(sum, red, &all);
+  for (int i = 0; i < kBins / 256 && before < s.k; ++i) {
+    const uint32_t c = count[threadIdx.x * (kBins / 256) + i];
+    if (c) atomicAdd(&w.count[threadIdx.x * (kBins / 256) + i], c);
+    before += c;
+  }
+}
+
+// Launch 3: the tokens that the border is among. top_k: all up to the end of its bin; top_p: its bin's.
+template <int DT>
+__global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
+  __shared__ uint64_t red[4];
+  __shared__ uint64_t pick[2];
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
+  const RowSettings s = settings(a, r);
+  if (s.kind != kFront && s.kind != kShare) return;
+  const RowReader<DT> row(a, r);
+  RowWork& w = a.work[r];
+  const RowRange range = row_range(a, w);
+  if (!(fabsf(range.top) < __builtin_inff())) return;
+  const Bins bin(range.top, range.least, a.shift, s.t);
+  constexpr int N = kBins / 256, E = RowReader<DT>::E;
+  uint64_t v[N], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = s.kind == kFront ? w.count[threadIdx.x * N + i] : w.mass[threadIdx.x * N + i];
+    sum += v[i];
+  }
+  uint64_t before = scan_block<4>(sum, red, &all);
+  const uint64_t goal = s.kind == kFront ? s.k : mass_goal(s.p, all);
+  if (threadIdx.x == 0) pick[0] = kBins;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (before < goal && before + v[i] >= goal) pick[0] = threadIdx.x * N + i, pick[1] = before;
+    before += v[i];
+  }
+  __syncthreads();
+  const int border = (int)pick[0];
+  if (at == 0 && threadIdx.x == 0) {
+    w.before = pick[1], w.goal = goal;
+    if (border == kBins) w.n = kList + 1;  // fewer tokens than top_k: as if there were too many
+  }
+  if (border == kBins) return;
+  const bool front = s.kind == kFront;
+  const int g0 = at * a.per * a.chunk_units, g1 = min(row.units, (at + 1) * a.per * a.chunk_units);
+  row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& u) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float x = RowReader<DT>::value(u, j);
+      const int b = bin(x);
+      if (x != kDead && (front ? b <= border : b == border)) {
+        const uint32_t to = atomicAdd(&w.n, 1u);
+        if (to < kList) w.list[to] = place(key_of(x), unit * E - row.off + j);
+      }
+    }
+  });
+}
+
+// Launch 4, a workgroup a row: its token, or (top_p) the last place kept.
+template <int DT>
+__global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
   __shared__ SampleShared sm;
   const int r = blockIdx.x;
-  const double t = a.temperature ? (double)a.temperature[r] : a.t;
-  const double p = a.top_p ? (double)a.top_p[r] : a.p, m0 = a.min_p ? (double)a.min_p[r] : a.m;
-  const double m = m0 > 0.0 ? fmin(m0, 1.0) : 0.0;
-  const double u = a.u64 ? ((const double*)a.u)[r] : (double)((const float*)a.u)[r];
-  uint64_t k = max(a.top_k ? a.top_k[r] : a.k, 0);
-  if (k >= (uint64_t)a.vocab) k = 0;
-  Sampler<DT> s{a, sm, RowReader<DT>(a, r)};
-  if (!(t > 0.0)) {
+  const RowSettings s = settings(a, r);
+  RowWork& w = a.work[r];
+  const RowRange range = row_range(a, w);
+  int token = -1;
+  if (s.kind == kGreedy) {
     uint64_t best = 0;
-    s.tokens([&](int i, float x) {
-      const uint64_t v = place(key_of(x), i);
-      best = v > best ? v : best;
-    });
-    best = max_block(best, sm.red);
-    if (threadIdx.x == 0) a.token[r] = best ? token_of(best) : -1;
-    return;
+    for (int i = 0; i < a.splits; ++i) best = max(best, w.top[i]);
+    if (best) token = token_of(best);
+  } else if (range.top != kDead) {
+    const Weigh weigh = {(double)range.top, 1.4426950408889634074 / s.t, a.shift};
+    const RowReader<DT> row(a, r);
+    const bool list = s.kind == kFront || s.kind == kShare;
+    if (s.kind == kWhole || range.top == __builtin_inff() || (list && w.n > kList)) {
+      Sampler<DT> whole{a, sm, row, weigh, Bins(range.top, range.least, a.shift, s.t)};
+      token = whole.whole(s);
+    } else if (s.kind == kAll) {
+      const uint64_t least = (uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift));
+      const uint64_t mine = (int)threadIdx.x < a.chunks ? w.chunk[threadIdx.x] : 0;
+      uint64_t all;
+      if ((int)threadIdx.x < a.chunks) sm.chunk[threadIdx.x] = mine;
+      scan_block<16>(mine, sm.red, &all);
+      token = find<DT>(a, sm, row, pick_goal(s.u, all), [&](int, float x) {
+        const uint64_t y = weigh(x);
+        return y >= least ? y : 0;
+      });
+    } else {
+      const int n = (int)w.n;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if ((int)threadIdx.x + 1024 * e < n) sm.list[threadIdx.x + 1024 * e] = w.list[threadIdx.x + 1024 * e];
+      __syncthreads();
+      if (s.kind == kShare) {
+        const uint64_t cut = n > 1024 ? last_kept<2>(sm, weigh, n, w.before, w.goal)
+                                      : last_kept<1>(sm, weigh, n, w.before, w.goal);
+        if (threadIdx.x == 0) w.cut = cut;
+        return;
+      }
+      token = n > 1024 ? choose<2>(sm, weigh, n, s) : choose<1>(sm, weigh, n, s);
+    }
   }
-  float top = kDead, least = __builtin_inff();
-  uint32_t alive = 0;
-  s.tokens([&](int, float x) {
-    top = fmaxf(top, x), least = fminf(least, x);
-    ++alive;
-  });
-  top = value_of((uint32_t)max_block(key_of(top), sm.red));
-  least = value_of(~(uint32_t)max_block(~key_of(least), sm.red));
+  if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
+}
+
+// What a token at or before the cut of its row weighs, if that is enough for min_p.
+struct Kept {
+  Weigh weigh;
+  float x;       // of the last token kept
+  int i;
+  uint64_t least;
+  __device__ __forceinline__ Kept(const SampleArgs& a, const RowSettings& s, const RowWork& w, float top)
+      : weigh{(double)top, 1.4426950408889634074 / s.t, a.shift}, x(value_of((uint32_t)(w.cut >> 32))), i(token_of(w.cut)),
+        least((uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift))) {}
+  __device__ __forceinline__ uint64_t operator()(int at, float y) const {
+    const uint64_t v = weigh(y);
+    return (y > x || (y == x && at <= i)) && v >= least ? v : 0;
+  }
+};
+
+// Launch 5: the kept tokens' weights, by chunks.
+template <int DT>
+__global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
+  RowWork& w = a.work[r];
+  if (w.done) return;
+  const RowSettings s = settings(a, r);
+  const RowReader<DT> row(a, r);
+  const Kept kept(a, s, w, row_range(a, w).top);
+  const int c0 = at * a.per, c1 = min(a.chunks, c0 + a.per);
+  for (int c = c0 + (threadIdx.x >> 6); c < c1; c += 4) {
+    const uint64_t v = chunk_sum<DT>(a, row, c, kept);
+    if ((threadIdx.x & 63) == 0) w.chunk[c] = v;
+  }
+}
+
+// Launch 6: the token of the rows that have none.
+template <int DT>
+__global__ __launch_bounds__(1024) void sample_find_kernel(SampleArgs a) {
+  __shared__ SampleShared sm;
+  const int r = blockIdx.x;
+  RowWork& w = a.work[r];
+  if (w.done) return;
+  const RowSettings s = settings(a, r);
+  const RowReader<DT> row(a, r);
+  const Kept kept(a, s, w, row_range(a, w).top);
+  const uint64_t mine = (int)threadIdx.x < a.chunks ? w.chunk[threadIdx.x] : 0;
   uint64_t all;
-  scan_block(alive, sm.red, &all);
-  if (all == 0) {
-    if (threadIdx.x == 0) a.token[r] = -1;
-    return;
-  }
-  if (k >= all) k = 0;
-  s.unit = __builtin_bit_cast(double, (uint64_t)(a.shift + 1023) << 52);
-  s.weigh = {(double)top, 1.4426950408889634074 / t, s.unit};
-  s.top = top;
-  // bins down to the least logit, or to where weights are 0
-  const double span = fmin((double)top - (double)least, (double)(a.shift + 2) * 0.6931471805599453 * t);
-  s.per_bin = span > 0.0 ? (float)fmin((double)kBins / span, 3e38) : 0.0f;
-  if (!(s.per_bin > 0.0f)) s.per_bin = 0.0f;
-  uint64_t cut = 0;
-  if (k) {
-    s.clear_bins();
-    s.tokens([&](int, float x) { atomicAdd(&sm.count[s.bin(x)], 1u); });
-    __syncthreads();
-    int at;
-    uint64_t count, mass;
-    s.border(k, 0, &at, &count, &mass);
-    const Cut c = s.front(0, k, 0, at, count, 0);
-    if (c.list) {
-      const int token = s.choose(c.n, k, p, m, u);
-      if (threadIdx.x == 0) a.token[r] = token;
-      return;
-    }
-    cut = c.place;
-  }
-  if (p < 1.0) {
-    s.clear_bins();
-    s.tokens([&](int i, float x) {
-      if (place(key_of(x), i) < cut) return;
-      const int b = s.bin(x);
-      atomicAdd(&sm.count[b], 1u);
-      atomicAdd((unsigned long long*)&sm.mass[b], (unsigned long long)s.weigh(x));
-    });
-    __syncthreads();
-    uint64_t v = 0, total;
-    for (int i = threadIdx.x; i < kBins; i += 1024) v += sm.mass[i];
-    scan_block(v, sm.red, &total);
-    const uint64_t goal = Sampler<DT>::mass_goal(p, total);
-    int at;
-    uint64_t count, mass;
-    s.border(0, goal, &at, &count, &mass);
-    const Cut c = s.front(cut, 0, goal, at, count, mass);
-    if (c.list) {
-      // the list holds tokens past the border, too: whole bins. Their sum is not the row's
-      const int t0 = threadIdx.x;
-      const uint64_t place = sort_block(t0 < c.n ? sm.list[t0] : 0, c.n, sm.list);
-      const uint64_t w = t0 < c.n ? s.weigh(value_of((uint32_t)(place >> 32))) : 0;
-      uint64_t sum;
-      const uint64_t before = scan_block(w, sm.red, &sum);
-      const bool keep = t0 < c.n && (t0 == 0 || before < goal);
-      uint64_t n;
-      scan_block(keep, sm.red, &n);
-      __syncthreads();
-      sm.list[t0] = keep ? place : 0;
-      __syncthreads();
-      const int token = s.choose((int)n, 0, 1.0, m, u);
-      if (threadIdx.x == 0) a.token[r] = token;
-      return;
-    }
-    cut = c.place;
-  }
-  const double least_w = m * s.unit;
-  auto value = [&](int i, float x) -> uint64_t {
-    if (place(key_of(x), i) < cut) return 0;
-    const uint64_t w = s.weigh(x);
-    return (double)w >= least_w || x == top ? w : 0;
-  };
-  s.chunk_sums(value);
-  uint64_t v = 0, total;
-  for (int i = threadIdx.x; i < kChunks; i += 1024) v += sm.chunk[i];
-  scan_block(v, sm.red, &total);
-  const int token = s.find(Sampler<DT>::pick_goal(u, total), value);
+  if ((int)threadIdx.x < a.chunks) sm.chunk[threadIdx.x] = mine;
+  scan_block<16>(mine, sm.red, &all);
+  const int token = find<DT>(a, sm, row, pick_goal(s.u, all), kept);
   if (threadIdx.x == 0) a.token[r] = token;
+}
+
+constexpr int64_t kRowsAtOnce = 1024;  // rows of a batch of launches: 50 MB of workspace
+
+template <int DT>
+static int sample_rows(SampleArgs a, hipStream_t st) {
+  const dim3 many((unsigned)(a.rows * a.splits)), one((unsigned)a.rows);
+  // what no row can need is left out
+  const bool greedy = !a.temperature && !(a.t > 0.0);
+  const bool front = !greedy && (a.top_k || (a.k > 0 && a.k < a.vocab));
+  const bool share = !greedy && (a.top_p || a.p < 1.0) && (a.top_k || !front);
+  sample_range_kernel<DT><<<many, 256, 0, st>>>(a);
+  if (!greedy) sample_weigh_kernel<DT><<<many, 256, 0, st>>>(a);
+  if (front || share) sample_collect_kernel<DT><<<many, 256, 0, st>>>(a);
+  sample_choose_kernel<DT><<<one, 1024, 0, st>>>(a);
+  if (share) {
+    sample_kept_kernel<DT><<<many, 256, 0, st>>>(a);
+    sample_find_kernel<DT><<<one, 1024, 0, st>>>(a);
+  }
+  CP_LAUNCHED("sampling");
+  return CP_OK;
 }
 
 }  // namespace cp
 
 extern "C" {
 
+size_t cp_sample_ws_bytes(int64_t rows, int64_t vocab) {
+  return rows < 1 || vocab < 1 ? 0 : (size_t)std::min(rows, cp::kRowsAtOnce) * sizeof(cp::RowWork);
+}
+
 int cp_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_step, const void* u, int u_f64,
               const float* temperature, double temperature_all, const int32_t* top_k, int top_k_all, const float* top_p,
-              double top_p_all, const float* min_p, double min_p_all, int32_t* token, void* stream) {
+              double top_p_all, const float* min_p, double min_p_all, int32_t* token, void* ws, size_t ws_bytes,
+              void* stream) {
   cp::clear_error();
   const int es = cp::dtype_bytes(dtype);
   if (!es) return cp::set_error(CP_ERR_ARG, "dtype code %d", dtype);
   if (vocab < 1 || vocab > 1 << 24) return cp::set_error(CP_ERR_SHAPE, "%lld tokens", (long long)vocab);
-  if (rows < 0 || rows > cp::most_workgroups(1024)) return cp::set_error(CP_ERR_SHAPE, "%lld rows", (long long)rows);
+  if (rows < 0 || rows > 0x7FFFFFFF) return cp::set_error(CP_ERR_SHAPE, "%lld rows", (long long)rows);
   if (row_step < 0) return cp::set_error(CP_ERR_SHAPE, "negative stride of logits");
   if (rows == 0) return CP_OK;
   if (!logits || !u || !token) return cp::set_error(CP_ERR_ARG, "null logits / u / token");
   if (!cp::aligned(logits, es) || !cp::aligned(u, u_f64 ? 8 : 4))
     return cp::set_error(CP_ERR_ALIGN, "logits and u need their elements' alignment");
-  cp::SampleArgs a;
-  a.logits = logits;
-  a.step = row_step;
-  a.rows = (int)rows;
-  a.vocab = (int)vocab;
+  if (!ws || ws_bytes < cp_sample_ws_bytes(rows, vocab))
+    return cp::set_error(CP_ERR_WORKSPACE, "workspace of %zu bytes needs %zu", ws_bytes, cp_sample_ws_bytes(rows, vocab));
+  if (!cp::aligned(ws, 256)) return cp::set_error(CP_ERR_ALIGN, "workspace needs 256-byte alignment");
   int bits = 0;
   while (((int64_t)1 << bits) < vocab) ++bits;
-  a.shift = std::min(51, 62 - bits);
-  a.u = u;
-  a.u64 = u_f64;
-  a.temperature = temperature;
-  a.top_p = top_p;
-  a.min_p = min_p;
-  a.top_k = top_k;
-  a.t = temperature_all;
-  a.p = top_p_all;
-  a.m = min_p_all;
-  a.k = top_k_all;
-  a.token = token;
-  const dim3 grid((unsigned)rows);
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == CP_F32) cp::sample_kernel<CP_F32><<<grid, 1024, 0, st>>>(a);
-  if (dtype == CP_BF16) cp::sample_kernel<CP_BF16><<<grid, 1024, 0, st>>>(a);
-  if (dtype == CP_F16) cp::sample_kernel<CP_F16><<<grid, 1024, 0, st>>>(a);
-  CP_LAUNCHED("sampling");
+  const int per_unit = 16 / es;
+  const int64_t units = (vocab + 2 * per_unit - 2) / per_unit;  // wherever a row begins in its first one
+  int64_t chunk = cp::kChunkUnits;
+  while ((units + chunk - 1) / chunk > cp::kChunks) chunk *= 2;
+  for (int64_t r0 = 0; r0 < rows; r0 += cp::kRowsAtOnce) {
+    cp::SampleArgs a;
+    a.logits = (const char*)logits + r0 * row_step * es;
+    a.step = row_step;
+    a.rows = (int)std::min(rows - r0, cp::kRowsAtOnce);
+    a.vocab = (int)vocab;
+    a.shift = std::min(51, 62 - bits);
+    a.u = (const char*)u + r0 * (u_f64 ? 8 : 4);
+    a.u64 = u_f64;
+    a.temperature = temperature ? temperature + r0 : nullptr;
+    a.top_p = top_p ? top_p + r0 : nullptr;
+    a.min_p = min_p ? min_p + r0 : nullptr;
+    a.top_k = top_k ? top_k + r0 : nullptr;
+    a.t = temperature_all;
+    a.p = top_p_all;
+    a.m = min_p_all;
+    a.k = top_k_all;
+    a.token = token + r0;
+    a.work = (cp::RowWork*)ws;
+    a.chunk_units = (int)chunk;
+    a.chunks = (int)((units + chunk - 1) / chunk);
+    // enough workgroups for every CU, and several for the rows with more to do
+    const int64_t want = std::min({(int64_t)cp::kSplits, (int64_t)a.chunks, std::max(2048 / (int64_t)a.rows, (int64_t)4)});
+    a.per = (int)((a.chunks + want - 1) / want);
+    a.splits = (a.chunks + a.per - 1) / a.per;
+    const int s = dtype == CP_F32    ? cp::sample_rows<CP_F32>(a, (hipStream_t)stream)
+                  : dtype == CP_BF16 ? cp::sample_rows<CP_BF16>(a, (hipStream_t)stream)
+                                     : cp::sample_rows<CP_F16>(a, (hipStream_t)stream);
+    if (s) return s;
+  }
   return CP_OK;
 }
 

@@ -69,8 +69,10 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         logits = logits.contiguous()
     u = u.contiguous()
     token = logits.new_empty((rows,), dtype=torch.int32)
+    nws = lib.cp_sample_ws_bytes(rows, vocab)
+    ws = _lib.workspace(nws, logits.device)
     _lib.check(lib.cp_sample(logits.data_ptr(), code, rows, vocab, logits.stride(0), u.data_ptr(),
                              int(u.dtype == torch.float64), _lib.ptr(t), t_all, _lib.ptr(k), k_all,
                              _lib.ptr(p), p_all, _lib.ptr(m), m_all, token.data_ptr(),
-                             _lib.stream_ptr()))
+                             _lib.ptr(ws), nws, _lib.stream_ptr()))
     return token

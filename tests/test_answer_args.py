@@ -79,13 +79,14 @@ def test_copy(lib, a, b, kw, status):  # noqa: F811
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dt=3), ARG), (dict(vocab=0), SHAPE), (dict(vocab=2 ** 24 + 1), SHAPE), (dict(rows=-1), SHAPE),
-    (dict(rows=2 ** 22), SHAPE), (dict(step=-1), SHAPE), (dict(logits=None), ARG), (dict(u=None), ARG), (dict(token=None), ARG),
-    (dict(logits=P + 1), ALIGN), (dict(u=P + 4, u64=1), ALIGN), (dict(rows=0, logits=None), OK)])
+    (dict(rows=2 ** 31), SHAPE), (dict(step=-1), SHAPE), (dict(logits=None), ARG), (dict(u=None), ARG), (dict(token=None), ARG),
+    (dict(logits=P + 1), ALIGN), (dict(u=P + 4, u64=1), ALIGN), (dict(rows=0, logits=None), OK), (dict(ws=None), WS),
+    (dict(nws=1024), WS), (dict(ws=P + 16), ALIGN)])
 def test_sample(lib, kw, status):  # noqa: F811
-    a = dict(logits=P, dt=1, rows=2, vocab=100, step=100, u=P, u64=0, token=P)
+    a = dict(logits=P, dt=1, rows=2, vocab=100, step=100, u=P, u64=0, token=P, ws=P, nws=1 << 30)
     a.update(kw)
     got = lib.cp_sample(a["logits"], a["dt"], a["rows"], a["vocab"], a["step"], a["u"], a["u64"], None, 1.0, None, 0, None,
-                        1.0, None, 0.0, a["token"], None)
+                        1.0, None, 0.0, a["token"], a["ws"], a["nws"], None)
     assert got == status
 
 

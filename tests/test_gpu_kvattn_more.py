@@ -88,7 +88,7 @@ def test_changed_scores(kv, block, heads, d, group, scores, dtype):  # noqa: F81
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("d,scores", itertools.product((64, 128), [dict(), *SCORES]), ids=str)
+@pytest.mark.parametrize("d,scores", itertools.product((64, 96, 128, 256), [dict(), *SCORES]), ids=str)
 def test_tiles_of_many_rows(kv, d, scores, dtype):  # noqa: F811
     """Prompts of hundreds of rows over thousands of tokens, in the kernel of 128 rows a workgroup: documents,
     a prefix, a window, and weights of every size."""
