@@ -27,6 +27,9 @@ constexpr int kList = 2048;    // tokens that are sorted at most: two a thread
 constexpr int kChunks = 1024;  // pieces of a row whose weights are summed by themselves, at most
 constexpr int kChunkUnits = 256;  // of 16 bytes in a piece, at least
 constexpr int kSplits = 64;     // workgroups of a row at most
+constexpr int kFrontMost = 1024;  // top_k that several workgroups share
+constexpr int kPeaks = 8;       // of a thread
+constexpr int kMostPeaks = 4096;  // of a row
 constexpr float kDead = -__builtin_inff();
 
 struct SampleArgs {
@@ -41,6 +44,8 @@ struct SampleArgs {
   int k;
   int* token;          // [rows]
   struct RowWork* work;  // [rows]
+  uint32_t* peaks;       // [rows][splits][peaks_each]: largest keys of parts of the row
+  int peaks_each;        // 64 .. 2048, a power of two
   int splits;          // workgroups of a row, where it is read by several
   int chunk_units, chunks, per;  // units of a chunk, chunks of a row and of a workgroup
 };
@@ -58,26 +63,33 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 __device__ __forceinline__ uint64_t place(uint32_t key, int i) { return (uint64_t)key << 32 | (0xFFFFFFFFu - (uint32_t)i); }
 __device__ __forceinline__ int token_of(uint64_t place) { return (int)(0xFFFFFFFFu - (uint32_t)place); }
 
-// round(2^s e^((x - max) / T)) with scale = log2 e / T: 2^n times the series of 2^f, |f| <= 1/2, to the 12th
-// term, off by 6e-15. Numbers round as 1.5 x 2^52 (n) and 2^52 (the weight) are added, and lie in
-// the low bits then. NaN and minus infinity weigh 0: fmax leaves the other. The largest logit is finite here.
+__device__ __forceinline__ double fma_to(double a, double b, double c) {  // a b + c with c left as it is
+  double y;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(a), "v"(b), "s"(c));
+  return y;
+}
+
+// round(2^s e^((x - max) / T)) with scale = log2 e / T: 2^n p(f), where p is the polynomial of degree 10 whose
+// largest relative distance from 2^f over |f| <= 1/2 is least, 2.2e-16 (found by exchange). Numbers round as
+// 1.5 x 2^52 (n) and 2^52 (the weight) are added, and lie in the low bits then. NaN and minus infinity weigh 0: fmax
+// leaves the other. The largest logit is finite here.
 struct Weigh {
   double top, scale;
   int shift;  // s
+  __device__ __forceinline__ Weigh(float largest, double t, int s)
+      : top(largest), scale(1.4426950408889634074 / t), shift(s) {}
   __device__ __forceinline__ uint64_t operator()(float x) const {
     const double r = fmax(((double)x - top) * scale, -64.0);
     const double big = r + 6755399441055744.0, f = r - (big - 6755399441055744.0);
-    double y = 4.44553827187081e-10;  // ln2^k / k!
-    y = __builtin_fma(y, f, 7.054911620801121e-09);
-    y = __builtin_fma(y, f, 1.0178086009239696e-07);
-    y = __builtin_fma(y, f, 1.3215486790144305e-06);
-    y = __builtin_fma(y, f, 1.5252733804059838e-05);
-    y = __builtin_fma(y, f, 1.5403530393381606e-04);
-    y = __builtin_fma(y, f, 1.3333558146428441e-03);
-    y = __builtin_fma(y, f, 9.618129107628477e-03);
-    y = __builtin_fma(y, f, 5.5504108664821576e-02);
-    y = __builtin_fma(y, f, 2.402265069591007e-01);
-    y = __builtin_fma(y, f, 6.931471805599453e-01);
+    double y = fma_to(7.037270609916633e-09, f, 1.0208537624759209e-07);
+    y = fma_to(y, f, 1.321566288002748e-06);
+    y = fma_to(y, f, 1.5252658118053735e-05);
+    y = fma_to(y, f, 0.00015403529961050233);
+    y = fma_to(y, f, 0.0013333558228558876);
+    y = fma_to(y, f, 0.009618129108034647);
+    y = fma_to(y, f, 0.05550410866445885);
+    y = fma_to(y, f, 0.24022650695908768);
+    y = fma_to(y, f, 0.6931471805599497);
     y = __builtin_fma(y, f, 1.0);
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, big) + shift;
     const uint64_t b = __builtin_bit_cast(uint64_t, y);
@@ -85,8 +97,10 @@ struct Weigh {
                      4503599627370496.0;
     return __builtin_bit_cast(uint64_t, w) & 0xFFFFFFFFFFFFFull;
   }
-  // Where the largest may be an infinity, too.
-  __device__ __forceinline__ uint64_t any(float x) const { return (double)x == top ? (uint64_t)1 << shift : (*this)(x); }
+  // Of any logit, also where the largest is an infinity.
+  __device__ __forceinline__ uint64_t any(float x) const {
+    return (double)x == top ? (uint64_t)1 << shift : (*this)(x);
+  }
 };
 
 // One row's elements, 16 bytes a thread and step.
@@ -110,22 +124,21 @@ struct RowReader {
     for (int j = 0; j < E; ++j) e[j] = i0 + j >= 0 && i0 + j < vocab ? p[i0 + j] : (T)kDead;
     return __builtin_bit_cast(u32x4, e);
   }
-  // Element j of a unit: NaN as minus infinity, -0 as 0.
-  static __device__ __forceinline__ float value(const u32x4& w, int j) {
-    float x;
+  // Element j of a unit as it stands, and with NaN as minus infinity, -0 as 0.
+  static __device__ __forceinline__ float raw(const u32x4& w, int j) {
     if constexpr (DT == CP_F32) {
       const uint32_t b = w[j];
-      x = __uint_as_float(b);
+      return __uint_as_float(b);
     } else {
       const uint32_t b = w[j >> 1];
       if constexpr (DT == CP_BF16)
-        x = __uint_as_float(j & 1 ? b & 0xFFFF0000u : b << 16);
+        return __uint_as_float(j & 1 ? b & 0xFFFF0000u : b << 16);
       else
-        x = (float)__builtin_bit_cast(f16x2, b)[j & 1];
+        return (float)__builtin_bit_cast(f16x2, b)[j & 1];
     }
-    return fmaxf(x, kDead) + 0.0f;
   }
-  // f(unit, its 16 bytes) for the units first, first + by, ... before `end`; four loads in flight.
+  static __device__ __forceinline__ float value(const u32x4& w, int j) { return fmaxf(raw(w, j), kDead) + 0.0f; }
+  // f(unit, its 16 bytes, which of four) for the units first, first + by, ... before `end`; four loads in flight.
   template <class F>
   __device__ __forceinline__ void each(int first, int by, int end, F f) const {
     constexpr int U = 4;
@@ -136,7 +149,7 @@ struct RowReader {
         if (g + x * by < end) w[x] = load(g + x * by);
 #pragma unroll
       for (int x = 0; x < U; ++x)
-        if (g + x * by < end) f(g + x * by, w[x]);
+        if (g + x * by < end) f(g + x * by, w[x], x);
     }
   }
 };
@@ -144,14 +157,16 @@ struct RowReader {
 // What the launches of a call hand on about a row.
 struct RowWork {
   uint64_t mass[kBins];
-  uint32_t count[kBins];
-  uint64_t list[kList];
+  uint64_t list[2 * kList];  // tokens among which the border is; top_p: and the ones ahead of them
   uint64_t chunk[kChunks];
-  uint64_t top[kSplits], least[kSplits];  // of every workgroup: its largest place, its least key's complement
-  uint64_t before, goal;  // weight ahead of the border's bin, and the border's
-  uint64_t cut;           // place of the last token kept
-  uint32_t n;             // tokens on the list, or that there were for it
-  uint32_t done;          // the row has its token
+  uint64_t first[kSplits];   // of every workgroup: its largest place,
+  uint32_t top[kSplits], least[kSplits];  // its largest key, its least key's complement
+  uint64_t before, goal;     // weight ahead of the border's bin, and the border's
+  uint64_t cut;              // place of the last token kept
+  uint32_t least_kept;       // key of the least logit that min_p leaves
+  uint32_t n, ahead;         // tokens on either list, or that there were for it
+  uint32_t from;             // top_k: a key that at least k tokens reach
+  uint32_t done, whole;      // the row has its token; it is left to one workgroup
 };
 
 // How a row is dealt with.
@@ -172,7 +187,7 @@ __device__ __forceinline__ RowSettings settings(const SampleArgs& a, int r) {
   s.u = a.u64 ? ((const double*)a.u)[r] : (double)((const float*)a.u)[r];
   const int k = max(a.top_k ? a.top_k[r] : a.k, 0);
   s.k = k >= a.vocab ? 0 : k;
-  s.kind = !(s.t > 0.0) ? kGreedy : s.k > kList ? kWhole : s.k ? kFront : s.p < 1.0 ? kShare : kAll;
+  s.kind = !(s.t > 0.0) ? kGreedy : s.k > kFrontMost ? kWhole : s.k ? kFront : s.p < 1.0 ? kShare : kAll;
   return s;
 }
 
@@ -282,10 +297,34 @@ struct Bins {
     per = span > 0.0 ? (float)fmin((double)kBins / span, 3e38) : 0.0f;
     if (!(per > 0.0f)) per = 0.0f;
   }
-  __device__ __forceinline__ int operator()(float x) const {
-    return x == top ? 0 : min((int)fminf((top - x) * per, 4e6f), kBins - 1);
-  }
+  __device__ __forceinline__ int operator()(float x) const { return x == top ? 0 : finite(x); }
+  // The same where the largest is finite.
+  __device__ __forceinline__ int finite(float x) const { return min((int)fminf((top - x) * per, 4e6f), kBins - 1); }
 };
+
+// The least key in (lo, hi] of which `enough` holds, as it does of hi and of all above one it holds of. A wave
+// tries 64 at a time.
+template <class F>
+__device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F enough) {
+  const uint32_t lane = threadIdx.x & 63;
+  while (hi - lo > 1) {
+    const uint32_t step = (hi - lo + 63) / 64, mine = hi - lo > step * (lane + 1) ? lo + step * (lane + 1) : hi;
+    const int at = __ffsll((unsigned long long)__ballot(enough(mine))) - 1;
+    const uint32_t end = hi - lo > step * (at + 1) ? lo + step * (at + 1) : hi;
+    lo += step * at;
+    hi = end;
+  }
+  return __builtin_amdgcn_readfirstlane(hi);
+}
+constexpr uint32_t kDeadKey = 0x007FFFFFu;  // of minus infinity
+
+// The least key whose weight min_p leaves: the largest one's does.
+__device__ __forceinline__ uint32_t least_kept(const Weigh& weigh, float top, double m) {
+  if (!(m > 0.0)) return kDeadKey + 1;
+  const double least = ceil(m * (double)((uint64_t)1 << weigh.shift));
+  return least_key(kDeadKey, key_of(top),
+                   [&](uint32_t k) { return k == key_of(top) || (double)weigh(value_of(k)) >= least; });
+}
 
 struct SampleShared {
   uint64_t mass[kBins];  // of a histogram
@@ -298,11 +337,12 @@ struct SampleShared {
 };
 
 // Chooses among the n tokens of the list in LDS, all that may be kept, by their places: k, p, m and u as
-// in the file's heading (k 0: all n).
+// in the file's heading (k 0: all n). goal: top_p's, where the list is not all the weight there is (0: it is).
 template <int E>
-__device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int n, const RowSettings& s) {
+__device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int n, const RowSettings& s,
+                                      uint64_t goal) {
   const int t = threadIdx.x;
-  const double unit = (double)((uint64_t)1 << weigh.shift);
+  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);  // the largest logit is finite here
   uint64_t v[E], w[E], before[E], total = 0, kept = 0, sum;
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
@@ -315,10 +355,10 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
     before[e] = total + scan_block<16>(w[e], sm.red, &sum);
     total += sum;
   }
-  const uint64_t share = s.p < 1.0 ? mass_goal(s.p, total) : total;
+  const uint64_t share = goal ? goal : s.p < 1.0 ? mass_goal(s.p, total) : total;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool keep = t + 1024 * e < last && (t + 1024 * e == 0 || (before[e] < share && (double)w[e] >= s.m * unit));
+    const bool keep = t + 1024 * e < last && (t + 1024 * e == 0 || (before[e] < share && (uint32_t)(v[e] >> 32) >= least));
     w[e] = keep ? w[e] : 0;
     sm.mass[t + 1024 * e] = w[e];
     // by rising number, the kept ones first
@@ -326,7 +366,7 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
     scan_block<16>(w[e], sm.red, &sum);
     kept += sum;
   }
-  const uint64_t goal = pick_goal(s.u, kept);
+  const uint64_t pick = pick_goal(s.u, kept);
   sort_block<E>(v, n, sm.list);
   total = 0;
 #pragma unroll
@@ -334,7 +374,7 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
     const uint64_t mine = v[e] ? sm.mass[(uint32_t)v[e]] : 0;
     const uint64_t b = total + scan_block<16>(mine, sm.red, &sum);
     total += sum;
-    if (b <= goal && b + mine > goal) sm.pick[2] = (uint64_t)(0xFFFFFFFFu - (uint32_t)(v[e] >> 32));
+    if (b <= pick && b + mine > pick) sm.pick[2] = (uint64_t)(0xFFFFFFFFu - (uint32_t)(v[e] >> 32));
   }
   __syncthreads();
   return (int)sm.pick[2];
@@ -376,7 +416,7 @@ __device__ __forceinline__ uint64_t chunk_sum(const SampleArgs& a, const RowRead
       if (g + 64 * x < g1) {
 #pragma unroll
         for (int j = 0; j < RowReader<DT>::E; ++j)
-          v += value((g + 64 * x) * RowReader<DT>::E - row.off + j, RowReader<DT>::value(w[x], j));
+          v += value((g + 64 * x) * RowReader<DT>::E - row.off + j, RowReader<DT>::raw(w[x], j));
       }
   }
   return wave_sum64(v);
@@ -402,7 +442,7 @@ __device__ __forceinline__ int find(const SampleArgs& a, SampleShared& sm, const
       const u32x4 w = row.load(g);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        v[j] = value(g * E - row.off + j, RowReader<DT>::value(w, j));
+        v[j] = value(g * E - row.off + j, RowReader<DT>::raw(w, j));
         all += v[j];
       }
     }
@@ -434,7 +474,7 @@ struct Sampler {
 
   template <class F>
   __device__ __forceinline__ void tokens(F f) const {
-    row.each(threadIdx.x, 1024, row.units, [&](int unit, const u32x4& w) {
+    row.each(threadIdx.x, 1024, row.units, [&](int unit, const u32x4& w, int) {
       const int i0 = unit * E - row.off;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -487,7 +527,7 @@ struct Sampler {
   }
 
   // The least key of a bin: keys rise as bins fall.
-  __device__ __forceinline__ uint32_t least_key(int b) const {
+  __device__ __forceinline__ uint32_t bin_start(int b) const {
     uint32_t lo = key_of(kDead) + 1, hi = key_of(bin.top);  // bin(hi) = 0 <= b
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo) / 2;
@@ -504,7 +544,7 @@ struct Sampler {
   // the list, or are all equal.
   __device__ __forceinline__ uint64_t front(uint64_t cut, uint64_t by_count, uint64_t by_mass, int at, uint64_t count,
                                        uint64_t mass) {
-    uint32_t hi = at == 0 ? key_of(bin.top) : least_key(at - 1) - 1, lo = least_key(at);
+    uint32_t hi = at == 0 ? key_of(bin.top) : bin_start(at - 1) - 1, lo = bin_start(at);
     for (;;) {
       int n;
       const uint64_t in_bin = sm.count[at];
@@ -569,7 +609,7 @@ struct Sampler {
 
   // The place of the need'th token with this key at or above `cut`, by number.
   __device__ __forceinline__ uint64_t nth(uint32_t key, uint64_t cut, uint64_t need) {
-    auto one = [&](int i, float x) -> uint64_t { return x != kDead && key_of(x) == key && place(key, i) >= cut; };
+    auto one = [&](int i, float x) -> uint64_t { return x == value_of(key) && place(key, i) >= cut; };
     chunk_sums(one);
     uint64_t all;
     scan_block<16>((int)threadIdx.x < a.chunks ? sm.chunk[threadIdx.x] : 0, sm.red, &all);
@@ -607,7 +647,7 @@ struct Sampler {
     }
     const double least = s.m * (double)((uint64_t)1 << weigh.shift);
     auto value = [&](int i, float x) -> uint64_t {
-      if (place(key_of(x), i) < cut) return 0;
+      if (!(x > kDead) || place(key_of(x + 0.0f), i) < cut) return 0;
       const uint64_t w = weigh.any(x);
       return (double)w >= least ? w : 0;
     };
@@ -622,13 +662,20 @@ struct RowRange {
   float top, least;
 };
 __device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork& w) {
-  uint64_t top = 0, least = 0;
-  for (int i = 0; i < a.splits; ++i) top = max(top, w.top[i]), least = max(least, w.least[i]);
-  return {top ? value_of((uint32_t)(top >> 32)) : kDead, value_of(~(uint32_t)least)};
+  const int lane = threadIdx.x & 63;
+  uint32_t top = lane < a.splits ? w.top[lane] : 0, least = lane < a.splits ? w.least[lane] : 0;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    top = max(top, (uint32_t)__shfl_xor((int)top, k));
+    least = max(least, (uint32_t)__shfl_xor((int)least, k));
+  }
+  top = __builtin_amdgcn_readfirstlane(top), least = __builtin_amdgcn_readfirstlane(least);
+  return {top ? value_of(top) : kDead, value_of(~least)};
 }
 
 // Launch 1, a.splits workgroups a row as all others that read it: its largest logit (and the first token that
-// has it, where that is the answer), its least, and what the next ones add to cleared.
+// has it, where that is the answer), its least, and what the next ones add to cleared. top_k: also the
+// largest of every thread's loads, from which the next launch tells how far down to look.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a) {
   __shared__ uint64_t red[4];
@@ -640,7 +687,7 @@ __global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a) {
   constexpr int E = RowReader<DT>::E;
   if (s.kind == kGreedy) {
     uint64_t best = 0;
-    row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& v) {
+    row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& v, int) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float x = RowReader<DT>::value(v, j);
@@ -649,205 +696,285 @@ __global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a) {
       }
     });
     best = max_block<4>(best, red);
-    if (threadIdx.x == 0) w.top[at] = best;
+    if (threadIdx.x == 0) w.first[at] = best;
   } else {
-    float top = kDead, least = __builtin_inff();
-    row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
+    float peak[kPeaks], least = __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kPeaks; ++i) peak[i] = kDead;
+    row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v, int x) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float x = RowReader<DT>::value(v, j);
-        top = fmaxf(top, x);
-        least = fminf(least, x == kDead ? __builtin_inff() : x);
+        const float y = RowReader<DT>::raw(v, j);
+        float& to = peak[2 * x + (j >= E / 2)];
+        to = fmaxf(to, y);
+        least = fminf(least, y == kDead ? __builtin_inff() : y);
       }
     });
-    const uint64_t hi = max_block<4>(top == kDead ? 0 : place(key_of(top), 0), red);
-    const uint64_t lo = max_block<4>(~key_of(least), red);
-    if (threadIdx.x == 0) w.top[at] = hi, w.least[at] = lo;
+    if (s.kind == kFront) {
+      uint32_t* to = a.peaks + (int64_t)blockIdx.x * a.peaks_each;
+      float p[kPeaks];
+#pragma unroll
+      for (int i = 0; i < kPeaks; ++i) p[i] = peak[i];
+#pragma unroll
+      for (int n = kPeaks / 2; n > 0; n >>= 1)
+        if (a.peaks_each <= 256 * n) {
+#pragma unroll
+          for (int i = 0; i < n; ++i) p[i] = fmaxf(p[i], p[i + n]);
+        }
+      int stride = 1;  // threads that share a peak
+      for (; a.peaks_each * stride < 256; stride *= 2) p[0] = fmaxf(p[0], __shfl_xor(p[0], stride));
+#pragma unroll
+      for (int i = 0; i < kPeaks; ++i)
+        if ((i == 0 || 256 * i < a.peaks_each) && threadIdx.x % stride == 0)
+          to[256 * i + threadIdx.x / stride] = p[i] == kDead ? 0 : key_of(p[i] + 0.0f);
+    }
+    float top = peak[0];
+#pragma unroll
+    for (int i = 1; i < kPeaks; ++i) top = fmaxf(top, peak[i]);
+    const uint64_t hi = max_block<4>(top == kDead ? 0 : key_of(top + 0.0f), red);
+    const uint64_t lo = max_block<4>((uint32_t)~key_of(least + 0.0f), red);
+    if (threadIdx.x == 0) w.top[at] = (uint32_t)hi, w.least[at] = (uint32_t)lo;
     if (s.kind == kShare)
       for (int i = at * 256 + threadIdx.x; i < kBins; i += a.splits * 256) w.mass[i] = 0;
-    if (s.kind == kFront)
-      for (int i = at * 256 + threadIdx.x; i < kBins; i += a.splits * 256) w.count[i] = 0;
   }
-  if (at == 0 && threadIdx.x == 0) w.n = w.done = 0;
+  if (at == 0 && threadIdx.x == 0) w.n = w.ahead = w.done = w.whole = 0;
 }
 
-// Launch 2. top_k: how many tokens are in each bin, as far as this workgroup's part reaches k. top_p: the bins'
-// weights. Neither: the chunks' weights.
+// Launch 2. top_k: a logit that k tokens reach, as k of the peaks do. top_p: the weight in each bin. Neither: the
+// chunks' weights.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
   __shared__ uint64_t mass[kBins];
   __shared__ uint64_t red[4];
+  __shared__ uint32_t pick;
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   const RowSettings s = settings(a, r);
-  if (s.kind == kGreedy || s.kind == kWhole) return;
-  const RowReader<DT> row(a, r);
+  if (s.kind == kGreedy || s.kind == kWhole || (s.kind == kFront && at > 0)) return;
   RowWork& w = a.work[r];
   const RowRange range = row_range(a, w);
   if (!(fabsf(range.top) < __builtin_inff())) return;  // an infinity: one workgroup deals with it
+  constexpr int N = kBins / 256;
+  if (s.kind == kFront) {
+    uint32_t* count = reinterpret_cast<uint32_t*>(mass);
+    const uint32_t* peaks = a.peaks + (int64_t)r * a.splits * a.peaks_each;
+    const int n = a.splits * a.peaks_each;  // at most kMostPeaks
+    uint32_t mine[kMostPeaks / 256], low = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < kMostPeaks / 256; ++i) {
+      const int at = threadIdx.x + 256 * i;
+      mine[i] = at < n ? peaks[at] : 0;
+    }
+    for (int i = threadIdx.x; i < kBins; i += 256) count[i] = 0;
+    if (threadIdx.x == 0) pick = kBins;
+    // bins over the peaks alone
+#pragma unroll
+    for (int i = 0; i < kMostPeaks / 256; ++i) low = min(low, mine[i] ? mine[i] : 0xFFFFFFFFu);
+    low = ~(uint32_t)max_block<4>((uint32_t)~low, red);
+    const Bins bin(range.top, value_of(low), a.shift, __builtin_inf());
+#pragma unroll
+    for (int i = 0; i < kMostPeaks / 256; ++i)
+      if (mine[i]) atomicAdd(&count[bin(value_of(mine[i]))], 1u);
+    __syncthreads();
+    uint64_t sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += count[threadIdx.x * N + i];
+    uint64_t before = scan_block<4>(sum, red, &all);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t c = count[threadIdx.x * N + i];
+      if (before < s.k && before + c >= s.k) pick = threadIdx.x * N + i;
+      before += c;
+    }
+    __syncthreads();
+    const int border = (int)pick;
+    // fewer peaks than top_k: every token may be kept
+    const uint32_t from = border == kBins ? kDeadKey + 1
+                                          : least_key(kDeadKey, key_of(range.top),
+                                                      [&](uint32_t k) { return bin(value_of(k)) <= border; });
+    if (threadIdx.x == 0) w.from = from;
+    return;
+  }
+  const RowReader<DT> row(a, r);
   const int c0 = at * a.per, c1 = min(a.chunks, c0 + a.per);
-  const int g0 = c0 * a.chunk_units, g1 = min(row.units, c1 * a.chunk_units);
   constexpr int E = RowReader<DT>::E;
-  const Weigh weigh = {(double)range.top, 1.4426950408889634074 / s.t, a.shift};
+  const Weigh weigh(range.top, s.t, a.shift);
   if (s.kind == kAll) {
-    const uint64_t least = (uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift));
+    const uint32_t least = least_kept(weigh, range.top, s.m);
+    const float from = value_of(least);
     for (int c = c0 + (threadIdx.x >> 6); c < c1; c += 4) {
-      const uint64_t v = chunk_sum<DT>(a, row, c, [&](int, float x) {
-        const uint64_t y = weigh(x);
-        return y >= least ? y : 0;
-      });
+      const uint64_t v = chunk_sum<DT>(a, row, c, [&](int, float x) { return weigh(x >= from ? x : kDead); });
       if ((threadIdx.x & 63) == 0) w.chunk[c] = v;
     }
+    if (at == 0 && threadIdx.x == 0) w.least_kept = least;
     return;
   }
+  const int g0 = c0 * a.chunk_units, g1 = min(row.units, c1 * a.chunk_units);
   const Bins bin(range.top, range.least, a.shift, s.t);
-  if (s.kind == kShare) {
-    for (int i = threadIdx.x; i < kBins; i += 256) mass[i] = 0;
-    __syncthreads();
-    row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float x = RowReader<DT>::value(v, j);
-        const uint64_t y = weigh(x);
-        if (y) atomicAdd((unsigned long long*)&mass[bin(x)], (unsigned long long)y);
-      }
-    });
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += 256)
-      if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
-    return;
-  }
-  uint32_t* count = reinterpret_cast<uint32_t*>(mass);
-  for (int i = threadIdx.x; i < kBins; i += 256) count[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += 256) mass[i] = 0;
   __syncthreads();
-  row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v) {
+  row.each(g0 + threadIdx.x, 256, g1, [&](int, const u32x4& v, int) {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const float x = RowReader<DT>::value(v, j);
-      if (x != kDead) atomicAdd(&count[bin(x)], 1u);
+      const float x = RowReader<DT>::raw(v, j);
+      const uint64_t y = weigh(x);
+      if (y) atomicAdd((unsigned long long*)&mass[bin.finite(x)], (unsigned long long)y);
     }
   });
   __syncthreads();
-  uint64_t sum = 0, all;
-  for (int i = 0; i < kBins / 256; ++i) sum += count[threadIdx.x * (kBins / 256) + i];
-  uint64_t before = scan_block<4>(sum, red, &all);
-  for (int i = 0; i < kBins / 256 && before < s.k; ++i) {
-    const uint32_t c = count[threadIdx.x * (kBins / 256) + i];
-    if (c) atomicAdd(&w.count[threadIdx.x * (kBins / 256) + i], c);
-    before += c;
-  }
+  for (int i = threadIdx.x; i < kBins; i += 256)
+    if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
 }
 
-// Launch 3: the tokens that the border is among. top_k: all up to the end of its bin; top_p: its bin's.
+// Launch 3: the tokens that the border is among. top_k: all that reach its logit. top_p: those of its bin, and on
+// a list of their own those ahead of it, as long as they are few.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
   __shared__ uint64_t red[4];
   __shared__ uint64_t pick[2];
-  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits, lane = threadIdx.x & 63;
   const RowSettings s = settings(a, r);
   if (s.kind != kFront && s.kind != kShare) return;
   const RowReader<DT> row(a, r);
   RowWork& w = a.work[r];
   const RowRange range = row_range(a, w);
   if (!(fabsf(range.top) < __builtin_inff())) return;
-  const Bins bin(range.top, range.least, a.shift, s.t);
   constexpr int N = kBins / 256, E = RowReader<DT>::E;
-  uint64_t v[N], sum = 0, all;
+  const bool share = s.kind == kShare;
+  uint32_t from, to = 0xFFFFFFFFu;  // keys of the list
+  if (!share) {
+    from = w.from;
+  } else {
+    uint64_t v[N], sum = 0, all;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = s.kind == kFront ? w.count[threadIdx.x * N + i] : w.mass[threadIdx.x * N + i];
-    sum += v[i];
-  }
-  uint64_t before = scan_block<4>(sum, red, &all);
-  const uint64_t goal = s.kind == kFront ? s.k : mass_goal(s.p, all);
-  if (threadIdx.x == 0) pick[0] = kBins;
-  __syncthreads();
+    for (int i = 0; i < N; ++i) {
+      v[i] = w.mass[threadIdx.x * N + i];
+      sum += v[i];
+    }
+    uint64_t before = scan_block<4>(sum, red, &all);
+    const uint64_t goal = mass_goal(s.p, all);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (before < goal && before + v[i] >= goal) pick[0] = threadIdx.x * N + i, pick[1] = before;
-    before += v[i];
+    for (int i = 0; i < N; ++i) {
+      if (before < goal && before + v[i] >= goal) pick[0] = threadIdx.x * N + i, pick[1] = before;
+      before += v[i];
+    }
+    __syncthreads();
+    const int border = (int)pick[0];
+    const Bins bin(range.top, range.least, a.shift, s.t);
+    from = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) <= border; });
+    if (border > 0) to = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) < border; }) - 1;
+    if (at == 0 && threadIdx.x == 0) w.before = pick[1], w.goal = goal;
   }
-  __syncthreads();
-  const int border = (int)pick[0];
-  if (at == 0 && threadIdx.x == 0) {
-    w.before = pick[1], w.goal = goal;
-    if (border == kBins) w.n = kList + 1;  // fewer tokens than top_k: as if there were too many
-  }
-  if (border == kBins) return;
-  const bool front = s.kind == kFront;
+  const float low = value_of(from);
   const int g0 = at * a.per * a.chunk_units, g1 = min(row.units, (at + 1) * a.per * a.chunk_units);
-  row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& u) {
+  // one addition a wave for its tokens on a list; how many were there before
+  auto put = [&](bool mine, uint32_t* n, uint64_t* list, uint64_t what) -> uint32_t {
+    const unsigned long long m = __ballot(mine);
+    if (!m) return 0;
+    uint32_t base = 0;
+    if (lane == 0) base = atomicAdd(n, (uint32_t)__popcll(m));
+    base = __builtin_amdgcn_readfirstlane(base);
+    const uint32_t to = base + __popcll(m & ((1ull << lane) - 1));
+    if (mine && to < kList) list[to] = what;
+    return base;
+  };
+  bool few = share;  // as far as this wave knows
+  const int last = g0 + (g1 - g0 + 63) / 64 * 64;  // whole waves
+  for (int g = g0 + threadIdx.x; g < last; g += 1024) {
+    u32x4 u[4];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float x = RowReader<DT>::value(u, j);
-      const int b = bin(x);
-      if (x != kDead && (front ? b <= border : b == border)) {
-        const uint32_t to = atomicAdd(&w.n, 1u);
-        if (to < kList) w.list[to] = place(key_of(x), unit * E - row.off + j);
+    for (int x = 0; x < 4; ++x)
+      if (g + 256 * x < g1) u[x] = row.load(g + 256 * x);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      bool any = false;
+      if (g + 256 * x < g1) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) any |= RowReader<DT>::raw(u[x], j) >= low;
+      }
+      if (!__any(any)) continue;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float y = RowReader<DT>::value(u[x], j);
+        const bool mine = any && y >= low;
+        if (!__any(mine)) continue;
+        const uint32_t k = key_of(y);
+        const uint64_t p = place(k, (g + 256 * x) * E - row.off + j);
+        put(mine && k <= to, &w.n, w.list, p);
+        if (few) few = put(mine && k > to, &w.ahead, w.list + kList, p) <= kList;
       }
     }
-  });
+  }
 }
 
-// Launch 4, a workgroup a row: its token, or (top_p) the last place kept.
+// Launch 4, a workgroup a row: its token, or (top_p with many tokens kept) the last place kept.
 template <int DT>
 __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
   __shared__ SampleShared sm;
   const int r = blockIdx.x;
   const RowSettings s = settings(a, r);
   RowWork& w = a.work[r];
-  const RowRange range = row_range(a, w);
   int token = -1;
   if (s.kind == kGreedy) {
-    uint64_t best = 0;
-    for (int i = 0; i < a.splits; ++i) best = max(best, w.top[i]);
+    const int lane = threadIdx.x & 63;
+    uint64_t best = lane < a.splits ? w.first[lane] : 0;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const uint64_t o = shfl_xor64(best, k);
+      best = o > best ? o : best;
+    }
     if (best) token = token_of(best);
-  } else if (range.top != kDead) {
-    const Weigh weigh = {(double)range.top, 1.4426950408889634074 / s.t, a.shift};
+    if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
+    return;
+  }
+  const RowRange range = row_range(a, w);
+  if (range.top != kDead) {
+    const Weigh weigh(range.top, s.t, a.shift);
     const RowReader<DT> row(a, r);
     const bool list = s.kind == kFront || s.kind == kShare;
-    if (s.kind == kWhole || range.top == __builtin_inff() || (list && w.n > kList)) {
-      Sampler<DT> whole{a, sm, row, weigh, Bins(range.top, range.least, a.shift, s.t)};
-      token = whole.whole(s);
+    const uint32_t n = list ? w.n : 0, ahead = s.kind == kShare ? w.ahead : 0;
+    if (s.kind == kWhole || range.top == __builtin_inff() || n > kList) {
+      if (threadIdx.x == 0) w.whole = 1;
+      return;
     } else if (s.kind == kAll) {
-      const uint64_t least = (uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift));
+      const float from = value_of(w.least_kept);
       const uint64_t mine = (int)threadIdx.x < a.chunks ? w.chunk[threadIdx.x] : 0;
       uint64_t all;
       if ((int)threadIdx.x < a.chunks) sm.chunk[threadIdx.x] = mine;
       scan_block<16>(mine, sm.red, &all);
-      token = find<DT>(a, sm, row, pick_goal(s.u, all), [&](int, float x) {
-        const uint64_t y = weigh(x);
-        return y >= least ? y : 0;
-      });
+      token = find<DT>(a, sm, row, pick_goal(s.u, all), [&](int, float x) { return weigh(x >= from ? x : kDead); });
     } else {
-      const int n = (int)w.n;
+      const bool some = n + ahead <= kList;  // all that may be kept is at hand
+      const int have = (int)(some ? n + ahead : n);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if ((int)threadIdx.x + 1024 * e < n) sm.list[threadIdx.x + 1024 * e] = w.list[threadIdx.x + 1024 * e];
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t i = threadIdx.x + 1024 * e;
+        if ((int)i < have) sm.list[i] = i < n ? w.list[i] : w.list[kList + i - n];
+      }
       __syncthreads();
-      if (s.kind == kShare) {
-        const uint64_t cut = n > 1024 ? last_kept<2>(sm, weigh, n, w.before, w.goal)
-                                      : last_kept<1>(sm, weigh, n, w.before, w.goal);
-        if (threadIdx.x == 0) w.cut = cut;
+      if (!some) {
+        const uint64_t cut = n > 1024 ? last_kept<2>(sm, weigh, (int)n, w.before, w.goal)
+                                      : last_kept<1>(sm, weigh, (int)n, w.before, w.goal);
+        const uint32_t least = least_kept(weigh, range.top, s.m);
+        if (threadIdx.x == 0) w.cut = cut, w.least_kept = least;
         return;
       }
-      token = n > 1024 ? choose<2>(sm, weigh, n, s) : choose<1>(sm, weigh, n, s);
+      // what is on the lists is not all the row's weight, but the border's goal is of that
+      const uint64_t goal = s.kind == kShare ? w.goal : 0;
+      token = have > 1024 ? choose<2>(sm, weigh, have, s, goal) : choose<1>(sm, weigh, have, s, goal);
     }
   }
   if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
 }
 
-// What a token at or before the cut of its row weighs, if that is enough for min_p.
+// What a token weighs that is at or before the cut of its row and enough for min_p.
 struct Kept {
   Weigh weigh;
-  float x;       // of the last token kept
+  float x, from;  // logit of the last token kept, and the least that min_p leaves
   int i;
-  uint64_t least;
   __device__ __forceinline__ Kept(const SampleArgs& a, const RowSettings& s, const RowWork& w, float top)
-      : weigh{(double)top, 1.4426950408889634074 / s.t, a.shift}, x(value_of((uint32_t)(w.cut >> 32))), i(token_of(w.cut)),
-        least((uint64_t)ceil(s.m * (double)((uint64_t)1 << a.shift))) {}
+      : weigh(top, s.t, a.shift), x(value_of((uint32_t)(w.cut >> 32))), from(value_of(w.least_kept)), i(token_of(w.cut)) {}
   __device__ __forceinline__ uint64_t operator()(int at, float y) const {
-    const uint64_t v = weigh(y);
-    return (y > x || (y == x && at <= i)) && v >= least ? v : 0;
+    return weigh((y > x || (y == x && at <= i)) && y >= from ? y : kDead);
   }
 };
 
@@ -856,24 +983,33 @@ template <int DT>
 __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   RowWork& w = a.work[r];
-  if (w.done) return;
+  if (w.done || w.whole) return;
   const RowSettings s = settings(a, r);
   const RowReader<DT> row(a, r);
   const Kept kept(a, s, w, row_range(a, w).top);
   const int c0 = at * a.per, c1 = min(a.chunks, c0 + a.per);
   for (int c = c0 + (threadIdx.x >> 6); c < c1; c += 4) {
-    const uint64_t v = chunk_sum<DT>(a, row, c, kept);
+    // equal logits are kept up to the cut's number: all of a chunk's, or none but in its own
+    const int i0 = c * a.chunk_units * RowReader<DT>::E - row.off, i1 = i0 + a.chunk_units * RowReader<DT>::E;
+    uint64_t v;
+    if (kept.i >= i1 || kept.i < i0 || kept.from > kept.x) {
+      const uint32_t k = key_of(kept.x) + (kept.i < i0 ? 1 : 0);
+      const float from = fmaxf(value_of(k), kept.from);
+      v = chunk_sum<DT>(a, row, c, [&](int, float y) { return kept.weigh(y >= from ? y : kDead); });
+    } else {
+      v = chunk_sum<DT>(a, row, c, kept);
+    }
     if ((threadIdx.x & 63) == 0) w.chunk[c] = v;
   }
 }
 
-// Launch 6: the token of the rows that have none.
+// Launch 6: the token of the rows whose kept weights are summed.
 template <int DT>
 __global__ __launch_bounds__(1024) void sample_find_kernel(SampleArgs a) {
   __shared__ SampleShared sm;
   const int r = blockIdx.x;
   RowWork& w = a.work[r];
-  if (w.done) return;
+  if (w.done || w.whole) return;
   const RowSettings s = settings(a, r);
   const RowReader<DT> row(a, r);
   const Kept kept(a, s, w, row_range(a, w).top);
@@ -885,7 +1021,25 @@ __global__ __launch_bounds__(1024) void sample_find_kernel(SampleArgs a) {
   if (threadIdx.x == 0) a.token[r] = token;
 }
 
-constexpr int64_t kRowsAtOnce = 1024;  // rows of a batch of launches: 50 MB of workspace
+// Last launch: rows with more tokens around the border than the list holds, with larger top_k, or with an
+// infinity, a workgroup each. It is there for any row that needs it; most calls have none.
+template <int DT>
+__global__ __launch_bounds__(1024) void sample_whole_kernel(SampleArgs a) {
+  __shared__ SampleShared sm;
+  const int r = blockIdx.x;
+  RowWork& w = a.work[r];
+  if (!w.whole) return;
+  const RowSettings s = settings(a, r);
+  const RowRange range = row_range(a, w);
+  Sampler<DT> whole{a, sm, RowReader<DT>(a, r), Weigh(range.top, s.t, a.shift), Bins(range.top, range.least, a.shift, s.t)};
+  const int token = whole.whole(s);
+  if (threadIdx.x == 0) a.token[r] = token;
+}
+
+constexpr int64_t kRowsAtOnce = 1024;  // rows of a batch of launches: 80 MB of workspace
+
+// Workgroups of a row at most: enough for every CU, and several for the rows with more to do.
+static int64_t most_splits(int64_t rows) { return std::min((int64_t)kSplits, std::max(2048 / rows, (int64_t)4)); }
 
 template <int DT>
 static int sample_rows(SampleArgs a, hipStream_t st) {
@@ -902,6 +1056,7 @@ static int sample_rows(SampleArgs a, hipStream_t st) {
     sample_kept_kernel<DT><<<many, 256, 0, st>>>(a);
     sample_find_kernel<DT><<<one, 1024, 0, st>>>(a);
   }
+  if (!greedy) sample_whole_kernel<DT><<<one, 1024, 0, st>>>(a);
   CP_LAUNCHED("sampling");
   return CP_OK;
 }
@@ -911,7 +1066,9 @@ static int sample_rows(SampleArgs a, hipStream_t st) {
 extern "C" {
 
 size_t cp_sample_ws_bytes(int64_t rows, int64_t vocab) {
-  return rows < 1 || vocab < 1 ? 0 : (size_t)std::min(rows, cp::kRowsAtOnce) * sizeof(cp::RowWork);
+  if (rows < 1 || vocab < 1) return 0;
+  const int64_t n = std::min(rows, cp::kRowsAtOnce);
+  return (size_t)n * sizeof(cp::RowWork) + (size_t)n * cp::kMostPeaks * 4;
 }
 
 int cp_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_step, const void* u, int u_f64,
@@ -958,10 +1115,12 @@ int cp_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_
     a.work = (cp::RowWork*)ws;
     a.chunk_units = (int)chunk;
     a.chunks = (int)((units + chunk - 1) / chunk);
-    // enough workgroups for every CU, and several for the rows with more to do
-    const int64_t want = std::min({(int64_t)cp::kSplits, (int64_t)a.chunks, std::max(2048 / (int64_t)a.rows, (int64_t)4)});
+    const int64_t want = std::min((int64_t)a.chunks, cp::most_splits(a.rows));
     a.per = (int)((a.chunks + want - 1) / want);
     a.splits = (a.chunks + a.per - 1) / a.per;
+    a.peaks = (uint32_t*)((char*)ws + a.rows * sizeof(cp::RowWork));
+    a.peaks_each = 256 * cp::kPeaks;
+    while (a.splits * a.peaks_each > cp::kMostPeaks) a.peaks_each /= 2;
     const int s = dtype == CP_F32    ? cp::sample_rows<CP_F32>(a, (hipStream_t)stream)
                   : dtype == CP_BF16 ? cp::sample_rows<CP_BF16>(a, (hipStream_t)stream)
                                      : cp::sample_rows<CP_F16>(a, (hipStream_t)stream);
