@@ -202,16 +202,44 @@ __device__ __forceinline__ uint64_t pick_goal(double u, uint64_t total) {
 }
 
 __device__ __forceinline__ uint64_t join64(int lo, int hi) { return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo; }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int s) {
-  return join64(__shfl_xor((int)(uint32_t)v, s), __shfl_xor((int)(v >> 32), s));
+// The value of lane ^ S, without LDS: within rows of 16 lanes by moves, beyond by swapping rows of two copies.
+template <int S>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (S == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);   // within four: 1 0 3 2
+  if constexpr (S == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);   // 2 3 0 1
+  if constexpr (S == 4)  // eight in reverse, then each four of them
+    return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);
+  if constexpr (S == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, true);  // sixteen turned by eight
+  if constexpr (S == 16) {
+    const auto w = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? w[0] : w[1];
+  } else {
+    const auto w = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? w[0] : w[1];
+  }
+}
+template <int S>
+__device__ __forceinline__ uint64_t lane_xor64(uint64_t v) {
+  return (uint64_t)lane_xor<S>((uint32_t)(v >> 32)) << 32 | lane_xor<S>((uint32_t)v);
+}
+// v put together over the wave, in every lane.
+template <class F>
+__device__ __forceinline__ uint64_t wave_all64(uint64_t v, F f) {
+  v = f(v, lane_xor64<1>(v));
+  v = f(v, lane_xor64<2>(v));
+  v = f(v, lane_xor64<4>(v));
+  v = f(v, lane_xor64<8>(v));
+  v = f(v, lane_xor64<16>(v));
+  return f(v, lane_xor64<32>(v));
 }
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int s) {
   return join64(__shfl_up((int)(uint32_t)v, s), __shfl_up((int)(v >> 32), s));
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) v += shfl_xor64(v, s);
-  return v;
+  return wave_all64(v, [](uint64_t a, uint64_t b) { return a + b; });
+}
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+  return wave_all64(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 
 // Sum of v over the threads before this one, and over all W waves.
@@ -239,11 +267,7 @@ __device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64
 
 template <int W>
 __device__ __forceinline__ uint64_t max_block(uint64_t v, uint64_t* red) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint64_t o = shfl_xor64(v, s);
-    v = o > v ? o : v;
-  }
+  v = wave_max64(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
 #pragma unroll
@@ -252,38 +276,54 @@ __device__ __forceinline__ uint64_t max_block(uint64_t v, uint64_t* red) {
   return v;
 }
 
-// Up to 1024 E values, number t + 1024 e in thread t's v[e], sorted, the largest first; n of them are not
-// 0. Steps within a wave exchange by shuffles: up to 64 values need no other.
+// A step of the sort: value number at against partner o, J apart, in runs of k that fall and rise in turn.
+template <int E>
+__device__ __forceinline__ void sort_keep(uint64_t (&v)[E], const uint64_t (&o)[E], int j, int k) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool first = !(threadIdx.x & j), down = !(((int)threadIdx.x + 1024 * e) & k);  // down: the larger one first
+    v[e] = (first == down) == (v[e] > o[e]) ? v[e] : o[e];
+  }
+}
+template <int J, int E>
+__device__ __forceinline__ void sort_step(uint64_t (&v)[E], int k) {
+  uint64_t o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = lane_xor64<J>(v[e]);
+  sort_keep<E>(v, o, J, k);
+}
+
+// Up to 1024 E values, number t + 1024 e in thread t's v[e], sorted, the largest first (threads past the n
+// of them hold 0): a bitonic sort, whose steps within a wave need no LDS.
 template <int E>
 __device__ __forceinline__ void sort_block(uint64_t (&v)[E], int n, uint64_t* list) {
   const int t = threadIdx.x;
   int size = 64;
   while (size < n) size <<= 1;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (E > 1 && j == 1024) {
-        const uint64_t a = v[0], b = v[E - 1];
-        v[0] = a > b ? a : b, v[E - 1] = a > b ? b : a;
-        continue;
-      }
-      uint64_t o[E];
-      if (j < 64) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = shfl_xor64(v[e], j);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) list[t + 1024 * e] = v[e];
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = list[(t ^ j) + 1024 * e];
-        __syncthreads();
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool first = !(t & j), down = !((t + 1024 * e) & k);  // down: the larger one first
-        v[e] = (first == down) == (v[e] > o[e]) ? v[e] : o[e];
-      }
+  for (int k = 2; k <= size; k <<= 1) {
+    int j = k >> 1;
+    if (E > 1 && j == 1024) {
+      const uint64_t a = v[0], b = v[E - 1];
+      v[0] = a > b ? a : b, v[E - 1] = a > b ? b : a;
+      j >>= 1;
     }
+    for (; j >= 64; j >>= 1) {
+      uint64_t o[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) list[t + 1024 * e] = v[e];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = list[(t ^ j) + 1024 * e];
+      __syncthreads();
+      sort_keep<E>(v, o, j, k);
+    }
+    if (j >= 32) sort_step<32>(v, k);
+    if (j >= 16) sort_step<16>(v, k);
+    if (j >= 8) sort_step<8>(v, k);
+    if (j >= 4) sort_step<4>(v, k);
+    if (j >= 2) sort_step<2>(v, k);
+    sort_step<1>(v, k);
+  }
 }
 
 // Bins of falling logits, as many as bring the least logit, or the one from which on weights are 0, to the
@@ -340,7 +380,7 @@ struct SampleShared {
 // in the file's heading (k 0: all n). goal: top_p's, where the list is not all the weight there is (0: it is).
 template <int E>
 __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int n, const RowSettings& s,
-                                      uint64_t goal) {
+                                      uint64_t goal, int vocab) {
   const int t = threadIdx.x;
   const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);  // the largest logit is finite here
   uint64_t v[E], w[E], before[E], total = 0, kept = 0, sum;
@@ -360,21 +400,37 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
   for (int e = 0; e < E; ++e) {
     const bool keep = t + 1024 * e < last && (t + 1024 * e == 0 || (before[e] < share && (uint32_t)(v[e] >> 32) >= least));
     w[e] = keep ? w[e] : 0;
-    sm.mass[t + 1024 * e] = w[e];
-    // by rising number, the kept ones first
-    v[e] = keep ? (uint64_t)(uint32_t)v[e] << 32 | (uint32_t)(t + 1024 * e) : 0;
     scan_block<16>(w[e], sm.red, &sum);
     kept += sum;
   }
   const uint64_t pick = pick_goal(s.u, kept);
-  sort_block<E>(v, n, sm.list);
-  total = 0;
+  // In the order of numbers: weights by bins of numbers, then the border's bin, of a 2048th of the vocabulary.
+  for (int i = t; i < kBins; i += 1024) sm.mass[i] = 0;
+  if (t == 0) sm.n = 0;
+  __syncthreads();
+  int bin[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const uint64_t mine = v[e] ? sm.mass[(uint32_t)v[e]] : 0;
-    const uint64_t b = total + scan_block<16>(mine, sm.red, &sum);
-    total += sum;
-    if (b <= pick && b + mine > pick) sm.pick[2] = (uint64_t)(0xFFFFFFFFu - (uint32_t)(v[e] >> 32));
+    bin[e] = (int)((int64_t)token_of(v[e]) * kBins / vocab);
+    if (w[e]) atomicAdd((unsigned long long*)&sm.mass[bin[e]], (unsigned long long)w[e]);
+  }
+  __syncthreads();
+  const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = scan_block<16>(m0 + m1, sm.red, &sum);
+  if (b <= pick && b + m0 > pick) sm.pick[0] = 2 * t, sm.pick[1] = b;
+  else if (b + m0 <= pick && b + m0 + m1 > pick) sm.pick[0] = 2 * t + 1, sm.pick[1] = b + m0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (w[e] && bin[e] == (int)sm.pick[0]) {
+      const uint32_t at = atomicAdd(&sm.n, 1u);
+      sm.list[at] = (uint32_t)v[e];  // larger for smaller numbers
+      sm.mass[at] = w[e];
+    }
+  __syncthreads();
+  for (int i = t; i < (int)sm.n; i += 1024) {
+    uint64_t before = sm.pick[1];
+    for (int j = 0; j < (int)sm.n; ++j) before += sm.list[j] > sm.list[i] ? sm.mass[j] : 0;
+    if (before <= pick && before + sm.mass[i] > pick) sm.pick[2] = 0xFFFFFFFFu - (uint32_t)sm.list[i];
   }
   __syncthreads();
   return (int)sm.pick[2];
@@ -418,6 +474,58 @@ __device__ __forceinline__ uint64_t chunk_sum(const SampleArgs& a, const RowRead
         for (int j = 0; j < RowReader<DT>::E; ++j)
           v += value((g + 64 * x) * RowReader<DT>::E - row.off + j, RowReader<DT>::raw(w[x], j));
       }
+  }
+  return wave_sum64(v);
+}
+
+// The weights of chunk c's logits from `from` on, by one wave. Where they are fewer than three in four, they are
+// put side by side first (in keep, which holds four loads of a wave's logits): a weight costs as much as seven
+// such moves. 256 rows of which a fifth is kept 43 us without, SIDE with.
+template <int DT>
+__device__ __forceinline__ uint64_t chunk_sum_from(const SampleArgs& a, const RowReader<DT>& row, int c, const Weigh& weigh,
+                                                   float from, float* keep) {
+  constexpr int E = RowReader<DT>::E;
+  const int lane = threadIdx.x & 63, g0 = c * a.chunk_units, g1 = min(row.units, g0 + a.chunk_units);
+  uint64_t v = 0;
+  for (int g = g0; g < g1; g += 256) {
+    u32x4 w[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (g + 64 * x + lane < g1) w[x] = row.load(g + 64 * x + lane);
+    int n = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        n += __popcll(__ballot(g + 64 * x + lane < g1 && RowReader<DT>::raw(w[x], j) >= from));
+    if (n > 3 * 64 * E) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (g + 64 * x + lane < g1) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const float y = RowReader<DT>::raw(w[x], j);
+            v += weigh(y >= from ? y : kDead);
+          }
+        }
+      continue;
+    }
+    int at = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float y = RowReader<DT>::raw(w[x], j);
+        const bool mine = g + 64 * x + lane < g1 && y >= from;
+        const unsigned long long m = __ballot(mine);
+        if (mine) keep[at + __popcll(m & ((1ull << lane) - 1))] = y;
+        at += __popcll(m);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int i = lane; i < n; i += 64) v += weigh(keep[i]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
   return wave_sum64(v);
 }
@@ -663,13 +771,10 @@ struct RowRange {
 };
 __device__ __forceinline__ RowRange row_range(const SampleArgs& a, const RowWork& w) {
   const int lane = threadIdx.x & 63;
-  uint32_t top = lane < a.splits ? w.top[lane] : 0, least = lane < a.splits ? w.least[lane] : 0;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    top = max(top, (uint32_t)__shfl_xor((int)top, k));
-    least = max(least, (uint32_t)__shfl_xor((int)least, k));
-  }
-  top = __builtin_amdgcn_readfirstlane(top), least = __builtin_amdgcn_readfirstlane(least);
+  const uint64_t both = wave_all64(lane < a.splits ? (uint64_t)w.top[lane] << 32 | w.least[lane] : 0, [](uint64_t a, uint64_t b) {
+    return (uint64_t)max((uint32_t)(a >> 32), (uint32_t)(b >> 32)) << 32 | max((uint32_t)a, (uint32_t)b);
+  });
+  const uint32_t top = __builtin_amdgcn_readfirstlane((uint32_t)(both >> 32)), least = __builtin_amdgcn_readfirstlane((uint32_t)both);
   return {top ? value_of(top) : kDead, value_of(~least)};
 }
 
@@ -749,7 +854,7 @@ __global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
   __shared__ uint32_t pick;
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   const RowSettings s = settings(a, r);
-  if (s.kind == kGreedy || s.kind == kWhole || (s.kind == kFront && at > 0)) return;
+  if (s.kind == kGreedy || s.kind == kWhole || (s.kind == kFront && at != r % a.splits)) return;  // on every XCD in turn
   RowWork& w = a.work[r];
   const RowRange range = row_range(a, w);
   if (!(fabsf(range.top) < __builtin_inff())) return;  // an infinity: one workgroup deals with it
@@ -831,7 +936,9 @@ template <int DT>
 __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
   __shared__ uint64_t red[4];
   __shared__ uint64_t pick[2];
-  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits, lane = threadIdx.x & 63;
+  __shared__ uint64_t list[2][kList];
+  __shared__ uint32_t have[2], base[2];
+  const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   const RowSettings s = settings(a, r);
   if (s.kind != kFront && s.kind != kShare) return;
   const RowReader<DT> row(a, r);
@@ -866,44 +973,30 @@ __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
   }
   const float low = value_of(from);
   const int g0 = at * a.per * a.chunk_units, g1 = min(row.units, (at + 1) * a.per * a.chunk_units);
-  // one addition a wave for its tokens on a list; how many were there before
-  auto put = [&](bool mine, uint32_t* n, uint64_t* list, uint64_t what) -> uint32_t {
-    const unsigned long long m = __ballot(mine);
-    if (!m) return 0;
-    uint32_t base = 0;
-    if (lane == 0) base = atomicAdd(n, (uint32_t)__popcll(m));
-    base = __builtin_amdgcn_readfirstlane(base);
-    const uint32_t to = base + __popcll(m & ((1ull << lane) - 1));
-    if (mine && to < kList) list[to] = what;
-    return base;
-  };
-  bool few = share;  // as far as this wave knows
-  const int last = g0 + (g1 - g0 + 63) / 64 * 64;  // whole waves
-  for (int g = g0 + threadIdx.x; g < last; g += 1024) {
-    u32x4 u[4];
+  // lists of the workgroup: [0] the border's, [1] ahead of it, which is left alone once it is too long
+  const float high = to == 0xFFFFFFFFu ? __builtin_inff() : value_of(to + 1);
+  if (threadIdx.x < 2) have[threadIdx.x] = 0;
+  __syncthreads();
+  row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& u, int) {
+    const float end = *(volatile uint32_t*)&have[1] > kList ? high : __builtin_inff();
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (g + 256 * x < g1) u[x] = row.load(g + 256 * x);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      bool any = false;
-      if (g + 256 * x < g1) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) any |= RowReader<DT>::raw(u[x], j) >= low;
-      }
-      if (!__any(any)) continue;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float y = RowReader<DT>::value(u[x], j);
-        const bool mine = any && y >= low;
-        if (!__any(mine)) continue;
-        const uint32_t k = key_of(y);
-        const uint64_t p = place(k, (g + 256 * x) * E - row.off + j);
-        put(mine && k <= to, &w.n, w.list, p);
-        if (few) few = put(mine && k > to, &w.ahead, w.list + kList, p) <= kList;
-      }
+    for (int j = 0; j < E; ++j) {
+      const float x = RowReader<DT>::raw(u, j);
+      if (!(x >= low && x < end)) continue;
+      const uint32_t k = key_of(x + 0.0f);
+      const int which = k > to;
+      const uint32_t n = atomicAdd(&have[which], 1u);
+      if (n < kList) list[which][n] = place(k, unit * E - row.off + j);
     }
-  }
+  });
+  __syncthreads();
+  // the row's lists: room for the workgroup's tokens, then they
+  if (threadIdx.x < 2) base[threadIdx.x] = have[threadIdx.x] ? atomicAdd(threadIdx.x ? &w.ahead : &w.n, have[threadIdx.x]) : 0;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    for (uint32_t i = threadIdx.x; i < min(have[x], (uint32_t)kList) && base[x] + i < kList; i += 256)
+      w.list[x * kList + base[x] + i] = list[x][i];
 }
 
 // Launch 4, a workgroup a row: its token, or (top_p with many tokens kept) the last place kept.
@@ -916,12 +1009,7 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
   int token = -1;
   if (s.kind == kGreedy) {
     const int lane = threadIdx.x & 63;
-    uint64_t best = lane < a.splits ? w.first[lane] : 0;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const uint64_t o = shfl_xor64(best, k);
-      best = o > best ? o : best;
-    }
+    const uint64_t best = wave_max64(lane < a.splits ? w.first[lane] : 0);
     if (best) token = token_of(best);
     if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
     return;
@@ -960,7 +1048,7 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
       }
       // what is on the lists is not all the row's weight, but the border's goal is of that
       const uint64_t goal = s.kind == kShare ? w.goal : 0;
-      token = have > 1024 ? choose<2>(sm, weigh, have, s, goal) : choose<1>(sm, weigh, have, s, goal);
+      token = have > 1024 ? choose<2>(sm, weigh, have, s, goal, a.vocab) : choose<1>(sm, weigh, have, s, goal, a.vocab);
     }
   }
   if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
@@ -981,6 +1069,7 @@ struct Kept {
 // Launch 5: the kept tokens' weights, by chunks.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
+  __shared__ float keep[4][256 * RowReader<DT>::E];
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   RowWork& w = a.work[r];
   if (w.done || w.whole) return;
@@ -995,7 +1084,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
     if (kept.i >= i1 || kept.i < i0 || kept.from > kept.x) {
       const uint32_t k = key_of(kept.x) + (kept.i < i0 ? 1 : 0);
       const float from = fmaxf(value_of(k), kept.from);
-      v = chunk_sum<DT>(a, row, c, [&](int, float y) { return kept.weigh(y >= from ? y : kDead); });
+      v = chunk_sum_from<DT>(a, row, c, kept.weigh, from, keep[threadIdx.x >> 6]);
     } else {
       v = chunk_sum<DT>(a, row, c, kept);
     }
