@@ -165,7 +165,7 @@ struct RowWork {
   uint64_t cut;              // place of the last token kept
   uint32_t least_kept;       // key of the least logit that min_p leaves
   uint32_t n, ahead;         // tokens on either list, or that there were for it
-  uint32_t from;             // top_k: a key that at least k tokens reach
+  uint32_t from, to;         // keys of the border's list
   uint32_t done, whole;      // the row has its token; it is left to one workgroup
 };
 
@@ -232,8 +232,20 @@ __device__ __forceinline__ uint64_t wave_all64(uint64_t v, F f) {
   v = f(v, lane_xor64<16>(v));
   return f(v, lane_xor64<32>(v));
 }
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int s) {
-  return join64(__shfl_up((int)(uint32_t)v, s), __shfl_up((int)(v >> 32), s));
+// v of another lane by a move CTRL, 0 for lanes without one and in rows of 16 that ROWS leaves out.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lane_move64(uint64_t v) {
+  return join64(__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false),
+                __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false));
+}
+// Sum of v over the lanes up to this one: rows of 16 moved up by 1, 2, 4 and 8, then the last lanes of rows.
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
+  v += lane_move64<0x111, 0xF>(v);
+  v += lane_move64<0x112, 0xF>(v);
+  v += lane_move64<0x114, 0xF>(v);
+  v += lane_move64<0x118, 0xF>(v);
+  v += lane_move64<0x142, 0xA>(v);
+  return v + lane_move64<0x143, 0xC>(v);
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
   return wave_all64(v, [](uint64_t a, uint64_t b) { return a + b; });
@@ -246,12 +258,7 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 template <int W>
 __device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t sum = v;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint64_t o = shfl_up64(sum, s);
-    if (lane >= s) sum += o;
-  }
+  const uint64_t sum = wave_scan64(v);
   if (lane == 63) red[wave] = sum;
   __syncthreads();
   uint64_t base = 0, all = 0;
@@ -436,6 +443,34 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
   return (int)sm.pick[2];
 }
 
+// Leaves of the n > 1024 tokens on the list those up to the end of the bin in which the k'th lies: 1024 are sorted
+// in 8 us, twice as many in 20. Returns how many there are.
+__device__ __forceinline__ int drop_past(SampleShared& sm, const Bins& bin, int n, uint32_t k) {
+  const int t = threadIdx.x;
+  uint64_t v[2], all;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
+    sm.count[t + 1024 * e] = 0;
+  }
+  if (t == 0) sm.n = 0, sm.pick[0] = kBins;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (v[e]) atomicAdd(&sm.count[bin(value_of((uint32_t)(v[e] >> 32)))], 1u);
+  __syncthreads();
+  const uint32_t c0 = sm.count[2 * t], c1 = sm.count[2 * t + 1];
+  const uint64_t b = scan_block<16>(c0 + c1, sm.red, &all);
+  if (b < k && b + c0 >= k) sm.pick[0] = 2 * t;
+  else if (b + c0 < k && b + c0 + c1 >= k) sm.pick[0] = 2 * t + 1;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (v[e] && bin(value_of((uint32_t)(v[e] >> 32))) <= (int)sm.pick[0]) sm.list[atomicAdd(&sm.n, 1u)] = v[e];
+  __syncthreads();
+  return (int)sm.n;
+}
+
 // The place of the last token kept among the n of the list in LDS: the one before which, `before` included,
 // less than goal lies.
 template <int E>
@@ -478,54 +513,32 @@ __device__ __forceinline__ uint64_t chunk_sum(const SampleArgs& a, const RowRead
   return wave_sum64(v);
 }
 
-// The weights of chunk c's logits from `from` on, by one wave. Where they are fewer than three in four, they are
-// put side by side first (in keep, which holds four loads of a wave's logits): a weight costs as much as seven
-// such moves. 256 rows of which a fifth is kept 43 us without, SIDE with.
+// The weights of chunk c's logits from `from` on, by one wave. A lane weighs only those of its own that are: four
+// units lie in LDS (own, 16 bytes a thread and unit, 256 threads apart), from which it takes them one by one,
+// so that a step of a wave costs what its fullest lane has. 256 rows of which a ninth is kept: all
+// weighed 43 us, so 30.
 template <int DT>
 __device__ __forceinline__ uint64_t chunk_sum_from(const SampleArgs& a, const RowReader<DT>& row, int c, const Weigh& weigh,
-                                                   float from, float* keep) {
+                                                   float from, u32x4* own) {
+  typedef typename Elem<DT>::T T;
   constexpr int E = RowReader<DT>::E;
   const int lane = threadIdx.x & 63, g0 = c * a.chunk_units, g1 = min(row.units, g0 + a.chunk_units);
   uint64_t v = 0;
-  for (int g = g0; g < g1; g += 256) {
-    u32x4 w[4];
+  for (int g = g0 + lane; g < g1; g += 256) {
+    uint32_t mine = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (g + 64 * x + lane < g1) w[x] = row.load(g + 64 * x + lane);
-    int n = 0;
+    for (int x = 0; x < 4; ++x) {
+      if (g + 64 * x >= g1) break;
+      const u32x4 w = row.load(g + 64 * x);
+      own[256 * x] = w;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        n += __popcll(__ballot(g + 64 * x + lane < g1 && RowReader<DT>::raw(w[x], j) >= from));
-    if (n > 3 * 64 * E) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (g + 64 * x + lane < g1) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float y = RowReader<DT>::raw(w[x], j);
-            v += weigh(y >= from ? y : kDead);
-          }
-        }
-      continue;
+      for (int j = 0; j < E; ++j) mine |= (RowReader<DT>::raw(w, j) >= from ? 1u : 0u) << (E * x + j);
     }
-    int at = 0;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float y = RowReader<DT>::raw(w[x], j);
-        const bool mine = g + 64 * x + lane < g1 && y >= from;
-        const unsigned long long m = __ballot(mine);
-        if (mine) keep[at + __popcll(m & ((1ull << lane) - 1))] = y;
-        at += __popcll(m);
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    for (int i = lane; i < n; i += 64) v += weigh(keep[i]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    while (mine) {
+      const int i = __ffs(mine) - 1;
+      mine &= mine - 1;
+      v += weigh((float)reinterpret_cast<const T*>(own + 256 * (i / E))[i % E]);
+    }
   }
   return wave_sum64(v);
 }
@@ -896,7 +909,7 @@ __global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
     const uint32_t from = border == kBins ? kDeadKey + 1
                                           : least_key(kDeadKey, key_of(range.top),
                                                       [&](uint32_t k) { return bin(value_of(k)) <= border; });
-    if (threadIdx.x == 0) w.from = from;
+    if (threadIdx.x == 0) w.from = from, w.to = 0xFFFFFFFFu;
     return;
   }
   const RowReader<DT> row(a, r);
@@ -930,12 +943,45 @@ __global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
     if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
 }
 
-// Launch 3: the tokens that the border is among. top_k: all that reach its logit. top_p: those of its bin, and on
+// Launch 3, a workgroup a row with top_p: the bin in which its border lies, and that bin's keys. (The last
+// workgroup of the launch before could do it, but the fence that it takes costs each of them an L2
+// written back: 45 -> 303 us.)
+__global__ __launch_bounds__(256) void sample_border_kernel(SampleArgs a) {
+  __shared__ uint64_t red[4];
+  __shared__ int pick;
+  const int r = blockIdx.x;
+  const RowSettings s = settings(a, r);
+  if (s.kind != kShare) return;
+  RowWork& w = a.work[r];
+  const RowRange range = row_range(a, w);
+  if (!(fabsf(range.top) < __builtin_inff())) return;
+  constexpr int N = kBins / 256;
+  uint64_t v[N], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = w.mass[threadIdx.x * N + i];
+    sum += v[i];
+  }
+  uint64_t before = scan_block<4>(sum, red, &all);
+  const uint64_t goal = mass_goal(s.p, all);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (before < goal && before + v[i] >= goal) pick = threadIdx.x * N + i, w.before = before;
+    before += v[i];
+  }
+  __syncthreads();
+  const int border = pick;
+  const Bins bin(range.top, range.least, a.shift, s.t);
+  const uint32_t from = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) <= border; });
+  const uint32_t to = border == 0 ? 0xFFFFFFFFu
+                                  : least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) < border; }) - 1;
+  if (threadIdx.x == 0) w.from = from, w.to = to, w.goal = goal;
+}
+
+// Launch 4: the tokens that the border is among. top_k: all that reach its logit. top_p: those of its bin, and on
 // a list of their own those ahead of it, as long as they are few.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
-  __shared__ uint64_t red[4];
-  __shared__ uint64_t pick[2];
   __shared__ uint64_t list[2][kList];
   __shared__ uint32_t have[2], base[2];
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
@@ -943,34 +989,9 @@ __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
   if (s.kind != kFront && s.kind != kShare) return;
   const RowReader<DT> row(a, r);
   RowWork& w = a.work[r];
-  const RowRange range = row_range(a, w);
-  if (!(fabsf(range.top) < __builtin_inff())) return;
-  constexpr int N = kBins / 256, E = RowReader<DT>::E;
-  const bool share = s.kind == kShare;
-  uint32_t from, to = 0xFFFFFFFFu;  // keys of the list
-  if (!share) {
-    from = w.from;
-  } else {
-    uint64_t v[N], sum = 0, all;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = w.mass[threadIdx.x * N + i];
-      sum += v[i];
-    }
-    uint64_t before = scan_block<4>(sum, red, &all);
-    const uint64_t goal = mass_goal(s.p, all);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (before < goal && before + v[i] >= goal) pick[0] = threadIdx.x * N + i, pick[1] = before;
-      before += v[i];
-    }
-    __syncthreads();
-    const int border = (int)pick[0];
-    const Bins bin(range.top, range.least, a.shift, s.t);
-    from = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) <= border; });
-    if (border > 0) to = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) < border; }) - 1;
-    if (at == 0 && threadIdx.x == 0) w.before = pick[1], w.goal = goal;
-  }
+  if (!(fabsf(row_range(a, w).top) < __builtin_inff())) return;
+  constexpr int E = RowReader<DT>::E;
+  const uint32_t from = w.from, to = w.to;
   const float low = value_of(from);
   const int g0 = at * a.per * a.chunk_units, g1 = min(row.units, (at + 1) * a.per * a.chunk_units);
   // lists of the workgroup: [0] the border's, [1] ahead of it, which is left alone once it is too long
@@ -999,7 +1020,7 @@ __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
       w.list[x * kList + base[x] + i] = list[x][i];
 }
 
-// Launch 4, a workgroup a row: its token, or (top_p with many tokens kept) the last place kept.
+// Launch 5, a workgroup a row: its token, or (top_p with many tokens kept) the last place kept.
 template <int DT>
 __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
   __shared__ SampleShared sm;
@@ -1032,7 +1053,7 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
       token = find<DT>(a, sm, row, pick_goal(s.u, all), [&](int, float x) { return weigh(x >= from ? x : kDead); });
     } else {
       const bool some = n + ahead <= kList;  // all that may be kept is at hand
-      const int have = (int)(some ? n + ahead : n);
+      int have = (int)(some ? n + ahead : n);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t i = threadIdx.x + 1024 * e;
@@ -1045,6 +1066,9 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
         const uint32_t least = least_kept(weigh, range.top, s.m);
         if (threadIdx.x == 0) w.cut = cut, w.least_kept = least;
         return;
+      }
+      if (s.kind == kFront && have > 1024) {
+        have = drop_past(sm, Bins(range.top, value_of(w.from), a.shift, __builtin_inf()), have, (uint32_t)s.k);
       }
       // what is on the lists is not all the row's weight, but the border's goal is of that
       const uint64_t goal = s.kind == kShare ? w.goal : 0;
@@ -1066,10 +1090,10 @@ struct Kept {
   }
 };
 
-// Launch 5: the kept tokens' weights, by chunks.
+// Launch 6: the kept tokens' weights, by chunks.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
-  __shared__ float keep[4][256 * RowReader<DT>::E];
+  __shared__ u32x4 own[4 * 256];
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   RowWork& w = a.work[r];
   if (w.done || w.whole) return;
@@ -1084,7 +1108,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
     if (kept.i >= i1 || kept.i < i0 || kept.from > kept.x) {
       const uint32_t k = key_of(kept.x) + (kept.i < i0 ? 1 : 0);
       const float from = fmaxf(value_of(k), kept.from);
-      v = chunk_sum_from<DT>(a, row, c, kept.weigh, from, keep[threadIdx.x >> 6]);
+      v = chunk_sum_from<DT>(a, row, c, kept.weigh, from, own + threadIdx.x);
     } else {
       v = chunk_sum<DT>(a, row, c, kept);
     }
@@ -1092,36 +1116,30 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs a) {
   }
 }
 
-// Launch 6: the token of the rows whose kept weights are summed.
+// Last launch, a workgroup a row that has no token yet: rows whose kept weights are summed, and those with more
+// tokens around the border than the list holds, with larger top_k or with an infinity, all of which is
+// left to the workgroup. It is there for any row that needs it; with top_k most calls have none.
 template <int DT>
-__global__ __launch_bounds__(1024) void sample_find_kernel(SampleArgs a) {
+__global__ __launch_bounds__(1024) void sample_last_kernel(SampleArgs a) {
   __shared__ SampleShared sm;
   const int r = blockIdx.x;
   RowWork& w = a.work[r];
-  if (w.done || w.whole) return;
+  if (w.done) return;
   const RowSettings s = settings(a, r);
   const RowReader<DT> row(a, r);
-  const Kept kept(a, s, w, row_range(a, w).top);
-  const uint64_t mine = (int)threadIdx.x < a.chunks ? w.chunk[threadIdx.x] : 0;
-  uint64_t all;
-  if ((int)threadIdx.x < a.chunks) sm.chunk[threadIdx.x] = mine;
-  scan_block<16>(mine, sm.red, &all);
-  const int token = find<DT>(a, sm, row, pick_goal(s.u, all), kept);
-  if (threadIdx.x == 0) a.token[r] = token;
-}
-
-// Last launch: rows with more tokens around the border than the list holds, with larger top_k, or with an
-// infinity, a workgroup each. It is there for any row that needs it; most calls have none.
-template <int DT>
-__global__ __launch_bounds__(1024) void sample_whole_kernel(SampleArgs a) {
-  __shared__ SampleShared sm;
-  const int r = blockIdx.x;
-  RowWork& w = a.work[r];
-  if (!w.whole) return;
-  const RowSettings s = settings(a, r);
   const RowRange range = row_range(a, w);
-  Sampler<DT> whole{a, sm, RowReader<DT>(a, r), Weigh(range.top, s.t, a.shift), Bins(range.top, range.least, a.shift, s.t)};
-  const int token = whole.whole(s);
+  int token;
+  if (w.whole) {
+    Sampler<DT> whole{a, sm, row, Weigh(range.top, s.t, a.shift), Bins(range.top, range.least, a.shift, s.t)};
+    token = whole.whole(s);
+  } else {
+    const Kept kept(a, s, w, range.top);
+    const uint64_t mine = (int)threadIdx.x < a.chunks ? w.chunk[threadIdx.x] : 0;
+    uint64_t all;
+    if ((int)threadIdx.x < a.chunks) sm.chunk[threadIdx.x] = mine;
+    scan_block<16>(mine, sm.red, &all);
+    token = find<DT>(a, sm, row, pick_goal(s.u, all), kept);
+  }
   if (threadIdx.x == 0) a.token[r] = token;
 }
 
@@ -1139,13 +1157,11 @@ static int sample_rows(SampleArgs a, hipStream_t st) {
   const bool share = !greedy && (a.top_p || a.p < 1.0) && (a.top_k || !front);
   sample_range_kernel<DT><<<many, 256, 0, st>>>(a);
   if (!greedy) sample_weigh_kernel<DT><<<many, 256, 0, st>>>(a);
+  if (share) sample_border_kernel<<<one, 256, 0, st>>>(a);
   if (front || share) sample_collect_kernel<DT><<<many, 256, 0, st>>>(a);
   sample_choose_kernel<DT><<<one, 1024, 0, st>>>(a);
-  if (share) {
-    sample_kept_kernel<DT><<<many, 256, 0, st>>>(a);
-    sample_find_kernel<DT><<<one, 1024, 0, st>>>(a);
-  }
-  if (!greedy) sample_whole_kernel<DT><<<one, 1024, 0, st>>>(a);
+  if (share) sample_kept_kernel<DT><<<many, 256, 0, st>>>(a);
+  if (!greedy) sample_last_kernel<DT><<<one, 1024, 0, st>>>(a);
   CP_LAUNCHED("sampling");
   return CP_OK;
 }
