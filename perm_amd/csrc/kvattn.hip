@@ -869,7 +869,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     }
   };
   // MODE 2: the scores of unit s of the tile at j0, and the largest and least of them
-  auto change = [&](f32x16& x, int j0, int s, float kc) {
+  auto change = [&](f32x16& x, int j0, int s, float kc) __attribute__((always_inline)) {
     if constexpr (MODE > 1) {
       change_scores<16>(ext, x, kc, slope, (float)(pos - (j0 + 32 * s + 16 * hh)));
       top = bot = x[0];
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   };
   // Whether a row's weights need two terms: one is too small for float16, and not all of them for any.
   // (A distance's share leaves many rows' far tokens with no weight at all.)
-  auto deep_scores = [&](float kc, float lg) {
+  auto deep_scores = [&](float kc, float lg) __attribute__((always_inline)) {
     const bool small = __builtin_fmaf(bot, kc, lg) < m - kDeep;
     return MODE > 1 ? small && __builtin_fmaf(top, kc, lg) > m - kGone : small;
   };
@@ -914,6 +914,194 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
     lookup(tile + 3);
   };
   if (tb < te) enter();
+  if constexpr (MODE > 0) {
+    // Weights in one term while they fit, in two from the tile on in which a row's do not, until a tile needs
+    // no more of them; either way the next unit's scores are multiplied meanwhile. A tile that turns
+    // out to need them at its second unit has that one done by itself.
+    auto first_scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) read_k(buf, 0, k);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[0][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
+        sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
+      }
+      if constexpr (MODE < 2) {
+        top = bot = sc[0][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
+      }
+    };
+    // masks a unit's scores, moves the maximum, and says whether its weights need two terms
+    auto enter_unit = [&](auto S, float kc, float lg, int j0) __attribute__((always_inline)) {
+      constexpr int s = S;
+      change(sc[s], j0, s, ks[s] * a.scale);
+      if (edge) mask(sc[s], j0, s, have[s]);
+      const float tm = __builtin_fmaf(top, kc, lg);
+      if (__any(tm > m + kLag)) move_max(tm);
+      return (bool)__any(deep_scores(kc, lg));
+    };
+    auto nan_of_unit = [&](int j0, int s, bool hv) __attribute__((always_inline)) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= nan_flags(vr[i][k]);
+      if (__any(any != 0)) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) mine[64 * i] = vr[i];
+        take_nan(j0, s, hv);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) vr[i] = mine[64 * i];
+      }
+    };
+    // unit s of the tile at j0, its scores entered; the next one's are multiplied
+    auto unit = [&](auto S, auto Two, float kc, float lg, int j0) __attribute__((always_inline)) {
+      constexpr int s = S;
+      constexpr bool two = Two;
+      // one term: V's scale in the exponent, out of the sum again by iv; two: as in attn_few_kernel
+      const float off = (two ? 0.0f : lg) + kLift - (m == kNegInf ? 0.0f : m);
+      u32x4 wh[2], wl[2];
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sc[1 - s][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * NC; ++k) {
+        const u32x4 x = kr[k >> 1];
+        sc[1 - s] = mfma32<DT>(k & 1 ? codes_to_16<DT>(x[2], x[3]) : codes_to_16<DT>(x[0], x[1]), qf[k >> 1][k & 1],
+                               sc[1 - s]);
+#pragma unroll
+        for (int i = 8 * k / (2 * NC); i < 8 * (k + 1) / (2 * NC); ++i) {
+          const float e0 = exp2_fast(__builtin_fmaf(sc[s][2 * i], kc, off));
+          const float e1 = exp2_fast(__builtin_fmaf(sc[s][2 * i + 1], kc, off));
+          sum += e0 + e1;
+          if constexpr (two) {
+            Weights2 w = weights2(e0 * vs[s], e1 * vs[s]);
+            asm volatile("" : "+v"(w.hi), "+v"(w.lo));
+            wh[i >> 2][i & 3] = w.hi, wl[i >> 2][i & 3] = w.lo;
+          } else {
+            uint32_t e = pack2<CP_F16>(e0, e1);
+            asm volatile("" : "+v"(e));  // here, not past the branch below
+            wh[i >> 2][i & 3] = e;
+          }
+        }
+        if (k == NC) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) read_v(buf, s, i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (two) l += sum;
+      else l = __builtin_fmaf(sum, __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u)), l);
+      if (edge) nan_of_unit(j0, s, have[s]);
+      __builtin_amdgcn_s_setprio(0);
+      if constexpr (MODE < 2) top = bot = sc[1 - s][0];
+#pragma unroll
+      for (int k = 0; k < 2 * NC; ++k) {
+        const int i = k % NC;
+        const u32x4 x = vr[i];
+        if constexpr (two) {
+          const u32x4 c16 = k < NC ? codes_to_16<CP_BF16>(x[0], x[1]) : codes_to_16<CP_BF16>(x[2], x[3]);
+          o[i] = mfma32<CP_BF16>(c16, wh[k / NC], o[i]);
+          o[i] = mfma32<CP_BF16>(c16, wl[k / NC], o[i]);
+        } else {
+          o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), wh[k / NC], o[i]);
+        }
+        if constexpr (MODE < 2) {
+#pragma unroll
+          for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
+            top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(1);
+    };
+    auto scale_bits = [&](float v) __attribute__((always_inline)) { return (float)((int)(__float_as_uint(v) >> 23) - 127); };
+    auto next_tile = [&]() __attribute__((always_inline)) {
+      buf = nbuf;
+      nbuf = last;
+      ++tile;
+      enter();
+    };
+    if (tb < te) first_scores();
+    while (tile < te) {
+      wide = -1;
+      while (tile < te) {
+        const int j0 = tile * kTile;
+        unrolled2([&](auto S) {
+          constexpr int s = S;
+          if (s == 1 && wide >= 0) return;
+          const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
+          if constexpr (s == 1) advance();
+#pragma unroll
+          for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
+          if (enter_unit(S, kc, lg, j0)) {
+            wide = s;
+            return;
+          }
+          unit(S, std::false_type{}, kc, lg, j0);
+        });
+        if (wide >= 0) break;
+        next_tile();
+      }
+      if (tile >= te) break;
+      if (wide == 1) {  // by itself, from its scores on
+        const int j0 = tile * kTile;
+        const float kc0 = ks[1] * a.scale, kc = MODE > 1 ? 1.0f : kc0;
+        f32x16& x = sc[0];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          read_k(buf, 1, k);
+          x = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], x);
+          x = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], x);
+        }
+        change(x, j0, 1, kc0);
+        if (edge) mask(x, j0, 1, have[1]);  // the maximum has moved already
+        const float off = kLift - (m == kNegInf ? 0.0f : m);
+        u32x4 wh[2], wl[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float e0 = exp2_fast(__builtin_fmaf(x[2 * i], kc, off)), e1 = exp2_fast(__builtin_fmaf(x[2 * i + 1], kc, off));
+          sum += e0 + e1;
+          const Weights2 w = weights2(e0 * vs[1], e1 * vs[1]);
+          wh[i >> 2][i & 3] = w.hi, wl[i >> 2][i & 3] = w.lo;
+        }
+        l += sum;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) read_v(buf, 1, i);
+        if (edge) nan_of_unit(j0, 1, have[1]);
+#pragma unroll
+        for (int k = 0; k < 2 * NC; ++k) {
+          const int i = k % NC;
+          const u32x4 y = vr[i], c16 = k < NC ? codes_to_16<CP_BF16>(y[0], y[1]) : codes_to_16<CP_BF16>(y[2], y[3]);
+          o[i] = mfma32<CP_BF16>(c16, wh[k / NC], o[i]);
+          o[i] = mfma32<CP_BF16>(c16, wl[k / NC], o[i]);
+        }
+        next_tile();
+        if (tile >= te) break;
+      }
+      first_scores();  // again: the ones at hand are changed, or another tile's
+      for (bool deep = true; tile < te && deep;) {
+        const int j0 = tile * kTile;
+        deep = false;
+        unrolled2([&](auto S) {
+          constexpr int s = S;
+          const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
+          if constexpr (s == 1) advance();
+#pragma unroll
+          for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
+          deep |= enter_unit(S, kc, lg, j0);
+          unit(S, std::true_type{}, kc, lg, j0);
+        });
+        next_tile();
+      }
+    }
+  } else
   while (tile < te) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) read_k(buf, 0, k);
@@ -924,29 +1112,26 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
       sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
     }
-    if constexpr (MODE < 2) {
-      top = bot = sc[0][0];
+    top = bot = sc[0][0];
 #pragma unroll
-      for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
-    }
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
     wide = -1;
     while (tile < te) {
       const int j0 = tile * kTile;
       unrolled2([&](auto S) {
         constexpr int s = S;
         if (s == 1 && wide >= 0) return;
-        const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale;
+        const float kc = ks[s] * a.scale;
         const float lg = (float)((int)(__float_as_uint(vs[s]) >> 23) - 127);
         const float iv = __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u));
         if constexpr (s == 1) advance();
 #pragma unroll
         for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
-        change(sc[s], j0, s, ks[s] * a.scale);
         if (edge) mask(sc[s], j0, s, have[s]);
         // the largest t of the unit: kc > 0, so t rises with the raw score
         const float tm = __builtin_fmaf(top, kc, lg);
         if (__any(tm > m + kLag)) move_max(tm);
-        if (__any(deep_scores(kc, lg))) {
+        if (__any(__builtin_fmaf(bot, kc, lg) < m - kDeep)) {
           wide = s;
           return;
         }
@@ -995,17 +1180,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         // SIMD's other wave: its MFMAs need an issue slot in 32 clocks, the weights every slot, and
         // two waves that keep out of step overlap (335 -> 309 us for two prompts of 4096 rows).
         __builtin_amdgcn_s_setprio(0);
-        if constexpr (MODE < 2) top = bot = sc[1 - s][0];
+        top = bot = sc[1 - s][0];
 #pragma unroll
         for (int k = 0; k < 2 * NC; ++k) {
           const int i = k % NC;
           const u32x4 x = vr[i];
           o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), w[k / NC], o[i]);
-          if constexpr (MODE < 2) {
 #pragma unroll
-            for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
-              top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
-          }
+          for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
+            top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
           __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(1);
@@ -1025,7 +1208,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       if (s == 1 && !ahead) advance();
       ahead = false;
       const bool hv = s ? have[1] : have[0];
-      const float v1 = s ? vs[1] : vs[0], kc0 = (s ? ks[1] : ks[0]) * a.scale, kc = MODE > 1 ? 1.0f : kc0;
+      const float v1 = s ? vs[1] : vs[0], kc = (s ? ks[1] : ks[0]) * a.scale;
       const float lg = (float)((int)(__float_as_uint(v1) >> 23) - 127);
       f32x16& x = sc[0];
 #pragma unroll
@@ -1036,17 +1219,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         x = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], x);
         x = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], x);
       }
-      change(x, j0, s, kc0);
       if (edge) {
         mask(x, j0, s, hv);
-      } else if constexpr (MODE < 2) {
+      } else {
         top = bot = x[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
       }
       const float tm = __builtin_fmaf(top, kc, lg);
       if (__any(tm > m + kLag)) move_max(tm);
-      deep |= __any(deep_scores(kc, lg));
+      deep |= __any(__builtin_fmaf(bot, kc, lg) < m - kDeep);
       // as in attn_few_kernel, the sum's terms and the weights from them
       const float off = kLift - (m == kNegInf ? 0.0f : m);
       u32x4 wh[2], wl[2];
