@@ -39,6 +39,7 @@ constexpr float kNegInf = -__builtin_inff();
 // Weights are 2^kLift above 2^(t - m), which uses float16's range up to 2^15: m moves when a t
 // passes it by kLag. A t more than kDeep below m has a weight below float16's normal range.
 constexpr float kLift = 11.0f, kLag = 4.0f, kDeep = kLift + 14.0f;
+constexpr float kSmallCap = 0.6f;        // shares of the cap up to which tanh is a polynomial
 constexpr float kGone = kLift + 127.0f;  // a t more than this below m has no weight in bfloat16 either
 
 struct AttnArgs {
@@ -59,7 +60,7 @@ struct AttnArgs {
 };
 
 // What changes the masks and scores above, in kernels of their own (MODE 1: which tokens a row sees,
-// MODE 2: scores too):
+// MODE 2: capped scores, too, which rise with the products; MODE 3: scores that need not):
 //   first   a row sees no token before its own first one (the start of its document)
 //   prefix  a sequence's tokens before this are seen whatever a row's position
 //   shared  consecutive sequences (`group` of them) whose tables begin with the same pages: those are read once,
@@ -73,7 +74,7 @@ struct AttnMore {
   int phase;               // 0: no shared pages
   int slot0, slots;        // where this phase's splits lie among a row's
   const float* slopes;     // [q heads]
-  float cap, over;         // cap * log2 e (0: none) and 2 / cap
+  float cap, inv;          // cap * log2 e (0: none), and 1 over it
   int series;              // a large cap
 };
 struct AttnPlain {};
@@ -171,36 +172,46 @@ __device__ __forceinline__ bool whole_group(const AttnArgs& a, const AttnMore& x
 
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// N scores of tokens that follow one another, in base 2: products times kc, capped, less the distance's
-// share. far: position less the first token. tanh z = 1 - 2 / (1 + e^2z) errs by 1.5 x 2^-23, a capped
-// score by cap times that: up to caps of 128 no more than 2^-15 of a weight. Larger caps, of which
-// most scores are a small part, take the series below |z| = 1/4, whose error is relative.
+// N products x become x tanh(z) / z, z = x kz: what kc takes to the capped score then is cap tanh(z). `small`: all of
+// them have |z| <= 0.6, where tanh(z) / z = 1 + z^2 p(z^2) within 2^-23.5 (p found by exchange): seven
+// operations. Elsewhere tanh z = 1 - 2 / (1 + e^2z), two of whose five steps run at a quarter of
+// the rate; it errs by 1.5 x 2^-23, a score by cap times that: up to caps of 128 no more than 2^-15
+// of a weight. Under larger ones small scores take the first way one by one.
 template <int N, class V>
-__device__ __forceinline__ void change_scores(const AttnMore& x, V& v, float kc, float slope, float far) {
+__device__ __forceinline__ void cap_scores(const AttnMore& x, V& v, float kc, bool small) {
+  const float kz = kc * x.inv;
+  auto near = [&](float y) {
+    const float z = y * kz, q = z * z;
+    float p = __builtin_fmaf(q, 0.015612630648888721f, -0.05221180504288673f);
+    p = __builtin_fmaf(q, p, 0.1331311661378244f);
+    p = __builtin_fmaf(q, p, -0.3333259750323093f);
+    return y * __builtin_fmaf(q, p, 1.0f);
+  };
+  if (small) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] *= kc;
-  if (x.cap > 0.0f) {
+    for (int i = 0; i < N; ++i) v[i] = near(v[i]);
+  } else {
+    const float most = x.cap / kc, e2 = kz * (2.0f * kLog2e);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float z2 = v[i] * x.over, e = exp2_fast(z2);
-      float y = __builtin_fmaf(-2.0f * x.cap, __builtin_amdgcn_rcpf(1.0f + e), x.cap);
-      if (x.series) {
-        const float z = z2 * (0.5f / kLog2e), q = z * z;
-        float p = __builtin_fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f);
-        p = __builtin_fmaf(q, p, 2.0f / 15.0f);
-        p = __builtin_fmaf(q, p, -1.0f / 3.0f);
-        y = q < 0.0625f ? __builtin_fmaf(v[i] * q, p, v[i]) : y;
-      }
-      v[i] = y;
+      const float far = __builtin_fmaf(-2.0f * most, __builtin_amdgcn_rcpf(1.0f + exp2_fast(v[i] * e2)), most);
+      v[i] = x.series && fabsf(v[i] * kz) <= kSmallCap ? near(v[i]) : far;
     }
-  }
-  if (x.slopes) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __builtin_fmaf(-slope, fabsf(far - (float)i), v[i]);
   }
 }
 
-// Results of the rows [0, lead) and [tail, end): 0, lse -inf, nothing to join. Workgroup `at` of `of`.
+// N scores of tokens that follow one another, in base 2, capped, less the distance's share. far: position less the
+// first token.
+template <int N, class V>
+__device__ __forceinline__ void change_scores(const AttnMore& x, V& v, float slope, float far) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(v[i]));
+  if (x.cap > 0.0f) cap_scores<N>(x, v, 1.0f, __all(most * x.inv <= kSmallCap));
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __builtin_fmaf(-slope, fabsf(far - (float)i), v[i]);
+}
+
 template <int DT, class X>
 __device__ __forceinline__ void attn_clear(const AttnArgs& a, const X& x, int64_t lead, int64_t tail, int64_t end, int at, int of) {
   const int64_t per = (int64_t)a.group * a.c.heads, skip = (tail - lead) * per;
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
   if constexpr (MODE > 0) {
     const SeenRow s = seen_row(a, ext, bt, real, row0 + qi, b, row0, n_b);
     pos = s.pos, lo = s.lo, hi = s.hi;
-    if (MODE > 1 && ext.slopes && real) slope = ext.slopes[qh] * kLog2e;
+    if (MODE == 3 && real) slope = ext.slopes[qh] * kLog2e;
   }
   // tokens any row of the workgroup sees
   int jhi = hi, jlo = hi > lo ? lo : 0x7FFFFFFF;
@@ -420,12 +431,28 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
         sc[t] = mfma16<DT>(codes_to_16<DT>(kk[t][k][2], kk[t][k][3]), qf[k][1], sc[t]);
       }
     }
-    const float kc = MODE > 1 ? 1.0f : ks * a.scale;
+    const float kc = MODE == 3 ? 1.0f : ks * a.scale;
     const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
-    if constexpr (MODE > 1) {
-      const float far = (float)(pos - jv);
+    if constexpr (MODE == 2) {
+      float most = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) change_scores<4>(ext, sc[t], ks * a.scale, slope, far - 4.0f * t);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(sc[t][i]));
+      const bool small = __all(most * (kc * ext.inv) <= kSmallCap);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) cap_scores<4>(ext, sc[t], kc, small);
+    }
+    if constexpr (MODE == 3) {
+      const float far = (float)(pos - jv);
+      // All products are read before change_scores branches: with a branch right behind a matrix instruction, the
+      // compiler (ROCm 7.2) did not wait for that one's result on the way around what is skipped.
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = sc[i >> 2][i & 3] * (ks * a.scale);
+      change_scores<8>(ext, v, slope, far);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sc[i >> 2][i & 3] = v[i];
     }
     bool edge = false;  // a token of this lane that its row does not see
 #pragma unroll
@@ -620,11 +647,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   extern __shared__ __align__(16) uint8_t lds[];     // [3][BUF], then [4 waves][NC][64 lanes][16]
   const KvCacheArgs& c = a.c;
   const int h = (int)(blockIdx.x % c.heads);
-  const int split = (int)(blockIdx.x / c.heads % a.splits);
+  // MODE > 0: all first splits, then all second ones ..., as many have nothing to do where masks leave little. A
+  // launch deals its workgroups to the shader engines in turn: with an even number of splits side by
+  // side, the full ones would be on half of them (two rows of documents of up to 8192 tokens in four
+  // splits of at least 16 tiles 483 us, so 220).
+  const int split = (int)(MODE ? blockIdx.x / c.heads / items : blockIdx.x / c.heads % a.splits);
   int b, item, n_b;
   int64_t row0;
   // last items first: causal rows at the end of a prompt see the most tokens
-  const int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
+  const int from_end = items - 1 - (int)(MODE ? blockIdx.x / c.heads % items : blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
   if (!kv_locate(bt, from_end, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b,
                  &item, &row0, &n_b, each_of(ext)))
     return attn_unowned<DT>(a, ext, bt, item, items - from_end + item, piece, 0, 0);
@@ -721,8 +752,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   float m = kNegInf, l = 0.0f;
 
   float slope = 0.0f;
-  if constexpr (MODE > 1) {
-    if (ext.slopes && real) slope = ext.slopes[qh] * kLog2e;
+  if constexpr (MODE == 3) {
+    if (real) slope = ext.slopes[qh] * kLog2e;
   }
   const int* tab = c.table + (int64_t)b * each_of(ext) * c.max_pages;
   // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
@@ -868,10 +899,20 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       }
     }
   };
-  // MODE 2: the scores of unit s of the tile at j0, and the largest and least of them
+  // The scores of unit s of the tile at j0, and the largest and least of them: capped ones from those of the
+  // products.
   auto change = [&](f32x16& x, int j0, int s, float kc) __attribute__((always_inline)) {
-    if constexpr (MODE > 1) {
-      change_scores<16>(ext, x, kc, slope, (float)(pos - (j0 + 32 * s + 16 * hh)));
+    if constexpr (MODE == 2) {
+      const bool small = __all(fmaxf(fabsf(top), fabsf(bot)) * (kc * ext.inv) <= kSmallCap);
+      cap_scores<16>(ext, x, kc, small);
+      float ends[2] = {top, bot};
+      cap_scores<2>(ext, ends, kc, small);
+      top = ends[0], bot = ends[1];
+    }
+    if constexpr (MODE == 3) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] *= kc;
+      change_scores<16>(ext, x, slope, (float)(pos - (j0 + 32 * s + 16 * hh)));
       top = bot = x[0];
 #pragma unroll
       for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
@@ -881,7 +922,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   // (A distance's share leaves many rows' far tokens with no weight at all.)
   auto deep_scores = [&](float kc, float lg) __attribute__((always_inline)) {
     const bool small = __builtin_fmaf(bot, kc, lg) < m - kDeep;
-    return MODE > 1 ? small && __builtin_fmaf(top, kc, lg) > m - kGone : small;
+    return MODE == 3 ? small && __builtin_fmaf(top, kc, lg) > m - kGone : small;
   };
   // the running maximum and what hangs on it, when a row's t passes it by kLag; called seldom
   auto move_max = [&](float tm) {
@@ -928,7 +969,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], sc[0]);
         sc[0] = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], sc[0]);
       }
-      if constexpr (MODE < 2) {
+      if constexpr (MODE < 3) {
         top = bot = sc[0][0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, sc[0][j]), bot = fminf(bot, sc[0][j]);
@@ -997,7 +1038,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       else l = __builtin_fmaf(sum, __uint_as_float((254u << 23) - (__float_as_uint(vs[s]) & 0x7F800000u)), l);
       if (edge) nan_of_unit(j0, s, have[s]);
       __builtin_amdgcn_s_setprio(0);
-      if constexpr (MODE < 2) top = bot = sc[1 - s][0];
+      if constexpr (MODE < 3) top = bot = sc[1 - s][0];
 #pragma unroll
       for (int k = 0; k < 2 * NC; ++k) {
         const int i = k % NC;
@@ -1009,7 +1050,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         } else {
           o[i] = mfma32<CP_F16>(k < NC ? codes_to_16<CP_F16>(x[0], x[1]) : codes_to_16<CP_F16>(x[2], x[3]), wh[k / NC], o[i]);
         }
-        if constexpr (MODE < 2) {
+        if constexpr (MODE < 3) {
 #pragma unroll
           for (int j = 16 * k / (2 * NC); j < 16 * (k + 1) / (2 * NC); ++j)
             top = fmaxf(top, sc[1 - s][j]), bot = fminf(bot, sc[1 - s][j]);
@@ -1033,7 +1074,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         unrolled2([&](auto S) {
           constexpr int s = S;
           if (s == 1 && wide >= 0) return;
-          const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
+          const float kc = MODE == 3 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
           if constexpr (s == 1) advance();
 #pragma unroll
           for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
@@ -1049,7 +1090,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
       if (tile >= te) break;
       if (wide == 1) {  // by itself, from its scores on
         const int j0 = tile * kTile;
-        const float kc0 = ks[1] * a.scale, kc = MODE > 1 ? 1.0f : kc0;
+        const float kc0 = ks[1] * a.scale, kc = MODE == 3 ? 1.0f : kc0;
         f32x16& x = sc[0];
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = 0.0f;
@@ -1058,6 +1099,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
           read_k(buf, 1, k);
           x = mfma32<DT>(codes_to_16<DT>(kr[k][0], kr[k][1]), qf[k][0], x);
           x = mfma32<DT>(codes_to_16<DT>(kr[k][2], kr[k][3]), qf[k][1], x);
+        }
+        if constexpr (MODE == 2) {
+          top = bot = x[0];
+#pragma unroll
+          for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]), bot = fminf(bot, x[j]);
         }
         change(x, j0, 1, kc0);
         if (edge) mask(x, j0, 1, have[1]);  // the maximum has moved already
@@ -1091,7 +1137,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
         deep = false;
         unrolled2([&](auto S) {
           constexpr int s = S;
-          const float kc = MODE > 1 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
+          const float kc = MODE == 3 ? 1.0f : ks[s] * a.scale, lg = scale_bits(vs[s]);
           if constexpr (s == 1) advance();
 #pragma unroll
           for (int k = 0; k < NC; ++k) read_k(s ? nbuf : buf, 1 - s, k);
@@ -1668,16 +1714,17 @@ int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row,
   x.seqs = two ? (int)(batch / groups) : 1;
   x.slopes = more->slopes;
   x.cap = more->softcap * cp::kLog2e;
-  x.over = more->softcap > 0.0f ? 2.0f / more->softcap : 0.0f;
+  x.inv = more->softcap > 0.0f ? 1.0f / x.cap : 0.0f;
   x.series = more->softcap > 128.0f;
   const cp::KvBatch b = {offsets, (int)batch};
   hipStream_t st = (hipStream_t)stream;
-  const bool scores = more->softcap > 0.0f || more->slopes;
   if (dtype == CP_BF16)
-    return scores ? cp::attn_run_more<CP_BF16, 2>(a, b, x, p, sp, (int)groups, st)
-                  : cp::attn_run_more<CP_BF16, 1>(a, b, x, p, sp, (int)groups, st);
-  return scores ? cp::attn_run_more<CP_F16, 2>(a, b, x, p, sp, (int)groups, st)
-                : cp::attn_run_more<CP_F16, 1>(a, b, x, p, sp, (int)groups, st);
+    return more->slopes         ? cp::attn_run_more<CP_BF16, 3>(a, b, x, p, sp, (int)groups, st)
+           : more->softcap > 0.0f ? cp::attn_run_more<CP_BF16, 2>(a, b, x, p, sp, (int)groups, st)
+                                  : cp::attn_run_more<CP_BF16, 1>(a, b, x, p, sp, (int)groups, st);
+  return more->slopes         ? cp::attn_run_more<CP_F16, 3>(a, b, x, p, sp, (int)groups, st)
+         : more->softcap > 0.0f ? cp::attn_run_more<CP_F16, 2>(a, b, x, p, sp, (int)groups, st)
+                                : cp::attn_run_more<CP_F16, 1>(a, b, x, p, sp, (int)groups, st);
 }
 
 }  // extern "C"

@@ -13,6 +13,13 @@ pytestmark = pytest.mark.gpu
 HALVES = [torch.bfloat16, torch.float16]
 
 
+@pytest.fixture(autouse=True)
+def _fronts_apart(kv, monkeypatch, request):  # noqa: F811
+    """Common pages are read apart at every size here, but where the rule for it is tested."""
+    if "rule" not in request.node.name:
+        monkeypatch.setattr(kv, "_front_pays", lambda *a: True)
+
+
 def _check(kv, c, o, table, lens, counts, hq, dtype, rng, offsets=True, spread=1.0, slopes=None, first=None,  # noqa: F811
            prefix=None, shared=None, causal=True, window=0, scale=None, softcap=0.0):
     heads, d = o.k.shape[1], o.k.shape[3]
@@ -23,15 +30,15 @@ def _check(kv, c, o, table, lens, counts, hq, dtype, rng, offsets=True, spread=1
                 first=None if first is None else _i32(first), prefix=None if prefix is None else _i32(prefix),
                 shared=None if shared is None else _i32(shared))
     off = _offsets(counts) if offsets else None
+    table = np.array(table)
+    if shared is not None:  # a group's rows of the table begin alike
+        each = len(lens) // len(shared)
+        for b in range(len(lens)):
+            table[b, :max(shared[b // each], 0)] = table[b - b % each, :max(shared[b // each], 0)]
     out, lse = kv.attention(q, c, _i32(table), _i32(lens), off, return_lse=True, **args)
     again = kv.attention(q, c, _i32(table), _i32(lens), off, **args)
     assert torch.equal(again.view(torch.int16), out.view(torch.int16))
     assert out.shape == q.shape and out.dtype == dtype
-    table = np.array(table)
-    if shared is not None:  # a group's front is its first sequence's
-        each = len(lens) // len(shared)
-        for b in range(len(lens)):
-            table[b, :max(shared[b // each], 0)] = table[b - b % each, :max(shared[b // each], 0)]
     r = 0
     for b, n in enumerate(counts):
         k, v, have = (torch.from_numpy(t).cuda() for t in o.tokens(table[b], min(lens[b], table.shape[1] * o.block)))
@@ -154,6 +161,25 @@ def test_common_pages(kv, block, heads, d, group, dtype):  # noqa: F811
            spread=3.0)
     none = np.full_like(table, -1)
     _check(kv, c, o, none, lens, counts, hq, dtype, rng, shared=[4, 2])
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_rule_of_common_pages(kv, dtype):  # noqa: F811
+    """The same answers whichever way the rule takes, on both sides of it."""
+    rng = np.random.default_rng(6)
+    lens = [2100 + n for n in range(24)]
+    c, o, table = _filled_cache(kv, rng, lens, 1, 64, 16)
+    table[:, :130] = table[0, :130]
+    desc = kv._desc(c)
+    assert not kv._front_pays(desc, 24, 4, 24, 1, 2144) and not kv._front_pays(desc, 2400, 4, 24, 1, 1 << 20)
+    assert kv._front_pays(desc, 24, 4, 24, 1, 1 << 20) and not kv._front_pays(desc, 24, 4, 24, 24, 1 << 20)
+    for counts in ([1] * 24, [5, 0, 30] * 8):
+        _check(kv, c, o, table, lens, counts, 4, dtype, rng, shared=[130])
+        _check(kv, c, o, table, lens, counts, 4, dtype, rng, shared=[130, 100], softcap=9.0, window=900)
+    # a table wide enough for it, most of which is empty
+    wide = np.full((24, 1 << 16), -1)
+    wide[:, :table.shape[1]] = table
+    _check(kv, c, o, wide, lens, [1] * 24, 4, dtype, rng, shared=[130])
 
 
 @pytest.mark.parametrize("dtype", HALVES)
