@@ -117,7 +117,7 @@ __device__ __forceinline__ bool grow_wants(const GrowArgs& a, const GrowRange& g
 
 // f(sequence, its range, this thread's place among the ones that share it and their number, the last of its
 // entries in the row): a thread a sequence of up to four entries, as the next token has, then a
-// wave a longer one. (A wave for every one, 272 sequences: 46 us, so GROW.)
+// wave a longer one. (A wave for every one, 272 sequences: 46 us, so 12.)
 template <class F>
 __device__ __forceinline__ void for_sequences(const GrowArgs& a, F f) {
   const int lane = threadIdx.x & 63;

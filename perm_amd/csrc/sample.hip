@@ -23,7 +23,8 @@
 namespace cp {
 
 constexpr int kBins = 2048;    // of a histogram
-constexpr int kList = 2048;    // tokens that are sorted at most: two a thread
+constexpr int kList = 2048;    // tokens that are sorted at most: two a thread,
+constexpr int kFew = 1024;     // or one
 constexpr int kChunks = 1024;  // pieces of a row whose weights are summed by themselves, at most
 constexpr int kChunkUnits = 256;  // of 16 bytes in a piece, at least
 constexpr int kSplits = 64;     // workgroups of a row at most
@@ -157,7 +158,7 @@ struct RowReader {
 // What the launches of a call hand on about a row.
 struct RowWork {
   uint64_t mass[kBins];
-  uint64_t list[2 * kList];  // tokens among which the border is; top_p: and the ones ahead of them
+  uint64_t list[kList + kFew];  // tokens among which the border is; top_p: and the ones ahead of them
   uint64_t chunk[kChunks];
   uint64_t first[kSplits];   // of every workgroup: its largest place,
   uint32_t top[kSplits], least[kSplits];  // its largest key, its least key's complement
@@ -283,21 +284,34 @@ __device__ __forceinline__ uint64_t max_block(uint64_t v, uint64_t* red) {
   return v;
 }
 
-// A step of the sort: value number at against partner o, J apart, in runs of k that fall and rise in turn.
+// A step of a sort: values number t + 1024 e against partners o, j apart, in runs of k that fall and rise in turn.
 template <int E>
-__device__ __forceinline__ void sort_keep(uint64_t (&v)[E], const uint64_t (&o)[E], int j, int k) {
+__device__ __forceinline__ void sort_keep(uint64_t (&v)[E], const uint64_t (&o)[E], int t, int j, int k) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool first = !(threadIdx.x & j), down = !(((int)threadIdx.x + 1024 * e) & k);  // down: the larger one first
+    const bool first = !(t & j), down = !((t + 1024 * e) & k);  // down: the larger one first
     v[e] = (first == down) == (v[e] > o[e]) ? v[e] : o[e];
   }
 }
 template <int J, int E>
-__device__ __forceinline__ void sort_step(uint64_t (&v)[E], int k) {
+__device__ __forceinline__ void sort_step(uint64_t (&v)[E], int t, int k) {
   uint64_t o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = lane_xor64<J>(v[e]);
-  sort_keep<E>(v, o, J, k);
+  sort_keep<E>(v, o, t, J, k);
+}
+
+// The 64 values of a wave, sorted, the largest first.
+__device__ __forceinline__ void sort_lanes(uint64_t (&v)[1]) {
+  const int t = threadIdx.x & 63;
+  for (int k = 2; k <= 64; k <<= 1) {
+    if (k > 32) sort_step<32>(v, t, k);
+    if (k > 16) sort_step<16>(v, t, k);
+    if (k > 8) sort_step<8>(v, t, k);
+    if (k > 4) sort_step<4>(v, t, k);
+    if (k > 2) sort_step<2>(v, t, k);
+    sort_step<1>(v, t, k);
+  }
 }
 
 // Up to 1024 E values, number t + 1024 e in thread t's v[e], sorted, the largest first (threads past the n
@@ -322,14 +336,14 @@ __device__ __forceinline__ void sort_block(uint64_t (&v)[E], int n, uint64_t* li
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = list[(t ^ j) + 1024 * e];
       __syncthreads();
-      sort_keep<E>(v, o, j, k);
+      sort_keep<E>(v, o, t, j, k);
     }
-    if (j >= 32) sort_step<32>(v, k);
-    if (j >= 16) sort_step<16>(v, k);
-    if (j >= 8) sort_step<8>(v, k);
-    if (j >= 4) sort_step<4>(v, k);
-    if (j >= 2) sort_step<2>(v, k);
-    sort_step<1>(v, k);
+    if (j >= 32) sort_step<32>(v, t, k);
+    if (j >= 16) sort_step<16>(v, t, k);
+    if (j >= 8) sort_step<8>(v, t, k);
+    if (j >= 4) sort_step<4>(v, t, k);
+    if (j >= 2) sort_step<2>(v, t, k);
+    sort_step<1>(v, t, k);
   }
 }
 
@@ -383,35 +397,32 @@ struct SampleShared {
   uint64_t pick[4];
 };
 
-// Chooses among the n tokens of the list in LDS, all that may be kept, by their places: k, p, m and u as
-// in the file's heading (k 0: all n). goal: top_p's, where the list is not all the weight there is (0: it is).
+// The place of the last token kept among the n of the list in LDS: the one before which, `before` included,
+// less than goal lies.
 template <int E>
-__device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int n, const RowSettings& s,
-                                      uint64_t goal, int vocab) {
+__device__ __forceinline__ uint64_t last_kept(SampleShared& sm, const Weigh& weigh, int n, uint64_t before,
+                                              uint64_t goal) {
   const int t = threadIdx.x;
-  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);  // the largest logit is finite here
-  uint64_t v[E], w[E], before[E], total = 0, kept = 0, sum;
+  uint64_t v[E], sum, least = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
   __syncthreads();
   sort_block<E>(v, n, sm.list);
-  const int last = s.k ? min(n, (int)s.k) : n;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    w[e] = t + 1024 * e < last ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
-    before[e] = total + scan_block<16>(w[e], sm.red, &sum);
-    total += sum;
+    const uint64_t w = t + 1024 * e < n ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
+    const uint64_t b = before + scan_block<16>(w, sm.red, &sum);
+    before += sum;
+    if (t + 1024 * e < n && b < goal && ~v[e] > least) least = ~v[e];
   }
-  const uint64_t share = goal ? goal : s.p < 1.0 ? mass_goal(s.p, total) : total;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const bool keep = t + 1024 * e < last && (t + 1024 * e == 0 || (before[e] < share && (uint32_t)(v[e] >> 32) >= least));
-    w[e] = keep ? w[e] : 0;
-    scan_block<16>(w[e], sm.red, &sum);
-    kept += sum;
-  }
-  const uint64_t pick = pick_goal(s.u, kept);
-  // In the order of numbers: weights by bins of numbers, then the border's bin, of a 2048th of the vocabulary.
+  return ~max_block<16>(least, sm.red);
+}
+
+// The token at which u falls among those of places v and weights w (0: not kept), in the order of numbers:
+// weights by bins of numbers, then the border's bin, of a 2048th of the vocabulary.
+template <int E>
+__device__ __forceinline__ int by_number(SampleShared& sm, const uint64_t (&v)[E], const uint64_t (&w)[E], double u, int vocab) {
+  const int t = threadIdx.x;
   for (int i = t; i < kBins; i += 1024) sm.mass[i] = 0;
   if (t == 0) sm.n = 0;
   __syncthreads();
@@ -422,7 +433,9 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
     if (w[e]) atomicAdd((unsigned long long*)&sm.mass[bin[e]], (unsigned long long)w[e]);
   }
   __syncthreads();
-  const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = scan_block<16>(m0 + m1, sm.red, &sum);
+  uint64_t kept;
+  const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = scan_block<16>(m0 + m1, sm.red, &kept);
+  const uint64_t pick = pick_goal(u, kept);
   if (b <= pick && b + m0 > pick) sm.pick[0] = 2 * t, sm.pick[1] = b;
   else if (b + m0 <= pick && b + m0 + m1 > pick) sm.pick[0] = 2 * t + 1, sm.pick[1] = b + m0;
   __syncthreads();
@@ -443,53 +456,129 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, int 
   return (int)sm.pick[2];
 }
 
-// Leaves of the n > 1024 tokens on the list those up to the end of the bin in which the k'th lies: 1024 are sorted
-// in 8 us, twice as many in 20. Returns how many there are.
-__device__ __forceinline__ int drop_past(SampleShared& sm, const Bins& bin, int n, uint32_t k) {
+__device__ __forceinline__ uint64_t lane_value64(uint64_t v, int lane) {
+  return join64(__shfl((int)(uint32_t)v, lane), __shfl((int)(v >> 32), lane));
+}
+
+// choose() of up to 64 tokens, by one wave: two sorts and three sums in registers (8 us a row as the file's histograms
+// do it, 6 so).
+__device__ __forceinline__ int choose_few(const uint64_t* list, const Weigh& weigh, int n, const RowSettings& s, uint64_t goal) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);
+  uint64_t v[1] = {lane < n ? list[lane] : 0};
+  sort_lanes(v);
+  const int last = s.k ? min(n, (int)min(s.k, (uint64_t)64)) : n;
+  uint64_t w = lane < last ? weigh.any(value_of((uint32_t)(v[0] >> 32))) : 0;
+  uint64_t sum = wave_scan64(w);
+  const uint64_t total = lane_value64(sum, 63), share = goal ? goal : s.p < 1.0 ? mass_goal(s.p, total) : total;
+  const bool keep = lane < last && (lane == 0 || (sum - w < share && (uint32_t)(v[0] >> 32) >= least));
+  w = keep ? w : 0;
+  const uint64_t pick = pick_goal(s.u, lane_value64(wave_scan64(w), 63));
+  uint64_t by[1] = {keep ? (uint64_t)(uint32_t)v[0] << 32 | (uint32_t)lane : 0};  // by rising number, the kept ones first
+  sort_lanes(by);
+  const uint64_t own = lane_value64(w, (int)(by[0] & 63)), mine = by[0] ? own : 0;
+  sum = wave_scan64(mine);
+  const unsigned long long hit = __ballot(sum > pick && sum - mine <= pick);
+  return token_of((uint64_t)(uint32_t)__shfl((int)(by[0] >> 32), __ffsll(hit) - 1));
+}
+
+// The bin, of values x0 in bin 2 t and x1 in the next, in which their sum reaches goal, and the sum before it.
+__device__ __forceinline__ int border_bin(SampleShared& sm, uint64_t x0, uint64_t x1, uint64_t b, uint64_t goal, uint64_t* before) {
   const int t = threadIdx.x;
-  uint64_t v[2], all;
+  if (b < goal && b + x0 >= goal) sm.pick[0] = 2 * t, sm.pick[1] = b;
+  else if (b + x0 < goal && b + x0 + x1 >= goal) sm.pick[0] = 2 * t + 1, sm.pick[1] = b + x0;
+  __syncthreads();
+  *before = sm.pick[1];
+  return (int)sm.pick[0];
+}
+
+// Chooses among the n tokens of the list in LDS, all that may be kept: k, p, m and u as in the file's heading (k 0:
+// all n). goal: top_p's, where the list is not all the weight there is (0: it is). Each border is found by a
+// histogram of the list over `bin`, and the tokens of its bin alone are sorted: by every wave for itself where they are up
+// to 64 (1100 tokens sorted as a whole 21 us a row, so 15).
+__device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, const Bins& bin, int n, const RowSettings& s,
+                                      uint64_t goal, int vocab) {
+  const int t = threadIdx.x, lane = t & 63;
+  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);  // the largest logit is finite here
+  uint64_t v[2], w[2], sum, before;
+  int at[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
+    at[e] = v[e] ? bin(value_of((uint32_t)(v[e] >> 32))) : kBins;
     sm.count[t + 1024 * e] = 0;
+    sm.mass[t + 1024 * e] = 0;
   }
-  if (t == 0) sm.n = 0, sm.pick[0] = kBins;
-  __syncthreads();
+  // puts the tokens of one bin on the list, side by side: how many
+  auto gather = [&](int border) __attribute__((always_inline)) {
+    if (t == 0) sm.n = 0;
+    __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (v[e]) atomicAdd(&sm.count[bin(value_of((uint32_t)(v[e] >> 32)))], 1u);
-  __syncthreads();
-  const uint32_t c0 = sm.count[2 * t], c1 = sm.count[2 * t + 1];
-  const uint64_t b = scan_block<16>(c0 + c1, sm.red, &all);
-  if (b < k && b + c0 >= k) sm.pick[0] = 2 * t;
-  else if (b + c0 < k && b + c0 + c1 >= k) sm.pick[0] = 2 * t + 1;
-  __syncthreads();
+    for (int e = 0; e < 2; ++e)
+      if (at[e] == border) sm.list[atomicAdd(&sm.n, 1u)] = v[e];
+    __syncthreads();
+    return (int)sm.n;
+  };
+  auto drop = [&](int border, uint64_t cut) __attribute__((always_inline)) {
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (v[e] && bin(value_of((uint32_t)(v[e] >> 32))) <= (int)sm.pick[0]) sm.list[atomicAdd(&sm.n, 1u)] = v[e];
+    for (int e = 0; e < 2; ++e)
+      if (at[e] > border || (at[e] == border && v[e] < cut)) v[e] = 0, at[e] = kBins;
+  };
   __syncthreads();
-  return (int)sm.n;
-}
-
-// The place of the last token kept among the n of the list in LDS: the one before which, `before` included,
-// less than goal lies.
-template <int E>
-__device__ __forceinline__ uint64_t last_kept(SampleShared& sm, const Weigh& weigh, int n, uint64_t before,
-                                              uint64_t goal) {
-  const int t = threadIdx.x;
-  uint64_t v[E], sum, least = 0;
+  if (s.k && (uint64_t)n > s.k) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
-  __syncthreads();
-  sort_block<E>(v, n, sm.list);
+    for (int e = 0; e < 2; ++e)
+      if (v[e]) atomicAdd(&sm.count[at[e]], 1u);
+    __syncthreads();
+    const uint64_t c0 = sm.count[2 * t], c1 = sm.count[2 * t + 1], b = scan_block<16>(c0 + c1, sm.red, &sum);
+    const int border = border_bin(sm, c0, c1, b, s.k, &before);
+    const int m = gather(border), need = (int)(s.k - before);  // of m
+    uint64_t cut;
+    if (m <= 64) {
+      uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
+      sort_lanes(x);
+      cut = join64(__shfl((int)(uint32_t)x[0], need - 1), __shfl((int)(x[0] >> 32), need - 1));
+    } else {
+      uint64_t x[2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const uint64_t w = t + 1024 * e < n ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
-    const uint64_t b = before + scan_block<16>(w, sm.red, &sum);
-    before += sum;
-    if (t + 1024 * e < n && b < goal && ~v[e] > least) least = ~v[e];
+      for (int e = 0; e < 2; ++e) x[e] = t + 1024 * e < m ? sm.list[t + 1024 * e] : 0;
+      __syncthreads();
+      sort_block<2>(x, m, sm.list);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (t + 1024 * e == need - 1) sm.pick[3] = x[e];
+      __syncthreads();
+      cut = sm.pick[3];
+    }
+    drop(border, cut);
   }
-  return ~max_block<16>(least, sm.red);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) w[e] = v[e] ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
+  if (goal || s.p < 1.0) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (w[e]) atomicAdd((unsigned long long*)&sm.mass[at[e]], (unsigned long long)w[e]);
+    __syncthreads();
+    const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = scan_block<16>(m0 + m1, sm.red, &sum);
+    const uint64_t share = goal ? goal : mass_goal(s.p, sum);
+    const int border = border_bin(sm, m0, m1, b, share, &before);
+    const int m = gather(border);
+    uint64_t cut;
+    if (m <= 64) {
+      uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
+      sort_lanes(x);
+      const uint64_t y = lane < m ? weigh.any(value_of((uint32_t)(x[0] >> 32))) : 0;
+      const int last = __popcll(__ballot(lane < m && before + wave_scan64(y) - y < share)) - 1;  // a front of the lanes
+      cut = join64(__shfl((int)(uint32_t)x[0], last), __shfl((int)(x[0] >> 32), last));
+    } else {
+      cut = last_kept<2>(sm, weigh, m, before, share);
+    }
+    drop(border, cut);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) w[e] = v[e] && (uint32_t)(v[e] >> 32) >= least ? w[e] : 0;
+  __syncthreads();
+  return by_number<2>(sm, v, w, s.u, vocab);
 }
 
 // The sum of value(i, x) over chunk c, by one wave.
@@ -982,7 +1071,7 @@ __global__ __launch_bounds__(256) void sample_border_kernel(SampleArgs a) {
 // a list of their own those ahead of it, as long as they are few.
 template <int DT>
 __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
-  __shared__ uint64_t list[2][kList];
+  __shared__ uint64_t list[2][kFew];
   __shared__ uint32_t have[2], base[2];
   const int r = blockIdx.x / a.splits, at = blockIdx.x % a.splits;
   const RowSettings s = settings(a, r);
@@ -999,7 +1088,7 @@ __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
   if (threadIdx.x < 2) have[threadIdx.x] = 0;
   __syncthreads();
   row.each(g0 + threadIdx.x, 256, g1, [&](int unit, const u32x4& u, int) {
-    const float end = *(volatile uint32_t*)&have[1] > kList ? high : __builtin_inff();
+    const float end = *(volatile uint32_t*)&have[1] > kFew ? high : __builtin_inff();
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const float x = RowReader<DT>::raw(u, j);
@@ -1007,16 +1096,25 @@ __global__ __launch_bounds__(256) void sample_collect_kernel(SampleArgs a) {
       const uint32_t k = key_of(x + 0.0f);
       const int which = k > to;
       const uint32_t n = atomicAdd(&have[which], 1u);
-      if (n < kList) list[which][n] = place(k, unit * E - row.off + j);
+      const uint64_t p = place(k, unit * E - row.off + j);
+      if (n < kFew) {
+        list[which][n] = p;
+      } else if (!which) {  // LDS is full: one by one
+        const uint32_t at = atomicAdd(&w.n, 1u);
+        if (at < kList) w.list[at] = p;
+      }
     }
   });
   __syncthreads();
   // the row's lists: room for the workgroup's tokens, then they
-  if (threadIdx.x < 2) base[threadIdx.x] = have[threadIdx.x] ? atomicAdd(threadIdx.x ? &w.ahead : &w.n, have[threadIdx.x]) : 0;
+  if (threadIdx.x < 2) {
+    const uint32_t n = threadIdx.x ? have[1] : min(have[0], (uint32_t)kFew);
+    base[threadIdx.x] = n ? atomicAdd(threadIdx.x ? &w.ahead : &w.n, n) : 0;
+  }
   __syncthreads();
 #pragma unroll
   for (int x = 0; x < 2; ++x)
-    for (uint32_t i = threadIdx.x; i < min(have[x], (uint32_t)kList) && base[x] + i < kList; i += 256)
+    for (uint32_t i = threadIdx.x; i < min(have[x], (uint32_t)kFew) && base[x] + i < (x ? kFew : kList); i += 256)
       w.list[x * kList + base[x] + i] = list[x][i];
 }
 
@@ -1052,8 +1150,8 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
       scan_block<16>(mine, sm.red, &all);
       token = find<DT>(a, sm, row, pick_goal(s.u, all), [&](int, float x) { return weigh(x >= from ? x : kDead); });
     } else {
-      const bool some = n + ahead <= kList;  // all that may be kept is at hand
-      int have = (int)(some ? n + ahead : n);
+      const bool some = s.kind == kFront || n + ahead <= kFew;  // all that may be kept is at hand
+      const int have = (int)(some ? n + ahead : n);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t i = threadIdx.x + 1024 * e;
@@ -1067,12 +1165,10 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
         if (threadIdx.x == 0) w.cut = cut, w.least_kept = least;
         return;
       }
-      if (s.kind == kFront && have > 1024) {
-        have = drop_past(sm, Bins(range.top, value_of(w.from), a.shift, __builtin_inf()), have, (uint32_t)s.k);
-      }
       // what is on the lists is not all the row's weight, but the border's goal is of that
       const uint64_t goal = s.kind == kShare ? w.goal : 0;
-      token = have > 1024 ? choose<2>(sm, weigh, have, s, goal, a.vocab) : choose<1>(sm, weigh, have, s, goal, a.vocab);
+      if (have <= 64) token = choose_few(sm.list, weigh, have, s, goal);
+      else token = choose(sm, weigh, Bins(range.top, value_of(w.from), a.shift, __builtin_inf()), have, s, goal, a.vocab);
     }
   }
   if (threadIdx.x == 0) a.token[r] = token, w.done = 1;
