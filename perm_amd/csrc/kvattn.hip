@@ -647,15 +647,16 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   extern __shared__ __align__(16) uint8_t lds[];     // [3][BUF], then [4 waves][NC][64 lanes][16]
   const KvCacheArgs& c = a.c;
   const int h = (int)(blockIdx.x % c.heads);
-  // MODE > 0: all first splits, then all second ones ..., as many have nothing to do where masks leave little. A
-  // launch deals its workgroups to the shader engines in turn: with an even number of splits side by
-  // side, the full ones would be on half of them (two rows of documents of up to 8192 tokens in four
-  // splits of at least 16 tiles 483 us, so 220).
-  const int split = (int)(MODE ? blockIdx.x / c.heads / items : blockIdx.x / c.heads % a.splits);
+  // MODE > 0: an item's splits begin at another one than the item's before, as many have nothing to do where masks
+  // leave little. A launch deals its workgroups to the shader engines in turn: with an even number of
+  // splits the full ones would be on half of them (two sequences of documents, 8192 rows, in four splits of
+  // at least 16 tiles 483 us; all first splits ahead of all second ones 220, but 2162 rows on 4096 tokens in
+  // three full splits 204 that way, 188 this one).
+  const int split = (int)((blockIdx.x / c.heads + (MODE ? blockIdx.x / c.heads / a.splits : 0)) % a.splits);
   int b, item, n_b;
   int64_t row0;
   // last items first: causal rows at the end of a prompt see the most tokens
-  const int from_end = items - 1 - (int)(MODE ? blockIdx.x / c.heads % items : blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
+  const int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
   if (!kv_locate(bt, from_end, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b,
                  &item, &row0, &n_b, each_of(ext)))
     return attn_unowned<DT>(a, ext, bt, item, items - from_end + item, piece, 0, 0);
