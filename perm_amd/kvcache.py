@@ -207,6 +207,9 @@ def _more(desc, table, rows, heads, device, softcap, slopes, first, prefix, shar
         if groups == 0 or batch % groups:
             raise ValueError(f"{batch} sequences in {groups} groups")
     keep = slopes, first, prefix, shared
+    for t in keep:
+        if t is not None and t.device != device:
+            raise ValueError(f"an argument on {t.device}, q on {device}")
     return _lib.KvMore(softcap, *(None if t is None else t.data_ptr() for t in keep), groups), keep
 
 

@@ -36,10 +36,12 @@ def new(pages, device="cuda"):
     return torch.zeros((pages,), dtype=torch.int32, device=device)
 
 
-def _ints(t, dims, what, size=None):
+def _ints(t, dims, what, device, size=None):
     """An int32 CUDA tensor of ``dims`` dimensions (of ``size``, where it has one)."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ValueError(f"{what} must be a CUDA tensor")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not {device}")
     if t.dtype != torch.int32 or t.dim() != dims:
         raise IndexError(f"{what} must be int32 with {dims} dimension(s), got {t.dtype} "
                          f"{tuple(t.shape)}")
@@ -51,11 +53,9 @@ def _ints(t, dims, what, size=None):
 def _books(refs, table):
     """The two checked: they are changed in place, so neither is copied."""
     for t, dims, what in ((refs, 1, "refs"), (table, 2, "table")):
-        if _ints(t, dims, what) is not t:
+        if _ints(t, dims, what, getattr(refs, "device", None)) is not t:
             raise ValueError(f"{what} is changed in place and must be contiguous")
     _lib.here(refs.device)
-    if table.device != refs.device:
-        raise ValueError(f"refs on {refs.device}, table on {table.device}")
     return refs.data_ptr(), refs.shape[0], table.data_ptr(), table.shape[0], table.shape[1]
 
 
@@ -73,9 +73,9 @@ def fork(refs, table, lens, parents, children, block):
     children's lengths are the caller's to set."""
     lib = _lib.load()
     books = _books(refs, table)
-    lens = _ints(lens, 1, "lens", table.shape[0])
-    children = _ints(children, 1, "children")
-    parents = _ints(parents, 1, "parents", children.shape[0])
+    lens = _ints(lens, 1, "lens", refs.device, table.shape[0])
+    children = _ints(children, 1, "children", refs.device)
+    parents = _ints(parents, 1, "parents", refs.device, children.shape[0])
     _lib.check(lib.cp_kv_fork(*books, lens.data_ptr(), _block(block), parents.data_ptr(),
                               children.data_ptr(), children.shape[0], _lib.stream_ptr()))
 
@@ -94,10 +94,10 @@ def grow(refs, table, filled, new, block):
     lib = _lib.load()
     books = _books(refs, table)
     batch = table.shape[0]
-    filled = _ints(filled, 1, "filled", batch)
+    filled = _ints(filled, 1, "filled", refs.device, batch)
     each = 0
     if isinstance(new, torch.Tensor):
-        new = _ints(new, 1, "new", batch)
+        new = _ints(new, 1, "new", refs.device, batch)
     else:
         each, new = operator.index(new), None
         if not 0 <= each < 2 ** 31:
@@ -117,7 +117,7 @@ def free(refs, table, rows=None):
     lib = _lib.load()
     books = _books(refs, table)
     if rows is not None:
-        rows = _ints(rows, 1, "rows")
+        rows = _ints(rows, 1, "rows", refs.device)
         if rows.shape[0] == 0:
             return
     _lib.check(lib.cp_kv_free(*books, _lib.ptr(rows), 0 if rows is None else rows.shape[0],
@@ -147,8 +147,11 @@ def copy(cache, src, dst, into=None):
     lib = _lib.load()
     desc = _desc(cache)
     to = desc if into is None else _desc(into)
-    src = _ints(src, 1, "src")
-    dst = _ints(dst, 1, "dst", src.shape[0])
-    _lib.here(cache[0].device)
+    device = cache[0].device
+    _lib.here(device)
+    if into is not None and into[0].device != device:
+        raise ValueError(f"a cache on {device} into one on {into[0].device}")
+    src = _ints(src, 1, "src", device)
+    dst = _ints(dst, 1, "dst", device, src.shape[0])
     _lib.check(lib.cp_kv_copy(ctypes.byref(desc), ctypes.byref(to), src.data_ptr(), dst.data_ptr(),
                               src.shape[0], _lib.stream_ptr()))

@@ -27,11 +27,11 @@ from . import _lib
 from .mxfp4 import DTYPES
 
 
-def _setting(v, rows, dtype, what, low, high):
+def _setting(v, rows, dtype, what, low, high, device):
     """(tensor or None, number): a setting of each row, or one for all."""
     if isinstance(v, torch.Tensor):
-        if not v.is_cuda:
-            raise ValueError(f"{what} must be a number or on the GPU")
+        if v.device != device:
+            raise ValueError(f"{what} must be a number or on {device}")
         if v.dtype != dtype or v.shape != (rows,):
             raise ValueError(f"{what} of each row must be {dtype} [{rows}], got {v.dtype} "
                              f"{tuple(v.shape)}")
@@ -55,22 +55,23 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         raise ValueError("logits must be on the GPU")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocab], got {tuple(logits.shape)}")
-    _lib.here(logits.device)
+    dev = logits.device
+    _lib.here(dev)
     rows, vocab = logits.shape
-    if not (isinstance(u, torch.Tensor) and u.is_cuda) or u.shape != (rows,):
-        raise ValueError(f"u must be a CUDA tensor [{rows}]")
+    if not isinstance(u, torch.Tensor) or u.device != dev or u.shape != (rows,):
+        raise ValueError(f"u must be a tensor [{rows}] on {dev}")
     if u.dtype not in (torch.float32, torch.float64):
         raise TypeError(f"u must be float32 or float64, got {u.dtype}")
-    t, t_all = _setting(temperature, rows, torch.float32, "temperature", 0.0, float("inf"))
-    k, k_all = _setting(top_k, rows, torch.int32, "top_k", 0, 2 ** 31 - 1)
-    p, p_all = _setting(top_p, rows, torch.float32, "top_p", 0.0, 1.0)
-    m, m_all = _setting(min_p, rows, torch.float32, "min_p", 0.0, 1.0)
-    if logits.stride(1) != 1 and vocab > 1 or rows > 1 and logits.stride(0) < 0:
+    t, t_all = _setting(temperature, rows, torch.float32, "temperature", 0.0, float("inf"), dev)
+    k, k_all = _setting(top_k, rows, torch.int32, "top_k", 0, 2 ** 31 - 1, dev)
+    p, p_all = _setting(top_p, rows, torch.float32, "top_p", 0.0, 1.0, dev)
+    m, m_all = _setting(min_p, rows, torch.float32, "min_p", 0.0, 1.0, dev)
+    if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
     u = u.contiguous()
     token = logits.new_empty((rows,), dtype=torch.int32)
     nws = lib.cp_sample_ws_bytes(rows, vocab)
-    ws = _lib.workspace(nws, logits.device)
+    ws = _lib.workspace(nws, dev)
     _lib.check(lib.cp_sample(logits.data_ptr(), code, rows, vocab, logits.stride(0), u.data_ptr(),
                              int(u.dtype == torch.float64), _lib.ptr(t), t_all, _lib.ptr(k), k_all,
                              _lib.ptr(p), p_all, _lib.ptr(m), m_all, token.data_ptr(),
