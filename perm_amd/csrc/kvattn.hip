@@ -76,6 +76,7 @@ struct AttnMore {
   const float* slopes;     // [q heads]
   float cap, inv;          // cap * log2 e (0: none), and 1 over it
   int series;              // a large cap
+  int *cost, *order;       // [items]: tiles of the row tiles of 128, and these by falling cost (null: as they come)
 };
 struct AttnPlain {};
 template <int MODE>
@@ -656,7 +657,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   int b, item, n_b;
   int64_t row0;
   // last items first: causal rows at the end of a prompt see the most tokens
-  const int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits), piece = h * a.splits + split;
+  int from_end = items - 1 - (int)(blockIdx.x / c.heads / a.splits);
+  if constexpr (MODE > 0) {
+    if (ext.order) from_end = ext.order[blockIdx.x / c.heads / a.splits];
+  }
+  const int piece = h * a.splits + split;
   if (!kv_locate(bt, from_end, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b,
                  &item, &row0, &n_b, each_of(ext)))
     return attn_unowned<DT>(a, ext, bt, item, items - from_end + item, piece, 0, 0);
@@ -1435,6 +1440,68 @@ __global__ __launch_bounds__(256) void attn_join_kernel(SplitParts sp, int64_t r
   if (lse && c == 0) lse[row] = row_lse(mm, ll);
 }
 
+// The row tiles of attn_many_kernel by falling number of token tiles. Masks leave each its own, and a launch
+// that starts long ones late ends with those alone: two sequences of documents, 1048 workgroups of very different
+// numbers of tiles, take 235 us in the rows' order, the CUs busy for 62 % of them, and 172 in this one with the 4.8
+// and 4.9 us of the two launches that find it. Here a wave a row tile counts.
+__global__ __launch_bounds__(256) void attn_cost_kernel(AttnArgs a, KvBatch bt, int items, AttnMore x) {
+  const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (at >= items) return;
+  int b, item, n_b, tiles = 0;
+  int64_t row0;
+  if (kv_locate(bt, at, [&](int, int n) { return (int)(((int64_t)n * a.group + kManyRows - 1) / kManyRows); }, &b, &item,
+                &row0, &n_b) &&
+      row0 >= 0 && row0 + n_b <= a.rows) {
+    int lo = 0x7FFFFFFF, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = (int64_t)item * kManyRows + 64 * i + lane;
+      const SeenRow s = seen_row(a, x, bt, r < (int64_t)n_b * a.group, row0 + r / a.group, b, row0, n_b);
+      if (s.hi > s.lo) lo = min(lo, s.lo), hi = max(hi, s.hi);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      lo = min(lo, __shfl_xor(lo, s));
+      hi = max(hi, __shfl_xor(hi, s));
+    }
+    tiles = hi > lo ? (hi + kTile - 1) / kTile - lo / kTile : 0;
+  }
+  if (lane == 0) x.cost[at] = tiles;
+}
+
+// Sorted by counting, in 1024 steps of the largest; items of one step in any order, which changes when they run and
+// nothing else.
+__global__ __launch_bounds__(1024) void attn_order_kernel(int items, AttnMore x) {
+  __shared__ int count[1024], red[16];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  int most = 0;
+  for (int i = t; i < items; i += 1024) most = max(most, x.cost[i]);
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) most = max(most, __shfl_xor(most, s));
+  if (lane == 0) red[wave] = most;
+  count[t] = 0;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) most = max(most, red[w]);
+  __syncthreads();
+  int shift = 0;
+  while (most >> shift > 1023) ++shift;
+  for (int i = t; i < items; i += 1024) atomicAdd(&count[1023 - (x.cost[i] >> shift)], 1);
+  __syncthreads();
+  int sum = count[t];
+  const int own = sum;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int o = __shfl_up(sum, s);
+    if (lane >= s) sum += o;
+  }
+  if (lane == 63) red[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += red[w];
+  count[t] = sum - own;  // where the step begins
+  __syncthreads();
+  for (int i = t; i < items; i += 1024) x.order[atomicAdd(&count[1023 - (x.cost[i] >> shift)], 1)] = i;
+}
+
 struct AttnPlan {
   bool many;
   int64_t items;  // upper bound of the batch's row tiles, and one more where rows may have no sequence
@@ -1556,11 +1623,25 @@ static SharedPlan shared_plan(int64_t rows, int64_t batch, int64_t groups, bool 
           attn_plan(rows, batch, ragged, group, heads, d, cap, window)};
 }
 
+// Whether a call's row tiles are put in order first: two rounds of workgroups or more, and an upper bound of the
+// pairs of rows and tokens that takes twenty times as long as the ordering. (One sequence whose rows begin at one
+// token is in order from its end; where masks leave much less than the bound, the ordering's 10 us stand beside
+// the less that it can win.)
+static bool attn_ordered(const AttnPlan& p, int64_t rows, int group, int heads, int64_t cap, int window) {
+  return p.many && p.items * heads >= 1024 &&
+         (double)rows * group * heads * (window > 0 ? std::min(cap, (int64_t)window + kManyRows) : cap) > 1 << 28;
+}
+
 template <int DT, int MODE>
 static int attn_run_more(AttnArgs a, KvBatch b, AttnMore x, const AttnPlan& p, const SharedPlan& sp, int groups,
                          hipStream_t st) {
   if (!x.shared) {
     x.slots = a.splits = p.splits, a.least = p.least;
+    if (x.order) {
+      attn_cost_kernel<<<dim3((unsigned)((p.items + 3) / 4)), 256, 0, st>>>(a, b, (int)p.items, x);
+      attn_order_kernel<<<dim3(1), 1024, 0, st>>>((int)p.items, x);
+      CP_LAUNCHED("order of the cache attention's rows");
+    }
     const int s = attn_launch_d<DT, MODE>(a, b, p, x, st);
     return s || a.splits == 1 ? s : attn_join<DT, false>(a, a.splits, 0, st);
   }
@@ -1648,10 +1729,15 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
 
 size_t cp_kv_attention_more_ws_bytes(const cp_kv_cache* cache, int64_t rows, int q_heads, int64_t batch,
                                      int64_t max_pages, int ragged, int window, int64_t groups) {
-  if (groups <= 0) return cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, ragged, window);
-  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 1 || max_pages < 1) return 0;
-  const cp::SharedPlan p = cp::shared_plan(rows, batch, groups, ragged != 0, q_heads / cache->heads, cache->heads,
-                                           cache->head_dim, max_pages * cache->block, window);
+  if (!cache || cache->heads < 1 || rows < 1 || q_heads < 1 || batch < 0 || max_pages < 1) return 0;
+  const int group = q_heads / cache->heads;
+  const int64_t cap = max_pages * cache->block;
+  if (groups <= 0 || batch < 1) {
+    const cp::AttnPlan p = cp::attn_plan(rows, batch, ragged != 0, group, cache->heads, cache->head_dim, cap, window);
+    const size_t order = cp::attn_ordered(p, rows, group, cache->heads, cap, window) ? 2 * (size_t)p.items * 4 : 0;
+    return order + cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, ragged, window);
+  }
+  const cp::SharedPlan p = cp::shared_plan(rows, batch, groups, ragged != 0, group, cache->heads, cache->head_dim, cap, window);
   return (size_t)rows * q_heads * ((size_t)(p.front.splits + p.rest.splits) * (cache->head_dim + 2) + 2) * 4;
 }
 
@@ -1717,6 +1803,10 @@ int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row,
   x.cap = more->softcap * cp::kLog2e;
   x.inv = more->softcap > 0.0f ? 1.0f / x.cap : 0.0f;
   x.series = more->softcap > 128.0f;
+  if (!two && (batch > 1 || more->first) && cp::attn_ordered(p, rows, group, cache->heads, cap, window)) {  // behind the splits' sums
+    x.cost = (int*)((char*)ws + cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window));
+    x.order = x.cost + p.items;
+  }
   const cp::KvBatch b = {offsets, (int)batch};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CP_BF16)

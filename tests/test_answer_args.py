@@ -114,3 +114,7 @@ def test_workspaces_of_common_pages(lib):  # noqa: F811
     # two phases: two splits of every row and head at the least, and two counts
     assert lib.cp_kv_attention_more_ws_bytes(c, 64, 4, 64, 1, 0, 0, 1) >= 64 * 4 * (2 * (64 + 2) + 2) * 4
     assert lib.cp_kv_attention_more_ws_bytes(c, 0, 4, 64, 1, 0, 0, 1) == 0
+    # many rows of many tokens: their row tiles in order, two numbers for each
+    more = lib.cp_kv_attention_more_ws_bytes(c, 40000, 4, 2, 1024, 1, 0, 0)
+    tiles = (40000 * 2) // 128 + 2 + 1
+    assert more - lib.cp_kv_attention_ws_bytes(c, 40000, 4, 2, 1024, 1, 0) == 8 * tiles

@@ -246,6 +246,40 @@ def test_many_rows_that_hide_nan(kv):  # noqa: F811
             _check(kv, c, o, table, lens, counts, hq, torch.bfloat16, rng, first=first, shared=shared, **more)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("scores", [dict(), dict(softcap=20.0), dict(slopes=True)], ids=str)
+def test_row_tiles_in_order_of_their_work(kv, scores, dtype):  # noqa: F811
+    """Thousands of rows under a table for thousands of tokens, whose row tiles run in another order: what the
+    same call gives under a narrow table, and the definition. Rows of no sequence and empty rows among them."""
+    rng = np.random.default_rng(17)
+    hq, width = 16, 32
+    scores = dict(scores)
+    if scores.get("slopes"):
+        scores["slopes"] = _slopes(hq)
+    counts = [500, 0, 1, 300, 128, 33, 500] + [int(x) for x in rng.integers(200, 480, 26)]
+    lens = [int(rng.integers(n, 513)) if n else 0 for n in counts]
+    c, o, table = _filled_cache(kv, rng, lens, 4, 64, 16)
+    narrow = np.full((len(lens), width), -1, np.int32)
+    narrow[:, :table.shape[1]] = table[:, :width]
+    wide = np.full((len(lens), 160), -1, np.int32)
+    wide[:, :width] = narrow
+    rows = sum(counts)
+    # past 2^28 pairs under the wide table and not under the narrow one, and four workgroups a CU in both
+    assert rows * hq * 160 * 16 > 1 << 28 > rows * hq * width * 16 and rows * 4 // 128 * 4 >= 1024
+    first = np.concatenate([np.maximum.accumulate(rng.integers(0, 2, n) * (np.arange(n) + m - n)) if i % 3 else
+                            rng.integers(0, 520, n) for i, (n, m) in enumerate(zip(counts, lens))]).astype(np.int64)
+    q = torch.from_numpy(rng.standard_normal((rows + 300, hq, 64))).to(dtype).cuda()
+    args = {k: torch.tensor(v, dtype=torch.float32, device="cuda") if k == "slopes" else v for k, v in scores.items()}
+    for begin in (first, np.zeros_like(first)):
+        more = dict(first=_i32(np.concatenate([begin, np.zeros(300, np.int64)])), **args)
+        a, al = kv.attention(q, c, _i32(narrow), _i32(lens), _offsets(counts), return_lse=True, **more)
+        b, bl = kv.attention(q, c, _i32(wide), _i32(lens), _offsets(counts), return_lse=True, **more)
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16)) and torch.equal(al, bl)
+        assert not bool(b[rows:].any())
+    some = slice(0, 7)
+    _check(kv, c, o, wide[some], lens[some], counts[some], hq, dtype, rng, first=first[:sum(counts[some])], **scores)
+
+
 def test_values_under_scales_far_apart(kv):  # noqa: F811
     """V scales from 2^-30 to 2^7 in and past the common pages, scores of hundreds."""
     rng = np.random.default_rng(7)
