@@ -182,6 +182,7 @@ struct RowSettings {
 __device__ __forceinline__ RowSettings settings(const SampleArgs& a, int r) {
   RowSettings s;
   s.t = a.temperature ? (double)a.temperature[r] : a.t;
+  if (s.t > 0.0) s.t = fmax(s.t, 1e-290);  // 1 / T stays finite; logits 2^-149 apart already weigh 0 there
   s.p = a.top_p ? (double)a.top_p[r] : a.p;
   const double m = a.min_p ? (double)a.min_p[r] : a.m;
   s.m = m > 0.0 ? fmin(m, 1.0) : 0.0;
@@ -1239,7 +1240,7 @@ __global__ __launch_bounds__(1024) void sample_last_kernel(SampleArgs a) {
   if (threadIdx.x == 0) a.token[r] = token;
 }
 
-constexpr int64_t kRowsAtOnce = 1024;  // rows of a batch of launches: 80 MB of workspace
+constexpr int64_t kRowsAtOnce = 1024;  // rows of a batch of launches: 68 MB of workspace
 
 // Workgroups of a row at most: enough for every CU, and several for the rows with more to do.
 static int64_t most_splits(int64_t rows) { return std::min((int64_t)kSplits, std::max(2048 / rows, (int64_t)4)); }

@@ -125,6 +125,17 @@ def test_extremes(sampling, dtype):
         _check(sampling, x, u, **settings)
 
 
+def test_temperatures_whose_reciprocal_is_no_number(sampling):
+    """Numbers for all rows come in double precision: the largest logits alone weigh, all the same."""
+    x, u = _logits(11, 6, 5000, torch.float32)
+    x[3, [7, 70, 700]] = 100.0
+    for t in (5e-324, 1e-320, 1e-308, 1e-291):
+        for more in (dict(), dict(top_p=0.9), dict(top_k=5), dict(top_k=2000), dict(min_p=0.5)):
+            got = sampling.sample(x, u, temperature=t, **more)
+            assert torch.equal(x.gather(1, got.long()[:, None])[:, 0], x.amax(1)), (t, more)
+            assert torch.equal(got, sampling.sample(x, u, temperature=1e-30, **more)), (t, more)
+
+
 def test_numbers_at_the_ends_of_their_range(sampling):
     x, _ = _logits(9, 6, 5000, torch.float32)
     u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 0.5, 0.25, 1.0, float("nan")], device="cuda")
