@@ -75,7 +75,7 @@ struct AttnMore {
   int slot0, slots;        // where this phase's splits lie among a row's
   const float* slopes;     // [q heads]
   float cap, inv;          // cap * log2 e (0: none), and 1 over it
-  int series;              // a large cap
+  int series;              // a large cap, or a scale under which cap over scale is none
   int *cost, *order;       // [items]: tiles of the row tiles of 128, and these by falling cost (null: as they come)
 };
 struct AttnPlain {};
@@ -177,7 +177,8 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 // them have |z| <= 0.6, where tanh(z) / z = 1 + z^2 p(z^2) within 2^-23.5 (p found by exchange): seven
 // operations. Elsewhere tanh z = 1 - 2 / (1 + e^2z), two of whose five steps run at a quarter of
 // the rate; it errs by 1.5 x 2^-23, a score by cap times that: up to caps of 128 no more than 2^-15
-// of a weight. Under larger ones small scores take the first way one by one.
+// of a weight. Under larger ones small scores take the first way one by one, and under scales so
+// small that cap / kc may be infinite, which only infinite products leave.
 template <int N, class V>
 __device__ __forceinline__ void cap_scores(const AttnMore& x, V& v, float kc, bool small) {
   const float kz = kc * x.inv;
@@ -1802,7 +1803,7 @@ int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row,
   x.slopes = more->slopes;
   x.cap = more->softcap * cp::kLog2e;
   x.inv = more->softcap > 0.0f ? 1.0f / x.cap : 0.0f;
-  x.series = more->softcap > 128.0f;
+  x.series = more->softcap > 128.0f || scale < 1e-12f;
   if (!two && (batch > 1 || more->first) && cp::attn_ordered(p, rows, group, cache->heads, cap, window)) {  // behind the splits' sums
     x.cost = (int*)((char*)ws + cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window));
     x.order = x.cost + p.items;

@@ -227,6 +227,31 @@ def test_unseen_tokens_do_not_reach_a_row(kv):  # noqa: F811
             _check(kv, c, o, table, lens, counts, 4, dtype, rng, first=first, shared=shared, **more)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("many", [False, True])
+def test_an_infinite_query_stays_in_its_row(kv, many, dtype):  # noqa: F811
+    """Infinities and NaN in some queries, under caps and scales of every size: the other rows are as without."""
+    rng = np.random.default_rng(12)
+    lens, counts = ([2500], [700]) if many else ([100, 40], [9, 1])
+    c, o, table = _filled_cache(kv, rng, lens, 1, 64, 16)
+    rows, hq = sum(counts), 12
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 64))).to(dtype).cuda()
+    bad = q.clone()
+    bad[1, 3, 5], bad[4, 0, 0], bad[4, 7, 1] = float("inf"), float("-inf"), float("nan")
+    left = torch.ones((rows, hq), dtype=torch.bool, device="cuda")
+    left[1, 3] = left[4, 0] = left[4, 7] = False
+    if many:
+        _many(c, counts, hq, table)
+    for scale, cap, slopes in itertools.product((None, 1e-13, 1e-30, 1e-37), (0.5, 30.0, 1000.0, 1e29), (None, True)):
+        more = dict(scale=scale, softcap=cap, slopes=slopes and torch.tensor(_slopes(hq), device="cuda"))
+        a = kv.attention(q, c, _i32(table), _i32(lens), _offsets(counts), **more)
+        b = kv.attention(bad, c, _i32(table), _i32(lens), _offsets(counts), **more)
+        assert bool(torch.isfinite(b[left]).all()), (scale, cap)
+        # where all are small they take the shorter way together; two ways differ by less than a result's rounding
+        tol = 4 * HALF_ULP[dtype] * float(a.double().abs().max())
+        assert float((a[left].double() - b[left].double()).abs().max()) <= tol, (scale, cap)
+
+
 def test_many_rows_that_hide_nan(kv):  # noqa: F811
     """The same in tiles of 128 rows."""
     rng = np.random.default_rng(9)
