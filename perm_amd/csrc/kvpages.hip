@@ -164,7 +164,7 @@ __device__ __forceinline__ T scan1024(T v, T* sm, T* total) {
   return base + sum - v;
 }
 
-// One workgroup does it all, phase by phase. 1: every sequence's wants, a wave each. 2: their sums
+// One workgroup does it all, phase by phase. 1: every sequence's wants. 2: their sums
 // in order, and which sequences are served: those up to the first whose sum passes the free pages.
 // 3: the free pages in order. 4: entries. 5: holders, once nobody reads them any more.
 __global__ __launch_bounds__(1024) void kv_grow_kernel(GrowArgs a) {
@@ -218,13 +218,22 @@ __global__ __launch_bounds__(1024) void kv_grow_kernel(GrowArgs a) {
   }
   __syncthreads();
   const int given = sm_given;
-  // the first `given` free pages, a wave a block
+  // the first `given` free pages: 64 blocks' counts at a time, a wave a block that has any (294912 pages with
+  // the last 300 free: block by block 66 us, so 18)
   int before = 0;
-  for (int at = 0; at < a.blocks && before < given; ++at) {
-    const int here = min(k.pages - at * kPagesBlock, kPagesBlock) - a.counts[at];
-    if (at % 16 == wave && here > 0) {
+  for (int at0 = 0; at0 < a.blocks && before < given; at0 += 64) {
+    const int own = at0 + lane < a.blocks ? min(k.pages - (at0 + lane) * kPagesBlock, kPagesBlock) - a.counts[at0 + lane] : 0;
+    int sum = own;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int o = __shfl_up(sum, s);
+      if (lane >= s) sum += o;
+    }
+    for (unsigned long long left = __ballot(own > 0) & 0x0001000100010001ull << wave; left; left &= left - 1) {
+      const int l = __ffsll(left) - 1, at = at0 + l;
+      int r = before + __shfl(sum - own, l);
+      if (r >= given) break;
       const uint32_t bits = in_use(k, at);
-      int r = before;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const bool fr = !(bits >> i & 1);
@@ -234,7 +243,7 @@ __global__ __launch_bounds__(1024) void kv_grow_kernel(GrowArgs a) {
         r += __popcll(m);
       }
     }
-    before += here;
+    before += __shfl(sum, 63);
   }
   __syncthreads();
   for_sequences(a, [&](int b, const GrowRange& g, int at, int by, int64_t end) {

@@ -69,7 +69,7 @@ def fork(refs, table, lens, parents, children, block):
     """Row children[i] of the table becomes row parents[i] as far as its lens[parents[i]] tokens
     go, and -1 past them; the pages gain a holder each. parents and children: int32 [n]. A child's row
     should hold no pages (``free`` it first), is named once and is no parent of the same call.
-    Numbers that are no row of the table are left out. lens (int32 [batch]) is read alone: the
+    Numbers that are no row of the table are left out, and a row into itself. lens (int32 [batch]) is read alone: the
     children's lengths are the caller's to set."""
     lib = _lib.load()
     books = _books(refs, table)
