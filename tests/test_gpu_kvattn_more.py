@@ -227,6 +227,41 @@ def test_unseen_tokens_do_not_reach_a_row(kv):  # noqa: F811
             _check(kv, c, o, table, lens, counts, 4, dtype, rng, first=first, shared=shared, **more)
 
 
+def test_ordered_calls_captured_and_on_streams(kv):  # noqa: F811
+    """Calls whose row tiles are put in order: replayed under other documents and lengths, and two at once."""
+    rng = np.random.default_rng(18)
+    counts, lens = [4000, 300, 4000], [4000, 900, 4090]
+    c, o, table = _filled_cache(kv, rng, lens, 4, 64, 16)
+    rows, hq = sum(counts), 16
+    assert rows * hq * table.shape[1] * 16 > 1 << 28 and rows * 4 // 128 * 4 >= 1024
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 64))).to(torch.bfloat16).cuda()
+    table, held, off = _i32(table), _i32(lens), _offsets(counts)
+    first = _i32(rng.integers(0, 4000, rows))
+
+    def call():
+        return kv.attention(q, c, table, held, off, first=first, softcap=20.0)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    alone = call()
+    torch.cuda.synchronize()
+    both = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            both.append([call() for _ in range(3)])
+    torch.cuda.synchronize()
+    for x in (*both[0], *both[1]):
+        assert torch.equal(x.view(torch.int16), alone.view(torch.int16))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got.view(torch.int16), call().view(torch.int16)), i
+        held -= 50
+        first.copy_(_i32(np.sort(rng.integers(0, 4000 >> i, rows))))
+
+
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("many", [False, True])
 def test_an_infinite_query_stays_in_its_row(kv, many, dtype):  # noqa: F811

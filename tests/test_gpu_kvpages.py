@@ -237,6 +237,34 @@ def test_graph_replays(mods):
         new[2] += 3
 
 
+def test_books_on_two_streams(mods):
+    """Two pairs of books at once, each on a stream of its own."""
+    _, kp = mods
+    rng = np.random.default_rng(4)
+    streams, runs = [torch.cuda.Stream() for _ in range(2)], []
+    inputs = [[_i32(rng.integers(0, 300, 40)) for _ in range(6)] for _ in streams]
+    rows = [_i32(rng.permutation(40)[:9]) for _ in range(6)]
+    torch.cuda.synchronize()
+
+    def run(new):
+        refs, table = kp.new(3000), torch.full((40, 130), -1, dtype=torch.int32, device="cuda")
+        lens, outs = torch.zeros(40, dtype=torch.int32, device="cuda"), []
+        for n, r in zip(new, rows):
+            outs += kp.grow(refs, table, lens, n, 16)
+            lens = lens + n
+            kp.free(refs, table, r)
+            lens.index_fill_(0, r.long(), 0)
+            outs += kp.compact(refs, table)
+        return [refs, table, *outs]
+    for s, new in zip(streams, inputs):
+        with torch.cuda.stream(s):
+            runs.append([run(new) for _ in range(2)])
+    torch.cuda.synchronize()
+    for got, new in zip(runs, inputs):
+        for want, *both in zip(run(new), *got):
+            assert all(torch.equal(want, t) for t in both)
+
+
 def test_refusals(mods, monkeypatch):
     kv, kp = mods
     refs, table = kp.new(8), torch.full((2, 4), -1, dtype=torch.int32, device="cuda")

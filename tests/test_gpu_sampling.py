@@ -213,6 +213,21 @@ def test_graph_replays(sampling):
         t.mul_(0.8)
 
 
+def test_two_streams_at_once(sampling):
+    x, u = _logits(12, 200, 50000, torch.bfloat16)
+    kinds = [dict(top_p=0.9), dict(top_k=50, top_p=0.95), dict(min_p=0.02), dict(top_k=1500)]
+    want = [sampling.sample(x, u, **k) for k in kinds]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([sampling.sample(x, u, **k) for k in kinds])
+    torch.cuda.synchronize()
+    for tokens in got:
+        assert all(torch.equal(a, b) for a, b in zip(tokens, want))
+
+
 def test_refusals(sampling, monkeypatch):
     x, u = _logits(1, 4, 100, torch.float32)
     with pytest.raises(TypeError):
