@@ -23,8 +23,8 @@
 namespace cp {
 
 constexpr int kBins = 2048;    // of a histogram
-constexpr int kList = 2048;    // tokens that are sorted at most: two a thread,
-constexpr int kFew = 1024;     // or one
+constexpr int kList = 2048;    // tokens that are sorted at most: two a thread
+constexpr int kFew = 1024;     // tokens of a workgroup's lists, and ahead of the border that are listed
 constexpr int kChunks = 1024;  // pieces of a row whose weights are summed by themselves, at most
 constexpr int kChunkUnits = 256;  // of 16 bytes in a piece, at least
 constexpr int kSplits = 64;     // workgroups of a row at most
@@ -256,6 +256,11 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
   return wave_all64(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 
+// The value of one lane, the same number in all.
+__device__ __forceinline__ uint64_t read_lane64(uint64_t v, int lane) {
+  return join64(__builtin_amdgcn_readlane((int)(uint32_t)v, lane), __builtin_amdgcn_readlane((int)(v >> 32), lane));
+}
+
 // Sum of v over the threads before this one, and over all W waves.
 template <int W>
 __device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64_t* total) {
@@ -263,14 +268,19 @@ __device__ __forceinline__ uint64_t scan_block(uint64_t v, uint64_t* red, uint64
   const uint64_t sum = wave_scan64(v);
   if (lane == 63) red[wave] = sum;
   __syncthreads();
-  uint64_t base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    base += w < wave ? red[w] : 0;
-    all += red[w];
+  // the waves' sums in the first lanes of each row of 16 (by every thread for itself: 16 reads and 96 more operations)
+  const int at = lane & 15;
+  uint64_t s = at < W ? red[at] : 0;
+  s += lane_move64<0x111, 0xF>(s);
+  s += lane_move64<0x112, 0xF>(s);
+  if (W > 4) {
+    s += lane_move64<0x114, 0xF>(s);
+    s += lane_move64<0x118, 0xF>(s);
   }
+  const int w = __builtin_amdgcn_readfirstlane(wave);
+  const uint64_t base = w ? read_lane64(s, w - 1) : 0;
   __syncthreads();
-  *total = all;
+  *total = read_lane64(s, W - 1);
   return base + sum - v;
 }
 
@@ -380,10 +390,15 @@ __device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F enough
 }
 constexpr uint32_t kDeadKey = 0x007FFFFFu;  // of minus infinity
 
-// The least key whose weight min_p leaves: the largest one's does.
+// The least weight that min_p leaves: the largest logit's is one.
+__device__ __forceinline__ double least_weight(const Weigh& weigh, double m) {
+  return ceil(m * (double)((uint64_t)1 << weigh.shift));
+}
+
+// The least key whose weight is one.
 __device__ __forceinline__ uint32_t least_kept(const Weigh& weigh, float top, double m) {
   if (!(m > 0.0)) return kDeadKey + 1;
-  const double least = ceil(m * (double)((uint64_t)1 << weigh.shift));
+  const double least = least_weight(weigh, m);
   return least_key(kDeadKey, key_of(top),
                    [&](uint32_t k) { return k == key_of(top) || (double)weigh(value_of(k)) >= least; });
 }
@@ -397,6 +412,20 @@ struct SampleShared {
   uint32_t n;
   uint64_t pick[4];
 };
+
+// Number `at` of the n tokens of the list in LDS, sorted, into sm.pick[3].
+template <int E>
+__device__ __forceinline__ void pick_sorted(SampleShared& sm, int n, int at) {
+  const int t = threadIdx.x;
+  uint64_t v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = t + 1024 * e < n ? sm.list[t + 1024 * e] : 0;
+  __syncthreads();
+  sort_block<E>(v, n, sm.list);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (t + 1024 * e == at) sm.pick[3] = v[e];
+}
 
 // The place of the last token kept among the n of the list in LDS: the one before which, `before` included,
 // less than goal lies.
@@ -465,14 +494,14 @@ __device__ __forceinline__ uint64_t lane_value64(uint64_t v, int lane) {
 // do it, 6 so).
 __device__ __forceinline__ int choose_few(const uint64_t* list, const Weigh& weigh, int n, const RowSettings& s, uint64_t goal) {
   const int lane = threadIdx.x & 63;
-  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);
+  const double least = least_weight(weigh, s.m);
   uint64_t v[1] = {lane < n ? list[lane] : 0};
   sort_lanes(v);
   const int last = s.k ? min(n, (int)min(s.k, (uint64_t)64)) : n;
   uint64_t w = lane < last ? weigh.any(value_of((uint32_t)(v[0] >> 32))) : 0;
   uint64_t sum = wave_scan64(w);
   const uint64_t total = lane_value64(sum, 63), share = goal ? goal : s.p < 1.0 ? mass_goal(s.p, total) : total;
-  const bool keep = lane < last && (lane == 0 || (sum - w < share && (uint32_t)(v[0] >> 32) >= least));
+  const bool keep = lane < last && (lane == 0 || (sum - w < share && (double)w >= least));
   w = keep ? w : 0;
   const uint64_t pick = pick_goal(s.u, lane_value64(wave_scan64(w), 63));
   uint64_t by[1] = {keep ? (uint64_t)(uint32_t)v[0] << 32 | (uint32_t)lane : 0};  // by rising number, the kept ones first
@@ -493,14 +522,54 @@ __device__ __forceinline__ int border_bin(SampleShared& sm, uint64_t x0, uint64_
   return (int)sm.pick[0];
 }
 
+// The values v in bin `border` of theirs (at) onto the list, side by side: how many.
+__device__ __forceinline__ int gather(SampleShared& sm, const uint64_t (&v)[2], const int (&at)[2], int border) {
+  if (threadIdx.x == 0) sm.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (at[e] == border) sm.list[atomicAdd(&sm.n, 1u)] = v[e];
+  __syncthreads();
+  return (int)sm.n;
+}
+
+// The place of the last token kept among those of places v, weights w and bins at, and its bin: the one before which,
+// `before` included, less than goal lies (goal 0: the share p of their sum). A histogram finds the bin, and its
+// tokens alone are sorted: by one wave where they are up to 64. sm.mass is 0 on entry.
+__device__ __forceinline__ uint64_t last_by_mass(SampleShared& sm, const Weigh& weigh, const uint64_t (&v)[2], const uint64_t (&w)[2],
+                                                 const int (&at)[2], uint64_t before, uint64_t goal, double p, int* border) {
+  const int t = threadIdx.x, lane = t & 63;
+  uint64_t sum;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (w[e]) atomicAdd((unsigned long long*)&sm.mass[at[e]], (unsigned long long)w[e]);
+  __syncthreads();
+  const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = before + scan_block<16>(m0 + m1, sm.red, &sum);
+  const uint64_t share = goal ? goal : mass_goal(p, sum);
+  *border = border_bin(sm, m0, m1, b, share, &before);
+  const int m = gather(sm, v, at, *border);
+  if (m > 1024) return last_kept<2>(sm, weigh, m, before, share);
+  if (m > 64) return last_kept<1>(sm, weigh, m, before, share);
+  if (t < 64) {
+    uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
+    sort_lanes(x);
+    const uint64_t y = lane < m ? weigh.any(value_of((uint32_t)(x[0] >> 32))) : 0;
+    const uint64_t sum = wave_scan64(y);
+    const unsigned long long kept = __ballot(lane < m && before + sum - y < share);  // a front of the lanes
+    if (lane == __popcll(kept) - 1) sm.pick[3] = x[0];
+  }
+  __syncthreads();
+  return sm.pick[3];
+}
+
 // Chooses among the n tokens of the list in LDS, all that may be kept: k, p, m and u as in the file's heading (k 0:
 // all n). goal: top_p's, where the list is not all the weight there is (0: it is). Each border is found by a
-// histogram of the list over `bin`, and the tokens of its bin alone are sorted: by every wave for itself where they are up
-// to 64 (1100 tokens sorted as a whole 21 us a row, so 15).
+// histogram of the list over `bin`, and the tokens of its bin alone are sorted (1100 tokens sorted as a whole 21 us a
+// row, so 13).
 __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, const Bins& bin, int n, const RowSettings& s,
                                       uint64_t goal, int vocab) {
   const int t = threadIdx.x, lane = t & 63;
-  const uint32_t least = least_kept(weigh, (float)weigh.top, s.m);  // the largest logit is finite here
+  const double least = least_weight(weigh, s.m);
   uint64_t v[2], w[2], sum, before;
   int at[2];
 #pragma unroll
@@ -510,16 +579,6 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, cons
     sm.count[t + 1024 * e] = 0;
     sm.mass[t + 1024 * e] = 0;
   }
-  // puts the tokens of one bin on the list, side by side: how many
-  auto gather = [&](int border) __attribute__((always_inline)) {
-    if (t == 0) sm.n = 0;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (at[e] == border) sm.list[atomicAdd(&sm.n, 1u)] = v[e];
-    __syncthreads();
-    return (int)sm.n;
-  };
   auto drop = [&](int border, uint64_t cut) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -533,51 +592,30 @@ __device__ __forceinline__ int choose(SampleShared& sm, const Weigh& weigh, cons
     __syncthreads();
     const uint64_t c0 = sm.count[2 * t], c1 = sm.count[2 * t + 1], b = scan_block<16>(c0 + c1, sm.red, &sum);
     const int border = border_bin(sm, c0, c1, b, s.k, &before);
-    const int m = gather(border), need = (int)(s.k - before);  // of m
-    uint64_t cut;
+    const int m = gather(sm, v, at, border), need = (int)(s.k - before);  // of m
     if (m <= 64) {
-      uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
-      sort_lanes(x);
-      cut = join64(__shfl((int)(uint32_t)x[0], need - 1), __shfl((int)(x[0] >> 32), need - 1));
+      if (t < 64) {
+        uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
+        sort_lanes(x);
+        if (lane == need - 1) sm.pick[3] = x[0];
+      }
+    } else if (m <= 1024) {
+      pick_sorted<1>(sm, m, need - 1);
     } else {
-      uint64_t x[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) x[e] = t + 1024 * e < m ? sm.list[t + 1024 * e] : 0;
-      __syncthreads();
-      sort_block<2>(x, m, sm.list);
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (t + 1024 * e == need - 1) sm.pick[3] = x[e];
-      __syncthreads();
-      cut = sm.pick[3];
+      pick_sorted<2>(sm, m, need - 1);
     }
-    drop(border, cut);
+    __syncthreads();
+    drop(border, sm.pick[3]);
   }
 #pragma unroll
   for (int e = 0; e < 2; ++e) w[e] = v[e] ? weigh.any(value_of((uint32_t)(v[e] >> 32))) : 0;
   if (goal || s.p < 1.0) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (w[e]) atomicAdd((unsigned long long*)&sm.mass[at[e]], (unsigned long long)w[e]);
-    __syncthreads();
-    const uint64_t m0 = sm.mass[2 * t], m1 = sm.mass[2 * t + 1], b = scan_block<16>(m0 + m1, sm.red, &sum);
-    const uint64_t share = goal ? goal : mass_goal(s.p, sum);
-    const int border = border_bin(sm, m0, m1, b, share, &before);
-    const int m = gather(border);
-    uint64_t cut;
-    if (m <= 64) {
-      uint64_t x[1] = {lane < m ? sm.list[lane] : 0};
-      sort_lanes(x);
-      const uint64_t y = lane < m ? weigh.any(value_of((uint32_t)(x[0] >> 32))) : 0;
-      const int last = __popcll(__ballot(lane < m && before + wave_scan64(y) - y < share)) - 1;  // a front of the lanes
-      cut = join64(__shfl((int)(uint32_t)x[0], last), __shfl((int)(x[0] >> 32), last));
-    } else {
-      cut = last_kept<2>(sm, weigh, m, before, share);
-    }
+    int border;
+    const uint64_t cut = last_by_mass(sm, weigh, v, w, at, 0, goal, s.p, &border);
     drop(border, cut);
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e) w[e] = v[e] && (uint32_t)(v[e] >> 32) >= least ? w[e] : 0;
+  for (int e = 0; e < 2; ++e) w[e] = v[e] && (double)w[e] >= least ? w[e] : 0;
   __syncthreads();
   return by_number<2>(sm, v, w, s.u, vocab);
 }
@@ -762,15 +800,7 @@ struct Sampler {
       if (in_bin <= kList) {
         collect(lo, hi, cut, &n);
         if (by_count) {
-          uint64_t v[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) v[e] = (int)threadIdx.x + 1024 * e < n ? sm.list[threadIdx.x + 1024 * e] : 0;
-          __syncthreads();
-          sort_block<2>(v, n, sm.list);
-          const int at = (int)(by_count - count) - 1;  // of the sorted list
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if ((int)threadIdx.x + 1024 * e == at) sm.pick[3] = v[e];
+          pick_sorted<2>(sm, n, (int)(by_count - count) - 1);
           __syncthreads();
           return sm.pick[3];
         }
@@ -1033,7 +1063,7 @@ __global__ __launch_bounds__(256) void sample_weigh_kernel(SampleArgs a) {
     if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
 }
 
-// Launch 3, a workgroup a row with top_p: the bin in which its border lies, and that bin's keys. (The last
+// Launch 3, a workgroup a row with top_p: the bin in which its border lies, that bin's keys, and min_p's. (The last
 // workgroup of the launch before could do it, but the fence that it takes costs each of them an L2
 // written back: 45 -> 303 us.)
 __global__ __launch_bounds__(256) void sample_border_kernel(SampleArgs a) {
@@ -1062,10 +1092,19 @@ __global__ __launch_bounds__(256) void sample_border_kernel(SampleArgs a) {
   __syncthreads();
   const int border = pick;
   const Bins bin(range.top, range.least, a.shift, s.t);
-  const uint32_t from = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) <= border; });
-  const uint32_t to = border == 0 ? 0xFFFFFFFFu
-                                  : least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) < border; }) - 1;
-  if (threadIdx.x == 0) w.from = from, w.to = to, w.goal = goal;
+  // three searches, a wave each
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave == 0) {
+    const uint32_t from = least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) <= border; });
+    if (lane == 0) w.from = from, w.goal = goal;
+  } else if (wave == 1) {
+    const uint32_t to = border == 0 ? 0xFFFFFFFFu
+                                    : least_key(kDeadKey, key_of(range.top), [&](uint32_t k) { return bin(value_of(k)) < border; }) - 1;
+    if (lane == 0) w.to = to;
+  } else if (wave == 2) {
+    const uint32_t least = least_kept(Weigh(range.top, s.t, a.shift), range.top, s.m);
+    if (lane == 0) w.least_kept = least;
+  }
 }
 
 // Launch 4: the tokens that the border is among. top_k: all that reach its logit. top_p: those of its bin, and on
@@ -1160,14 +1199,26 @@ __global__ __launch_bounds__(1024) void sample_choose_kernel(SampleArgs a) {
       }
       __syncthreads();
       if (!some) {
-        const uint64_t cut = n > 1024 ? last_kept<2>(sm, weigh, (int)n, w.before, w.goal)
-                                      : last_kept<1>(sm, weigh, (int)n, w.before, w.goal);
-        const uint32_t least = least_kept(weigh, range.top, s.m);
-        if (threadIdx.x == 0) w.cut = cut, w.least_kept = least;
+        const int t = threadIdx.x;
+        const Bins bin(value_of(min(w.to, key_of(range.top))), value_of(w.from), a.shift, __builtin_inf());
+        uint64_t v[2], y[2];
+        int at[2], border;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          v[e] = t + 1024 * e < have ? sm.list[t + 1024 * e] : 0;
+          const float x = value_of((uint32_t)(v[e] >> 32));
+          at[e] = v[e] ? bin(x) : kBins;
+          y[e] = v[e] ? weigh(x) : 0;
+          sm.mass[t + 1024 * e] = 0;
+        }
+        __syncthreads();
+        const uint64_t cut = last_by_mass(sm, weigh, v, y, at, w.before, w.goal, 0.0, &border);
+        if (threadIdx.x == 0) w.cut = cut;
         return;
       }
       // what is on the lists is not all the row's weight, but the border's goal is of that
       const uint64_t goal = s.kind == kShare ? w.goal : 0;
+      if (have <= 64 && threadIdx.x >= 64) return;
       if (have <= 64) token = choose_few(sm.list, weigh, have, s, goal);
       else token = choose(sm, weigh, Bins(range.top, value_of(w.from), a.shift, __builtin_inf()), have, s, goal, a.vocab);
     }
