@@ -14,6 +14,11 @@
 // Which token u falls on must not hang on the order in which weights are added: a vocabulary of 2^17
 // tokens has borders 2^-17 apart, float32 sums err by 2^-20 of the whole. A weight is the whole
 // number round(w 2^s), computed in float64, s = 62 - log2(vocabulary) up to 51, and sums are exact in 64 bits.
+//
+// A row is read two to four times, out of the caches but for the first, as a border has to be known before what it
+// leaves can be summed. 256 rows of 151936 bfloat16 with settings of their own (78 MB): range 18.5 us, weigh 30
+// (float64, the VALU two-thirds busy), collect 17, kept 16, and 26 in three launches of a workgroup a row. One row with
+// top_k: five launches, 18.6 us, each as long as its latencies.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -490,8 +495,8 @@ __device__ __forceinline__ uint64_t lane_value64(uint64_t v, int lane) {
   return join64(__shfl((int)(uint32_t)v, lane), __shfl((int)(v >> 32), lane));
 }
 
-// choose() of up to 64 tokens, by one wave: two sorts and three sums in registers (8 us a row as the file's histograms
-// do it, 6 so).
+// choose() of up to 64 tokens, by one wave: two sorts and three sums in registers (a launch of one row 8 us as choose
+// does it, 4.3 so).
 __device__ __forceinline__ int choose_few(const uint64_t* list, const Weigh& weigh, int n, const RowSettings& s, uint64_t goal) {
   const int lane = threadIdx.x & 63;
   const double least = least_weight(weigh, s.m);

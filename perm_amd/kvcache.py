@@ -6,7 +6,10 @@ tokens) and head. A sequence's position p is slot p % block of page table[b][p /
   new(pages, heads, head_dim, block)             an empty KvCache
   write(cache, k, v, table, filled, offsets)     quantizes and appends rows
   read(cache, table, offsets, total, dtype)      the tokens held, back in floating point
-  attention(q, cache, table, lens, offsets)      softmax(q K^T) V over the codes
+  attention(q, cache, table, lens, offsets)      softmax(q K^T) V over the codes, also of capped
+                                                 scores, of documents, and of pages in common
+
+Who holds which page is the caller's to say; ``perm_amd.kvpages`` keeps such books on the GPU.
 
 Ragged batches: ``offsets`` int32 [batch + 1] gives each sequence's first row of k, v or q;
 None means one row a sequence, as in decoding. table int32 [batch, max_pages], filled and
