@@ -279,7 +279,7 @@ def ptr(t):
 
 class _NoBackward(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, name, x):
+    def forward(ctx, y, name, *xs):
         ctx.name = name
         ctx.mark_dirty(y)  # the result itself, not a view of it
         return y
@@ -289,11 +289,12 @@ class _NoBackward(torch.autograd.Function):
         raise NotImplementedError(f"{ctx.name} has no backward pass")
 
 
-def no_backward(y, name, x):
-    """y, with a backward pass that raises where autograd would want one: an operator without
-    gradients must not pass for one that has none to give."""
-    if x.requires_grad and torch.is_grad_enabled():
-        return _NoBackward.apply(y, name, x)
+def no_backward(y, name, *xs):
+    """y, with a backward pass that raises where autograd would want one for any of the inputs xs
+    (None: not given): an operator without gradients must not pass for one that has none to give."""
+    for x in xs:
+        if x is not None and x.requires_grad and torch.is_grad_enabled():
+            return _NoBackward.apply(y, name, *xs)
     return y
 
 

@@ -19,8 +19,8 @@ reads as 0, and attention does not see its tokens. Offsets do not decrease; rows
 first and past the last (a padded batch) have no sequence: write leaves them out, read and
 attention give 0 there.
 
-For inference: rows written keep no graph, and a backward pass through attention raises
-NotImplementedError.
+For inference: rows written keep no graph, and a backward pass through attention, to its queries
+or its slopes, raises NotImplementedError.
 """
 import ctypes
 import operator
@@ -280,5 +280,5 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
         _lib.check(lib.cp_kv_attention(*args, *ends))
     else:
         _lib.check(lib.cp_kv_attention_more(*args, ctypes.byref(more), *ends))
-    out = _lib.no_backward(out, "kvcache.attention", q)
-    return (out, _lib.no_backward(lse, "kvcache.attention", q)) if return_lse else out
+    out = _lib.no_backward(out, "kvcache.attention", q, slopes)
+    return (out, _lib.no_backward(lse, "kvcache.attention", q, slopes)) if return_lse else out
