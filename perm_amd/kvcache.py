@@ -178,7 +178,7 @@ def _front_pays(desc, rows, heads, batch, groups, tokens):
     on 32768, 64 sequences 395 and 91, 16 110 and 53, 4 39 and 32; 300 rows of each of 32 in four
     groups on 4096 193 and 189, 30 rows 40 and 54."""
     pairs = rows * heads // desc.heads
-    if batch == groups or pairs > 64 * batch:
+    if batch == groups or pairs == 0 or pairs > 64 * batch:
         return False
     without = 8 + batch * -(-pairs // (16 * batch)) * tokens * desc.heads * desc.head_dim * 2 / 11e6
     return without > 1.25 * (30 + rows * heads * tokens * desc.head_dim * 4 / 6e8)
@@ -207,7 +207,7 @@ def _more(desc, table, rows, heads, device, softcap, slopes, first, prefix, shar
     if shared is not None:
         shared = _index(shared, 1, "shared")
         groups = shared.shape[0]
-        if groups == 0 or batch % groups:
+        if batch and (groups == 0 or batch % groups):
             raise ValueError(f"{batch} sequences in {groups} groups")
     keep = slopes, first, prefix, shared
     for t in keep:

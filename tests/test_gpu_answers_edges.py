@@ -21,3 +21,24 @@ def test_slopes_that_want_a_gradient(kv, heads):  # noqa: F811
             got.float().sum().backward()
     with torch.no_grad():
         assert not kv.attention(q, c, t, n, slopes=slopes).requires_grad
+
+
+@pytest.mark.parametrize("rows", [0, 3])
+@pytest.mark.parametrize("apart", [None, True], ids=["rule", "apart"])
+def test_common_pages_of_an_empty_batch(kv, monkeypatch, apart, rows):  # noqa: F811
+    """A step without sequences, of any number of groups: what the call without common pages gives."""
+    if apart:
+        monkeypatch.setattr(kv, "_front_pays", lambda *a: True)
+    c = kv.new(4, 2, 64, 16)
+    q = torch.ones((rows, 8, 64), dtype=torch.bfloat16, device="cuda")
+    table, lens = torch.empty((0, 5), dtype=torch.int32, device="cuda"), _i32([])
+    for offsets in (_i32([0]), None) if rows == 0 else (_i32([0]),):
+        for groups in (0, 1, 3):
+            for more in (dict(), dict(softcap=5.0), dict(window=9)):
+                out, lse = kv.attention(q, c, table, lens, offsets, return_lse=True, shared=_i32([1] * groups), **more)
+                assert out.shape == q.shape and not out.any() and lse.shape == (rows, 8) and torch.isneginf(lse).all()
+    # sequences, but no rows of theirs
+    out = kv.attention(q[:0], c, _i32([[0], [1]]), _i32([9, 9]), _i32([0, 0, 0]), shared=_i32([1]))
+    assert out.shape == (0, 8, 64)
+    with pytest.raises(ValueError, match="groups"):
+        kv.attention(q[:0], c, _i32([[0], [1]]), _i32([9, 9]), _i32([0, 0, 0]), shared=_i32([]))
