@@ -499,6 +499,7 @@ int cp_kv_compact(int32_t* refs, int64_t pages, int32_t* table, int64_t batch, i
   cp::kv_moves_kernel<<<dim3((unsigned)a.blocks), 1024, 0, st>>>(a);
   CP_LAUNCHED("moves");
   const int64_t items = std::max(batch * max_pages, pages / 2);
+  if (items == 0) return CP_OK;  // one page and no entries
   cp::kv_moved_kernel<<<dim3((unsigned)std::min((items + 255) / 256, (int64_t)2048)), 256, 0, st>>>(a);
   CP_LAUNCHED("moved entries");
   return CP_OK;

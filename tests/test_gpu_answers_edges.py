@@ -42,3 +42,20 @@ def test_common_pages_of_an_empty_batch(kv, monkeypatch, apart, rows):  # noqa: 
     assert out.shape == (0, 8, 64)
     with pytest.raises(ValueError, match="groups"):
         kv.attention(q[:0], c, _i32([[0], [1]]), _i32([9, 9]), _i32([0, 0, 0]), shared=_i32([]))
+
+
+@pytest.mark.parametrize("pages", [1, 2, 3, 2000])
+@pytest.mark.parametrize("width", [1, 5])
+def test_compaction_under_a_table_of_no_rows(pages, width):
+    """Holders that no table names (another's, or none): pages in use move all the same."""
+    from perm_amd import kvpages
+    table = torch.empty((0, width), dtype=torch.int32, device="cuda")
+    for held in ([], [pages - 1], list(range(0, pages, 2))):
+        refs = kvpages.new(pages)
+        refs[held] = 1
+        src, dst, used = kvpages.compact(refs, table)
+        n = len(held)
+        assert used.tolist() == [n] and refs.tolist() == [1] * n + [0] * (pages - n)
+        moved, free = [p for p in held if p >= n], [p for p in range(n) if p not in held]
+        assert src.tolist() == moved + [-1] * (pages // 2 - len(moved))
+        assert dst.tolist() == free + [-1] * (pages // 2 - len(moved))
