@@ -1,8 +1,12 @@
 """The operators for several answers at the edges of what their calls allow."""
+import numpy as np
 import pytest
 import torch
 
 from test_gpu_kvcache import _i32, kv  # noqa: F401
+from test_gpu_kvpages import _books, _same
+from test_gpu_sampling import DTYPES, _logits
+from test_gpu_sampling import _check as _check_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +63,56 @@ def test_compaction_under_a_table_of_no_rows(pages, width):
         moved, free = [p for p in held if p >= n], [p for p in range(n) if p not in held]
         assert src.tolist() == moved + [-1] * (pages // 2 - len(moved))
         assert dst.tolist() == free + [-1] * (pages // 2 - len(moved))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sampling_of_more_rows_than_a_batch_of_launches(dtype):
+    """1500 rows of their own, part of a wider tensor, all four settings and a number for each."""
+    from perm_amd import sampling
+    rows, vocab = 1500, 500
+    x, u = _logits(21, rows, vocab + 13, dtype)
+    rng = np.random.default_rng(21)
+    settings = dict(temperature=rng.choice([0.0, 0.3, 0.7, 1.0, 1.5], rows), top_k=rng.choice([0, 0, 1, 20, 50, 499], rows),
+                    top_p=rng.choice([1.0, 1.0, 0.5, 0.9, 0.95], rows), min_p=rng.choice([0.0, 0.0, 0.02, 0.1], rows))
+    for y, v in ((x[:, 5:5 + vocab], u), (x[:, :vocab], u.double())):
+        assert y.stride(0) > vocab
+        _check_tokens(sampling, y, v, **settings)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 5000011), (torch.bfloat16, 1 << 24)])
+def test_sampling_of_the_largest_vocabularies(dtype, vocab):
+    """Pieces of a row of more than 1024 units of 16 bytes, one to four steps each: nothing left out, a share, long lists,
+    and (bfloat16) thousands of equal logits at every border. Weights are multiples of 2^-39 and 2^-38 of the
+    largest here and what a row keeps sums to more than 2^6 of it: they err by under 2^-21 of the whole in all."""
+    from perm_amd import sampling
+    print(f"sample {vocab} {dtype}", flush=True)
+    x, _ = _logits(22, 1, vocab, dtype)
+    kinds = [dict(), dict(top_p=0.9), dict(top_k=1500), dict(top_k=3000000, min_p=1e-4), dict(top_k=40, top_p=0.95)]
+    numbers = [[0.03, 0.41, 0.77], [0.999], [0.5], [0.86], [0.2]]
+    for kind, us in zip(kinds, numbers):
+        _check_tokens(sampling, x.expand(len(us), vocab), torch.tensor(us, dtype=torch.float64, device="cuda"), **kind)
+
+
+def test_growth_of_thousands_of_sequences():
+    """2100 of them, of one entry to wave-wide ranges, some past the table's end: pages run short behind the first 1024."""
+    from oracle import pages_oracle as O
+    from perm_amd import kvpages
+    rng = np.random.default_rng(23)
+    batch, cap, block = 2100, 12, 16
+    lens = rng.integers(0, 60, batch)
+    lens[5::40] = 0
+    new = rng.choice([0, 1, 1, 1, 20, 110], batch)
+    new[[300, 1400]] = 300  # more than the table's row holds
+    need = -(-(lens + new) // block) + (-lens // block)
+    for short in (1030, 1500, None):
+        pages = int((-(-lens // block)).sum() + need[:short].sum()) + (0 if short else 2000)
+        refs, table = _books(rng, pages, batch, cap, lens, block)
+        o = O.Books(refs, table, block)
+        refs, table = _i32(refs), _i32(table)
+        want = o.grow(lens, new)
+        unserved = [b for b in np.flatnonzero(want[2]) if b not in (300, 1400)]
+        assert len(unserved) > 100 and unserved[0] >= short if short else not unserved
+        got = kvpages.grow(refs, table, _i32(lens), _i32(new), block)
+        for g, w, name in zip(got, want, ("src", "dst", "missing")):
+            assert g.tolist() == w, (short, name)
+        _same(o, refs, table)
