@@ -266,11 +266,13 @@ def stream_ptr():
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
-def here(device):
-    """Refuses tensors of another device than the current one, on whose stream kernels run."""
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}, but the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+def here(*tensors):
+    """Refuses tensors (None: not given) of another device than the current one, on whose stream
+    kernels run."""
+    at = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"a tensor on {t.device}, but the current device is cuda:{at}")
 
 
 def ptr(t):

@@ -57,7 +57,8 @@ def new(pages, heads, head_dim, block=16, device="cuda"):
 
 
 def _desc(c):
-    """struct cp_kv_cache of a KvCache, its buffers checked against each other."""
+    """struct cp_kv_cache of a KvCache, its buffers checked against each other (but for their
+    device: ``_lib.here`` with the call's other tensors)."""
     if not (isinstance(c, (tuple, list)) and len(c) == 4):
         raise TypeError(f"cache must be a KvCache, got {type(c).__name__}")
     k, v, ks, vs = c
@@ -71,9 +72,8 @@ def _desc(c):
     if k.dtype != torch.uint8 or v.dtype != torch.uint8 \
             or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise TypeError("cache codes are uint8 and scales float32")
-    if not (k.is_cuda and v.is_cuda and ks.is_cuda and vs.is_cuda and k.is_contiguous()
-            and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        raise ValueError("cache buffers must be contiguous and on the GPU")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("cache buffers must be contiguous")
     return _lib.KvCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages,
                             heads, block, d)
 
@@ -141,6 +141,7 @@ def write(cache, k, v, table, filled, offsets=None):
     if v.shape[0] != rows:
         raise ValueError(f"{rows} keys and {v.shape[0]} values")
     table, filled, offsets = _batch(table, filled, "filled", offsets, rows)
+    _lib.here(k, v, table, filled, offsets, *cache)
     if table.shape[0] == 0:
         return
     _lib.check(lib.cp_kv_write(
@@ -160,6 +161,7 @@ def read(cache, table, offsets, total, dtype=torch.bfloat16):
     if offsets is None:
         raise ValueError("read needs offsets")
     table, _, offsets = _batch(table, None, "", offsets, total)
+    _lib.here(table, offsets, *cache)
     shape = total, desc.heads, desc.head_dim
     k = cache.k.new_empty(shape, dtype=dtype)
     v = torch.empty_like(k)
@@ -186,7 +188,6 @@ def _front_pays(desc, rows, heads, batch, groups, tokens):
 
 def _more(desc, table, rows, heads, device, softcap, slopes, first, prefix, shared):
     """struct cp_kv_more of attention's arguments, and what keeps its arrays alive."""
-    _lib.here(device)
     softcap = float(softcap)
     if not 0.0 <= softcap < 1e30 or 0.0 < softcap < 1e-30:
         raise ValueError(f"softcap {softcap} must be 0 (none) or positive")
@@ -250,6 +251,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
+    _lib.here(q, table, lens, offsets, *cache)
     more = None
     if softcap or slopes is not None or first is not None or prefix is not None or shared is not None:
         more, keep = _more(desc, table, rows, heads, q.device, softcap, slopes, first, prefix, shared)

@@ -55,7 +55,7 @@ def _books(refs, table):
     for t, dims, what in ((refs, 1, "refs"), (table, 2, "table")):
         if _ints(t, dims, what, getattr(refs, "device", None)) is not t:
             raise ValueError(f"{what} is changed in place and must be contiguous")
-    _lib.here(refs.device)
+    _lib.here(refs)
     return refs.data_ptr(), refs.shape[0], table.data_ptr(), table.shape[0], table.shape[1]
 
 
@@ -148,9 +148,7 @@ def copy(cache, src, dst, into=None):
     desc = _desc(cache)
     to = desc if into is None else _desc(into)
     device = cache[0].device
-    _lib.here(device)
-    if into is not None and into[0].device != device:
-        raise ValueError(f"a cache on {device} into one on {into[0].device}")
+    _lib.here(*cache, *(into or ()))
     src = _ints(src, 1, "src", device)
     dst = _ints(dst, 1, "dst", device, src.shape[0])
     _lib.check(lib.cp_kv_copy(ctypes.byref(desc), ctypes.byref(to), src.data_ptr(), dst.data_ptr(),

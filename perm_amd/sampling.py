@@ -56,7 +56,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocab], got {tuple(logits.shape)}")
     dev = logits.device
-    _lib.here(dev)
+    _lib.here(logits)
     rows, vocab = logits.shape
     if not isinstance(u, torch.Tensor) or u.device != dev or u.shape != (rows,):
         raise ValueError(f"u must be a tensor [{rows}] on {dev}")
