@@ -457,14 +457,16 @@ typedef struct cp_kv_cache {
  * [-60, 60], with max |x| <= 448 * 2^e over the finite values written, or the scale it had
  * where it holds tokens already and that is larger; a scale that grows moves the codes held.
  * Values beyond 448 * scale saturate, NaN stays. Tokens past the table's end or on a page
- * outside [0, pages) are dropped. Sequences written in one call must not share a page. */
+ * outside [0, pages) are dropped, and so are sequences that begin before row 0 and pages whose rows
+ * pass the last one. Sequences written in one call must not share a page. */
 int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t k_head,
                 const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows,
                 const int32_t* table, int64_t batch, int64_t max_pages, const int32_t* filled,
                 const int32_t* offsets, void* stream);
 
 /* The first offsets[b + 1] - offsets[b] tokens of every sequence into k and v [total, heads,
- * head_dim]; tokens without a page, and rows that no sequence has, read as 0. */
+ * head_dim]; tokens without a page, those of a sequence that begins before row 0, and rows that no
+ * sequence has, read as 0. */
 int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, int64_t max_pages,
                const int32_t* offsets, int64_t total, void* k, void* v, int dtype, void* stream);
 

@@ -1649,7 +1649,7 @@ static int attn_run_more(AttnArgs a, KvBatch b, AttnMore x, const AttnPlan& p, c
   x.slots = sp.front.splits + sp.rest.splits;
   x.phase = 1;
   a.splits = sp.front.splits, a.least = sp.front.least;
-  const KvBatch bg = {b.offsets, groups};
+  const KvBatch bg = {b.offsets, groups, b.rows};
   if (int s = attn_launch_d<DT, MODE>(a, bg, sp.front, x, st)) return s;
   x.phase = 2;
   x.slot0 = sp.front.splits;
@@ -1723,7 +1723,7 @@ int cp_kv_attention(const cp_kv_cache* cache, const void* q, int64_t q_row, int6
   a.splits = p.splits;
   a.least = p.least;
   a.scale = scale * cp::kLog2e;
-  const cp::KvBatch b = {offsets, (int)batch};
+  const cp::KvBatch b = {offsets, (int)batch, (int)rows};
   return dtype == CP_BF16 ? cp::attn_run<CP_BF16>(a, b, p, (hipStream_t)stream)
                           : cp::attn_run<CP_F16>(a, b, p, (hipStream_t)stream);
 }
@@ -1808,7 +1808,7 @@ int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row,
     x.cost = (int*)((char*)ws + cp_kv_attention_ws_bytes(cache, rows, q_heads, batch, max_pages, offsets != nullptr, window));
     x.order = x.cost + p.items;
   }
-  const cp::KvBatch b = {offsets, (int)batch};
+  const cp::KvBatch b = {offsets, (int)batch, (int)rows};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CP_BF16)
     return more->slopes         ? cp::attn_run_more<CP_BF16, 3>(a, b, x, p, sp, (int)groups, st)

@@ -18,6 +18,7 @@ struct KvCacheArgs {
 struct KvBatch {
   const int* offsets;  // [batch + 1] first row of each sequence; null: one row each
   int batch;
+  int rows;            // of the call
 };
 
 // Work item `at` of a ragged batch: sequence b, its item'th piece, its first row and row
@@ -26,6 +27,10 @@ struct KvBatch {
 // not know the lengths. False: the grid is an upper bound and this item is past the end; *item
 // is then which one past it. each: so many consecutive sequences count as one, of which q.batch
 // are given.
+//
+// Offsets may leave the call's rows: a sequence that begins before row 0 is given as one that
+// begins at row -1, one that passes the last row as one that passes it by a row, and pieces
+// count the rows that there are, so that the grid holds all of the other sequences'.
 template <class F>
 __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int* b, int* item,
                                           int64_t* row0, int* n, int each = 1) {
@@ -34,10 +39,10 @@ __device__ __forceinline__ bool kv_locate(const KvBatch& q, int at, F count, int
     const int s = base + lane;
     int r = 0, m = 0, pieces = 0;
     if (s < q.batch) {
-      r = q.offsets ? q.offsets[s * each] : s * each;
-      m = q.offsets ? q.offsets[(s + 1) * each] - r : each;
-      m = m < 0 ? 0 : m;
-      pieces = count(s, m);
+      r = q.offsets ? max(q.offsets[s * each], -1) : s * each;
+      const int end = q.offsets ? min(q.offsets[(s + 1) * each], q.rows + 1) : r + each;
+      m = end > r ? end - r : 0;
+      pieces = count(s, max(min(end, q.rows) - max(r, 0), 0));
     }
     int sum = pieces;  // inclusive scan
 #pragma unroll

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256, KEEP ? 4 : 3) void kv_write_kernel(KvCacheArgs
   const int done = item == 0 ? 0 : item * c.block - held % c.block;  // rows in earlier pages
   const int n = min(n_b - done, c.block - s0);
   const int64_t r0 = row0 + done;
-  if (pg >= c.max_pages || r0 < 0 || r0 + n > rows) return;
+  if (pg >= c.max_pages || row0 < 0 || r0 + n > rows) return;
   const int page = c.table[(int64_t)b * c.max_pages + pg];
   if ((unsigned)page >= (unsigned)c.pages) return;
   const int64_t ph = (int64_t)page * c.heads + h;
@@ -283,11 +283,12 @@ __global__ __launch_bounds__(256, 5) void kv_read_kernel(KvCacheArgs c, KvBatch 
     }
     return;
   }
-  const int64_t r0 = row0 + (int64_t)item * 16;
-  if (r0 < 0) return;
-  const int n = (int)min((int64_t)min(n_b - item * 16, 16), total - r0);  // rows that there are
+  // a sequence that begins before row 0 holds no tokens
+  const bool none = row0 < 0;
+  const int64_t r0 = (none ? 0 : row0) + (int64_t)item * 16;
+  const int n = (int)min((int64_t)min(n_b - (none ? 1 : 0) - item * 16, 16), total - r0);  // rows that there are
   const int64_t pg = (int64_t)item * 16 / c.block;
-  const int page = pg < c.max_pages ? c.table[(int64_t)b * c.max_pages + pg] : -1;
+  const int page = !none && pg < c.max_pages ? c.table[(int64_t)b * c.max_pages + pg] : -1;
   const bool have = (unsigned)page < (unsigned)c.pages;
   const int64_t ph = have ? (int64_t)page * c.heads + h : 0;
   const int d = c.d, blk = c.block, dc = d / 8, slot = item * 16 % blk;
@@ -396,7 +397,7 @@ int cp_kv_write(const cp_kv_cache* cache, const void* k, int64_t k_row, int64_t 
   if (items * cache->heads > 4 * cp::most_workgroups(256)) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
   const cp::KvRows kr = {k, k_row, k_head}, vr = {v, v_row, v_head};
-  const cp::KvBatch q = {offsets, (int)batch};
+  const cp::KvBatch q = {offsets, (int)batch, (int)rows};
   const dim3 grid((unsigned)((items * cache->heads + 3) / 4));
   const bool keep = cache->block == 16 && cache->head_dim <= 128;
   hipStream_t st = (hipStream_t)stream;
@@ -426,7 +427,7 @@ int cp_kv_read(const cp_kv_cache* cache, const int32_t* table, int64_t batch, in
   const int64_t items = total / 16 + batch + 1;  // one more than sequences can need
   if (items * cache->heads > 4 * cp::most_workgroups(256)) return cp::set_error(CP_ERR_SHAPE, "too many rows");
   const cp::KvCacheArgs a = cp::kv_args(cache, table, max_pages);
-  const cp::KvBatch q = {offsets, (int)batch};
+  const cp::KvBatch q = {offsets, (int)batch, (int)total};
   const dim3 grid((unsigned)((items * cache->heads + 3) / 4));
   hipStream_t st = (hipStream_t)stream;
   if (dtype == CP_F32) cp::kv_read_kernel<CP_F32><<<grid, 256, 0, st>>>(a, q, (int)items, total, (float*)k, (float*)v);

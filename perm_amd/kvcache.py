@@ -17,7 +17,8 @@ lens int32 [batch] stay on the GPU and are read there: a call never waits for th
 entry of table outside the cache's pages is no page: what is written there is dropped, it
 reads as 0, and attention does not see its tokens. Offsets do not decrease; rows before the
 first and past the last (a padded batch) have no sequence: write leaves them out, read and
-attention give 0 there.
+attention give 0 there. So they do with a sequence that begins before row 0. Of one that passes
+the last row the rows that there are are read and whole pages of them written; attention gives 0.
 
 For inference: rows written keep no graph, and a backward pass through attention, to its queries
 or its slopes, raises NotImplementedError.

@@ -3,7 +3,9 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kvcache import _i32, kv  # noqa: F401
+from test_gpu_kvcache import _filled_cache, _i32, kv  # noqa: F401
+from test_gpu_kvcache_padding import _dirty
+from test_gpu_kvcache_tiles import _long
 from test_gpu_kvpages import _books, _same
 from test_gpu_sampling import DTYPES, _logits
 from test_gpu_sampling import _check as _check_tokens
@@ -116,3 +118,78 @@ def test_growth_of_thousands_of_sequences():
         for g, w, name in zip(got, want, ("src", "dst", "missing")):
             assert g.tolist() == w, (short, name)
         _same(o, refs, table)
+
+
+# first rows of three sequences among 40 rows, some of which are no rows of the call
+OUTSIDE = [[-1000, 5, 9, 40], [-3, -2, 0, 40], [-90000, -500, 12, 30], [7, 20, 10 ** 6, 10 ** 6], [7, 10 ** 6, 10 ** 6, 10 ** 6],
+           [-5, 10 ** 6, 10 ** 6, 10 ** 6], [-2 ** 31, 11, 25, 2 ** 31 - 1], [-2 ** 31, -2 ** 31, 2 ** 31 - 1, 2 ** 31 - 1],
+           [50, 60, 70, 80], [-9, -8, -7, -6], [40, 40, 40, 41], [3, 3, 40, 41]]
+
+
+@pytest.mark.parametrize("tiles", [False, True], ids=["few", "tiles"])
+@pytest.mark.parametrize("offsets", OUTSIDE, ids=str)
+def test_attention_of_sequences_with_rows_outside_the_call(kv, monkeypatch, offsets, tiles):  # noqa: F811
+    """They have no results, the rows of no sequence neither, and the others theirs, whatever memory held."""
+    monkeypatch.setattr(kv, "_front_pays", lambda *a: True)
+    print(f"outside {offsets} {tiles}", flush=True)
+    rng = np.random.default_rng(31)
+    rows, hq, lens = 40, 32, [70, 90, 60]
+    c, o, table = _filled_cache(kv, rng, lens, 1, 64, 16)
+    table[:, 0] = table[0, 0]
+    t = _i32(_long(table, rows, hq, 16) if tiles else table)
+    q = torch.from_numpy(rng.standard_normal((rows, hq, 64))).to(torch.bfloat16).cuda()
+    whole = [b for b in range(3) if 0 <= offsets[b] < offsets[b + 1] <= rows]
+    for more in (dict(), dict(softcap=20.0), dict(slopes=torch.full((hq,), 0.1, device="cuda")), dict(shared=_i32([1, 1, 1])),
+                 dict(shared=_i32([1]))):
+        results = [] if len(more.get("shared", "___")) == 1 and not 0 <= offsets[0] <= offsets[3] <= rows else whole
+        _dirty(((rows, hq, 64), torch.bfloat16), ((rows, hq), torch.float32), ((rows * hq * 64 * 16,), torch.float32))
+        out, lse = kv.attention(q, c, t, _i32(lens), _i32(offsets), return_lse=True, **more)
+        left = torch.ones(rows, dtype=torch.bool, device="cuda")
+        for b in results:
+            at = slice(offsets[b], offsets[b + 1])
+            left[at] = False
+            alone = {k: v[b:b + 1] if k == "shared" else v for k, v in more.items()}
+            want, wl = kv.attention(q[at], c, t[b:b + 1], _i32(lens[b:b + 1]), _i32([0, offsets[b + 1] - offsets[b]]),
+                                    return_lse=True, **alone)
+            # the same to the order of float32 sums, which moves a result by one rounding to 16 bits at most
+            assert float((out[at].float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+            assert float((lse[at] - wl).abs().max()) <= 1e-4
+        assert not out[left].any() and bool((lse[left] == float("-inf")).all())
+
+
+@pytest.mark.parametrize("offsets", OUTSIDE, ids=str)
+def test_rows_outside_the_call_written_and_read(kv, offsets):  # noqa: F811
+    """A sequence that begins before row 0 is neither written nor read (0); one that passes the last row is read as
+    far as there are rows."""
+    rng = np.random.default_rng(32)
+    rows, lens = 40, [70, 90, 60]
+    c, o, table = _filled_cache(kv, rng, lens, 2, 48, 16)
+    for dtype in (torch.bfloat16, torch.float32):
+        _dirty(((rows, 2, 48), dtype))
+        k, v = kv.read(c, _i32(table), _i32(offsets), rows, dtype)
+        left = torch.ones(rows, dtype=torch.bool, device="cuda")
+        for b in range(3):
+            n = min(offsets[b + 1], rows) - offsets[b]
+            if offsets[b] < 0 or n <= 0:
+                continue
+            at = slice(offsets[b], offsets[b] + n)
+            left[at] = False
+            want = kv.read(c, _i32(table[b:b + 1]), _i32([0, n]), n, dtype)
+            assert torch.equal(k[at], want[0]) and torch.equal(v[at], want[1])
+        assert not k[left].any() and not v[left].any()
+    # written: whole pages of rows that there are
+    x = torch.from_numpy(rng.standard_normal((rows, 2, 48))).to(torch.bfloat16).cuda()
+    a, b = kv.new(*_geometry(c)), kv.new(*_geometry(c))
+    kv.write(a, x, x, _i32(table), _i32([0, 0, 0]), _i32(offsets))
+    for s in range(3):
+        n = offsets[s + 1] - offsets[s]
+        if offsets[s] < 0 or n <= 0 or offsets[s] >= rows:
+            continue
+        n = n if offsets[s + 1] <= rows else (rows - offsets[s]) // 16 * 16
+        kv.write(b, x[offsets[s]:offsets[s] + n], x[offsets[s]:offsets[s] + n], _i32(table[s:s + 1]), _i32([0]), _i32([0, n]))
+    assert all(torch.equal(y, z) for y, z in zip(a, b))
+
+
+def _geometry(c):
+    pages, heads, block, d = c.k.shape
+    return pages, heads, d, block
