@@ -193,7 +193,8 @@ __device__ __forceinline__ void cap_scores(const AttnMore& x, V& v, float kc, bo
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = near(v[i]);
   } else {
-    const float most = x.cap / kc, e2 = kz * (2.0f * kLog2e);
+    // finite, where a large kc over a small cap is not: products of 0 stay 0
+    const float most = x.cap / kc, e2 = fminf(kz * (2.0f * kLog2e), 3e38f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float far = __builtin_fmaf(-2.0f * most, __builtin_amdgcn_rcpf(1.0f + exp2_fast(v[i] * e2)), most);

@@ -193,3 +193,24 @@ def test_rows_outside_the_call_written_and_read(kv, offsets):  # noqa: F811
 def _geometry(c):
     pages, heads, block, d = c.k.shape
     return pages, heads, d, block
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("many", [False, True])
+def test_small_caps_of_large_keys(kv, many, dtype):  # noqa: F811
+    """Keys under the largest scale and caps down to the least: scores are at most the cap, 2^-60 or less of one, so
+    every row is the mean of the values it sees. Queries of 0 among them, whose scores are 0 under any cap."""
+    rng = np.random.default_rng(41)
+    n, rows = (2500, 700) if many else (100, 9)
+    c, o, table = _filled_cache(kv, rng, [n], 1, 64, 16)
+    c.k_scale.fill_(2.0 ** 60)
+    q = torch.from_numpy(rng.standard_normal((rows, 12, 64))).to(dtype).cuda()
+    q[1], q[5, 3:] = 0, 0
+    assert not many or rows * 12 * table.shape[1] * 16 > 1 << 24
+    v = kv.read(c, _i32(table), _i32([0, n]), n, torch.float32)[1][:, 0].double()
+    want = (v.cumsum(0)[n - rows:] / torch.arange(n - rows + 1, n + 1, device="cuda")[:, None])[:, None]
+    # one rounding to 16 bits and one of each weight: 2^-11 at most, of values up to max |v|
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -11 * v.abs().max()
+    for cap in (1e-30, 1e-25, 1e-20):
+        out = kv.attention(q, c, _i32(table), _i32([n]), _i32([0, rows]), softcap=cap)
+        assert bool(((out.double() - want).abs() <= tol).all()), cap
