@@ -505,8 +505,9 @@ size_t cp_kv_attention_more_ws_bytes(const cp_kv_cache* cache, int64_t rows, int
 
 /* As cp_kv_attention, with scores and masks changed as ``more`` says. A row at position p sees token j
  * where j < lens[b], j <= p or j < prefix[b] (causal), j > p - window (window > 0), and j >= first[row].
- * Common pages are looked up in the table row of a group's first sequence. With them, a group of
- * sequences whose rows are not all among the call's has no results. */
+ * Common pages are looked up in a group's first row of the table whose first entry is a page (a sequence
+ * that has ended, of 0 tokens, may have given its own back). With them, a group of sequences whose
+ * rows are not all among the call's has no results. */
 int cp_kv_attention_more(const cp_kv_cache* cache, const void* q, int64_t q_row, int64_t q_head,
                          int dtype, int64_t rows, int q_heads, const int32_t* table, int64_t batch,
                          int64_t max_pages, const int32_t* lens, const int32_t* offsets, int causal,

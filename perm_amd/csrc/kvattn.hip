@@ -113,6 +113,20 @@ __device__ __forceinline__ int pieces_of(int used, const AttnMore& x) { return x
 // sequences that kv_locate takes as one
 __device__ __forceinline__ int each_of(const AttnPlain&) { return 1; }
 __device__ __forceinline__ int each_of(const AttnMore& x) { return x.phase == 1 ? x.seqs : 1; }
+// The row of the table in which pages of b are looked up: of a group (phase 1) the first whose first entry is a
+// page, as a sequence that has ended may have given its own back. All lanes of a wave.
+__device__ __forceinline__ int64_t table_row(const AttnArgs&, const AttnPlain&, int b) { return b; }
+__device__ __forceinline__ int64_t table_row(const AttnArgs& a, const AttnMore& x, int b) {
+  if (x.phase != 1) return b;
+  const int64_t first = (int64_t)b * x.seqs;
+  for (int s0 = 0; s0 < x.seqs; s0 += 64) {
+    const int s = s0 + (threadIdx.x & 63);
+    const int p = s < x.seqs ? a.c.table[(first + s) * a.c.max_pages] : -1;
+    const unsigned long long held = __ballot((unsigned)p < (unsigned)a.c.pages);
+    if (held) return first + s0 + __ffsll(held) - 1;
+  }
+  return first;
+}
 
 // A row of the call: its position, the tokens [lo, hi) it sees in this phase (0, 0: none).
 struct SeenRow {
@@ -383,7 +397,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 2 : 4) void attn_few_kernel(AttnArg
 #pragma unroll
   for (int i = 0; i < ND; ++i) o[i] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
-  const int* tab = c.table + (int64_t)b * each_of(ext) * c.max_pages;
+  const int* tab = c.table + table_row(a, ext, b) * c.max_pages;
   // columns past d read the row's first ones instead: their q is 0, and a NaN there makes the
   // score NaN anyway
   int kcol[NC];
@@ -763,7 +777,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(AttnAr
   if constexpr (MODE == 3) {
     if (real) slope = ext.slopes[qh] * kLog2e;
   }
-  const int* tab = c.table + (int64_t)b * each_of(ext) * c.max_pages;
+  const int* tab = c.table + table_row(a, ext, b) * c.max_pages;
   // direct loads. K: rows 1024 / DP each, all in the wave's 16-token group. V: 16 columns
   // each, four token groups. Chunks past d repeat the row's first, rows past d its last 16
   // (their q is 0, their results are dropped).

@@ -238,7 +238,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
 
     shared (int32 [groups]): the batch is groups of as many consecutive sequences each, and in
     group g all rows of the table begin with the same shared[g] pages, as ``kvpages.fork``
-    leaves them. Where sizes say that it pays, those pages are read once for the whole group.
+    leaves them (a sequence that has ended, of 0 tokens, need not hold them any more). Where sizes say that it pays, those pages are read once for the whole group.
     The result is the same, up to the order of the sums."""
     lib = _lib.load()
     desc = _desc(cache)

@@ -214,3 +214,35 @@ def test_small_caps_of_large_keys(kv, many, dtype):  # noqa: F811
     for cap in (1e-30, 1e-25, 1e-20):
         out = kv.attention(q, c, _i32(table), _i32([n]), _i32([0, rows]), softcap=cap)
         assert bool(((out.double() - want).abs() <= tol).all()), cap
+
+
+@pytest.mark.parametrize("counts", [[1] * 6, [0, 30, 30, 0, 1, 30]], ids=["tokens", "rows"])
+@pytest.mark.parametrize("ended", [[0], [0, 1, 3], [0, 1, 2, 3, 4], [0, 1, 2, 4]], ids=str)
+def test_common_pages_of_a_group_whose_first_sequences_have_ended(kv, monkeypatch, ended, counts):  # noqa: F811
+    """Rows given back hold no pages: the others' front is looked up in one that does. Groups of six and of three."""
+    from perm_amd import kvpages
+    rng = np.random.default_rng(51)
+    front, block, own = 40, 16, [20, 33, 50, 7, 1, 64]
+    lens = [front * block + n for n in own]
+    c, o, table = _filled_cache(kv, rng, lens, 2, 64, block)
+    for g in (1, 2):
+        t = table.copy()
+        for b in range(6):
+            t[b, :front] = t[b - b % (6 // g), :front]
+        refs = np.zeros(c.k.shape[0], int)
+        np.add.at(refs, t[t >= 0], 1)
+        refs, t = _i32(refs), _i32(t)
+        kvpages.free(refs, t, _i32(ended))
+        held = _i32([0 if b in ended else n for b, n in enumerate(lens)])
+        n = [0 if b in ended else x for b, x in enumerate(counts)] if max(counts) > 1 else counts
+        offsets = None if max(counts) == 1 else _i32(np.concatenate([[0], np.cumsum(n)]))
+        q = torch.from_numpy(rng.standard_normal((sum(n), 8, 64))).to(torch.bfloat16).cuda()
+        for more in (dict(), dict(softcap=9.0), dict(window=500)):
+            want, wl = kv.attention(q, c, t, held, offsets, return_lse=True, **more)
+            monkeypatch.setattr(kv, "_front_pays", lambda *a: True)
+            got, gl = kv.attention(q, c, t, held, offsets, return_lse=True, shared=_i32([front] * g), **more)
+            monkeypatch.undo()
+            # the same but for the order of float32 sums and one rounding to bfloat16
+            assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max()) + 1e-30
+            some = torch.isfinite(wl)
+            assert torch.equal(some, torch.isfinite(gl)) and bool(((gl - wl).abs()[some] <= 1e-4).all())
