@@ -532,7 +532,8 @@ size_t cp_kv_grow_ws_bytes(int64_t pages, int64_t batch);
 /* Pages for the next fresh[b] (fresh NULL: each) tokens of sequence b, which holds filled[b].
  * Of the entries those tokens fall into, one without a page gets a free one (but not one that
  * tokens held were in), and one whose page has other holders gets a free one in its place: where
- * tokens held are in it, src[b] and dst[b] name the pages to copy from and to (otherwise -1).
+ * tokens held are in it, src[b] and dst[b] name the pages to copy from and to (otherwise -1). Holders
+ * count as before the call: where all of a page's are to write into it, all get one, and it is free then.
  * Sequences are served in order, each wholly or not at all: missing[b] is 0, or the pages it
  * wanted, from the first on for which the free pages do not suffice; also where its tokens pass
  * the end of its row. Free pages are handed out by number. */

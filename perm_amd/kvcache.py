@@ -179,7 +179,10 @@ def _front_pays(desc, rows, heads, batch, groups, tokens):
     launches more and every pair's arithmetic at 0.6 PFLOP/s. One token of 16 heads each on 4096 common
     tokens and up to 512 own: 64 sequences 61 us without and 36 with, 16 sequences 25 and 25; of 32 heads
     on 32768, 64 sequences 395 and 91, 16 110 and 53, 4 39 and 32; 300 rows of each of 32 in four
-    groups on 4096 193 and 189, 30 rows 40 and 54."""
+    groups on 4096 193 and 189, 30 rows 40 and 54.
+
+    tokens is the table's width: lengths are on the GPU. Under a table far wider than its sequences that is
+    a wrong guess (eight of 32 heads with 128 tokens each, 131072 wide: 17 without and 22 with)."""
     pairs = rows * heads // desc.heads
     if batch == groups or pairs == 0 or pairs > 64 * batch:
         return False
@@ -238,8 +241,10 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
 
     shared (int32 [groups]): the batch is groups of as many consecutive sequences each, and in
     group g all rows of the table begin with the same shared[g] pages, as ``kvpages.fork``
-    leaves them (a sequence that has ended, of 0 tokens, need not hold them any more). Where sizes say that it pays, those pages are read once for the whole group.
-    The result is the same, up to the order of the sums."""
+    leaves them (a sequence that has ended, of 0 tokens, need not hold them any more). Where
+    sizes say that it pays, those pages are read once for the whole group. The sizes are the
+    table's: where it is far wider than its sequences, leave ``shared`` away for short fronts. The
+    result is the same, up to the order of the sums."""
     lib = _lib.load()
     desc = _desc(cache)
     if _dtype(q, "q") not in (torch.bfloat16, torch.float16):

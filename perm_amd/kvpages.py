@@ -85,12 +85,13 @@ def grow(refs, table, filled, new, block):
     may be a number for all): (src, dst, missing), int32 [batch] each.
 
     An entry that those tokens fall into gets a page where it has none, and one of its own where
-    other sequences hold its page too. Only the first of them can hold tokens already: src[b] and dst[b] then name the
-    pages that ``copy`` has to copy, and are -1 otherwise; such an entry without a page stays as
-    it is. Free pages are handed out by number, to the sequences in order, until one wants more
-    than there are: it and the ones after it that want any get none, and missing[b] says how many
-    they wanted (also for tokens past the table's end). Write no rows of such a sequence: its
-    last page may be another's too."""
+    other sequences hold its page too. Holders count as before the call: where all of a page's are
+    to write into it, each gets a page, and theirs is free after the call. Only the first entry
+    can hold tokens already: src[b] and dst[b] then name the pages that ``copy`` has to copy, and
+    are -1 otherwise; such an entry without a page stays as it is. Free pages are handed out by
+    number, to the sequences in order, until one wants more than there are: it and the ones after
+    it that want any get none, and missing[b] says how many they wanted (also for tokens past the
+    table's end). Write no rows of such a sequence: its last page may be another's too."""
     lib = _lib.load()
     books = _books(refs, table)
     batch = table.shape[0]
