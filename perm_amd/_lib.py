@@ -260,19 +260,22 @@ def check_index(p, size, what="index", permutation=False):
     return a.astype(np.int32)
 
 
-def stream_ptr():
-    """The current stream's hipStream_t, without the Stream object torch.cuda.current_stream()
-    builds each time (0.1 us instead of 2.8)."""
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+def stream_ptr(device=None):
+    """The current stream's hipStream_t (of ``device``, the current one's number where it is known),
+    without the Stream object torch.cuda.current_stream() builds each time (0.1 us instead of 2.8)."""
+    if device is None:
+        device = torch.cuda.current_device()
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device))
 
 
 def here(*tensors):
     """Refuses tensors (None: not given) of another device than the current one, on whose stream
-    kernels run."""
+    kernels run: that device's number."""
     at = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != at:
             raise ValueError(f"a tensor on {t.device}, but the current device is cuda:{at}")
+    return at
 
 
 def ptr(t):

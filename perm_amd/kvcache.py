@@ -80,8 +80,8 @@ def _desc(c):
 
 
 def _index(t, dims, what):
-    """An int32 CUDA tensor of ``dims`` dimensions, contiguous."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+    """An int32 tensor of ``dims`` dimensions, contiguous (its device: ``_lib.here``)."""
+    if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what} must be a CUDA tensor")
     if t.dtype != torch.int32 or t.dim() != dims:
         raise IndexError(f"{what} must be int32 with {dims} dimension(s), got {t.dtype} "
@@ -114,8 +114,6 @@ def _dtype(x, what):
 
 def _heads(x, heads, d, what):
     """x [rows, heads, d] in strides the kernels read in place (copied where they cannot)."""
-    if not x.is_cuda:
-        raise ValueError(f"{what} must be on the GPU")
     if x.dim() != 3 or x.shape[2] != d or (heads is not None and x.shape[1] != heads):
         raise ValueError(f"{what} is {tuple(x.shape)}: [rows, {heads or 'heads'}, {d}]")
     step = 16 // x.element_size()
@@ -142,13 +140,13 @@ def write(cache, k, v, table, filled, offsets=None):
     if v.shape[0] != rows:
         raise ValueError(f"{rows} keys and {v.shape[0]} values")
     table, filled, offsets = _batch(table, filled, "filled", offsets, rows)
-    _lib.here(k, v, table, filled, offsets, *cache)
+    device = _lib.here(k, v, table, filled, offsets, *cache)
     if table.shape[0] == 0:
         return
     _lib.check(lib.cp_kv_write(
         ctypes.byref(desc), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
         v.stride(1), DTYPES[dtype], rows, table.data_ptr(), table.shape[0], table.shape[1],
-        filled.data_ptr(), _lib.ptr(offsets), _lib.stream_ptr()))
+        filled.data_ptr(), _lib.ptr(offsets), _lib.stream_ptr(device)))
 
 
 def read(cache, table, offsets, total, dtype=torch.bfloat16):
@@ -162,13 +160,13 @@ def read(cache, table, offsets, total, dtype=torch.bfloat16):
     if offsets is None:
         raise ValueError("read needs offsets")
     table, _, offsets = _batch(table, None, "", offsets, total)
-    _lib.here(table, offsets, *cache)
+    device = _lib.here(table, offsets, *cache)
     shape = total, desc.heads, desc.head_dim
     k = cache.k.new_empty(shape, dtype=dtype)
     v = torch.empty_like(k)
     _lib.check(lib.cp_kv_read(ctypes.byref(desc), table.data_ptr(), table.shape[0],
                               table.shape[1], offsets.data_ptr(), total, k.data_ptr(),
-                              v.data_ptr(), DTYPES[dtype], _lib.stream_ptr()))
+                              v.data_ptr(), DTYPES[dtype], _lib.stream_ptr(device)))
     return k, v
 
 
@@ -257,7 +255,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     if window < 0:
         raise ValueError(f"window {window}")
     table, lens, offsets = _batch(table, lens, "lens", offsets, rows)
-    _lib.here(q, table, lens, offsets, *cache)
+    device = _lib.here(q, table, lens, offsets, *cache)
     more = None
     if softcap or slopes is not None or first is not None or prefix is not None or shared is not None:
         more, keep = _more(desc, table, rows, heads, q.device, softcap, slopes, first, prefix, shared)
@@ -283,7 +281,7 @@ def attention(q, cache, table, lens, offsets=None, *, causal=True, window=0, sca
     args = [ctypes.byref(desc), q.data_ptr(), q.stride(0), q.stride(1), DTYPES[q.dtype], rows,
             heads, table.data_ptr(), batch, max_pages, lens.data_ptr(), _lib.ptr(offsets),
             int(causal), window, desc.head_dim ** -0.5 if scale is None else float(scale)]
-    ends = [out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr()]
+    ends = [out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), nws, _lib.stream_ptr(device)]
     if more is None:
         _lib.check(lib.cp_kv_attention(*args, *ends))
     else:

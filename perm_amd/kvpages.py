@@ -149,8 +149,8 @@ def copy(cache, src, dst, into=None):
     desc = _desc(cache)
     to = desc if into is None else _desc(into)
     device = cache[0].device
-    _lib.here(*cache, *(into or ()))
+    at = _lib.here(*cache, *(into or ()))
     src = _ints(src, 1, "src", device)
     dst = _ints(dst, 1, "dst", device, src.shape[0])
     _lib.check(lib.cp_kv_copy(ctypes.byref(desc), ctypes.byref(to), src.data_ptr(), dst.data_ptr(),
-                              src.shape[0], _lib.stream_ptr()))
+                              src.shape[0], _lib.stream_ptr(at)))

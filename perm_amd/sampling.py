@@ -56,7 +56,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocab], got {tuple(logits.shape)}")
     dev = logits.device
-    _lib.here(logits)
+    at = _lib.here(logits)
     rows, vocab = logits.shape
     if not isinstance(u, torch.Tensor) or u.device != dev or u.shape != (rows,):
         raise ValueError(f"u must be a tensor [{rows}] on {dev}")
@@ -75,5 +75,5 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     _lib.check(lib.cp_sample(logits.data_ptr(), code, rows, vocab, logits.stride(0), u.data_ptr(),
                              int(u.dtype == torch.float64), _lib.ptr(t), t_all, _lib.ptr(k), k_all,
                              _lib.ptr(p), p_all, _lib.ptr(m), m_all, token.data_ptr(),
-                             _lib.ptr(ws), nws, _lib.stream_ptr()))
+                             _lib.ptr(ws), nws, _lib.stream_ptr(at)))
     return token
